@@ -238,6 +238,96 @@ int zh_moe_weighted_acc(zh_ctx *ctx, zh_buf *a, const zh_buf *b, const zh_buf *r
  * as sampleGreedy's CPU scan (forward.zig:10343-10356). result: u32. */
 int zh_argmax(zh_ctx *ctx, const zh_buf *logits, uint32_t n, zh_buf *result, uint64_t result_off);
 
+/* ---- batches over one layer's paged cache (no counterpart in the reference,
+ *      whose engine decodes one sequence) -------------------------------- */
+/* One layer's K and V caches, fp16 [n_kv_heads][cache_tokens][head_dim] each
+ * (cache_tokens a multiple of 16), and the page tables of a batch: u32
+ * [n_seq][table_stride], logical 16-token page i of sequence s in physical
+ * page tables[s * table_stride + i]. Sequences may share pages (zh_kv_pool_fork).
+ * The tables are read on the device. */
+typedef struct zh_kv_batch {
+    zh_buf *k_cache, *v_cache;
+    const zh_buf *tables;
+    uint32_t n_seq, table_stride, cache_tokens, n_kv_heads, head_dim, reserved;
+} zh_kv_batch;
+/* q, k and v rows of a batch of tokens: row t of a matrix is at its offset
+ * (bytes) + t * stride elements (0: rows without gaps; the three may be parts
+ * of one stacked projection's rows). Row t is the token of sequence seq[t] at position pos[t]
+ * (seq NULL: sequence t); the rows of a sequence may stand anywhere. */
+typedef struct zh_qkv_rows {
+    const zh_buf *q, *k, *v;
+    uint64_t q_off, k_off, v_off;
+    uint32_t q_stride, k_stride, v_stride;
+    uint32_t type;                   /* of q, k and v: ZH_F32 or ZH_F16 */
+    zh_buf *q_out;                   /* may be q's own rows (same offset, stride and type) */
+    uint64_t q_out_off;
+    uint32_t q_out_stride, q_out_type;
+    const zh_buf *q_norm_w, *k_norm_w; /* f32 [head_dim]; NULL: not normalised */
+    const zh_buf *inv_freq;          /* f32 [rope_dim / 2] */
+    const zh_buf *seq, *pos;         /* u32 [n_rows] */
+    uint32_t n_rows, n_q_heads, rope_dim;
+    float eps;
+} zh_qkv_rows;
+/* zh_qk_norm_rope_kv_write for a batch, enqueued without waiting: per head
+ * h = w * (x / sqrt(mean x^2 + eps)) of q and k, dims i and i + rope_dim / 2
+ * (i < rope_dim / 2) rotated by pos * inv_freq[i], the dims from rope_dim on
+ * passed through; q to q_out, k and v (as it is) to the row's cache slot. The
+ * angle is taken and reduced in 64 bits, the rest in 32 and rounded once.
+ * pos[t] == ZH_POS_NONE: a padded row, nothing of it is read or written. A row
+ * whose sequence, page entry or page lies outside has its q_out written and no
+ * cache slot, and the next zh_sync returns ZH_ERR_INVALID_ARGUMENT. Where rows
+ * of one call name the same slot it holds, head by head, one of them. head_dim
+ * even and at most 512, rope_dim even and at most head_dim (0: no rotation). */
+#define ZH_POS_NONE 0xFFFFFFFFu
+int zh_qk_norm_rope_kv_write_batched(zh_ctx *ctx, const zh_kv_batch *kv, const zh_qkv_rows *rows);
+/* One query row per sequence of a batch and where its result goes (strides in
+ * elements, 0: rows without gaps; offsets in bytes; rows 16-byte aligned; out
+ * may be q's own rows). */
+typedef struct zh_decode_rows {
+    const zh_buf *q;
+    zh_buf *out;
+    uint64_t q_off, out_off;
+    uint32_t q_stride, out_stride;
+    uint32_t type;                   /* of q and out: ZH_F32 or ZH_F16 */
+    uint32_t n_heads;                /* a multiple of n_kv_heads, at most 16 per kv head */
+    const zh_buf *seq_lens;          /* u32 [n_seq], on the device */
+    zh_buf *ws;                      /* zh_flash_decode_shared_ws bytes */
+    uint32_t prefix_len, max_len;
+    float attn_scale;                /* 0: 1/sqrt(head_dim) */
+    uint32_t reserved;
+} zh_decode_rows;
+/* Paged decode attention of a batch whose sequences share their first
+ * prefix_len tokens: out[s] = softmax(scale q[s] K^T) V over the tokens
+ * t < seq_lens[s] of sequence s (its new token's K and V are in the cache).
+ * K and V of the tokens below prefix_len are read once for all sequences,
+ * through sequence 0's table; a sequence shorter than prefix_len attends
+ * through its own table alone. prefix_len 0: nothing shared. seq_lens[s] == 0:
+ * the row is zero. A length past max_len or the table is cut there, a page
+ * outside the cache reads as page 0, and the next zh_sync then returns
+ * ZH_ERR_INVALID_ARGUMENT. Nothing past a sequence's end enters its result,
+ * whatever the cache holds there. head_dim 64 or 128. ZH_F32: q and the
+ * probabilities in two fp16 pieces each (22 bits); ZH_F16: in one; sums and
+ * softmax in 32 bits. Allocates nothing and adds in a fixed order; calls that
+ * may overlap (other contexts, replayed graphs) need a ws each. */
+int zh_flash_decode_shared(zh_ctx *ctx, const zh_kv_batch *kv, const zh_decode_rows *rows);
+/* Bytes of ws for a call of these sizes (0: refused sizes). */
+uint64_t zh_flash_decode_shared_ws(zh_ctx *ctx, const zh_kv_batch *kv, uint32_t n_heads, uint32_t prefix_len,
+                                   uint32_t max_len);
+/* A set of caches of one shape (the K and V caches of some or all layers). */
+typedef struct zh_kv_caches {
+    zh_buf *const *caches;
+    uint32_t n_caches, cache_tokens, n_kv_heads, head_dim;
+} zh_kv_caches;
+/* Copies page src_pages[i] of every cache of src to page dst_pages[i] of the
+ * same cache of dst (i < n_pages; the page numbers are host memory, read before
+ * the call returns; the copies are enqueued). dst and src may be the same
+ * caches or those of another sequence or engine, with as many heads and dims;
+ * a source page may go to several places. Refused with ZH_ERR_INVALID_ARGUMENT
+ * and nothing copied: a page outside its caches, two copies to one page, and a
+ * page both read and written where dst and src share a cache. */
+int zh_kv_copy_pages(zh_ctx *ctx, const zh_kv_caches *dst, const zh_kv_caches *src, const uint32_t *dst_pages,
+                     const uint32_t *src_pages, uint32_t n_pages);
+
 /* ---- engine: InferenceEngine surface (forward.zig:1226-10983) ---------- */
 /* Batched prefill projection (dispatchProjectionBatched, forward.zig:8147-8216;
  * recordMulMmQ4K dmmv.zig:1045-1094 / mul_mm_q4k.comp): Y[n][m] (+= when
@@ -364,8 +454,37 @@ int      zh_kv_pool_alloc(zh_kv_pool *pool, uint64_t request_id, uint32_t count,
 void     zh_kv_pool_free(zh_kv_pool *pool, uint64_t request_id);                          /* freePages */
 uint32_t zh_kv_pool_free_count(const zh_kv_pool *pool);                                  /* freeCount */
 uint32_t zh_kv_pool_max_context(const zh_kv_pool *pool, uint32_t page_count);            /* maxContext */
+/* Sharing pages (no counterpart in the reference, where a page has one owner).
+ * A request's pages keep the order in which it got them: entry i of
+ * zh_kv_pool_pages is logical page i of its page table. */
+/* child (a request without pages) gets the first n_pages pages of parent,
+ * shared: they are free again when every holder has given them back. */
+int      zh_kv_pool_fork(zh_kv_pool *pool, uint64_t parent, uint64_t child, uint32_t n_pages);
+/* Before request_id writes into its logical page `index`: if the page is
+ * shared, it is replaced by a free one of its own (*src: the shared page, *dst:
+ * the new one, for zh_kv_copy_pages; ZH_ERR_KV_CACHE_EXHAUSTED if none is
+ * free); a page of its own stays (*src == *dst). */
+int      zh_kv_pool_unshare(zh_kv_pool *pool, uint64_t request_id, uint32_t index, uint32_t *src, uint32_t *dst);
+/* Gives back the pages past the first `keep`. */
+int      zh_kv_pool_trim(zh_kv_pool *pool, uint64_t request_id, uint32_t keep);
+/* The number of pages of request_id; the first `cap` of them into page_ids. */
+uint32_t zh_kv_pool_pages(const zh_kv_pool *pool, uint64_t request_id, uint32_t *page_ids, uint32_t cap);
+uint32_t zh_kv_pool_refs(const zh_kv_pool *pool, uint32_t page);  /* holders of a page; 0: free */
+/* Renumbers the pages in use to 0 .. n - 1: the pages past that move to the
+ * free ones below, src[i] to dst[i] (the copies the caller then makes with
+ * zh_kv_copy_pages, before the next use of the tables; *n_moves of them). With
+ * fewer than *n_moves places in the arrays (cap) nothing is renumbered and
+ * ZH_ERR_INVALID_ARGUMENT returned; total_pages / 2 always suffice. */
+int      zh_kv_pool_compact(zh_kv_pool *pool, uint32_t *src, uint32_t *dst, uint32_t cap, uint32_t *n_moves);
 int zh_engine_read_kv(zh_engine *eng, uint32_t layer, uint32_t which, uint32_t t0, uint32_t n,
                       uint16_t *dst);
+/* Copies the K and V of the first n_tokens positions of src's sequence into
+ * dst's (whole pages through both page tables, in dst's stream after src's work
+ * so far; nothing of dst's other positions): a prompt is prefilled once and
+ * continued by several engines (zh_engine_generate_batch). Same layers, kv
+ * heads and head dims; n_tokens within both capacities. The page of dst in
+ * which n_tokens ends is copied whole. */
+int zh_engine_fork_kv(zh_engine *dst, zh_engine *src, uint32_t n_tokens);
 /* Model bytes touched per decoded token at context length L (weights + fp16
  * KV + activations), the numerator of the bandwidth roofline. */
 uint64_t zh_engine_bytes_per_token(zh_engine *eng, uint32_t L);

@@ -1,0 +1,624 @@
+"""The batched operators over a paged KV cache on the GPU, against plain numpy
+in 64 bits on the same fp16 cache and page tables.
+
+Tolerances. An f32 rounding is off by 2^-24 of the value, an fp16 one by 2^-11
+(or 2^-25 below the normal range).
+  rope: mean of squares, square root, division and the products before the
+    rotation: at most 24 roundings of 2^-24; the angle enters as a fraction of a
+    turn within 2^-26 (2^-23.3 radians), its sine and cosine within 2^-22; three
+    roundings of the rotation. Together less than 2^-19 (|a| + |b|) for the pair
+    (a, b), and the store's own rounding.
+  attention: a score is off by at most 2^-18 A, A = 1.45 scale sum |q_i k_i| of
+    its row's largest (q in two pieces: 2^-22; 8 chained matrix instructions of
+    32 products, each step within 2^-22 of the sum of magnitudes; the scaling and
+    the subtraction of the maximum 2^-23 each), and with it a weight by 2^-18 A
+    relative plus 2^-21 (exp2, two pieces). That enters the numerator and the sum
+    of weights; the sums over n tokens add n / 32 + 64 steps of 2^-23:
+    |error| <= W (2^-17 A + (n / 32 + 80) 2^-23), W = sum w |v| of the output.
+    ZH_F16 adds 2^-11 W for the weights in one piece and the store's rounding.
+"""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+NONE = 0xFFFFFFFF
+
+
+@pytest.fixture(scope="module")
+def zh():
+    import zinc_amd
+    return zinc_amd
+
+
+@pytest.fixture()
+def ctx(zh):
+    c = zh.Context(0)
+    yield c
+    c.close()
+
+
+NP_TYPE = {0: np.float32, 1: np.float16}
+
+
+def store_error(t, y):
+    """The rounding of a stored y of type t."""
+    return np.abs(y) * 2.0 ** (-24 if t == 0 else -11) + (0 if t == 0 else 2.0 ** -25)
+
+
+def close(got, want, tol, where=...):
+    err = np.abs(got - want)
+    ok = (err <= tol)[where].all()
+    assert ok, (float(np.nanmax(err)), float(np.nanmax((err - tol)[where])), int((~(err <= tol))[where].sum()))
+
+
+# ---------------------------------------------------------------------------
+# page copies
+# ---------------------------------------------------------------------------
+def copied(caches, dst, src, nkv, hd):
+    out = []
+    for c in caches:
+        c = c.copy().reshape(nkv, -1, 16, hd)
+        c[:, dst] = c[:, src]
+        out.append(c.reshape(-1))
+    return out
+
+
+@pytest.mark.parametrize("n_caches,nkv,hd,pool,n", [
+    (1, 1, 64, 4, 1), (2, 8, 128, 40, 13), (97, 2, 64, 9, 3), (3, 3, 80, 700, 300), (2, 1, 2, 30, 11), (4, 5, 6, 20, 9),
+    (2, 2, 512, 12, 5), (2, 4, 128, 1100, 513)])
+def test_copy_pages(zh, ctx, n_caches, nkv, hd, pool, n):
+    rng = np.random.default_rng(pool + n)
+    caches = [rng.integers(0, 1 << 16, nkv * pool * 16 * hd).astype(np.uint16) for _ in range(n_caches)]
+    bufs = [ctx.upload(c) for c in caches]
+    s = zh.KvCaches(bufs, pool * 16, nkv, hd)
+    perm = rng.permutation(pool)
+    dst, src = perm[:n], rng.choice(perm[n:], n)  # a source may go to several places
+    ctx.kv_copy_pages(s, s, dst, src)
+    for b, want in zip(bufs, copied(caches, dst, src, nkv, hd)):
+        assert np.array_equal(b.download(np.uint16, want.size), want)
+
+
+def test_copy_between_caches_of_other_sizes(zh, ctx):
+    rng = np.random.default_rng(3)
+    nkv, hd = 2, 64
+    a = [rng.integers(0, 1 << 16, (nkv, 10, 16, hd)).astype(np.uint16) for _ in range(2)]
+    b = [rng.integers(0, 1 << 16, (nkv, 7, 16, hd)).astype(np.uint16) for _ in range(2)]
+    A, B = [ctx.upload(x) for x in a], [ctx.upload(x) for x in b]
+    ctx.kv_copy_pages(zh.KvCaches(B, 7 * 16, nkv, hd),
+                      zh.KvCaches(A, 160, nkv, hd), [6, 0, 3], [9, 3, 0])
+    for x, y, Y in zip(a, b, B):
+        y[:, [6, 0, 3]] = x[:, [9, 3, 0]]
+        assert np.array_equal(Y.download(np.uint16, y.size), y.reshape(-1))
+    for x, X in zip(a, A):
+        assert np.array_equal(X.download(np.uint16, x.size), x.reshape(-1))
+
+
+def test_copy_refusal_changes_nothing_and_none_is_fine(zh, ctx):
+    c = np.arange(4 * 16 * 64, dtype=np.uint16)
+    b = ctx.upload(c)
+    s = zh.KvCaches([b], 64, 1, 64)
+    for d, q in (([1, 1], [2, 3]), ([1, 2], [2, 3]), ([1], [4])):
+        with pytest.raises(zh.ZincError) as e:
+            ctx.kv_copy_pages(s, s, d, q)
+        assert e.value.name == "InvalidArgument"
+    ctx.kv_copy_pages(s, s, [], [])
+    ctx.sync()
+    assert np.array_equal(b.download(np.uint16, c.size), c)
+
+
+# ---------------------------------------------------------------------------
+# q/k norm + rotation + KV write
+# ---------------------------------------------------------------------------
+def rope64(x, w, freq, pos, eps, rd):
+    """x [T][heads][hd]: the rotated rows and sum |a| + |b| of each pair."""
+    x = x.astype(np.float64)
+    if w is not None:
+        x = w.astype(np.float64) * (x / np.sqrt((x * x).mean(-1, keepdims=True) + eps))
+    y, mag = x.copy(), np.abs(x)
+    h = rd // 2
+    if h:
+        th = (pos.astype(np.float64)[:, None] * freq.astype(np.float64))[:, None]
+        a, b = x[..., :h], x[..., h:rd]
+        y[..., :h], y[..., h:rd] = a * np.cos(th) - b * np.sin(th), a * np.sin(th) + b * np.cos(th)
+        mag[..., :h] = mag[..., h:rd] = np.abs(a) + np.abs(b)
+    return y, mag
+
+
+ROPE = [  # rows, seqs, q heads, kv heads, head_dim, rope_dim, type, q type, norm, stacked
+    (1, 1, 4, 2, 128, 128, 0, 0, True, False),
+    (5, 3, 32, 8, 128, 128, 0, 0, True, True),
+    (33, 4, 10, 2, 128, 64, 0, 1, True, True),
+    (70, 2, 7, 7, 64, 64, 1, 1, True, True),
+    (300, 9, 8, 1, 64, 32, 1, 0, False, True),
+    (19, 19, 6, 3, 256, 256, 0, 1, True, True),
+    (9, 2, 3, 1, 80, 80, 0, 0, True, False),     # no power of two
+    (9, 2, 3, 1, 96, 40, 1, 1, True, True),
+    (12, 3, 2, 2, 6, 4, 1, 1, True, True),       # odd sizes, 2-byte aligned rows
+    (4, 1, 2, 1, 2, 2, 0, 0, False, False),
+    (8, 2, 4, 4, 512, 512, 0, 0, True, True),
+    (8, 2, 4, 2, 128, 0, 0, 1, True, True),      # norm alone
+    (40, 5, 16, 4, 128, 128, 1, 1, False, True),
+    (1030, 3, 5, 5, 128, 128, 0, 1, True, True),
+]
+
+
+@pytest.mark.parametrize("case", ROPE, ids=lambda c: "-".join(map(str, c)))
+def test_rope_batched(zh, ctx, case):
+    T, S, nq, nkv, hd, rd, ti, tq, norm, stacked = case
+    rng = np.random.default_rng(T * 7 + hd)
+    far = 200000
+    stride = far // 16 + 1
+    # rows of sequences in any order, distinct positions, some rows padded
+    seq = rng.integers(0, S, T)
+    pos = rng.choice(far, T, replace=False)
+    pos[0] = far - 1
+    pages_needed = sorted({(s, p // 16) for s, p in zip(seq, pos)})
+    pool = len(pages_needed) + 2
+    perm = rng.permutation(pool).astype(np.uint32)
+    tables = np.full((S, stride), pool + 7, dtype=np.uint32)  # (entries that no row uses lie outside)
+    for i, (s, p) in enumerate(pages_needed):
+        tables[s, p] = perm[i]
+    pad = rng.random(T) < 0.1
+    pad[0] = False
+    tokens = pool * 16
+    kc, vc = (rng.standard_normal((nkv, tokens, hd)).astype(np.float16) for _ in range(2))
+    qkv = (rng.standard_normal((T, nq + 2 * nkv, hd)) * 3).astype(NP_TYPE[ti])
+    qw, kw = ((1 + 0.2 * rng.standard_normal(hd)).astype(np.float32) for _ in range(2))
+    freq = (1e6 ** (-np.arange(0, rd, 2) / max(rd, 1))).astype(np.float32)
+    size, width = np.dtype(NP_TYPE[ti]).itemsize, (nq + 2 * nkv) * hd
+    gap = 8 if stacked else 0
+    out0 = rng.standard_normal((T + 1, nq * hd + gap)).astype(NP_TYPE[tq])
+    u = ctx.upload
+    kcb, vcb = u(kc), u(vc)
+    kv = zh.KvBatch(kcb, vcb, u(tables), S, stride, tokens, nkv, hd)
+    if stacked:
+        X = u(qkv)
+        where = dict(q=X, k=X, v=X, k_off=nq * hd * size, v_off=(nq + nkv) * hd * size, q_stride=width, k_stride=width,
+                     v_stride=width)
+    else:
+        where = dict(q=u(qkv[:, :nq]), k=u(qkv[:, nq:nq + nkv]), v=u(qkv[:, nq + nkv:]))
+    outb = u(out0)
+    rows = zh.QkvRows(q_out=outb, q_out_stride=nq * hd + gap, pos=u(np.where(pad, NONE, pos).astype(np.uint32)),
+                      seq=u(seq.astype(np.uint32)), n_rows=T, n_q_heads=nq, rope_dim=rd,
+                      inv_freq=u(freq) if rd else None, q_norm_w=u(qw) if norm else None,
+                      k_norm_w=u(kw) if norm else None, type=ti, q_out_type=tq, eps=1e-5, **where)
+    ctx.qk_norm_rope_kv_write_batched(kv, rows)
+    ctx.sync()
+    got = outb.download(NP_TYPE[tq], out0.size).reshape(out0.shape)
+    want, mag = rope64(qkv[:, :nq], qw if norm else None, freq, pos, 1e-5, rd)
+    live = ~pad
+    err = np.abs(got[:T, :nq * hd].reshape(T, nq, hd).astype(np.float64) - want)
+    assert (err <= mag * 2.0 ** -19 + store_error(tq, want))[live].all(), err[live].max()
+    # padded rows, the gaps and the row behind are as they were
+    assert np.array_equal(got[:T][pad], out0[:T][pad]) and np.array_equal(got[T], out0[T])
+    assert np.array_equal(got[:, nq * hd:], out0[:, nq * hd:])
+    k64, kmag = rope64(qkv[:, nq:nq + nkv], kw if norm else None, freq, pos, 1e-5, rd)
+    wk, wv, tol = kc.astype(np.float64), vc.astype(np.float64), np.zeros(kc.shape)
+    for t in np.flatnonzero(live):
+        slot = int(tables[seq[t], pos[t] // 16]) * 16 + pos[t] % 16
+        wk[:, slot], wv[:, slot] = k64[t], qkv[t, nq + nkv:].astype(np.float16)
+        tol[:, slot] = kmag[t] * 2.0 ** -19 + store_error(1, k64[t])
+    gk, gv = (b.download(np.float16, kc.size).reshape(kc.shape).astype(np.float64) for b in (kcb, vcb))
+    assert (np.abs(gk - wk) <= tol).all() and np.array_equal(gv, wv)
+
+
+def test_rope_in_place_and_like_the_single_token_entry(zh, ctx):
+    """One row through both entries (near positions, where a 32-bit angle is
+    good to 2^-24 of itself: at most 40 radians), q in place."""
+    rng = np.random.default_rng(1)
+    nq, nkv, hd, tokens = 8, 2, 128, 64
+    q, k, v = (rng.standard_normal(n * hd).astype(np.float32) for n in (nq, nkv, nkv))
+    qw, kw = ((1 + 0.1 * rng.standard_normal(hd)).astype(np.float32) for _ in range(2))
+    freq = (1e6 ** (-np.arange(0, hd, 2) / hd)).astype(np.float32)
+    pages = np.array([2, 0, 3, 1], dtype=np.uint32)
+    u = ctx.upload
+    got = []
+    for batched in (False, True):
+        Q, kc, vc = u(q), u(np.zeros((nkv, tokens, hd), np.float16)), u(np.zeros((nkv, tokens, hd), np.float16))
+        if batched:
+            kv = zh.KvBatch(kc, vc, u(pages), 1, 4, tokens, nkv, hd)
+            ctx.qk_norm_rope_kv_write_batched(kv, zh.QkvRows(
+                q=Q, k=u(k), v=u(v), q_out=Q, pos=u(np.array([39], np.uint32)), n_rows=1, n_q_heads=nq, rope_dim=hd,
+                inv_freq=u(freq), q_norm_w=u(qw), k_norm_w=u(kw), eps=1e-6))
+        else:
+            ctx.qk_norm_rope_kv_write(Q, u(qw), u(k), u(kw), u(v), u(freq), kc, vc, u(pages), 4, tokens, nq, nkv, hd,
+                                      39, 1e-6)
+        got.append((Q.download(np.float32, q.size), kc.download(np.float16, nkv * tokens * hd),
+                    vc.download(np.float16, nkv * tokens * hd)))
+    mag = 2 * np.abs(q).max() * 1.5 * 2
+    assert np.abs(got[0][0] - got[1][0]).max() <= mag * (39 * 2.0 ** -24 + 2.0 ** -18)
+    assert np.abs(got[0][1].astype(np.float64) - got[1][1]).max() <= mag * (39 * 2.0 ** -24 + 2.0 ** -18 + 2.0 ** -10)
+    assert np.array_equal(got[0][2], got[1][2])
+
+
+def test_rope_rows_outside_are_left_out_and_reported(zh, ctx):
+    rng = np.random.default_rng(2)
+    nq, nkv, hd, tokens, S, stride = 2, 1, 64, 64, 2, 3
+    x = rng.standard_normal((5, 4, hd)).astype(np.float32)
+    u = ctx.upload
+    kc0 = rng.standard_normal((nkv, tokens, hd)).astype(np.float16)
+    kc, vc = u(kc0), u(kc0)
+    tables = np.array([[0, 1, 4], [2, 0xFFFFFFFF, 0x10000000]], dtype=np.uint32)  # 4 and the last two lie outside
+    seq = np.array([0, 0, 1, 1, 2], dtype=np.uint32)
+    pos = np.array([48, 33, 17, 40, 3], dtype=np.uint32)  # past the table, page 4, no page, wrapped page, no sequence
+    out = ctx.alloc(4 * 5 * nq * hd)
+    X = u(x)
+    kv = zh.KvBatch(kc, vc, u(tables), S, stride, tokens, nkv, hd)
+    rows = dict(q=X, k=X, v=X, k_off=4 * 2 * hd, v_off=4 * 3 * hd, q_stride=4 * hd, k_stride=4 * hd, v_stride=4 * hd,
+                q_out=out, seq=u(seq), pos=u(pos), n_q_heads=nq)
+    ctx.qk_norm_rope_kv_write_batched(kv, zh.QkvRows(n_rows=5, **rows))
+    with pytest.raises(zh.ZincError) as e:
+        ctx.sync()
+    assert e.value.name == "InvalidArgument"
+    ctx.sync()  # reported once
+    assert np.array_equal(out.download(np.float32, 5 * nq * hd).reshape(5, nq, hd), x[:, :nq])
+    for b in (kc, vc):
+        assert np.array_equal(b.download(np.float16, kc0.size).reshape(kc0.shape), kc0)
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+def attend64(q, kc, vc, tables, lens, scale, t, P=0):
+    """(out, bound) of the module's formula; q [S][nh][hd]. The first P tokens
+    of the sequences that long are read through sequence 0's table."""
+    S, nh, hd = q.shape
+    nkv = kc.shape[0]
+    G = nh // nkv
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    for s in range(S):
+        n = int(lens[s])
+        if n == 0:
+            continue
+        tk = np.arange(n)
+        via = np.where((tk < P) & (n >= P), 0, s)
+        at = tables[via, tk // 16].astype(np.int64) * 16 + tk % 16
+        for h in range(nh):
+            k, v = kc[h // G, at].astype(np.float64), vc[h // G, at].astype(np.float64)
+            x = q[s, h].astype(np.float64)
+            sc = k @ x * scale
+            A = 1.45 * scale * (np.abs(k) @ np.abs(x)).max()
+            w = np.exp(sc - sc.max())
+            w /= w.sum()
+            out[s, h], W = w @ v, w @ np.abs(v)
+            tol[s, h] = W * (2.0 ** -17 * A + (n / 32 + 80) * 2.0 ** -23) + store_error(t, out[s, h])
+            if t == 1:
+                tol[s, h] += W * 2.0 ** -11
+    return out, tol
+
+
+def make(rng, S, nkv, hd, P, lens, shared=True, spare=2, poison=True):
+    """Caches and tables of sequences sharing their first P tokens; every slot
+    that no sequence uses, and the tables' unused entries, hold what must not
+    enter a result."""
+    lens = np.asarray(lens)
+    M = max(int(lens.max()), P, 1)
+    stride = -(-M // 16)
+    full = P // 16 if shared else 0
+    own = [max(0, -(-int(n) // 16) - full) if n >= P else -(-int(n) // 16) for n in lens]
+    own[0] = max(own[0], stride - full) if P else own[0]  # sequence 0's table covers the prefix
+    total = full + sum(own) + spare
+    perm = rng.permutation(total).astype(np.uint32)
+    tables = np.full((S, stride), 0xFFFFFFF0, dtype=np.uint32)
+    kc = np.full((nkv, total * 16, hd), np.nan if poison else 1.0, dtype=np.float16)
+    vc = kc.copy()
+    if poison:
+        vc[:, ::3] = np.inf
+    at = full
+    for s in range(S):
+        k = full if lens[s] >= P or s == 0 else 0
+        tables[s, :k] = perm[:k]
+        tables[s, k:k + own[s]] = perm[at:at + own[s]]
+        at += own[s]
+    base = [rng.standard_normal((P, nkv, hd)).astype(np.float16) for _ in range(2)]
+    for s in range(S):
+        n = int(lens[s])
+        if s == 0:
+            n = max(n, P)
+        t = np.arange(n)
+        slots = tables[s, t // 16].astype(np.int64) * 16 + t % 16
+        for c, b in zip((kc, vc), base):
+            x = rng.standard_normal((n, nkv, hd)).astype(np.float16)
+            if n >= P:
+                x[:P] = b
+            c[:, slots] = x.transpose(1, 0, 2)
+    return kc, vc, tables, total * 16, M
+
+
+def run_attention(zh, ctx, q, kc, vc, tables, lens, P, M, t, scale=0.0, gap=0, in_place=False, expect_error=False):
+    S, nh, hd = q.shape
+    u = ctx.upload
+    kv = zh.KvBatch(u(kc), u(vc), u(tables), S, tables.shape[1], kc.shape[1], kc.shape[0], hd)
+    rng = np.random.default_rng(9)
+    buf = rng.standard_normal((S + 1, nh * hd + gap)).astype(NP_TYPE[t])
+    buf[:S, :nh * hd] = q.reshape(S, -1)
+    out0 = buf.copy() if in_place else rng.standard_normal(buf.shape).astype(NP_TYPE[t])
+    Q = u(buf)
+    O = Q if in_place else u(out0)
+    n = ctx.flash_decode_shared_ws(kv, nh, P, M)
+    assert n > 0
+    guard = np.full(n // 4 + 64, 0x5A5A5A5A, dtype=np.uint32)
+    ws = u(guard)
+    rows = zh.DecodeRows(q=Q, out=O, seq_lens=u(np.asarray(lens, dtype=np.uint32)), ws=ws, n_heads=nh, prefix_len=P,
+                         max_len=M, type=t, q_stride=nh * hd + gap, out_stride=nh * hd + gap, attn_scale=scale)
+    ctx.flash_decode_shared(kv, rows)
+    if expect_error:
+        with pytest.raises(zh.ZincError) as e:
+            ctx.sync()
+        assert e.value.name == "InvalidArgument"
+    ctx.sync()
+    got = O.download(NP_TYPE[t], out0.size).reshape(out0.shape)
+    assert np.array_equal(got[:, nh * hd:], out0[:, nh * hd:]) and np.array_equal(got[S], out0[S])
+    assert (ws.download(np.uint32, guard.size)[(n + 3) // 4:] == 0x5A5A5A5A).all()
+    if not in_place:
+        ctx.flash_decode_shared(kv, rows)  # the same bits again
+        if expect_error:
+            with pytest.raises(zh.ZincError):
+                ctx.sync()
+        assert np.array_equal(O.download(NP_TYPE[t], out0.size).view(np.uint8), got.reshape(-1).view(np.uint8))
+    return got[:S, :nh * hd].reshape(S, nh, hd).astype(np.float64)
+
+
+ATTN = [  # q heads, kv heads, head_dim, prefix, lengths
+    (4, 4, 128, 0, [1]),
+    (32, 8, 128, 0, [17]),
+    (32, 8, 128, 16, [17, 16]),
+    (10, 2, 128, 200, [201, 240, 215]),
+    (3, 1, 64, 33, [33, 34, 49, 65, 33]),
+    (16, 1, 64, 0, [0, 5, 100, 0, 31, 32, 33]),
+    (16, 1, 128, 500, [700, 501, 500, 631]),
+    (8, 8, 128, 130, [300, 131, 20, 0, 129, 130, 131]),          # some shorter than the prefix
+    (7, 7, 64, 1000, [1000, 3, 1000, 999]),
+    (32, 4, 128, 1500, [1500 + 37 * i % 200 for i in range(21)]),  # 168 rows a kv head
+    (16, 8, 64, 777, [778 + 5 * i for i in range(70)]),
+    (14, 2, 128, 0, [4097, 63, 1024]),
+    (12, 4, 128, 2049, [2049 + 1 + i % 3 for i in range(40)]),
+    (8, 1, 128, 640, [640] * 64),                                 # nothing of their own
+    (2, 2, 128, 9000, [9001, 9100]),
+    (48, 4, 128, 300, [301 + i for i in range(90)]),              # 1080 rows a kv head
+]
+
+
+@pytest.mark.parametrize("t", [0, 1], ids=["f32", "f16"])
+@pytest.mark.parametrize("case", ATTN, ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}-{c[3]}-{len(c[4])}x{max(c[4])}")
+def test_attention(zh, ctx, case, t):
+    nh, nkv, hd, P, lens = case
+    rng = np.random.default_rng(nh * 100 + P)
+    kc, vc, tables, _, M = make(rng, len(lens), nkv, hd, P, lens)
+    q = (rng.standard_normal((len(lens), nh, hd)) * 1.5).astype(NP_TYPE[t])
+    got = run_attention(zh, ctx, q, kc, vc, tables, lens, P, M, t, gap=8 * (P % 2))
+    want, tol = attend64(q, kc, vc, tables, lens, hd ** -0.5, t, P)
+    close(got, want, tol)
+
+
+@pytest.mark.parametrize("t", [0, 1], ids=["f32", "f16"])
+def test_attention_in_place_other_scale_and_room_behind(zh, ctx, t):
+    rng = np.random.default_rng(4)
+    lens = [90, 61, 77]
+    kc, vc, tables, _, M = make(rng, 3, 2, 64, 48, lens)
+    q = rng.standard_normal((3, 6, 64)).astype(NP_TYPE[t])
+    wide = np.full((3, 40), 0xFFFFFFFF, dtype=np.uint32)  # a table and a max_len with room for more tokens
+    wide[:, :tables.shape[1]] = tables
+    for in_place in (False, True):
+        got = run_attention(zh, ctx, q, kc, vc, wide, lens, 48, 640, t, scale=0.31, gap=16, in_place=in_place)
+        want, tol = attend64(q, kc, vc, tables, lens, 0.31, t)
+        close(got, want, tol)
+
+
+@pytest.mark.parametrize("size", [1e-30, 3e-6, 1.0, 4e5, 1e30])
+def test_attention_of_f32_queries_of_any_size(zh, ctx, size):
+    """q far outside fp16's range (the scale takes it back)."""
+    rng = np.random.default_rng(6)
+    lens = [140, 139]
+    kc, vc, tables, _, M = make(rng, 2, 1, 128, 100, lens)
+    q = (rng.standard_normal((2, 4, 128)) * size).astype(np.float32)
+    scale = float(np.float32(0.09 / size))
+    got = run_attention(zh, ctx, q, kc, vc, tables, lens, 100, M, 0, scale=scale)
+    want, tol = attend64(q, kc, vc, tables, lens, scale, 0)
+    close(got, want, tol)
+
+
+def test_attention_peaked_weights_and_flat_ones(zh, ctx):
+    """One token takes everything / every token alike, over parts and steps."""
+    rng = np.random.default_rng(7)
+    P, lens = 1000, [1300, 1001, 1200]
+    kc, vc, tables, _, M = make(rng, 3, 1, 128, P, lens)
+    q = rng.standard_normal((3, 2, 128)).astype(np.float32)
+    for where in (3, 999, 1000):
+        k2 = kc.copy()
+        slot = int(tables[0, where // 16]) * 16 + where % 16
+        k2[0, slot] = (q[0, 0] * 3).astype(np.float16)
+        got = run_attention(zh, ctx, q, k2, vc, tables, lens, P, M, 0)
+        want, tol = attend64(q, k2, vc, tables, lens, 128 ** -0.5, 0, P)
+        close(got, want, tol)
+    q[:] = 0
+    got = run_attention(zh, ctx, q, kc, vc, tables, lens, P, M, 0)
+    want, tol = attend64(q, kc, vc, tables, lens, 128 ** -0.5, 0, P)
+    close(got, want, tol)
+
+
+def test_attention_nan_and_inf_stay_in_their_rows(zh, ctx):
+    """A NaN of one sequence's own token, or of one query, is no other row's."""
+    rng = np.random.default_rng(8)
+    P, lens = 96, [130, 97, 160, 40]
+    kc, vc, tables, _, M = make(rng, 4, 2, 128, P, lens)
+    q = rng.standard_normal((4, 8, 128)).astype(np.float32)
+    vc[1, int(tables[2, 150 // 16]) * 16 + 150 % 16, 5] = np.inf  # sequence 2, kv head 1, dim 5
+    q[0, 3, 7] = np.nan
+    got = run_attention(zh, ctx, q, kc, vc, tables, lens, P, M, 0)
+    ok = np.ones(got.shape, bool)
+    ok[2, 4:, 5] = False
+    ok[0, 3] = False
+    assert np.isnan(got[0, 3]).all() and not np.isfinite(got[2, 4:, 5]).any()
+    qq = q.copy()
+    qq[0, 3, 7] = 0
+    vc = np.where(np.isinf(vc), np.float16(0), vc)
+    want, tol = attend64(qq, kc, vc, tables, lens, 128 ** -0.5, 0)
+    close(got, want, tol, ok)
+
+
+def test_attention_cuts_lengths_and_reads_outside_pages_as_page_0(zh, ctx):
+    rng = np.random.default_rng(10)
+    lens = [64, 50]
+    kc, vc, tables, _, M = make(rng, 2, 1, 64, 0, lens, poison=False)
+    q = rng.standard_normal((2, 2, 64)).astype(np.float32)
+    got = run_attention(zh, ctx, q, kc, vc, tables, [64, 5000], 0, 50, 0, expect_error=True)
+    want, tol = attend64(q, kc, vc, tables, [50, 50], 0.125, 0)
+    close(got, want, tol)
+    for entry in (kc.shape[1] // 16, 0x10000000, 0xFFFFFFFF):
+        bad = tables.copy()
+        bad[1, 2] = entry
+        got = run_attention(zh, ctx, q, kc, vc, bad, lens, 0, M, 0, expect_error=True)
+        bad[1, 2] = 0
+        want, tol = attend64(q, kc, vc, bad, lens, 0.125, 0)
+        close(got, want, tol)
+
+
+def test_attention_like_one_sequence_at_a_time(zh, ctx):
+    """zh_flash_decode of each sequence: the same softmax within both bounds."""
+    rng = np.random.default_rng(11)
+    P, lens = 512, [700, 513, 612]
+    kc, vc, tables, tokens, M = make(rng, 3, 8, 128, P, lens, poison=False)
+    tables[tables == 0xFFFFFFF0] = 0
+    q = rng.standard_normal((3, 32, 128)).astype(np.float32)
+    got = run_attention(zh, ctx, q, kc, vc, tables, lens, P, M, 0)
+    _, tol = attend64(q, kc, vc, tables, lens, 128 ** -0.5, 0)
+    u = ctx.upload
+    K, V, out = u(kc), u(vc), ctx.alloc(4 * 32 * 128)
+    for s, n in enumerate(lens):
+        ctx.flash_decode(u(q[s]), K, V, u(tables[s]), tables.shape[1], tokens, out, 32, 8, 128, n)
+        one = out.download(np.float32, 32 * 128).reshape(32, 128)
+        assert (np.abs(got[s] - one) <= 2 * tol[s]).all()
+
+
+# ---------------------------------------------------------------------------
+# together: a pool, a prompt, forks, copies and decode steps
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("t", [0, 1], ids=["f32", "f16"])
+def test_fork_and_decode_together(zh, ctx, t):
+    """A prompt written in one call, forked five ways (copy on write of the page
+    it ends in), decoded some steps, one branch dropped, the pool compacted, and
+    decoded on: every step's attention against the formula over the K and V rows
+    of each branch, kept in 64 bits on the host."""
+    rng = np.random.default_rng(12)
+    nh, nkv, hd, pool_pages, P = 8, 2, 128, 64, 75
+    G = nh // nkv
+    pool = zh.KvPagePool(pool_pages)
+    tokens = pool_pages * 16
+    u = ctx.upload
+    kcb, vcb = (u(np.full((nkv, tokens, hd), np.nan, np.float16)) for _ in range(2))
+    caches = zh.KvCaches([kcb, vcb], tokens, nkv, hd)
+    freq = (1e4 ** (-np.arange(0, hd, 2) / hd)).astype(np.float32)
+    qw, kw = ((1 + 0.1 * rng.standard_normal(hd)).astype(np.float32) for _ in range(2))
+    F, QW, KW = u(freq), u(qw), u(kw)
+    stride = 12
+    history = {}  # request -> (K rows 64 bit, K tolerance, V rows)
+
+    def step(requests, positions, n_per):
+        """Writes n_per rows of each request at its next positions; returns q."""
+        T = len(requests) * n_per
+        x = rng.standard_normal((T, nh + 2 * nkv, hd)).astype(np.float32)
+        pos = np.concatenate([p + np.arange(n_per) for p in positions])
+        tables = np.zeros((len(requests), stride), np.uint32)
+        for i, r in enumerate(requests):
+            pg = pool.pages(r)
+            tables[i, :pg.size] = pg
+        X, out = u(x), ctx.alloc(T * nh * hd * (4 if t == 0 else 2))
+        TB = u(tables)
+        kv = zh.KvBatch(kcb, vcb, TB, len(requests), stride, tokens, nkv, hd)
+        w = (nh + 2 * nkv) * hd
+        ctx.qk_norm_rope_kv_write_batched(kv, zh.QkvRows(
+            q=X, k=X, v=X, k_off=4 * nh * hd, v_off=4 * (nh + nkv) * hd, q_stride=w, k_stride=w, v_stride=w, q_out=out,
+            q_out_type=t, pos=u(pos.astype(np.uint32)), seq=u(np.repeat(np.arange(len(requests)), n_per).astype(np.uint32)),
+            n_rows=T, n_q_heads=nh, rope_dim=hd, inv_freq=F, q_norm_w=QW, k_norm_w=KW))
+        k64, mag = rope64(x[:, nh:nh + nkv], kw, freq, pos, 1e-6, hd)
+        for i, r in enumerate(requests):
+            k, kt, v = history.setdefault(r, ([], [], []))
+            for j in range(n_per):
+                k.append(k64[i * n_per + j])
+                kt.append(mag[i * n_per + j] * 2.0 ** -19 + store_error(1, k64[i * n_per + j]))
+                v.append(x[i * n_per + j, nh + nkv:].astype(np.float16).astype(np.float64))
+        return kv, out, tables
+
+    def attention(requests, kv, q, prefix):
+        lens = [len(history[r][0]) for r in requests]
+        n = ctx.flash_decode_shared_ws(kv, nh, prefix, stride * 16)
+        out = ctx.alloc(len(requests) * nh * hd * 4)
+        ctx.flash_decode_shared(kv, zh.DecodeRows(q=q, out=out, seq_lens=u(np.array(lens, np.uint32)), ws=ctx.alloc(n),
+                                                  n_heads=nh, prefix_len=prefix, max_len=stride * 16, type=t))
+        ctx.sync()
+        got = out.download(NP_TYPE[t], len(requests) * nh * hd).reshape(-1, nh, hd).astype(np.float64)
+        qs = q.download(NP_TYPE[t], len(requests) * nh * hd).reshape(-1, nh, hd).astype(np.float64)
+        for i, r in enumerate(requests):
+            K, KT, V = (np.array(a) for a in history[r])
+            for h in range(nh):
+                sc = K[:, h // G] @ qs[i, h] * hd ** -0.5
+                # the cache holds K rounded: a score moves by at most d
+                d = (KT[:, h // G] @ np.abs(qs[i, h])).max() * hd ** -0.5
+                A = 1.45 * hd ** -0.5 * (np.abs(K[:, h // G]) @ np.abs(qs[i, h])).max()
+                w = np.exp(sc - sc.max())
+                w /= w.sum()
+                W = w @ np.abs(V[:, h // G])
+                want = w @ V[:, h // G]
+                tol = W * (2 * np.expm1(2 * d) + 2.0 ** -17 * A + (len(sc) / 32 + 80) * 2.0 ** -23 +
+                           (2.0 ** -11 if t else 0)) + store_error(t, want)
+                assert (np.abs(got[i, h] - want) <= tol).all(), (r, h)
+
+    pool.alloc_pages(0, -(-P // 16))
+    step([0], [0], P)
+    requests = [0, 1, 2, 3, 4, 5]
+    for c in requests[1:]:
+        pool.fork(0, c, -(-P // 16))
+        history[c] = tuple(list(a) for a in history[0])
+    for it in range(25):
+        if it == 12:  # a branch ends, the pool is compacted
+            pool.free_pages(3)
+            requests.remove(3)
+            src, dst = pool.compact()
+            ctx.kv_copy_pages(caches, caches, dst, src)
+            assert len(src)
+        moves = []
+        for r in requests:
+            n = len(history[r][0])
+            if n % 16 == 0:
+                pool.alloc_pages(r, 1)
+            else:
+                s, d = pool.unshare(r, n // 16)
+                if s != d:
+                    moves.append((d, s))
+        if moves:
+            ctx.kv_copy_pages(caches, caches, [m[0] for m in moves], [m[1] for m in moves])
+            assert it == 0
+        kv, q, _ = step(requests, [len(history[r][0]) for r in requests], 1)
+        attention(requests, kv, q, P if it % 2 else P // 16 * 16)
+
+
+def test_engine_fork_kv(zh, ctx):
+    """A prompt prefilled by one engine and forked into two of its context and
+    one of another context decodes like engines that prefilled it themselves."""
+    cfg = dict(n_layers=2, hidden=512, n_heads=4, n_kv_heads=2, head_dim=128, ffn=1024, vocab=1000, n_experts=0,
+               n_experts_used=0, expert_ffn=0, max_ctx=128, type_attn=12, type_ffn_gate_up=12, type_ffn_down=14,
+               type_lm_head=14, type_embd=12, type_router=8, rope_base=1e6, eps=1e-6, seed=5)
+    prompt = np.random.default_rng(3).integers(0, 1000, 37)
+    base = zh.InferenceEngine(ctx, cfg)
+    ctx2 = zh.Context(0)
+    engines = [base, base.share(ctx), base.share(ctx), base.share(ctx2, 64)]
+    order = np.random.default_rng(1).permutation(8).astype(np.uint32)
+    engines[2].set_pages(order)
+    base.prefill(prompt)
+    for e in engines[1:]:
+        e.fork_kv(base, 37)
+    want = [base.read_kv(l, w, 0, 37) for l in range(2) for w in range(2)]
+    for e in engines[1:]:
+        for i, x in enumerate(want):
+            assert np.array_equal(e.read_kv(i // 2, i % 2, 0, 37), x)
+    toks = [e.generate([7], 6, start_pos=37) for e in engines]
+    assert toks[1] == toks[0] and toks[2] == toks[0] and toks[3] == toks[0]
+    for e, n, name in ((base, 5, "InvalidArgument"), (engines[3], 65, "ContextLengthExceeded")):
+        with pytest.raises(zh.ZincError) as err:
+            e.fork_kv(base, n)
+        assert err.value.name == name
+    engines[1].fork_kv(base, 0)
+    for e in reversed(engines):
+        e.deinit()
+    ctx2.close()

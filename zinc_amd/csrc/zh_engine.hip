@@ -13,8 +13,10 @@
 
 #include <stdlib.h>
 
+#include <algorithm>
 #include <functional>
 #include <map>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -771,16 +773,25 @@ extern "C" int zh_engine_set_persistent(zh_engine *e, int on) {
 // pages in descending order), an owner per page, KvCacheExhausted when too
 // few pages are free.
 // ---------------------------------------------------------------------------
+// Pages may be shared (zh_kv_pool_fork): each request lists its pages in the
+// order it got them, a page counts its holders and is free at zero.
 struct zh_kv_pool {
-    std::vector<uint64_t> owner;  // request id + 1 (0: free)
+    std::vector<uint32_t> refs;  // holders per page (0: free)
     std::vector<uint32_t> free_list;
+    std::map<uint64_t, std::vector<uint32_t>> pages;  // by request id
     uint32_t page_size = 16;
 };
 extern "C" int zh_kv_pool_create(uint32_t total_pages, uint32_t page_size, zh_kv_pool **out) {
     if (!out || total_pages == 0 || page_size == 0) return ZH_ERR_INVALID_ARGUMENT;
-    zh_kv_pool *p = new zh_kv_pool;
-    p->owner.assign(total_pages, 0);
-    p->free_list.resize(total_pages);
+    zh_kv_pool *p = nullptr;
+    try {
+        p = new zh_kv_pool;
+        p->refs.assign(total_pages, 0);
+        p->free_list.resize(total_pages);
+    } catch (const std::bad_alloc &) {
+        delete p;
+        return ZH_ERR_OUT_OF_MEMORY;
+    }
     for (uint32_t i = 0; i < total_pages; i++) p->free_list[i] = i;
     p->page_size = page_size;
     *out = p;
@@ -790,21 +801,118 @@ extern "C" void zh_kv_pool_destroy(zh_kv_pool *p) { delete p; }
 extern "C" int zh_kv_pool_alloc(zh_kv_pool *p, uint64_t request_id, uint32_t count, uint32_t *page_ids) {
     if (!p || (count && !page_ids)) return ZH_ERR_INVALID_ARGUMENT;
     if (p->free_list.size() < count) return ZH_ERR_KV_CACHE_EXHAUSTED;
-    for (uint32_t i = 0; i < count; i++) {
-        const uint32_t id = p->free_list.back();
-        p->free_list.pop_back();
-        p->owner[id] = request_id + 1;
-        page_ids[i] = id;
+    if (count == 0) return ZH_OK;
+    try {
+        std::vector<uint32_t> &own = p->pages[request_id];
+        own.reserve(own.size() + count);
+        for (uint32_t i = 0; i < count; i++) {
+            const uint32_t id = p->free_list.back();
+            p->free_list.pop_back();
+            p->refs[id] = 1;
+            own.push_back(id);
+            page_ids[i] = id;
+        }
+    } catch (const std::bad_alloc &) {
+        return ZH_ERR_OUT_OF_MEMORY;
     }
     return ZH_OK;
 }
+// Gives back one hold of each page, the pages that become free in id order
+// (the free list has room for every page: it never grows past total_pages).
+static void pool_release(zh_kv_pool *p, uint32_t *ids, size_t n) {
+    std::sort(ids, ids + n);
+    for (size_t i = 0; i < n; i++)
+        if (--p->refs[ids[i]] == 0) p->free_list.push_back(ids[i]);
+}
 extern "C" void zh_kv_pool_free(zh_kv_pool *p, uint64_t request_id) {
     if (!p) return;
-    for (uint32_t id = 0; id < (uint32_t)p->owner.size(); id++)
-        if (p->owner[id] == request_id + 1) {
-            p->owner[id] = 0;
-            p->free_list.push_back(id);
+    const auto it = p->pages.find(request_id);
+    if (it == p->pages.end()) return;
+    pool_release(p, it->second.data(), it->second.size());
+    p->pages.erase(it);
+}
+extern "C" int zh_kv_pool_fork(zh_kv_pool *p, uint64_t parent, uint64_t child, uint32_t n_pages) {
+    if (!p || zh_kv_pool_pages(p, child, nullptr, 0)) return ZH_ERR_INVALID_ARGUMENT;
+    if (n_pages == 0) return ZH_OK;
+    const auto it = p->pages.find(parent);
+    if (it == p->pages.end() || it->second.size() < n_pages) return ZH_ERR_INVALID_ARGUMENT;
+    try {
+        p->pages[child] = std::vector<uint32_t>(it->second.begin(), it->second.begin() + n_pages);
+    } catch (const std::bad_alloc &) {
+        p->pages.erase(child);
+        return ZH_ERR_OUT_OF_MEMORY;
+    }
+    for (uint32_t i = 0; i < n_pages; i++) p->refs[it->second[i]]++;
+    return ZH_OK;
+}
+extern "C" int zh_kv_pool_unshare(zh_kv_pool *p, uint64_t request_id, uint32_t index, uint32_t *src, uint32_t *dst) {
+    if (!p || !src || !dst) return ZH_ERR_INVALID_ARGUMENT;
+    const auto it = p->pages.find(request_id);
+    if (it == p->pages.end() || index >= it->second.size()) return ZH_ERR_INVALID_ARGUMENT;
+    uint32_t &page = it->second[index];
+    if (p->refs[page] > 1) {
+        if (p->free_list.empty()) return ZH_ERR_KV_CACHE_EXHAUSTED;
+        const uint32_t id = p->free_list.back();
+        p->free_list.pop_back();
+        p->refs[id] = 1;
+        p->refs[page]--;
+        *src = page;
+        *dst = page = id;
+    } else {
+        *src = *dst = page;
+    }
+    return ZH_OK;
+}
+extern "C" int zh_kv_pool_trim(zh_kv_pool *p, uint64_t request_id, uint32_t keep) {
+    if (!p) return ZH_ERR_INVALID_ARGUMENT;
+    const auto it = p->pages.find(request_id);
+    if (it == p->pages.end() || it->second.size() <= keep) return ZH_OK;
+    pool_release(p, it->second.data() + keep, it->second.size() - keep);
+    it->second.resize(keep);
+    if (keep == 0) p->pages.erase(it);
+    return ZH_OK;
+}
+extern "C" uint32_t zh_kv_pool_pages(const zh_kv_pool *p, uint64_t request_id, uint32_t *page_ids, uint32_t cap) {
+    if (!p) return 0u;
+    const auto it = p->pages.find(request_id);
+    if (it == p->pages.end()) return 0u;
+    const uint32_t n = (uint32_t)it->second.size();
+    if (page_ids)
+        for (uint32_t i = 0; i < n && i < cap; i++) page_ids[i] = it->second[i];
+    return n;
+}
+extern "C" uint32_t zh_kv_pool_refs(const zh_kv_pool *p, uint32_t page) {
+    return p && page < p->refs.size() ? p->refs[page] : 0u;
+}
+extern "C" int zh_kv_pool_compact(zh_kv_pool *p, uint32_t *src, uint32_t *dst, uint32_t cap, uint32_t *n_moves) {
+    if (!p || !n_moves || (cap && (!src || !dst))) return ZH_ERR_INVALID_ARGUMENT;
+    const uint32_t total = (uint32_t)p->refs.size(), live = total - (uint32_t)p->free_list.size();
+    uint32_t n = 0;
+    for (uint32_t i = live; i < total; i++) n += p->refs[i] != 0;
+    *n_moves = n;
+    if (n > cap) return ZH_ERR_INVALID_ARGUMENT;
+    if (n) {
+        try {
+            std::vector<uint32_t> to(total);
+            uint32_t k = 0, hole = 0;
+            for (uint32_t i = 0; i < total; i++) to[i] = i;
+            for (uint32_t i = live; i < total; i++) {
+                if (!p->refs[i]) continue;
+                while (p->refs[hole]) hole++;  // (below live: as many holes as pages past it)
+                src[k] = i;
+                dst[k++] = to[i] = hole;
+                p->refs[hole] = p->refs[i];
+                p->refs[i] = 0;
+            }
+            for (auto &r : p->pages)
+                for (uint32_t &id : r.second) id = to[id];
+        } catch (const std::bad_alloc &) {
+            return ZH_ERR_OUT_OF_MEMORY;  // (before anything changed)
         }
+    }
+    // the free pages in id order, so that the next ones handed out are the highest
+    for (uint32_t i = live; i < total; i++) p->free_list[i - live] = i;
+    return ZH_OK;
 }
 extern "C" uint32_t zh_kv_pool_free_count(const zh_kv_pool *p) { return p ? (uint32_t)p->free_list.size() : 0u; }
 extern "C" uint32_t zh_kv_pool_max_context(const zh_kv_pool *p, uint32_t page_count) {
@@ -1712,6 +1820,46 @@ extern "C" int zh_engine_read_kv(zh_engine *e, uint32_t layer, uint32_t which, u
     ZH_LAUNCH_CHECK(e->ctx);
     EHIP(e, hipMemcpyAsync(dst, scr, cnt * 2, hipMemcpyDeviceToHost, e->ctx->stream));
     EHIP(e, hipStreamSynchronize(e->ctx->stream));
+    return ZH_OK;
+}
+
+// The prompt's K and V of one engine into another's cache: page copies of every
+// layer (zhk_kv_copy). Engines of one context are ordered by its stream; of two,
+// the call waits for src's work before it and for the copies after it, so that
+// src may go on at once.
+extern "C" int zh_engine_fork_kv(zh_engine *dst, zh_engine *src, uint32_t n_tokens) {
+    if (!dst || !src) return ZH_ERR_INVALID_ARGUMENT;
+    const zh_model_config &a = dst->c, &b = src->c;
+    if (dst == src || a.n_layers != b.n_layers || a.n_kv_heads != b.n_kv_heads || a.head_dim != b.head_dim ||
+        dst->ctx->device != src->ctx->device)
+        return zh_set_err(dst->ctx, ZH_ERR_INVALID_ARGUMENT, "fork: the engines' caches differ in layers, heads or device");
+    if (n_tokens > a.max_ctx || n_tokens > b.max_ctx)
+        return zh_set_err(dst->ctx, ZH_ERR_CONTEXT_LENGTH_EXCEEDED, "fork of %u tokens", n_tokens);
+    if (n_tokens == 0) return ZH_OK;
+    zh_device_scope dev(dst->ctx);
+    const uint32_t n = (n_tokens + 15) / 16;
+    try {
+        std::vector<uint32_t> dp(n), sp(n), seen(dst->n_pages, 0);
+        EHIP(dst, hipMemcpy(dp.data(), dst->pages, 4ull * n, hipMemcpyDeviceToHost));
+        EHIP(dst, hipMemcpy(sp.data(), src->pages, 4ull * n, hipMemcpyDeviceToHost));
+        for (uint32_t i = 0; i < n; i++)
+            if (seen[dp[i]]++)
+                return zh_set_err(dst->ctx, ZH_ERR_INVALID_ARGUMENT, "fork: page %u twice in the page table", dp[i]);
+        std::vector<void *> d;
+        std::vector<const void *> s;
+        for (uint32_t l = 0; l < a.n_layers; l++) {
+            d.push_back(dst->L[l].kc);
+            d.push_back(dst->L[l].vc);
+            s.push_back(src->L[l].kc);
+            s.push_back(src->L[l].vc);
+        }
+        if (src->ctx != dst->ctx) EHIP(dst, hipStreamSynchronize(src->ctx->stream));
+        ERC(zhk_kv_copy(dst->ctx, (uint32_t)d.size(), d.data(), s.data(), a.max_ctx, b.max_ctx, a.n_kv_heads,
+                        a.head_dim, dp.data(), sp.data(), n));
+        if (src->ctx != dst->ctx) EHIP(dst, hipStreamSynchronize(dst->ctx->stream));
+    } catch (const std::bad_alloc &) {
+        return zh_set_err(dst->ctx, ZH_ERR_OUT_OF_MEMORY, "fork: host memory");
+    }
     return ZH_OK;
 }
 

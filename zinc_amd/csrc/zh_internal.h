@@ -65,8 +65,13 @@ struct zh_ctx {
     // when it reports ZH_ERR_WAIT_TIMEOUT: the next launch starts at epoch 1.
     struct XWords { const void *owner; void *p; uint64_t bytes; };
     std::vector<XWords> xwords;
+    // zh_kv_copy_pages' check of its page numbers: the call that last named a
+    // page as a destination (a counter, so that no call clears the array).
+    std::vector<uint32_t> page_mark;
+    uint32_t page_call = 0;
 };
-enum : uint32_t { ZH_DEVERR_EXPERT_ID = 1u, ZH_DEVERR_ATTN_WAIT = 2u, ZH_DEVERR_STEP_BARRIER = 4u };
+enum : uint32_t { ZH_DEVERR_EXPERT_ID = 1u, ZH_DEVERR_ATTN_WAIT = 2u, ZH_DEVERR_STEP_BARRIER = 4u,
+                ZH_DEVERR_KV_ROW = 8u };
 // default merge wait: 50 ms
 constexpr uint32_t ZH_ATTN_WAIT_TICKS = 5000000u;
 
@@ -78,6 +83,19 @@ int zh_set_err(zh_ctx *ctx, int code, const char *fmt, ...);
             return zh_set_err((ctx), ZH_ERR_HIP, "%s failed: %s", #call, hipGetErrorString(e_)); \
     } while (0)
 #define ZH_LAUNCH_CHECK(ctx) ZH_HIP(ctx, hipGetLastError())
+
+// The context's device is the current one while this lives (entries called
+// from a thread whose current device is another).
+struct zh_device_scope {
+    int prev = -1;
+    explicit zh_device_scope(const zh_ctx *c) {
+        if (hipGetDevice(&prev) != hipSuccess || prev == c->device) prev = -1;
+        else hipSetDevice(c->device);
+    }
+    ~zh_device_scope() {
+        if (prev >= 0) hipSetDevice(prev);
+    }
+};
 
 // Scratch (grows; stream ordered, so reuse across sequential calls is safe).
 int zh_scratch(zh_ctx *ctx, uint64_t bytes, void **out);
@@ -180,6 +198,10 @@ int zhk_attn_decode_fused_z(zh_ctx *ctx, uint32_t n, const float *const *q, cons
                             uint32_t cache_tokens, float *const *out, void *const *xq_out, uint32_t nh, uint32_t nkv,
                             const uint32_t *const *pos_dev, uint32_t max_seq, float scale, float eps,
                             float *const *partials, bool ident_pages);
+// Page copies between raw caches (zh_kv.hip): the page numbers have been checked.
+int zhk_kv_copy(zh_ctx *ctx, uint32_t n_caches, void *const *dst, const void *const *src, uint32_t dst_tokens,
+                uint32_t src_tokens, uint32_t n_kv_heads, uint32_t head_dim, const uint32_t *dst_pages,
+                const uint32_t *src_pages, uint32_t n_pages);
 // Prefill (zh_prefill.hip)
 int zhk_gemm(zh_ctx *ctx, uint32_t qtype, const uint8_t *W, const _Float16 *X, uint32_t ldx, float *Y, uint32_t ldy,
              uint32_t M, uint32_t K, uint32_t N, uint32_t acc, const float *x_unscale = nullptr);

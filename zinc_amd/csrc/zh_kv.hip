@@ -1,0 +1,365 @@
+// zh_kv.hip — operators over a paged KV cache for batches: page copies and
+// the fused q/k RMSNorm + RoPE + KV write of many tokens.
+#include <new>
+
+#include "zh_device.h"
+#include "zh_internal.h"
+#include "zh_kv.h"
+
+// ---------------------------------------------------------------------------
+// Page copies. A page of one cache and head is 16 * head_dim halfs, contiguous
+// (4 KB at head_dim 128): nothing is computed, the copy is bound by HBM (or by
+// its launch for a few pages). The page numbers travel in the kernel arguments,
+// so a call needs no staging memory, is finished with its host arrays when it
+// returns and can be captured.
+// ---------------------------------------------------------------------------
+namespace {
+
+constexpr uint32_t KC_CACHES = 96, KC_PAGES = 256;  // per launch: 4 KB of arguments hold both lists
+struct KvCopyArgs {
+    const uint8_t *src[KC_CACHES];
+    uint8_t *dst[KC_CACHES];
+    uint32_t pages[KC_PAGES][2];  // source, destination
+    uint64_t src_head, dst_head;  // bytes of one head of a cache
+    uint32_t n_caches, n_pages, n_heads, seg;  // seg: bytes of a page of one head
+};
+static_assert(sizeof(KvCopyArgs) <= 4096, "kernel arguments");
+
+// One workgroup per (page, head, cache).
+__global__ __launch_bounds__(256) void k_kv_copy(KvCopyArgs a) {
+    const uint32_t p = blockIdx.x, h = blockIdx.y, c = blockIdx.z;
+    const u32x4 *s = (const u32x4 *)(a.src[c] + h * a.src_head + (uint64_t)a.pages[p][0] * a.seg);
+    u32x4 *d = (u32x4 *)(a.dst[c] + h * a.dst_head + (uint64_t)a.pages[p][1] * a.seg);
+    for (uint32_t i = threadIdx.x; i < a.seg / 16; i += 256) d[i] = s[i];
+}
+
+}  // namespace
+
+int zhk_kv_copy(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *const *src, uint32_t dst_tokens,
+                uint32_t src_tokens, uint32_t n_kv_heads, uint32_t head_dim, const uint32_t *dst_pages,
+                const uint32_t *src_pages, uint32_t n_pages) {
+    KvCopyArgs a;
+    a.seg = 32 * head_dim;
+    a.src_head = 2ull * src_tokens * head_dim;
+    a.dst_head = 2ull * dst_tokens * head_dim;
+    a.n_heads = n_kv_heads;
+    for (uint32_t c0 = 0; c0 < n_caches; c0 += KC_CACHES) {
+        a.n_caches = n_caches - c0 < KC_CACHES ? n_caches - c0 : KC_CACHES;
+        for (uint32_t i = 0; i < a.n_caches; i++) {
+            a.src[i] = (const uint8_t *)src[c0 + i];
+            a.dst[i] = (uint8_t *)dst[c0 + i];
+        }
+        for (uint32_t p0 = 0; p0 < n_pages; p0 += KC_PAGES) {
+            a.n_pages = n_pages - p0 < KC_PAGES ? n_pages - p0 : KC_PAGES;
+            for (uint32_t i = 0; i < a.n_pages; i++) {
+                a.pages[i][0] = src_pages[p0 + i];
+                a.pages[i][1] = dst_pages[p0 + i];
+            }
+            hipLaunchKernelGGL(k_kv_copy, dim3(a.n_pages, a.n_heads, a.n_caches), dim3(256), 0, c->stream, a);
+            ZH_LAUNCH_CHECK(c);
+        }
+    }
+    return ZH_OK;
+}
+
+static bool caches_ok(const zh_kv_caches *s) {
+    if (!s || !s->caches || s->n_caches == 0 || s->n_kv_heads == 0 || s->n_kv_heads > 65535 || s->head_dim == 0 ||
+        s->head_dim > 1024 || s->cache_tokens == 0)
+        return false;
+    for (uint32_t i = 0; i < s->n_caches; i++)
+        if (!kv_in_range(s->caches[i], 0, 2ull * s->n_kv_heads * s->cache_tokens * s->head_dim)) return false;
+    return true;
+}
+
+// The checks of zh_kv_copy_pages, of host data only (c may be null: no
+// message then). `mark` and `call`: see zh_ctx::page_mark.
+extern "C" int zh_check_kv_copy_pages(zh_ctx *c, const zh_kv_caches *dst, const zh_kv_caches *src,
+                                      const uint32_t *dst_pages, const uint32_t *src_pages, uint32_t n_pages) {
+    if (!caches_ok(dst) || !caches_ok(src) || dst->n_caches != src->n_caches || dst->n_kv_heads != src->n_kv_heads ||
+        dst->head_dim != src->head_dim)
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: cache sets");
+    if (n_pages && (!dst_pages || !src_pages))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: no page numbers");
+    bool alias = false;
+    for (uint32_t i = 0; i < dst->n_caches; i++) {
+        if (dst->caches[i]->ptr == src->caches[i]->ptr) alias = true;
+        for (uint32_t j = 0; j < i; j++) {
+            if (dst->caches[i]->ptr == dst->caches[j]->ptr)
+                return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: caches %u and %u of dst are one", j, i);
+            if (dst->caches[i]->ptr == src->caches[j]->ptr || dst->caches[j]->ptr == src->caches[i]->ptr) alias = true;
+        }
+    }
+    if (alias && dst->cache_tokens != src->cache_tokens)
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: one cache in two sizes");
+    const uint32_t np = dst->cache_tokens / 16;
+    for (uint32_t i = 0; i < n_pages; i++)
+        if (dst_pages[i] >= np || src_pages[i] >= src->cache_tokens / 16)
+            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: copy %u, page %u to %u, outside the cache", i,
+                              src_pages[i], dst_pages[i]);
+    try {
+        std::vector<uint32_t> own;
+        std::vector<uint32_t> &mark = c ? c->page_mark : own;
+        if (mark.size() < np) mark.resize(np, 0);
+        uint32_t one = 0, &call = c ? c->page_call : one;
+        if (++call == 0) {  // (wrapped: the old marks go)
+            std::fill(mark.begin(), mark.end(), 0u);
+            call = 1;
+        }
+        for (uint32_t i = 0; i < n_pages; i++) {
+            if (mark[dst_pages[i]] == call)
+                return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: two copies to page %u", dst_pages[i]);
+            mark[dst_pages[i]] = call;
+        }
+        if (alias)
+            for (uint32_t i = 0; i < n_pages; i++)
+                if (mark[src_pages[i]] == call)
+                    return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: page %u is read and written",
+                                      src_pages[i]);
+    } catch (const std::bad_alloc &) {
+        return zh_set_err(c, ZH_ERR_OUT_OF_MEMORY, "kv_copy_pages: host memory");
+    }
+    return ZH_OK;
+}
+
+extern "C" int zh_kv_copy_pages(zh_ctx *c, const zh_kv_caches *dst, const zh_kv_caches *src, const uint32_t *dst_pages,
+                                const uint32_t *src_pages, uint32_t n_pages) {
+    if (!c) return ZH_ERR_INVALID_ARGUMENT;
+    int rc = zh_check_kv_copy_pages(c, dst, src, dst_pages, src_pages, n_pages);
+    if (rc) return rc;
+    zh_device_scope dev(c);
+    // the buffers' addresses, KC_CACHES at a time
+    for (uint32_t c0 = 0; c0 < dst->n_caches; c0 += KC_CACHES) {
+        void *d[KC_CACHES];
+        const void *s[KC_CACHES];
+        const uint32_t n = dst->n_caches - c0 < KC_CACHES ? dst->n_caches - c0 : KC_CACHES;
+        for (uint32_t i = 0; i < n; i++) {
+            d[i] = dst->caches[c0 + i]->ptr;
+            s[i] = src->caches[c0 + i]->ptr;
+        }
+        rc = zhk_kv_copy(c, n, d, s, dst->cache_tokens, src->cache_tokens, dst->n_kv_heads, dst->head_dim, dst_pages,
+                         src_pages, n_pages);
+        if (rc) return rc;
+    }
+    return ZH_OK;
+}
+
+// ---------------------------------------------------------------------------
+// q/k RMSNorm + RoPE + KV write of a batch of rows:
+//   h = w (x / sqrt(mean x^2 + eps)) over a head (or x), then dims i and
+//   i + r/2 (i < r/2, r = rope_dim): (a cos - b sin, a sin + b cos) with the
+//   angle pos * inv_freq[i].
+// The angle is a 64-bit product (exact: 32 + 24 bits), reduced in 64 bits to a
+// fraction of a turn: in 32 bits a position of 2^17 alone would leave an error
+// of 2^-8 radians. Everything else is 32-bit and rounded once, at the store.
+// ---------------------------------------------------------------------------
+namespace {
+
+struct QkvArgs {
+    const uint8_t *q, *k, *v;
+    uint8_t *q_out;
+    uint64_t q_row, k_row, v_row, out_row;  // bytes between rows
+    const float *qw, *kw, *inv_freq;
+    uint16_t *kc, *vc;
+    const uint32_t *tables, *seq, *pos;
+    uint32_t *err;
+    uint32_t n_seq, stride, cache_tokens, nq, nkv, hd, rd;
+    float eps;
+};
+
+template <typename T>
+ZH_DEV void st1(uint8_t *p, uint32_t i, float v) {
+    if (sizeof(T) == 4) ((float *)p)[i] = v;
+    else ((uint16_t *)p)[i] = f2h_rn(v);
+}
+template <typename T>
+ZH_DEV float ld1(const uint8_t *p, uint32_t i) {
+    return sizeof(T) == 4 ? ((const float *)p)[i] : h2f(((const uint16_t *)p)[i]);
+}
+
+// cos and sin of pos * f.
+ZH_DEV void turn(uint32_t pos, float f, float &co, float &sn) {
+    double a = ((double)pos * (double)f) * 0.15915494309189533576888;  // turns
+    a -= __builtin_rint(a);
+    sincospif(2.0f * (float)a, &sn, &co);
+}
+
+// Any shape and alignment: one wave per head vector, workgroup = (head, row);
+// heads [0, nq) are q, then k, then v.
+template <typename TI, typename TQ>
+__global__ __launch_bounds__(64) void k_qkv_rows(QkvArgs a) {
+    const uint32_t t = blockIdx.y, lane = threadIdx.x, head = blockIdx.x;
+    const uint32_t pos = a.pos[t];
+    if (pos == ZH_POS_NONE) return;
+    const bool is_q = head < a.nq, is_v = head >= a.nq + a.nkv;
+    const uint32_t h = is_q ? head : (head - a.nq) % a.nkv;
+    uint32_t slot = 0;
+    if (!is_q) {
+        const uint32_t s = a.seq ? a.seq[t] : t;
+        if (!kv_slot(a.tables, a.n_seq, a.stride, a.cache_tokens, s, pos, slot)) {
+            if (lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+            return;
+        }
+    }
+    const uint8_t *x = is_q ? a.q + t * a.q_row : is_v ? a.v + t * a.v_row : a.k + t * a.k_row;
+    x += (size_t)h * a.hd * sizeof(TI);
+    uint16_t *cache = (is_v ? a.vc : a.kc) + ((size_t)h * a.cache_tokens + slot) * a.hd;
+    uint8_t *out = is_q ? a.q_out + t * a.out_row + (size_t)h * a.hd * sizeof(TQ) : (uint8_t *)cache;
+    auto put = [&](uint32_t i, float v) __attribute__((always_inline)) {
+        if (is_q) st1<TQ>(out, i, v);
+        else st1<uint16_t>(out, i, v);
+    };
+    if (is_v) {
+        for (uint32_t i = lane; i < a.hd; i += 64) put(i, ld1<TI>(x, i));
+        return;
+    }
+    const float *w = is_q ? a.qw : a.kw;
+    float ri = 1.f;
+    if (w) {
+        float sq = 0.f;
+        for (uint32_t i = lane; i < a.hd; i += 64) {
+            const float e = ld1<TI>(x, i);
+            sq = fmaf(e, e, sq);
+        }
+        ri = 1.0f / sqrtf(wave_sum(sq) / (float)a.hd + a.eps);
+    }
+    auto val = [&](uint32_t i) __attribute__((always_inline)) {
+        const float e = ld1<TI>(x, i);
+        return w ? w[i] * (e * ri) : e;
+    };
+    // (a lane reads and writes its own dims only: q_out may be q)
+    for (uint32_t i = lane; i < a.rd / 2; i += 64) {
+        float co, sn;
+        turn(pos, a.inv_freq[i], co, sn);
+        const float lo = val(i), hi = val(i + a.rd / 2);
+        put(i, lo * co - hi * sn);
+        put(i + a.rd / 2, lo * sn + hi * co);
+    }
+    for (uint32_t i = a.rd + lane; i < a.hd; i += 64) put(i, val(i));
+}
+
+}  // namespace
+
+// Bytes from the first to past the last element of `rows` rows of `width`.
+static uint64_t rows_bytes(uint32_t rows, uint32_t stride, uint64_t width, uint32_t size) {
+    return ((uint64_t)(rows - 1) * stride + width) * size;
+}
+
+bool kv_batch_ok(const zh_kv_batch *kv) {
+    return kv && kv->n_seq && kv->table_stride && kv->cache_tokens && kv->cache_tokens % 16 == 0 && kv->n_kv_heads &&
+           kv->n_kv_heads <= 65535 && kv->head_dim && kv->head_dim <= 512 &&
+           kv_in_range(kv->k_cache, 0, 2ull * kv->n_kv_heads * kv->cache_tokens * kv->head_dim) &&
+           kv_in_range(kv->v_cache, 0, 2ull * kv->n_kv_heads * kv->cache_tokens * kv->head_dim) &&
+           kv_in_range(kv->tables, 0, 4ull * kv->n_seq * kv->table_stride);
+}
+
+bool kv_rows_overlap(const zh_buf *a, uint64_t a0, uint64_t an, const zh_buf *b, uint64_t b0, uint64_t bn) {
+    const uint64_t pa = (uint64_t)(uintptr_t)a->ptr + a0, pb = (uint64_t)(uintptr_t)b->ptr + b0;
+    return pa < pb + bn && pb < pa + an;
+}
+
+// The rows with their strides (0: rows without gaps).
+static zh_qkv_rows with_strides(const zh_kv_batch *kv, const zh_qkv_rows *r) {
+    zh_qkv_rows x = *r;
+    if (!x.q_stride) x.q_stride = x.n_q_heads * kv->head_dim;
+    if (!x.q_out_stride) x.q_out_stride = x.n_q_heads * kv->head_dim;
+    if (!x.k_stride) x.k_stride = kv->n_kv_heads * kv->head_dim;
+    if (!x.v_stride) x.v_stride = kv->n_kv_heads * kv->head_dim;
+    return x;
+}
+
+// The checks of zh_qk_norm_rope_kv_write_batched, of host data only.
+extern "C" int zh_check_qkv_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_qkv_rows *rows) {
+    if (!kv_batch_ok(kv) || !rows) return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: cache or tables");
+    const zh_qkv_rows x = with_strides(kv, rows), *r = &x;
+    const uint32_t nkv = kv->n_kv_heads, hd = kv->head_dim, nq = r->n_q_heads, n = r->n_rows;
+    if (hd % 2 || nq == 0 || nq > 65535 || nq % nkv || (uint64_t)nq + 2ull * nkv > 65535)
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: heads %u / %u of %u", nq, nkv, hd);
+    if (r->rope_dim % 2 || r->rope_dim > hd)
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: rope_dim %u of %u", r->rope_dim, hd);
+    if ((r->type != ZH_F32 && r->type != ZH_F16) || (r->q_out_type != ZH_F32 && r->q_out_type != ZH_F16))
+        return zh_set_err(c, ZH_ERR_UNSUPPORTED_QUANT_TYPE, "qk_norm_rope_kv batch: types %u, %u", r->type, r->q_out_type);
+    if (n == 0) return ZH_OK;
+    const uint32_t si = r->type == ZH_F32 ? 4 : 2, so = r->q_out_type == ZH_F32 ? 4 : 2;
+    const uint64_t qw = (uint64_t)nq * hd, kw = (uint64_t)nkv * hd;
+    if (n > 1 && (r->q_stride < qw || r->k_stride < kw || r->v_stride < kw || r->q_out_stride < qw))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: rows overlap");
+    const uint64_t qb = rows_bytes(n, r->q_stride, qw, si), ob = rows_bytes(n, r->q_out_stride, qw, so);
+    if (!kv_in_range(r->q, r->q_off, qb) || !kv_in_range(r->k, r->k_off, rows_bytes(n, r->k_stride, kw, si)) ||
+        !kv_in_range(r->v, r->v_off, rows_bytes(n, r->v_stride, kw, si)) || !kv_in_range(r->q_out, r->q_out_off, ob) ||
+        !kv_in_range(r->pos, 0, 4ull * n) || (r->seq && !kv_in_range(r->seq, 0, 4ull * n)) ||
+        (!r->seq && n > kv->n_seq) || (r->q_norm_w && !kv_in_range(r->q_norm_w, 0, 4ull * hd)) ||
+        (r->k_norm_w && !kv_in_range(r->k_norm_w, 0, 4ull * hd)) ||
+        (r->rope_dim && !kv_in_range(r->inv_freq, 0, 2ull * r->rope_dim)))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: range");
+    if (r->q_off % si || r->k_off % si || r->v_off % si || r->q_out_off % so)
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: offset alignment");
+    // q_out: q's own rows, or apart from everything that is read
+    const bool same = r->q_out->ptr == r->q->ptr && r->q_out_off == r->q_off && r->q_out_type == r->type &&
+                      (r->q_out_stride == r->q_stride || n == 1);
+    if ((!same && kv_rows_overlap(r->q_out, r->q_out_off, ob, r->q, r->q_off, qb) &&
+         !(r->q_out_type == r->type && r->q_out_stride == r->q_stride && n > 1 &&
+           kv_columns_apart(r->q_out, r->q_out_off, r->q, r->q_off, r->q_stride, qw, qw, si))) ||
+        (kv_rows_overlap(r->q_out, r->q_out_off, ob, r->k, r->k_off, rows_bytes(n, r->k_stride, kw, si)) &&
+         !(r->q_out_type == r->type && r->q_out_stride == r->k_stride &&
+           kv_columns_apart(r->q_out, r->q_out_off, r->k, r->k_off, r->k_stride, qw, kw, si))) ||
+        (kv_rows_overlap(r->q_out, r->q_out_off, ob, r->v, r->v_off, rows_bytes(n, r->v_stride, kw, si)) &&
+         !(r->q_out_type == r->type && r->q_out_stride == r->v_stride &&
+           kv_columns_apart(r->q_out, r->q_out_off, r->v, r->v_off, r->v_stride, qw, kw, si))))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: q_out overlaps rows that are read");
+    return ZH_OK;
+}
+
+template <typename TI, typename TQ>
+static int qkv_launch(zh_ctx *c, const QkvArgs &a, uint32_t n) {
+    // (at most 65535 rows a launch: the grid's y)
+    for (uint32_t t0 = 0; t0 < n; t0 += 65535) {
+        QkvArgs b = a;
+        b.q += t0 * a.q_row;
+        b.k += t0 * a.k_row;
+        b.v += t0 * a.v_row;
+        b.q_out += t0 * a.out_row;
+        b.pos += t0;
+        if (b.seq) b.seq += t0;
+        hipLaunchKernelGGL((k_qkv_rows<TI, TQ>), dim3(a.nq + 2 * a.nkv, n - t0 < 65535 ? n - t0 : 65535), dim3(64), 0,
+                           c->stream, b);
+        ZH_LAUNCH_CHECK(c);
+    }
+    return ZH_OK;
+}
+
+extern "C" int zh_qk_norm_rope_kv_write_batched(zh_ctx *c, const zh_kv_batch *kv, const zh_qkv_rows *rows) {
+    if (!c) return ZH_ERR_INVALID_ARGUMENT;
+    const int rc = zh_check_qkv_rows(c, kv, rows);
+    if (rc || rows->n_rows == 0) return rc;
+    const zh_qkv_rows x = with_strides(kv, rows), *r = &x;
+    zh_device_scope dev(c);
+    const uint32_t si = r->type == ZH_F32 ? 4 : 2, so = r->q_out_type == ZH_F32 ? 4 : 2;
+    QkvArgs a = {};
+    a.q = (const uint8_t *)r->q->ptr + r->q_off;
+    a.k = (const uint8_t *)r->k->ptr + r->k_off;
+    a.v = (const uint8_t *)r->v->ptr + r->v_off;
+    a.q_out = (uint8_t *)r->q_out->ptr + r->q_out_off;
+    a.q_row = (uint64_t)r->q_stride * si;
+    a.k_row = (uint64_t)r->k_stride * si;
+    a.v_row = (uint64_t)r->v_stride * si;
+    a.out_row = (uint64_t)r->q_out_stride * so;
+    a.qw = r->q_norm_w ? (const float *)r->q_norm_w->ptr : nullptr;
+    a.kw = r->k_norm_w ? (const float *)r->k_norm_w->ptr : nullptr;
+    a.inv_freq = r->rope_dim ? (const float *)r->inv_freq->ptr : nullptr;
+    a.kc = (uint16_t *)kv->k_cache->ptr;
+    a.vc = (uint16_t *)kv->v_cache->ptr;
+    a.tables = (const uint32_t *)kv->tables->ptr;
+    a.seq = r->seq ? (const uint32_t *)r->seq->ptr : nullptr;
+    a.pos = (const uint32_t *)r->pos->ptr;
+    a.err = c->err_dev;
+    a.n_seq = kv->n_seq;
+    a.stride = kv->table_stride;
+    a.cache_tokens = kv->cache_tokens;
+    a.nq = r->n_q_heads;
+    a.nkv = kv->n_kv_heads;
+    a.hd = kv->head_dim;
+    a.rd = r->rope_dim;
+    a.eps = r->eps;
+    if (si == 4) return so == 4 ? qkv_launch<float, float>(c, a, r->n_rows) : qkv_launch<float, uint16_t>(c, a, r->n_rows);
+    return so == 4 ? qkv_launch<uint16_t, float>(c, a, r->n_rows) : qkv_launch<uint16_t, uint16_t>(c, a, r->n_rows);
+}

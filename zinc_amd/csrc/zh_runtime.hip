@@ -118,6 +118,9 @@ extern "C" int zh_sync(zh_ctx *c) {
         if (e & ZH_DEVERR_EXPERT_ID)
             return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "an expert id at or past the weights' expert count "
                                                           "(zh_dmmv_moe clamped it to the last expert)");
+        if (e & ZH_DEVERR_KV_ROW)
+            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "a batch named a sequence, position, length or page outside "
+                                                          "its tables or cache (the row was left out or cut)");
     }
     return ZH_OK;
 }

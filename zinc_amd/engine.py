@@ -190,6 +190,11 @@ class InferenceEngine:
         a = np.ascontiguousarray(pages, dtype=np.uint32)
         self.ctx.check(lib().zh_engine_set_pages(self.h, C.c_void_p(a.ctypes.data), len(a)))
 
+    def fork_kv(self, src, n_tokens):
+        """Copies the K and V of src's first n_tokens positions here (a prompt
+        prefilled once, continued by several engines)."""
+        self.ctx.check(lib().zh_engine_fork_kv(self.h, src.h, n_tokens))
+
     def set_persistent(self, on=True):
         """Run the step's layers as one persistent launch where the model takes it."""
         self.ctx.check(lib().zh_engine_set_persistent(self.h, int(bool(on))))
@@ -243,6 +248,7 @@ class KvPagePool:
             raise hip.ZincError(rc, "zh_kv_pool_create")
         self.h = h
         self.page_size = page_size
+        self.total_pages = total_pages
 
     def alloc_pages(self, request_id, count):
         out = np.empty(count, dtype=np.uint32)
@@ -253,6 +259,47 @@ class KvPagePool:
 
     def free_pages(self, request_id):
         lib().zh_kv_pool_free(self.h, request_id)
+
+    def fork(self, parent, child, n_pages):
+        """child (without pages so far) shares the first n_pages pages of parent."""
+        rc = lib().zh_kv_pool_fork(self.h, parent, child, n_pages)
+        if rc != hip.OK:
+            raise hip.ZincError(rc, f"fork {n_pages} pages of {parent} to {child}")
+
+    def unshare(self, request_id, index):
+        """(src, dst) page of the request's logical page `index` before it is
+        written: different ones where it was shared, its content then to be
+        copied (Context.kv_copy_pages)."""
+        src, dst = C.c_uint32(), C.c_uint32()
+        rc = lib().zh_kv_pool_unshare(self.h, request_id, index, C.byref(src), C.byref(dst))
+        if rc != hip.OK:
+            raise hip.ZincError(rc, f"unshare page {index} of {request_id}")
+        return src.value, dst.value
+
+    def trim(self, request_id, keep):
+        """Gives back the request's pages past the first `keep`."""
+        lib().zh_kv_pool_trim(self.h, request_id, keep)
+
+    def pages(self, request_id):
+        """The request's pages in logical order."""
+        out = np.empty(lib().zh_kv_pool_pages(self.h, request_id, None, 0), dtype=np.uint32)
+        lib().zh_kv_pool_pages(self.h, request_id, C.c_void_p(out.ctypes.data), out.size)
+        return out
+
+    def refs(self, page):
+        """Holders of a page (0: free)."""
+        return lib().zh_kv_pool_refs(self.h, page)
+
+    def compact(self):
+        """Renumbers the pages in use to the lowest ids; returns (src, dst) of
+        the copies to make (Context.kv_copy_pages)."""
+        n = C.c_uint32()
+        src, dst = (np.empty(self.total_pages // 2 + 1, dtype=np.uint32) for _ in range(2))
+        rc = lib().zh_kv_pool_compact(self.h, C.c_void_p(src.ctypes.data), C.c_void_p(dst.ctypes.data), src.size,
+                                      C.byref(n))
+        if rc != hip.OK:
+            raise hip.ZincError(rc, "compact")
+        return src[:n.value].copy(), dst[:n.value].copy()
 
     def free_count(self):
         return lib().zh_kv_pool_free_count(self.h)

@@ -108,6 +108,10 @@ SIGNATURES = {
                                         _u32, _f32]),
     "zh_flash_decode": (_i32, [_P, _P, _P, _P, _P, _u32, _u32, _P, _u32, _u32, _u32, _u32, _f32]),
     "zh_flash_decode_noalloc": (_i32, [_P, _P, _P, _P, _P, _u32, _u32, _P, _u32, _u32, _u32, _u32, _f32]),
+    "zh_qk_norm_rope_kv_write_batched": (_i32, [_P, _P, _P]),
+    "zh_flash_decode_shared": (_i32, [_P, _P, _P]),
+    "zh_flash_decode_shared_ws": (_u64, [_P, _P, _u32, _u32, _u32]),
+    "zh_kv_copy_pages": (_i32, [_P, _P, _P, _P, _P, _u32]),
     "zh_softmax_topk": (_i32, [_P, _P, _u32, _u32, _P]),
     "zh_moe_weighted_acc": (_i32, [_P, _P, _P, _P, _u32, _u32, _u32]),
     "zh_argmax": (_i32, [_P, _P, _u32, _P, _u64]),
@@ -138,6 +142,13 @@ SIGNATURES = {
     "zh_kv_pool_free": (None, [_P, _u64]),
     "zh_kv_pool_free_count": (_u32, [_P]),
     "zh_kv_pool_max_context": (_u32, [_P, _u32]),
+    "zh_kv_pool_fork": (_i32, [_P, _u64, _u64, _u32]),
+    "zh_kv_pool_unshare": (_i32, [_P, _u64, _u32, C.POINTER(_u32), C.POINTER(_u32)]),
+    "zh_kv_pool_trim": (_i32, [_P, _u64, _u32]),
+    "zh_kv_pool_pages": (_u32, [_P, _u64, _P, _u32]),
+    "zh_kv_pool_refs": (_u32, [_P, _u32]),
+    "zh_kv_pool_compact": (_i32, [_P, _P, _P, _u32, C.POINTER(_u32)]),
+    "zh_engine_fork_kv": (_i32, [_P, _P, _u32]),
     "zh_engine_bytes_per_token": (_u64, [_P, _u32]),
     "zh_engine_time_kernel": (_i32, [_P, _u32, _u32, _P]),
     "zh_engine_group_bytes": (_u64, [_P, _u32, _u32]),
@@ -169,6 +180,85 @@ SIGNATURES = {
                                       C.POINTER(_u64)]),
     "zh_gguf_model_config": (_i32, [_P, _u32, _P]),
 }
+
+
+
+class _Plan:
+    """A struct of the C ABI that a caller fills once and passes to many
+    calls: the buffers it names are kept alive with it."""
+
+    def _set(self, **fields):
+        self.c = self.Struct()
+        self._held = []
+        for name, v in fields.items():
+            if isinstance(v, Buffer):
+                self._held.append(v)
+                v = v.h
+            setattr(self.c, name, v)
+        self.ptr = C.byref(self.c)
+
+
+class KvBatch(_Plan):
+    """zh_kv_batch: one layer's paged caches and the page tables of a batch."""
+
+    class Struct(C.Structure):
+        _fields_ = [("k_cache", _P), ("v_cache", _P), ("tables", _P)] + [(n, _u32) for n in (
+            "n_seq", "table_stride", "cache_tokens", "n_kv_heads", "head_dim", "reserved")]
+
+    def __init__(self, k_cache, v_cache, tables, n_seq, table_stride, cache_tokens, n_kv_heads, head_dim):
+        self._set(k_cache=k_cache, v_cache=v_cache, tables=tables, n_seq=n_seq, table_stride=table_stride,
+                  cache_tokens=cache_tokens, n_kv_heads=n_kv_heads, head_dim=head_dim)
+
+
+class QkvRows(_Plan):
+    """zh_qkv_rows: the q, k and v rows of a batch of tokens, where the rotated
+    q goes, and each row's sequence and position. Strides in elements (0: rows
+    without gaps), offsets in bytes."""
+
+    class Struct(C.Structure):
+        _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_off", _u64), ("k_off", _u64), ("v_off", _u64),
+                    ("q_stride", _u32), ("k_stride", _u32), ("v_stride", _u32), ("type", _u32), ("q_out", _P),
+                    ("q_out_off", _u64), ("q_out_stride", _u32), ("q_out_type", _u32), ("q_norm_w", _P),
+                    ("k_norm_w", _P), ("inv_freq", _P), ("seq", _P), ("pos", _P), ("n_rows", _u32),
+                    ("n_q_heads", _u32), ("rope_dim", _u32), ("eps", _f32)]
+
+    def __init__(self, q, k, v, q_out, pos, n_rows, n_q_heads, inv_freq=None, seq=None, q_norm_w=None, k_norm_w=None,
+                 rope_dim=0, type=F32, q_out_type=None, q_off=0, k_off=0, v_off=0, q_out_off=0, q_stride=0, k_stride=0,
+                 v_stride=0, q_out_stride=0, eps=1e-6):
+        self._set(q=q, k=k, v=v, q_off=q_off, k_off=k_off, v_off=v_off, q_stride=q_stride, k_stride=k_stride,
+                  v_stride=v_stride, type=type, q_out=q_out, q_out_off=q_out_off, q_out_stride=q_out_stride,
+                  q_out_type=type if q_out_type is None else q_out_type, q_norm_w=q_norm_w, k_norm_w=k_norm_w,
+                  inv_freq=inv_freq, seq=seq, pos=pos, n_rows=n_rows, n_q_heads=n_q_heads, rope_dim=rope_dim, eps=eps)
+
+
+class DecodeRows(_Plan):
+    """zh_decode_rows: one query row per sequence and where its result goes."""
+
+    class Struct(C.Structure):
+        _fields_ = [("q", _P), ("out", _P), ("q_off", _u64), ("out_off", _u64), ("q_stride", _u32),
+                    ("out_stride", _u32), ("type", _u32), ("n_heads", _u32), ("seq_lens", _P), ("ws", _P),
+                    ("prefix_len", _u32), ("max_len", _u32), ("attn_scale", _f32), ("reserved", _u32)]
+
+    def __init__(self, q, out, seq_lens, ws, n_heads, max_len, prefix_len=0, type=F32, q_off=0, out_off=0, q_stride=0,
+                 out_stride=0, attn_scale=0.0):
+        self._set(q=q, out=out, q_off=q_off, out_off=out_off, q_stride=q_stride, out_stride=out_stride, type=type,
+                  n_heads=n_heads, seq_lens=seq_lens, ws=ws, prefix_len=prefix_len, max_len=max_len,
+                  attn_scale=attn_scale)
+
+
+class KvCaches(_Plan):
+    """zh_kv_caches: caches of one shape, whose pages are copied together."""
+
+    class Struct(C.Structure):
+        _fields_ = [("caches", C.POINTER(_P))] + [(n, _u32) for n in (
+            "n_caches", "cache_tokens", "n_kv_heads", "head_dim")]
+
+    def __init__(self, caches, cache_tokens, n_kv_heads, head_dim):
+        self._array = (_P * max(len(caches), 1))(*[b.h for b in caches])
+        self._set(caches=C.cast(self._array, C.POINTER(_P)), n_caches=len(caches), cache_tokens=cache_tokens,
+                  n_kv_heads=n_kv_heads, head_dim=head_dim)
+        self._held = list(caches)
+
 
 _lib = None
 
@@ -354,6 +444,25 @@ class Context:
                              attn_scale=0.0):
         self.check(lib().zh_flash_decode_noalloc(self.h, q.h, kc.h, vc.h, pages.h, n_pages, cache_tokens, out.h,
                                                  nh, nkv, hd, seq_len, attn_scale))
+
+    def qk_norm_rope_kv_write_batched(self, kv, rows):
+        """q/k norm, rotation and KV write of a batch (KvBatch, QkvRows)."""
+        self.check(lib().zh_qk_norm_rope_kv_write_batched(self.h, kv.ptr, rows.ptr))
+
+    def flash_decode_shared(self, kv, rows):
+        """Decode attention of a batch with a shared prefix (KvBatch, DecodeRows)."""
+        self.check(lib().zh_flash_decode_shared(self.h, kv.ptr, rows.ptr))
+
+    def flash_decode_shared_ws(self, kv, n_heads, prefix_len, max_len):
+        """Bytes of the workspace of such a call (0: refused sizes)."""
+        return lib().zh_flash_decode_shared_ws(self.h, kv.ptr, n_heads, prefix_len, max_len)
+
+    def kv_copy_pages(self, dst, src, dst_pages, src_pages):
+        """Page src_pages[i] of every cache of src to page dst_pages[i] of dst's (KvCaches)."""
+        d, s = np.ascontiguousarray(dst_pages, dtype=np.uint32), np.ascontiguousarray(src_pages, dtype=np.uint32)
+        if d.shape != s.shape or d.ndim != 1:
+            raise ValueError("one source page per destination page")
+        self.check(lib().zh_kv_copy_pages(self.h, dst.ptr, src.ptr, d.ctypes.data, s.ctypes.data, d.size))
 
     def softmax_topk(self, logits, n, k, routing):
         self.check(lib().zh_softmax_topk(self.h, logits.h, n, k, routing.h))
