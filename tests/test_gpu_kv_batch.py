@@ -622,3 +622,31 @@ def test_engine_fork_kv(zh, ctx):
     for e in reversed(engines):
         e.deinit()
     ctx2.close()
+
+
+def test_rope_of_more_rows_than_a_grid_is_high(zh, ctx):
+    """70000 rows without a sequence list, head_dim 2 (the kernel for any shape
+    takes at most 65535 rows a launch): row t is sequence t."""
+    rng = np.random.default_rng(13)
+    T, hd = 70000, 2
+    x = rng.standard_normal((T, 3, hd)).astype(np.float32)
+    pos = rng.integers(0, 16, T).astype(np.uint32)
+    pages = rng.permutation(T).astype(np.uint32)
+    freq = np.ones(1, np.float32)
+    u = ctx.upload
+    kc, vc, out = u(np.zeros((T * 16, hd), np.float16)), u(np.zeros((T * 16, hd), np.float16)), ctx.alloc(4 * T * hd)
+    X = u(x)
+    kv = zh.KvBatch(kc, vc, u(pages), T, 1, T * 16, 1, hd)
+    ctx.qk_norm_rope_kv_write_batched(kv, zh.QkvRows(
+        q=X, k=X, v=X, k_off=4 * hd, v_off=8 * hd, q_stride=3 * hd, k_stride=3 * hd, v_stride=3 * hd, q_out=out,
+        pos=u(pos), n_rows=T, n_q_heads=1, rope_dim=hd, inv_freq=u(freq)))
+    ctx.sync()
+    want, mag = rope64(x[:, :2], None, freq, pos, 1e-6, hd)
+    close(out.download(np.float32, T * hd).reshape(T, hd), want[:, 0], mag[:, 0] * 2.0 ** -19)
+    slot = pages.astype(np.int64) * 16 + pos
+    k64 = np.zeros((T * 16, hd))
+    k64[slot] = want[:, 1]
+    v64 = np.zeros((T * 16, hd))
+    v64[slot] = x[:, 2].astype(np.float16)
+    close(kc.download(np.float16, k64.size).reshape(k64.shape), k64, 2.0 ** -19 * 2 * np.abs(k64).max() + store_error(1, k64))
+    assert np.array_equal(vc.download(np.float16, v64.size).reshape(v64.shape).astype(np.float64), v64)

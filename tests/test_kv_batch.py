@@ -196,6 +196,10 @@ def test_copy_refusals():
     assert copy_check(KvCaches(bufs[:2], tokens + 16, nkv, hd), b, [1], [1]) == INVALID  # past the buffers
     assert copy_check(KvCaches([], tokens, nkv, hd), KvCaches([], tokens, nkv, hd), [1], [1]) == INVALID
     assert copy_check(KvCaches(bufs[:2], tokens // 2, nkv, hd), a, [1], [2]) == INVALID  # one cache in two sizes
+    many = [Fake(4096) for _ in range(256)]
+    assert copy_check(KvCaches(many, 16, 1, 64), KvCaches(many[::-1], 16, 1, 64), [0], [0]) == INVALID  # read and written
+    assert copy_check(KvCaches(many, 16, 1, 64), KvCaches([Fake(4096) for _ in range(256)], 16, 1, 64), [0], [0]) == OK
+    assert copy_check(KvCaches(many + bufs[:1], 16, 1, 64), KvCaches(many + bufs[:1], 16, 1, 64), [], []) == INVALID
     assert check("zh_check_kv_copy_pages", a.ptr, a.ptr, None, None, C.c_uint32(1)) == INVALID
     with pytest.raises(ValueError):
         hip.Context.kv_copy_pages(None, a, a, [1, 2], [3])

@@ -25,12 +25,33 @@ struct KvCopyArgs {
 };
 static_assert(sizeof(KvCopyArgs) <= 4096, "kernel arguments");
 
-// One workgroup per (page, head, cache).
+// One workgroup: KC_U pages of one head and cache, all loads before the stores.
+constexpr int KC_U = 2;  // (4 and 8: the same times)
+template <bool NT, int U>
+ZH_DEV void kv_copy_pages(const KvCopyArgs &a, uint32_t p0, const uint8_t *s, uint8_t *d) {
+    for (uint32_t i = threadIdx.x; i < a.seg / 16; i += blockDim.x) {
+        u32x4 v[U];
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const u32x4 *x = (const u32x4 *)(s + (uint64_t)a.pages[p0 + j][0] * a.seg) + i;
+            v[j] = NT ? __builtin_nontemporal_load(x) : *x;
+        }
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            u32x4 *x = (u32x4 *)(d + (uint64_t)a.pages[p0 + j][1] * a.seg) + i;
+            if (NT) __builtin_nontemporal_store(v[j], x);
+            else *x = v[j];
+        }
+    }
+}
+template <bool NT>
 __global__ __launch_bounds__(256) void k_kv_copy(KvCopyArgs a) {
-    const uint32_t p = blockIdx.x, h = blockIdx.y, c = blockIdx.z;
-    const u32x4 *s = (const u32x4 *)(a.src[c] + h * a.src_head + (uint64_t)a.pages[p][0] * a.seg);
-    u32x4 *d = (u32x4 *)(a.dst[c] + h * a.dst_head + (uint64_t)a.pages[p][1] * a.seg);
-    for (uint32_t i = threadIdx.x; i < a.seg / 16; i += 256) d[i] = s[i];
+    const uint32_t p0 = blockIdx.x * KC_U, h = blockIdx.y, c = blockIdx.z;
+    const uint8_t *s = a.src[c] + h * a.src_head;
+    uint8_t *d = a.dst[c] + h * a.dst_head;
+    if (p0 + KC_U <= a.n_pages) kv_copy_pages<NT, KC_U>(a, p0, s, d);
+    else
+        for (uint32_t p = p0; p < a.n_pages; p++) kv_copy_pages<NT, 1>(a, p, s, d);
 }
 
 }  // namespace
@@ -43,6 +64,10 @@ int zhk_kv_copy(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *cons
     a.src_head = 2ull * src_tokens * head_dim;
     a.dst_head = 2ull * dst_tokens * head_dim;
     a.n_heads = n_kv_heads;
+    const uint32_t threads = a.seg >= 4096 ? 256u : (a.seg / 16 + 63) / 64 * 64;
+    // past what the L2s hold, the pages go by them: 1024 pages of 32 caches of 8
+    // heads 382 us (5.6 TB/s read + written) against 408 through them
+    const bool nt = (uint64_t)n_caches * n_pages * n_kv_heads * a.seg > (32ull << 20);
     for (uint32_t c0 = 0; c0 < n_caches; c0 += KC_CACHES) {
         a.n_caches = n_caches - c0 < KC_CACHES ? n_caches - c0 : KC_CACHES;
         for (uint32_t i = 0; i < a.n_caches; i++) {
@@ -55,7 +80,9 @@ int zhk_kv_copy(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *cons
                 a.pages[i][0] = src_pages[p0 + i];
                 a.pages[i][1] = dst_pages[p0 + i];
             }
-            hipLaunchKernelGGL(k_kv_copy, dim3(a.n_pages, a.n_heads, a.n_caches), dim3(256), 0, c->stream, a);
+            const dim3 grid((a.n_pages + KC_U - 1) / KC_U, a.n_heads, a.n_caches);
+            if (nt) hipLaunchKernelGGL(k_kv_copy<true>, grid, dim3(threads), 0, c->stream, a);
+            else hipLaunchKernelGGL(k_kv_copy<false>, grid, dim3(threads), 0, c->stream, a);
             ZH_LAUNCH_CHECK(c);
         }
     }
@@ -63,7 +90,7 @@ int zhk_kv_copy(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *cons
 }
 
 static bool caches_ok(const zh_kv_caches *s) {
-    if (!s || !s->caches || s->n_caches == 0 || s->n_kv_heads == 0 || s->n_kv_heads > 65535 || s->head_dim == 0 ||
+    if (!s || !s->caches || s->n_caches == 0 || s->n_caches > 256 || s->n_kv_heads == 0 || s->n_kv_heads > 65535 || s->head_dim == 0 ||
         s->head_dim > 1024 || s->cache_tokens == 0)
         return false;
     for (uint32_t i = 0; i < s->n_caches; i++)
@@ -80,15 +107,22 @@ extern "C" int zh_check_kv_copy_pages(zh_ctx *c, const zh_kv_caches *dst, const 
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: cache sets");
     if (n_pages && (!dst_pages || !src_pages))
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: no page numbers");
+    // the caches' addresses in a small hash table (a fork copies a few pages of
+    // all layers: comparing every pair would take longer than the copy)
     bool alias = false;
+    uint16_t tab[1024] = {};
+    auto place = [&](const void *p) {  // p's entry, or the empty one it would take
+        uint32_t i = (uint32_t)(((uint64_t)(uintptr_t)p * 0x9E3779B97F4A7C15ull) >> 54);
+        while (tab[i] && dst->caches[tab[i] - 1]->ptr != p) i = (i + 1) % 1024;
+        return i;
+    };
     for (uint32_t i = 0; i < dst->n_caches; i++) {
-        if (dst->caches[i]->ptr == src->caches[i]->ptr) alias = true;
-        for (uint32_t j = 0; j < i; j++) {
-            if (dst->caches[i]->ptr == dst->caches[j]->ptr)
-                return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: caches %u and %u of dst are one", j, i);
-            if (dst->caches[i]->ptr == src->caches[j]->ptr || dst->caches[j]->ptr == src->caches[i]->ptr) alias = true;
-        }
+        uint16_t &e = tab[place(dst->caches[i]->ptr)];
+        if (e)
+            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: caches %u and %u of dst are one", e - 1u, i);
+        e = (uint16_t)(i + 1);
     }
+    for (uint32_t i = 0; i < src->n_caches && !alias; i++) alias = tab[place(src->caches[i]->ptr)] != 0;
     if (alias && dst->cache_tokens != src->cache_tokens)
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: one cache in two sizes");
     const uint32_t np = dst->cache_tokens / 16;
@@ -163,6 +197,7 @@ struct QkvArgs {
     const uint32_t *tables, *seq, *pos;
     uint32_t *err;
     uint32_t n_seq, stride, cache_tokens, nq, nkv, hd, rd;
+    uint32_t t0;  // rows before this launch's (k_qkv_rows)
     float eps;
 };
 
@@ -194,7 +229,7 @@ __global__ __launch_bounds__(64) void k_qkv_rows(QkvArgs a) {
     const uint32_t h = is_q ? head : (head - a.nq) % a.nkv;
     uint32_t slot = 0;
     if (!is_q) {
-        const uint32_t s = a.seq ? a.seq[t] : t;
+        const uint32_t s = a.seq ? a.seq[t] : a.t0 + t;
         if (!kv_slot(a.tables, a.n_seq, a.stride, a.cache_tokens, s, pos, slot)) {
             if (lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
             return;
@@ -235,6 +270,105 @@ __global__ __launch_bounds__(64) void k_qkv_rows(QkvArgs a) {
         put(i + a.rd / 2, lo * sn + hi * co);
     }
     for (uint32_t i = a.rd + lane; i < a.hd; i += 64) put(i, val(i));
+}
+
+// 8 elements of a row as floats / from floats.
+ZH_DEV void ld8(const float *p, float (&v)[8]) {
+    const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+ZH_DEV void ld8(const _Float16 *p, float (&v)[8]) {
+    const half8 a = *(const half8 *)p;
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (float)a[e];
+}
+ZH_DEV void st8(float *p, const float (&v)[8]) {
+    *(f32x4 *)p = f32x4{v[0], v[1], v[2], v[3]};
+    *(f32x4 *)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+}
+ZH_DEV void st8(_Float16 *p, const float (&v)[8]) {
+    half8 a;
+#pragma unroll
+    for (int e = 0; e < 8; e++) a[e] = (_Float16)v[e];
+    *(half8 *)p = a;
+}
+
+// Head dims of 8 L (L = 8, 16, 32 lanes of 8 dims), rope_dim / 16 zero or a
+// power of two, 16-byte aligned rows: a workgroup takes R x 256 / L heads of one
+// row (blockIdx.x) and works the row's angles out once, in LDS. The rotation's
+// partner dims lie rope_dim / 16 lanes away.
+template <typename TI, typename TQ, int L, int R>
+__global__ __launch_bounds__(256) void k_qkv_rows8(QkvArgs a) {
+    constexpr uint32_t HD = 8 * L, NS = 256 / L;
+    __shared__ float2 cs[HD / 2];
+    const uint32_t t = blockIdx.x, tid = threadIdx.x, l = tid % L, slot8 = tid / L;
+    const uint32_t pos = a.pos[t];
+    if (pos == ZH_POS_NONE) return;
+    const uint32_t h0 = blockIdx.y * (R * NS), H = a.nq + 2 * a.nkv;
+    float x[R][8];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const uint32_t h = min(h0 + r * NS + slot8, H - 1);
+        const uint8_t *p = h < a.nq ? a.q + t * a.q_row : h < a.nq + a.nkv ? a.k + t * a.k_row : a.v + t * a.v_row;
+        const uint32_t hh = h < a.nq ? h : h < a.nq + a.nkv ? h - a.nq : h - a.nq - a.nkv;
+        ld8((const TI *)p + hh * HD + 8 * l, x[r]);
+    }
+    uint32_t slot = 0;
+    bool ok = true;
+    if (h0 + R * NS > a.nq) {  // (uniform: some k or v head)
+        ok = kv_slot(a.tables, a.n_seq, a.stride, a.cache_tokens, a.seq ? a.seq[t] : t, pos, slot);
+        if (!ok && tid == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+    }
+    const uint32_t h2 = a.rd / 2;
+    if (h2 && h0 < a.nq + a.nkv) {  // (uniform: some q or k head)
+        if (tid < h2) turn(pos, a.inv_freq[tid], cs[tid].x, cs[tid].y);
+        __syncthreads();
+    }
+    const bool rot = 8 * l < a.rd, lower = 8 * l < h2;
+    float2 t8[8];
+    if (rot) {
+        const uint32_t b = lower ? 8 * l : 8 * l - h2;
+#pragma unroll
+        for (int e = 0; e < 8; e++) t8[e] = cs[b + e];
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const uint32_t h = h0 + r * NS + slot8;
+        if (h0 + r * NS >= H) break;  // uniform
+        const bool is_q = h < a.nq, is_v = h >= a.nq + a.nkv;
+        if (h0 + r * NS < a.nq + a.nkv) {  // (uniform; all lanes take part in the exchanges)
+            float y[8], sq = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) sq = fmaf(x[r][e], x[r][e], sq);
+            const float *w = is_q ? a.qw : a.kw;
+            if (a.qw || a.kw) {
+                const float ri = 1.0f / sqrtf(team_sum_dpp<L>(sq) / (float)HD + a.eps);
+                if (w && !is_v) {
+                    float wv[8];
+                    ld8(w + 8 * l, wv);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[r][e] = wv[e] * (x[r][e] * ri);
+                }
+            }
+            if (h2) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = __shfl_xor(x[r][e], h2 / 8, 64);
+                if (rot && !is_v)
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        x[r][e] = lower ? x[r][e] * t8[e].x - y[e] * t8[e].y : y[e] * t8[e].y + x[r][e] * t8[e].x;
+            }
+        }
+        if (h >= H) continue;
+        if (is_q) {
+            st8((TQ *)(a.q_out + t * a.out_row) + h * HD + 8 * l, x[r]);
+        } else if (ok) {
+            const uint32_t hh = is_v ? h - a.nq - a.nkv : h - a.nq;
+            st8((_Float16 *)(is_v ? a.vc : a.kc) + ((size_t)hh * a.cache_tokens + slot) * HD + 8 * l, x[r]);
+        }
+    }
 }
 
 }  // namespace
@@ -309,8 +443,27 @@ extern "C" int zh_check_qkv_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_qkv_
     return ZH_OK;
 }
 
+template <typename TI, typename TQ, int L>
+static void qkv_launch8(zh_ctx *c, const QkvArgs &a, uint32_t n) {
+    constexpr uint32_t NS = 256 / L;
+    const uint32_t H = a.nq + 2 * a.nkv;
+    // few rows: every workgroup one round of heads, for the most workgroups
+    if (n < 512) hipLaunchKernelGGL((k_qkv_rows8<TI, TQ, L, 1>), dim3(n, (H + NS - 1) / NS), dim3(256), 0, c->stream, a);
+    else hipLaunchKernelGGL((k_qkv_rows8<TI, TQ, L, 4>), dim3(n, (H + 4 * NS - 1) / (4 * NS)), dim3(256), 0, c->stream, a);
+}
+
 template <typename TI, typename TQ>
 static int qkv_launch(zh_ctx *c, const QkvArgs &a, uint32_t n) {
+    const uint32_t p2 = a.rd / 16;
+    const bool rows16 = (((uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v |
+                          (uint64_t)(uintptr_t)a.q_out | a.q_row | a.k_row | a.v_row | a.out_row) % 16) == 0;
+    if (rows16 && a.rd % 16 == 0 && (p2 & (p2 - 1)) == 0 && (a.hd == 64 || a.hd == 128 || a.hd == 256)) {
+        if (a.hd == 64) qkv_launch8<TI, TQ, 8>(c, a, n);
+        else if (a.hd == 128) qkv_launch8<TI, TQ, 16>(c, a, n);
+        else qkv_launch8<TI, TQ, 32>(c, a, n);
+        ZH_LAUNCH_CHECK(c);
+        return ZH_OK;
+    }
     // (at most 65535 rows a launch: the grid's y)
     for (uint32_t t0 = 0; t0 < n; t0 += 65535) {
         QkvArgs b = a;
@@ -320,6 +473,7 @@ static int qkv_launch(zh_ctx *c, const QkvArgs &a, uint32_t n) {
         b.q_out += t0 * a.out_row;
         b.pos += t0;
         if (b.seq) b.seq += t0;
+        b.t0 = t0;
         hipLaunchKernelGGL((k_qkv_rows<TI, TQ>), dim3(a.nq + 2 * a.nkv, n - t0 < 65535 ? n - t0 : 65535), dim3(64), 0,
                            c->stream, b);
         ZH_LAUNCH_CHECK(c);
@@ -360,6 +514,6 @@ extern "C" int zh_qk_norm_rope_kv_write_batched(zh_ctx *c, const zh_kv_batch *kv
     a.hd = kv->head_dim;
     a.rd = r->rope_dim;
     a.eps = r->eps;
-    if (si == 4) return so == 4 ? qkv_launch<float, float>(c, a, r->n_rows) : qkv_launch<float, uint16_t>(c, a, r->n_rows);
-    return so == 4 ? qkv_launch<uint16_t, float>(c, a, r->n_rows) : qkv_launch<uint16_t, uint16_t>(c, a, r->n_rows);
+    if (si == 4) return so == 4 ? qkv_launch<float, float>(c, a, r->n_rows) : qkv_launch<float, _Float16>(c, a, r->n_rows);
+    return so == 4 ? qkv_launch<_Float16, float>(c, a, r->n_rows) : qkv_launch<_Float16, _Float16>(c, a, r->n_rows);
 }

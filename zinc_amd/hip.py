@@ -462,7 +462,8 @@ class Context:
         d, s = np.ascontiguousarray(dst_pages, dtype=np.uint32), np.ascontiguousarray(src_pages, dtype=np.uint32)
         if d.shape != s.shape or d.ndim != 1:
             raise ValueError("one source page per destination page")
-        self.check(lib().zh_kv_copy_pages(self.h, dst.ptr, src.ptr, d.ctypes.data, s.ctypes.data, d.size))
+        self.check(lib().zh_kv_copy_pages(self.h, dst.ptr, src.ptr, d.__array_interface__["data"][0],
+                                          s.__array_interface__["data"][0], d.size))
 
     def softmax_topk(self, logits, n, k, routing):
         self.check(lib().zh_softmax_topk(self.h, logits.h, n, k, routing.h))
