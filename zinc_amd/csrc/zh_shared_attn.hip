@@ -21,9 +21,21 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr uint32_t SA_ROWS = 16;  // rows of a workgroup: one MFMA tile
+constexpr uint32_t SA_ROWS = 16;  // rows of an MFMA tile
 constexpr uint32_t SA_KB = 32;    // tokens of a wave's step
 constexpr int SA_W = 4;           // waves of a workgroup, each on its own steps
+#ifndef SA_TILE
+#define SA_TILE 96
+#endif
+#ifndef SA_RT
+#define SA_RT 2
+#endif
+#ifndef SA_PRE_PER
+#define SA_PRE_PER 2
+#endif
+#ifndef SA_OWN_PER
+#define SA_OWN_PER 8
+#endif
 
 struct SharedArgs {
     const uint8_t *q;
@@ -38,6 +50,7 @@ struct SharedArgs {
     uint32_t n_pre, n_own;           // parts of the prefix and of a sequence's own tokens
     uint32_t pre_tiles, pre_blocks;  // row tiles per kv head, workgroups of the prefix
     uint32_t pre_len;                // tokens of a prefix part (a multiple of SA_KB)
+    uint32_t pre_rows;               // rows of a prefix workgroup
     float scale;
 };
 
@@ -52,9 +65,9 @@ ZH_DEV float ld(const uint8_t *p, uint32_t i) {
     return sizeof(T) == 4 ? ((const float *)p)[i] : (float)((const _Float16 *)p)[i];
 }
 
-// One workgroup: 16 rows of one kv head over the tokens of one part. Each wave
-// takes steps of 32 tokens by itself, K and V straight from the cache into the
-// matrix operands' registers (no LDS, no barrier before the end):
+// One workgroup: up to 16 QT rows of one kv head over the tokens of one part.
+// Each wave takes steps of 32 tokens by itself, K and V straight from the cache
+// into the matrix operands' registers (no LDS, no barrier before the end):
 //   S^T = K q^T (tokens x rows): lane (li = lane % 16, lg = lane / 16) holds
 //   tokens 16 j + 4 lg + r of row li, so that a row's maximum is in-lane plus
 //   two lane exchanges, and its weights lie as the second product's operand
@@ -63,46 +76,26 @@ ZH_DEV float ld(const uint8_t *p, uint32_t i) {
 //   permutes; column li of the output tile n is dim HD/16 li + n.
 // NP pieces: q (scaled by a power of two to a maximum in [1, 2)) and P as sums
 // of NP fp16 values; 2 keep 22 bits of each.
-template <int HD, int NP, typename T>
-__global__ __launch_bounds__(64 * SA_W, 2) void k_shared_attn(SharedArgs a) {
+struct SharedPart {
+    uint32_t part, row0, nrow, t0, t1, tab;  // rows row0 .. (s * G + g), tokens [t0, t1) through table `tab`
+};
+
+template <int HD, int NP, int QT, typename T>
+ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, float *lds) {
     constexpr int K4 = HD / 32, ND = HD / 16;  // k-steps of the scores, dims per lane and output tiles
-    __shared__ float so[SA_W][SA_ROWS][HD + 4];
-    __shared__ float sm[SA_W][SA_ROWS], sl[SA_W][SA_ROWS];
+    constexpr int LD = HD + 4;
+    float *const so = lds, *const sm = lds + SA_W * SA_ROWS * LD, *const sl = sm + SA_W * SA_ROWS;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t li = lane % 16, lg = lane / 16;
-    const bool pre = blockIdx.x < a.pre_blocks;
-    // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
-    const uint32_t job = pre ? blockIdx.x : blockIdx.x - a.pre_blocks, kvh = job % a.nkv;
-    uint32_t part, row0, nrow, t0, t1, tab;  // rows row0 .. (s * G + g), tokens [t0, t1) through table `tab`
-    if (pre) {
-        const uint32_t tile = job / a.nkv % a.pre_tiles;
-        part = job / a.nkv / a.pre_tiles;
-        row0 = tile * SA_ROWS;
-        nrow = min(SA_ROWS, a.n_seq * a.G - row0);
-        tab = 0;
-        t0 = part * a.pre_len;
-        t1 = min(t0 + a.pre_len, a.prefix);
-    } else {
-        const uint32_t s = job / a.nkv % a.n_seq, p = job / a.nkv / a.n_seq;
-        part = a.n_pre + p;
-        row0 = s * a.G;
-        nrow = a.G;
-        tab = s;
-        const uint32_t len = seq_len(a, s);
-        if (tid == 0 && p == 0 && kvh == 0 && a.lens[s] > a.max_len) atomicOr(a.err, ZH_DEVERR_KV_ROW);
-        // a sequence shorter than the prefix: all of its tokens are its own
-        const uint32_t b = len < a.prefix ? 0u : a.prefix, n = (len - b + a.n_own - 1) / a.n_own;
-        const uint32_t c = (n + SA_KB - 1) / SA_KB * SA_KB;
-        t0 = min(b + p * c, len);
-        t1 = min(b + (p + 1) * c, len);
-    }
+    const uint32_t t0 = w.t0, t1 = w.t1;
     const uint32_t ta = t0 & ~15u;  // steps start on a page; tokens before t0 are masked
     const uint32_t nstep = t1 > t0 ? (t1 - ta + SA_KB - 1) / SA_KB : 0u;
-    // the row's q as operand fragments: dims 32 k4 + 8 lg ..
-    const uint32_t row = row0 + min(li, nrow - 1), rs = row / a.G, rh = kvh * a.G + row % a.G;
-    half8 qf[NP][K4];
-    float c = a.scale * 1.44269504088896340736f;  // scores in base 2
-    {
+    // the rows' q as operand fragments: dims 32 k4 + 8 lg ..
+    half8 qf[QT][NP][K4];
+    float c[QT];  // scores in base 2
+#pragma unroll
+    for (int q = 0; q < QT; q++) {
+        const uint32_t row = w.row0 + min(16u * q + li, w.nrow - 1), rs = row / a.G, rh = kvh * a.G + row % a.G;
         const uint8_t *qp = a.q + rs * a.q_row + (size_t)rh * HD * sizeof(T);
         float v[K4][8], mx = 0.f;
 #pragma unroll
@@ -113,13 +106,14 @@ __global__ __launch_bounds__(64 * SA_W, 2) void k_shared_attn(SharedArgs a) {
                 mx = fmaxf(mx, fabsf(v[k4][e]));
             }
         float up = 1.f;
+        c[q] = a.scale * 1.44269504088896340736f;
         if (NP > 1) {
             mx = xor32_max(xor16_max(mx));
             // 2^-E for a maximum in [2^E, 2^(E+1)) (not for zero, infinite or tiny rows)
             const uint32_t E = __float_as_uint(mx) >> 23;
             if (E >= 8 && E <= 246) {
                 up = __uint_as_float((254u - E) << 23);
-                c *= __uint_as_float(E << 23);
+                c[q] *= __uint_as_float(E << 23);
             }
         }
 #pragma unroll
@@ -129,17 +123,22 @@ __global__ __launch_bounds__(64 * SA_W, 2) void k_shared_attn(SharedArgs a) {
                 float x = v[k4][e] * up;
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
-                    qf[p][k4][e] = (_Float16)x;
-                    x -= (float)qf[p][k4][e];
+                    qf[q][p][k4][e] = (_Float16)x;
+                    x -= (float)qf[q][p][k4][e];
                 }
             }
     }
-    floatx4 o[ND];
+    floatx4 o[QT][ND];
+    float m[QT], l[QT];  // the row's maximum (every lg alike), this lane's share of its sum
 #pragma unroll
-    for (int n = 0; n < ND; n++) o[n] = floatx4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;  // the row's maximum (every lg alike), this lane's share of its sum
+    for (int q = 0; q < QT; q++) {
+        m[q] = -INFINITY;
+        l[q] = 0.f;
+#pragma unroll
+        for (int n = 0; n < ND; n++) o[q][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
     const uint16_t *kh = a.kc + (size_t)kvh * a.cache_tokens * HD, *vh = a.vc + (size_t)kvh * a.cache_tokens * HD;
-    const uint32_t *tb = a.tables + (size_t)tab * a.stride;
+    const uint32_t *tb = a.tables + (size_t)w.tab * a.stride;
     bool bad = false;
     for (uint32_t st = wave; st < nstep; st += SA_W) {
         const uint32_t tk = ta + st * SA_KB;
@@ -168,126 +167,464 @@ __global__ __launch_bounds__(64 * SA_W, 2) void k_shared_attn(SharedArgs a) {
             }
         }
         const bool whole = tk >= t0 && tk + SA_KB <= t1;
-        float s[2][4], mb = -INFINITY;
+        half8 pf[QT][NP];
+        float f[QT];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            floatx4 d = {0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < QT; q++) {
+            float s[2][4], mb = -INFINITY;
 #pragma unroll
-            for (int p = NP - 1; p >= 0; p--)
+            for (int j = 0; j < 2; j++) {
+                floatx4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k4 = 0; k4 < K4; k4++)
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[j][k4], qf[p][k4], d, 0, 0, 0);
+                for (int p = NP - 1; p >= 0; p--)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                s[j][r] = d[r] * c;
-                if (!whole) {
-                    // a token outside the part: no score, and no V (0 times
-                    // what the cache holds there may be NaN)
-                    const uint32_t t = tk + 16 * j + 4 * lg + r;
-                    if (t < t0 || t >= t1) {
-                        s[j][r] = -INFINITY;
+                    for (int k4 = 0; k4 < K4; k4++)
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[j][k4], qf[q][p][k4], d, 0, 0, 0);
 #pragma unroll
-                        for (int w = 0; w < ND / 2; w++) pv[j][r][w] = 0u;
+                for (int r = 0; r < 4; r++) {
+                    s[j][r] = d[r] * c[q];
+                    if (!whole) {
+                        const uint32_t t = tk + 16 * j + 4 * lg + r;
+                        if (t < t0 || t >= t1) s[j][r] = -INFINITY;
+                    }
+                    mb = fmaxf(mb, s[j][r]);
+                }
+            }
+            mb = xor32_max(xor16_max(mb));
+            // (weights up to 2^8, away from fp16's subnormals)
+            const float mn = fmaxf(m[q], mb - 8.f), ms = mn == -INFINITY ? 0.f : mn;
+            f[q] = __builtin_amdgcn_exp2f(m[q] - ms);  // (m = -inf: 0)
+            m[q] = mn;
+            float ls = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float p = __builtin_amdgcn_exp2f(s[j][r] - ms);
+                    ls += p;
+#pragma unroll
+                    for (int k = 0; k < NP; k++) {
+                        pf[q][k][4 * j + r] = (_Float16)p;
+                        p -= (float)pf[q][k][4 * j + r];
                     }
                 }
-                mb = fmaxf(mb, s[j][r]);
-            }
+            l[q] = fmaf(l[q], f[q], ls);
         }
-        mb = xor32_max(xor16_max(mb));
-        const float mn = fmaxf(m, mb), ms = mn == -INFINITY ? 0.f : mn;
-        const float f = __builtin_amdgcn_exp2f(m - ms);  // (m = -inf: 0)
-        m = mn;
-        half8 pf[NP];
-        float ls = 0.f;
+        if (!whole) {
+            // no V of a token outside the part (0 times what the cache holds there may be NaN)
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float p = __builtin_amdgcn_exp2f(s[j][r] - ms);
-                ls += p;
-                p *= 256.f;  // (away from fp16's subnormals; taken back at the end)
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t t = tk + 16 * j + 4 * lg + r;
 #pragma unroll
-                for (int k = 0; k < NP; k++) {
-                    pf[k][4 * j + r] = (_Float16)p;
-                    p -= (float)pf[k][4 * j + r];
+                    for (int x = 0; x < ND / 2; x++) pv[j][r][x] = t < t0 || t >= t1 ? 0u : pv[j][r][x];
                 }
-            }
-        l = fmaf(l, f, ls);
+        }
 #pragma unroll
         for (int n = 0; n < ND; n++) {
-            uint32_t w[4];
+            uint32_t x[4];
 #pragma unroll
             for (int i = 0; i < 4; i++)  // tokens 2 i, 2 i + 1 of the operand: their halfs of dim n
-                w[i] = __builtin_amdgcn_perm(pv[i >> 1][2 * (i & 1) + 1][n >> 1], pv[i >> 1][2 * (i & 1)][n >> 1],
+                x[i] = __builtin_amdgcn_perm(pv[i >> 1][2 * (i & 1) + 1][n >> 1], pv[i >> 1][2 * (i & 1)][n >> 1],
                                              (n & 1) ? 0x07060302u : 0x05040100u);
-            const u32x4 wv = {w[0], w[1], w[2], w[3]};
-            const half8 vf = __builtin_bit_cast(half8, wv);
+            const u32x4 xv = {x[0], x[1], x[2], x[3]};
+            const half8 vf = __builtin_bit_cast(half8, xv);
 #pragma unroll
-            for (int r = 0; r < 4; r++) o[n][r] *= f;
+            for (int q = 0; q < QT; q++) {
 #pragma unroll
-            for (int p = NP - 1; p >= 0; p--) o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[p], o[n], 0, 0, 0);
+                for (int r = 0; r < 4; r++) o[q][n][r] *= f[q];
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--)
+                    o[q][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[q][p], o[q][n], 0, 0, 0);
+            }
         }
     }
     if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
-    l = xor32_sum(xor16_sum(l));
-    // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-#pragma unroll
-        for (int n = 0; n < ND; n++) so[wave][li][ND * (4 * lg + r) + n] = o[n][r];
-    if (lg == 0) {
-        sm[wave][li] = m;
-        sl[wave][li] = l;
-    }
-    __syncthreads();
+    // ---- join the waves, 16 rows at a time; lane li, lg: row li, dims ND (4 lg + r) + n
     const bool direct = a.n_pre + a.n_own == 1;
-    for (uint32_t i = tid; i < nrow * HD; i += 64 * SA_W) {
-        const uint32_t r = i / HD, d = i % HD, R = row0 + r, s = R / a.G, h = kvh * a.G + R % a.G;
-        float M = sm[0][r], O = 0.f, L = 0.f;
 #pragma unroll
-        for (int w = 1; w < SA_W; w++) M = fmaxf(M, sm[w][r]);
-        const float Ms = M == -INFINITY ? 0.f : M;
+    for (int q = 0; q < QT; q++) {
+        if (16u * q >= w.nrow) break;  // uniform
+        if (q) __syncthreads();
+        const float lq = xor32_sum(xor16_sum(l[q]));
 #pragma unroll
-        for (int w = 0; w < SA_W; w++) {
-            const float f = __builtin_amdgcn_exp2f(sm[w][r] - Ms);
-            O = fmaf(so[w][r][d], f, O);
-            L = fmaf(sl[w][r], f, L);
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int n = 0; n < ND; n++) so[(wave * SA_ROWS + li) * LD + ND * (4 * lg + r) + n] = o[q][n][r];
+        if (lg == 0) {
+            sm[wave * SA_ROWS + li] = m[q];
+            sl[wave * SA_ROWS + li] = lq;
         }
-        O *= 1.f / 256.f;
-        if (direct) {
-            const float v = t1 > t0 ? O / L : 0.f;
-            uint8_t *op = a.out + s * a.out_row;
-            if (sizeof(T) == 4) ((float *)op)[h * HD + d] = v;
-            else ((_Float16 *)op)[h * HD + d] = (_Float16)v;
-        } else {
-            const size_t pr = (size_t)part * a.n_seq * a.nh + (size_t)s * a.nh + h;
-            a.part[pr * HD + d] = O;
-            if (d == 0) {
-                a.stat[2 * pr] = M;
-                a.stat[2 * pr + 1] = L;
+        __syncthreads();
+        const uint32_t nr = min(SA_ROWS, w.nrow - 16 * q);
+        for (uint32_t i = tid; i < nr * HD; i += 64 * SA_W) {
+            const uint32_t r = i / HD, d = i % HD, R = w.row0 + 16 * q + r, s = R / a.G, h = kvh * a.G + R % a.G;
+            float M = sm[r], O = 0.f, L = 0.f;
+#pragma unroll
+            for (int k = 1; k < SA_W; k++) M = fmaxf(M, sm[k * SA_ROWS + r]);
+            const float Ms = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int k = 0; k < SA_W; k++) {
+                const float fk = __builtin_amdgcn_exp2f(sm[k * SA_ROWS + r] - Ms);
+                O = fmaf(so[(k * SA_ROWS + r) * LD + d], fk, O);
+                L = fmaf(sl[k * SA_ROWS + r], fk, L);
+            }
+            if (direct) {
+                const float v = t1 > t0 ? O / L : 0.f;
+                uint8_t *op = a.out + s * a.out_row;
+                if (sizeof(T) == 4) ((float *)op)[h * HD + d] = v;
+                else ((_Float16 *)op)[h * HD + d] = (_Float16)v;
+            } else {
+                const size_t pr = (size_t)w.part * a.n_seq * a.nh + (size_t)s * a.nh + h;
+                a.part[pr * HD + d] = O;
+                if (d == 0) {
+                    a.stat[2 * pr] = M;
+                    a.stat[2 * pr + 1] = L;
+                }
             }
         }
     }
 }
 
-// Joins the parts of a row (one wave each).
+// The prefix's workgroups (16 QT rows each), then the sequences' own (16 rows).
+template <int HD, int NP, int QT, typename T>
+__global__ __launch_bounds__(64 * SA_W, QT * NP >= 4 ? 1 : 2) void k_shared_attn(SharedArgs a) {
+    __shared__ float lds[SA_W * SA_ROWS * (HD + 6)];
+    const bool pre = blockIdx.x < a.pre_blocks;
+    // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
+    const uint32_t job = pre ? blockIdx.x : blockIdx.x - a.pre_blocks, kvh = job % a.nkv;
+    SharedPart w;
+    if (pre) {
+        const uint32_t tile = job / a.nkv % a.pre_tiles;
+        w.part = job / a.nkv / a.pre_tiles;
+        w.row0 = tile * a.pre_rows;
+        w.nrow = min(a.pre_rows, a.n_seq * a.G - w.row0);
+        w.tab = 0;
+        w.t0 = w.part * a.pre_len;
+        w.t1 = min(w.t0 + a.pre_len, a.prefix);
+        shared_part<HD, NP, QT, T>(a, w, kvh, lds);
+    } else {
+        const uint32_t s = job / a.nkv % a.n_seq, p = job / a.nkv / a.n_seq;
+        w.part = a.n_pre + p;
+        w.row0 = s * a.G;
+        w.nrow = a.G;
+        w.tab = s;
+        const uint32_t len = seq_len(a, s);
+        if (threadIdx.x == 0 && p == 0 && kvh == 0 && a.lens[s] > a.max_len) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+        // a sequence shorter than the prefix: all of its tokens are its own
+        const uint32_t b = len < a.prefix ? 0u : a.prefix, n = (len - b + a.n_own - 1) / a.n_own;
+        const uint32_t c = (n + SA_KB - 1) / SA_KB * SA_KB;
+        w.t0 = min(b + p * c, len);
+        w.t1 = min(b + (p + 1) * c, len);
+        shared_part<HD, NP, 1, T>(a, w, kvh, lds);
+    }
+}
+
+// Many rows (a workgroup: 4 waves of 32 RT): K and V pass through LDS once for
+// all of them, in stages of 64 tokens copied there four ahead without passing
+// registers (each wave one page of a stage).
+//   S^T = K q^T by v_mfma_f32_32x32x16_f16: lane (i = lane % 32, h = lane / 32)
+//   holds tokens 8 (r / 4) + 4 h + r % 4 of row i in register r; registers
+//   8 s .. 8 s + 7 are the weights' operand of the s-th 16-token product
+//   O^T += V^T P^T. V stays row-major in LDS, its transposed fragments come from
+//   ds_read_b64_tr_b16. 16-byte pieces of a row lie at piece ^ (row % pieces),
+//   so that 32 rows' reads of one piece hit every bank alike.
+// The products of the next 32 tokens' scores run while the current ones' weights
+// are computed. The reference maximum moves only when a score passes it by 2^8
+// (the weights then reach 2^12 in fp16 at most), so the output is rarely rescaled.
+constexpr uint32_t ST_KB = 64, ST_NS = 4;
+template <int HD>
+constexpr uint32_t st_lds() { return 2 * ST_NS * ST_KB * HD * 2; }
+
+// 16 bytes per lane from base + off to LDS at the wave-uniform address + 16 lane.
+ZH_DEV void dma16_s(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int HD, int NP, int RT, typename T>
+__global__ __launch_bounds__(256, 1) void k_shared_tile(SharedArgs a) {
+    constexpr int KS = HD / 16, DT = HD / 32;       // k-steps of the scores, 32-dim tiles of the output
+    constexpr uint32_t ROWB = HD * 2, PPR = HD / 8;  // bytes and 16-byte pieces of a row
+    constexpr uint32_t STAGE = ST_KB * ROWB, NI = 16 * ROWB / 1024;  // bytes of a stage, copies of a page
+    extern __shared__ __align__(16) uint8_t lds[];
+    typedef __fp16 tr4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) tr4 lds_tr4;
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const uint32_t i32 = lane % 32, h = lane / 32;
+    // (the row tiles of one part and kv head on one XCD: they read the same K and V)
+    const uint32_t per = a.nkv * a.n_pre, tile = blockIdx.x / per, kvh = blockIdx.x % per % a.nkv;
+    const uint32_t part = blockIdx.x % per / a.nkv;
+    const uint32_t rows = a.n_seq * a.G, row0 = tile * (128 * RT) + wave * (32 * RT);
+    const bool mine = row0 < rows;  // (uniform per wave: it has rows)
+    const uint32_t t0 = part * a.pre_len, t1 = min(t0 + a.pre_len, a.prefix);
+    const uint32_t nst = (t1 - t0 + ST_KB - 1) / ST_KB;
+    // ---- the rows' q: dims 16 k + 8 h ..
+    half8 qf[RT][NP][KS];
+    float c[RT];
+#pragma unroll
+    for (int q = 0; q < RT; q++) {
+        const uint32_t row = min(row0 + 32 * q + i32, rows - 1);
+        const uint8_t *qp = a.q + row / a.G * a.q_row + (size_t)(kvh * a.G + row % a.G) * HD * sizeof(T);
+        float v[KS][8], mx = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[k][e] = ld<T>(qp, 16 * k + 8 * h + e);
+                mx = fmaxf(mx, fabsf(v[k][e]));
+            }
+        // (the scale's sign goes into q: the largest product is the largest score)
+        float up = a.scale < 0.f ? -1.f : 1.f;
+        c[q] = fabsf(a.scale) * 1.44269504088896340736f;
+        if (NP > 1) {
+            mx = xor32_max(mx);
+            const uint32_t E = __float_as_uint(mx) >> 23;
+            if (E >= 8 && E <= 246) {
+                up *= __uint_as_float((254u - E) << 23);
+                c[q] *= __uint_as_float(E << 23);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float x = v[k][e] * up;
+#pragma unroll
+                for (int p = 0; p < NP; p++) {
+                    qf[q][p][k][e] = (_Float16)x;
+                    x -= (float)qf[q][p][k][e];
+                }
+            }
+    }
+    // ---- copies: wave w page w of a stage, 1 KB (1024 / ROWB rows) each
+    const uint32_t lds0 = lds_addr(lds);
+    uint32_t off[NI];
+#pragma unroll
+    for (uint32_t i = 0; i < NI; i++) {
+        const uint32_t r = i * (64 / PPR) + lane / PPR;
+        off[i] = r * ROWB + ((lane % PPR) ^ (r % PPR)) * 16;
+    }
+    const uint8_t *kh = (const uint8_t *)(a.kc + (size_t)kvh * a.cache_tokens * HD);
+    const uint8_t *vh = (const uint8_t *)(a.vc + (size_t)kvh * a.cache_tokens * HD);
+    uint32_t pages = 0;  // lane l: page 64 (stage / 16) + l of the part
+    bool bad = false;
+    auto issue = [&](uint32_t st) __attribute__((always_inline)) {
+        if (st % 16 == 0) {
+            pages = a.tables[min(t0 / 16 + st * 4 + lane, (t1 - 1) / 16)];
+            if (pages >= a.cache_tokens / 16) {
+                bad = true;
+                pages = 0;
+            }
+        }
+        const uint32_t pg = __builtin_amdgcn_readlane(pages, st % 16 * 4 + wave);
+        const uint64_t at = (uint64_t)pg * (16 * ROWB);
+        const uint32_t to = lds0 + st % ST_NS * STAGE + wave * (16 * ROWB);
+#pragma unroll
+        for (uint32_t i = 0; i < NI; i++) dma16_s(kh + at, off[i], to + i * 1024);
+#pragma unroll
+        for (uint32_t i = 0; i < NI; i++) dma16_s(vh + at, off[i], to + ST_NS * STAGE + i * 1024);
+    };
+    f32x16 o[RT][DT];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int q = 0; q < RT; q++) {
+        m[q] = -INFINITY;
+        l[q] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[q][d][r] = 0.f;
+    }
+    // fragment addresses in a stage (their k-step and 32-dim tile by exclusive or)
+    const uint32_t ka = i32 * ROWB + ((h ^ (i32 % PPR)) * 16);
+    const uint32_t l16 = lane % 16, vr = 4 * h + l16 / 4, vp = 2 * (lane / 16 % 2) + l16 % 4 / 2;
+    const uint32_t va = vr * ROWB + ((vp ^ (vr % PPR)) * 16) + 8 * (l16 % 2);
+    f32x16 s[RT];
+    // scores of the 32 tokens at 32 kt of stage st
+    auto scores = [&](uint32_t st, uint32_t kt, f32x16 (&d)[RT]) __attribute__((always_inline)) {
+        const uint8_t *ks = lds + st % ST_NS * STAGE + kt * 32 * ROWB;
+#pragma unroll
+        for (int q = 0; q < RT; q++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) d[q][r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const half8 kf = *(const half8 *)(ks + (ka ^ (k * 32)));
+#pragma unroll
+            for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                for (int q = 0; q < RT; q++)
+                    d[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[q][p][k], d[q], 0, 0, 0);
+        }
+    };
+    // the reference maximum for scores d (raw): moved, and the sums with it, where one passes it by 2^8
+    auto refer = [&](f32x16 (&d)[RT]) __attribute__((always_inline)) {
+        float mb[RT];
+        bool up = false;
+#pragma unroll
+        for (int q = 0; q < RT; q++) {
+            float x = d[q][0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) x = fmaxf(x, d[q][r]);
+            mb[q] = xor32_max(x) * c[q];
+            up = up || mb[q] > m[q] + 8.f;
+        }
+        if (__builtin_amdgcn_ballot_w64(up)) {
+#pragma unroll
+            for (int q = 0; q < RT; q++) {
+                const float mn = fmaxf(m[q], mb[q]);
+                const float f = __builtin_amdgcn_exp2f(m[q] - (mn == -INFINITY ? 0.f : mn));
+                m[q] = mn;
+                l[q] *= f;
+#pragma unroll
+                for (int d2 = 0; d2 < DT; d2++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[q][d2][r] *= f;
+            }
+        }
+    };
+    // tokens past the part: no score
+    auto mask = [&](uint32_t t, f32x16 (&d)[RT]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            if (t + 8 * (r / 4) + 4 * h + r % 4 >= t1)
+#pragma unroll
+                for (int q = 0; q < RT; q++) d[q][r] = -INFINITY;
+    };
+    for (uint32_t st = 0; st < 3 && st < nst; st++) issue(st);
+    if (nst > 2) wait_vm<5 * NI>();
+    else wait_vm<0>();
+    lds_bar();
+    if (mine) {
+        scores(0, 0, s);
+        if (t0 + 32 > t1) mask(t0, s);
+        refer(s);
+    }
+    for (uint32_t st = 0; st < nst; st++) {
+        // landed: this stage's V and the next one's K (issued K, V by stage)
+        if (st + 2 < nst) wait_vm<3 * NI>();
+        else if (st + 1 < nst) wait_vm<NI>();
+        else wait_vm<0>();
+        lds_bar();
+        if (st + 3 < nst) issue(st + 3);
+        const uint32_t tk = t0 + st * ST_KB;
+        uint8_t *vs = lds + (ST_NS + st % ST_NS) * STAGE;
+        if (tk + ST_KB > t1) {  // V of the tokens past the part: zero (0 times NaN is NaN)
+            for (uint32_t i = (t1 - tk) * ROWB + tid * 16; i < STAGE; i += 256 * 16) *(u32x4 *)(vs + i) = u32x4{0, 0, 0, 0};
+            lds_bar();
+        }
+        if (!mine) continue;
+#pragma unroll
+        for (uint32_t kt = 0; kt < 2; kt++) {
+            f32x16 sn[RT];
+            const bool more = kt == 0 || st + 1 < nst;
+            if (more) scores(st + kt, 1 - kt, sn);
+            half8 pf[RT][NP][2];
+#pragma unroll
+            for (int q = 0; q < RT; q++) {
+                const float b = m[q] == -INFINITY ? 0.f : 4.f - m[q];
+                float ls = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    float p = __builtin_amdgcn_exp2f(fmaf(s[q][r], c[q], b));
+                    ls += p;
+#pragma unroll
+                    for (int k = 0; k < NP; k++) {
+                        pf[q][k][r / 8][r % 8] = (_Float16)p;
+                        p -= (float)pf[q][k][r / 8][r % 8];
+                    }
+                }
+                l[q] += ls;
+            }
+#pragma unroll
+            for (int s2 = 0; s2 < 2; s2++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    // tokens 16 s2 + 4 h .. +3 and those 8 on (8 rows on, the piece's bit 3 flipped)
+                    uint8_t *v0 = vs + (32 * kt + 16 * s2) * ROWB + (va ^ (d * 64));
+                    uint8_t *v1 = vs + (32 * kt + 16 * s2 + 8) * ROWB + (va ^ (d * 64) ^ (PPR > 8 ? 128 : 0));
+                    const tr4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)v0);
+                    const tr4 y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)v1);
+                    const half8 vf = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
+                                      (_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                        for (int q = 0; q < RT; q++)
+                            o[q][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[q][p][s2], o[q][d], 0, 0, 0);
+                }
+            if (more) {
+                const uint32_t tn = tk + 32 * (kt + 1);
+                if (tn + 32 > t1) mask(tn, sn);
+                refer(sn);
+#pragma unroll
+                for (int q = 0; q < RT; q++) s[q] = sn[q];
+            }
+        }
+    }
+    if (bad) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+    if (!mine) return;
+#pragma unroll
+    for (int q = 0; q < RT; q++) {
+        const uint32_t row = row0 + 32 * q + i32;
+        const float lq = xor32_sum(l[q]);
+        if (row >= rows) continue;
+        const size_t pr = (size_t)part * a.n_seq * a.nh + (size_t)(row / a.G) * a.nh + kvh * a.G + row % a.G;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                *(f32x4 *)(a.part + pr * HD + 32 * d + 8 * g + 4 * h) =
+                    f32x4{o[q][d][4 * g], o[q][d][4 * g + 1], o[q][d][4 * g + 2], o[q][d][4 * g + 3]};
+        if (h == 0) {
+            a.stat[2 * pr] = m[q] - 4.f;
+            a.stat[2 * pr + 1] = lq;
+        }
+    }
+}
+
+// Joins the parts of a row, one wave each: the lanes take the parts' statistics,
+// 64 at a time, then every lane HD / 64 dims of all of them, 8 loads in flight.
 template <int HD, typename T>
-__global__ __launch_bounds__(64) void k_shared_join(SharedArgs a) {
-    const uint32_t row = blockIdx.x, s = row / a.nh, lane = threadIdx.x;
-    const uint32_t len = seq_len(a, s), rows = a.n_seq * a.nh;
-    const uint32_t p0 = len < a.prefix ? a.n_pre : 0u;  // (such a sequence has no part in the prefix)
-    constexpr int E = HD / 64;
+__global__ __launch_bounds__(256) void k_shared_join(SharedArgs a) {
+    constexpr int E = HD / 64, U = 8;
+    const uint32_t rows = a.n_seq * a.nh, lane = threadIdx.x & 63;
+    const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (row >= rows) return;
+    const uint32_t s = row / a.nh, len = seq_len(a, s);
+    // (a sequence shorter than the prefix has no part in it)
+    const uint32_t p0 = len < a.prefix ? a.n_pre : 0u, p1 = a.n_pre + a.n_own;
     float M = -INFINITY, L = 0.f, O[E];
 #pragma unroll
     for (int e = 0; e < E; e++) O[e] = 0.f;
-    for (uint32_t p = p0; p < a.n_pre + a.n_own; p++) M = fmaxf(M, a.stat[2 * ((size_t)p * rows + row)]);
-    const float Ms = M == -INFINITY ? 0.f : M;
-    for (uint32_t p = p0; p < a.n_pre + a.n_own; p++) {
-        const size_t pr = (size_t)p * rows + row;
-        const float f = __builtin_amdgcn_exp2f(a.stat[2 * pr] - Ms);
-        L = fmaf(a.stat[2 * pr + 1], f, L);
+    for (uint32_t b = p0; b < p1; b += 64) {
+        const uint32_t n = min(64u, p1 - b);
+        const float2 st = *(const float2 *)(a.stat + 2 * ((size_t)(b + min(lane, n - 1)) * rows + row));
+        const float mn = fmaxf(M, wave_max(st.x)), ms = mn == -INFINITY ? 0.f : mn;
+        const float old = __builtin_amdgcn_exp2f(M - ms), w = lane < n ? __builtin_amdgcn_exp2f(st.x - ms) : 0.f;
+        M = mn;
+        L = fmaf(L, old, wave_sum(lane < n ? st.y * w : 0.f));
 #pragma unroll
-        for (int e = 0; e < E; e++) O[e] = fmaf(a.part[pr * HD + E * lane + e], f, O[e]);
+        for (int e = 0; e < E; e++) O[e] *= old;
+        for (uint32_t p = 0; p < n; p += U) {
+            float v[U][E];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float *pp = a.part + ((size_t)(b + min(p + u, n - 1)) * rows + row) * HD + E * lane;
+#pragma unroll
+                for (int e = 0; e < E; e++) v[u][e] = pp[e];
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {  // (past the last part: its values again, weight 0)
+                const float f = lane_f(w, p + u);
+#pragma unroll
+                for (int e = 0; e < E; e++) O[e] = fmaf(v[u][e], f, O[e]);
+            }
+        }
     }
     uint8_t *op = a.out + s * a.out_row;
 #pragma unroll
@@ -301,7 +638,8 @@ __global__ __launch_bounds__(64) void k_shared_join(SharedArgs a) {
 
 // How a call is cut (the same for every call of these sizes).
 struct SharedPlan {
-    uint32_t n_pre, n_own, pre_tiles, pre_len, pre_blocks, blocks;
+    uint32_t n_pre, n_own, pre_tiles, pre_len, pre_blocks, blocks, qt;
+    uint32_t tile, pre_rows;
     uint64_t stat_off, bytes;  // of ws
 };
 
@@ -310,20 +648,26 @@ uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); 
 bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t prefix, uint32_t max_len,
                  SharedPlan &p) {
     const uint32_t G = nh / nkv, own = max_len - prefix;
-    p.pre_tiles = ceil_div((uint64_t)n_seq * G, SA_ROWS);
-    // parts: two workgroups per CU, at least 128 tokens each
-    auto cut = [&](uint64_t jobs, uint32_t tokens) {
-        const uint32_t most = ceil_div(tokens, 128), want = ceil_div(2ull * cus, jobs);
+    const uint64_t rows_kv = (uint64_t)n_seq * G;
+    // rows of a prefix workgroup: 128 or 256 on LDS tiles, or 16 or 32 streamed
+    p.tile = rows_kv >= SA_TILE ? (rows_kv > 128 && SA_RT > 1 ? 2 : 1) : 0;
+    p.qt = rows_kv <= 16 ? 1 : 2;
+    p.pre_rows = p.tile ? 128u * p.tile : p.qt * SA_ROWS;
+    p.pre_tiles = ceil_div(rows_kv, p.pre_rows);
+    // parts: `per` workgroups per CU, at least 128 tokens each
+    auto cut = [&](uint64_t jobs, uint32_t tokens, uint32_t per) {
+        const uint32_t most = ceil_div(tokens, 128), want = ceil_div((uint64_t)per * cus, jobs);
         return want < most ? want : most;
     };
     p.n_pre = 0;
     p.pre_len = 0;
     if (prefix) {
-        const uint32_t n = cut((uint64_t)p.pre_tiles * nkv, prefix);
-        p.pre_len = ceil_div(ceil_div(prefix, n), SA_KB) * SA_KB;
+        const uint32_t n = cut((uint64_t)p.pre_tiles * nkv, prefix, p.tile ? 1 : SA_PRE_PER);
+        const uint32_t step = p.tile ? ST_KB : SA_KB;
+        p.pre_len = ceil_div(ceil_div(prefix, n), step) * step;
         p.n_pre = ceil_div(prefix, p.pre_len);
     }
-    p.n_own = own || !prefix ? cut((uint64_t)n_seq * nkv, own ? own : 1) : 1u;
+    p.n_own = own || !prefix ? cut((uint64_t)n_seq * nkv, own ? own : 1, SA_OWN_PER) : 1u;
     if (p.n_own == 0) p.n_own = 1;
     const uint64_t pre = (uint64_t)p.n_pre * p.pre_tiles * nkv, all = pre + (uint64_t)p.n_own * n_seq * nkv;
     if (all > 0x7FFFFFFFull || (uint64_t)n_seq * nh > 0x7FFFFFFFull) return false;
@@ -390,12 +734,36 @@ extern "C" uint64_t zh_flash_decode_shared_ws(zh_ctx *c, const zh_kv_batch *kv, 
     return p.bytes ? p.bytes : 16;
 }
 
+template <int HD, int NP, int RT, typename T>
+static int tile_launch(zh_ctx *c, const SharedArgs &a, const SharedPlan &p) {
+    static bool attr = false;
+    if (!attr) {
+        ZH_HIP(c, hipFuncSetAttribute((const void *)k_shared_tile<HD, NP, RT, T>,
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)st_lds<HD>()));
+        attr = true;
+    }
+    hipLaunchKernelGGL((k_shared_tile<HD, NP, RT, T>), dim3(p.pre_blocks), dim3(256), st_lds<HD>(), c->stream, a);
+    ZH_LAUNCH_CHECK(c);
+    return ZH_OK;
+}
+
 template <int HD, int NP, typename T>
 static int shared_launch(zh_ctx *c, const SharedArgs &a, const SharedPlan &p) {
-    hipLaunchKernelGGL((k_shared_attn<HD, NP, T>), dim3(p.blocks), dim3(64 * SA_W), 0, c->stream, a);
+    SharedArgs b = a;
+    uint32_t blocks = p.blocks;
+    if (p.n_pre && p.tile) {
+        const int rc = p.tile == 2 ? tile_launch<HD, NP, 2, T>(c, a, p) : tile_launch<HD, NP, 1, T>(c, a, p);
+        if (rc) return rc;
+        b.pre_blocks = 0;
+        blocks -= p.pre_blocks;
+    }
+#define SA_L(QT) hipLaunchKernelGGL((k_shared_attn<HD, NP, QT, T>), dim3(blocks), dim3(64 * SA_W), 0, c->stream, b)
+    if (p.qt == 1 || !b.pre_blocks) SA_L(1);
+    else SA_L(2);
+#undef SA_L
     ZH_LAUNCH_CHECK(c);
     if (a.n_pre + a.n_own > 1) {
-        hipLaunchKernelGGL((k_shared_join<HD, T>), dim3(a.n_seq * a.nh), dim3(64), 0, c->stream, a);
+        hipLaunchKernelGGL((k_shared_join<HD, T>), dim3((a.n_seq * a.nh + 3) / 4), dim3(256), 0, c->stream, a);
         ZH_LAUNCH_CHECK(c);
     }
     return ZH_OK;
@@ -435,6 +803,7 @@ extern "C" int zh_flash_decode_shared(zh_ctx *c, const zh_kv_batch *kv, const zh
     a.pre_tiles = p.pre_tiles;
     a.pre_blocks = p.pre_blocks;
     a.pre_len = p.pre_len;
+    a.pre_rows = p.pre_rows;
     a.scale = r->attn_scale != 0.f ? r->attn_scale : 1.0f / sqrtf((float)kv->head_dim);
     if (kv->head_dim == 128)
         return size == 4 ? shared_launch<128, 2, float>(c, a, p) : shared_launch<128, 1, _Float16>(c, a, p);
