@@ -345,8 +345,9 @@ ZH_DEV void dma16_s(const void *base, uint32_t off, uint32_t lds) {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <int HD, int NP, int RT, typename T>
-__global__ __launch_bounds__(256, 1) void k_shared_tile(SharedArgs a) {
+template <int HD, int NP, int NW, typename T>
+__global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
+    constexpr int RT = 1;
     constexpr int KS = HD / 16, DT = HD / 32;       // k-steps of the scores, 32-dim tiles of the output
     constexpr uint32_t ROWB = HD * 2, PPR = HD / 8;  // bytes and 16-byte pieces of a row
     constexpr uint32_t STAGE = ST_KB * ROWB, NI = 16 * ROWB / 1024;  // bytes of a stage, copies of a page
@@ -358,7 +359,7 @@ __global__ __launch_bounds__(256, 1) void k_shared_tile(SharedArgs a) {
     // (the row tiles of one part and kv head on one XCD: they read the same K and V)
     const uint32_t per = a.nkv * a.n_pre, tile = blockIdx.x / per, kvh = blockIdx.x % per % a.nkv;
     const uint32_t part = blockIdx.x % per / a.nkv;
-    const uint32_t rows = a.n_seq * a.G, row0 = tile * (128 * RT) + wave * (32 * RT);
+    const uint32_t rows = a.n_seq * a.G, row0 = tile * (32 * RT * NW) + wave * (32 * RT);
     const bool mine = row0 < rows;  // (uniform per wave: it has rows)
     const uint32_t t0 = part * a.pre_len, t1 = min(t0 + a.pre_len, a.prefix);
     const uint32_t nst = (t1 - t0 + ST_KB - 1) / ST_KB;
@@ -400,7 +401,8 @@ __global__ __launch_bounds__(256, 1) void k_shared_tile(SharedArgs a) {
                 }
             }
     }
-    // ---- copies: wave w page w of a stage, 1 KB (1024 / ROWB rows) each
+    // ---- copies, 1 KB (1024 / ROWB rows) each: 4 waves a page of K and of V of a
+    // stage; 8 waves a page of one of them
     const uint32_t lds0 = lds_addr(lds);
     uint32_t off[NI];
 #pragma unroll
@@ -420,13 +422,33 @@ __global__ __launch_bounds__(256, 1) void k_shared_tile(SharedArgs a) {
                 pages = 0;
             }
         }
-        const uint32_t pg = __builtin_amdgcn_readlane(pages, st % 16 * 4 + wave);
+        const uint32_t pg = __builtin_amdgcn_readlane(pages, st % 16 * 4 + wave % 4);
         const uint64_t at = (uint64_t)pg * (16 * ROWB);
-        const uint32_t to = lds0 + st % ST_NS * STAGE + wave * (16 * ROWB);
+        const uint32_t to = lds0 + st % ST_NS * STAGE + wave % 4 * (16 * ROWB);
+        if (NW == 4 || wave < 4) {
 #pragma unroll
-        for (uint32_t i = 0; i < NI; i++) dma16_s(kh + at, off[i], to + i * 1024);
+            for (uint32_t i = 0; i < NI; i++) dma16_s(kh + at, off[i], to + i * 1024);
+        }
+        if (NW == 4 || wave >= 4) {
 #pragma unroll
-        for (uint32_t i = 0; i < NI; i++) dma16_s(vh + at, off[i], to + ST_NS * STAGE + i * 1024);
+            for (uint32_t i = 0; i < NI; i++) dma16_s(vh + at, off[i], to + ST_NS * STAGE + i * 1024);
+        }
+    };
+    // waits until this wave's copies of V of stage st and K of stage st + 1 have
+    // landed, those of the two stages after it issued (as far as there are any)
+    auto landed = [&](uint32_t st) __attribute__((always_inline)) {
+        if (NW == 4) {
+            if (st + 2 < nst) wait_vm<3 * NI>();
+            else if (st + 1 < nst) wait_vm<NI>();
+            else wait_vm<0>();
+        } else if (wave < 4) {
+            if (st + 2 < nst) wait_vm<NI>();
+            else wait_vm<0>();
+        } else {
+            if (st + 2 < nst) wait_vm<2 * NI>();
+            else if (st + 1 < nst) wait_vm<NI>();
+            else wait_vm<0>();
+        }
     };
     f32x16 o[RT][DT];
     float m[RT], l[RT];
@@ -443,49 +465,41 @@ __global__ __launch_bounds__(256, 1) void k_shared_tile(SharedArgs a) {
     const uint32_t ka = i32 * ROWB + ((h ^ (i32 % PPR)) * 16);
     const uint32_t l16 = lane % 16, vr = 4 * h + l16 / 4, vp = 2 * (lane / 16 % 2) + l16 % 4 / 2;
     const uint32_t va = vr * ROWB + ((vp ^ (vr % PPR)) * 16) + 8 * (l16 % 2);
-    f32x16 s[RT];
-    // scores of the 32 tokens at 32 kt of stage st
-    auto scores = [&](uint32_t st, uint32_t kt, f32x16 (&d)[RT]) __attribute__((always_inline)) {
+    f32x16 s[RT], sn[RT];  // scores of the current and the next 32 tokens (raw)
+    half8 kf[KS];          // K fragments of the next ones
+    auto load_k = [&](uint32_t st, uint32_t kt) __attribute__((always_inline)) {
         const uint8_t *ks = lds + st % ST_NS * STAGE + kt * 32 * ROWB;
 #pragma unroll
-        for (int q = 0; q < RT; q++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) d[q][r] = 0.f;
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const half8 kf = *(const half8 *)(ks + (ka ^ (k * 32)));
-#pragma unroll
-            for (int p = NP - 1; p >= 0; p--)
-#pragma unroll
-                for (int q = 0; q < RT; q++)
-                    d[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[q][p][k], d[q], 0, 0, 0);
-        }
+        for (int k = 0; k < KS; k++) kf[k] = *(const half8 *)(ks + (ka ^ (k * 32)));
     };
-    // the reference maximum for scores d (raw): moved, and the sums with it, where one passes it by 2^8
-    auto refer = [&](f32x16 (&d)[RT]) __attribute__((always_inline)) {
-        float mb[RT];
+    // the reference maximum for scores d: moved, and the sums with it, where one
+    // (largest: mx) passes it by 2^8
+    auto refer = [&](float (&mx)[RT]) __attribute__((always_inline)) {
         bool up = false;
 #pragma unroll
         for (int q = 0; q < RT; q++) {
-            float x = d[q][0];
-#pragma unroll
-            for (int r = 1; r < 16; r++) x = fmaxf(x, d[q][r]);
-            mb[q] = xor32_max(x) * c[q];
-            up = up || mb[q] > m[q] + 8.f;
+            mx[q] = xor32_max(mx[q]) * c[q];
+            up = up || mx[q] > m[q] + 8.f;
         }
         if (__builtin_amdgcn_ballot_w64(up)) {
 #pragma unroll
             for (int q = 0; q < RT; q++) {
-                const float mn = fmaxf(m[q], mb[q]);
+                const float mn = fmaxf(m[q], mx[q]);
                 const float f = __builtin_amdgcn_exp2f(m[q] - (mn == -INFINITY ? 0.f : mn));
                 m[q] = mn;
                 l[q] *= f;
 #pragma unroll
-                for (int d2 = 0; d2 < DT; d2++)
+                for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) o[q][d2][r] *= f;
+                    for (int r = 0; r < 16; r++) o[q][d][r] *= f;
             }
         }
+    };
+    auto largest = [&](const f32x16 &d) __attribute__((always_inline)) {
+        float x = d[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) x = fmaxf(x, d[r]);
+        return x;
     };
     // tokens past the part: no score
     auto mask = [&](uint32_t t, f32x16 (&d)[RT]) __attribute__((always_inline)) {
@@ -496,52 +510,65 @@ __global__ __launch_bounds__(256, 1) void k_shared_tile(SharedArgs a) {
                 for (int q = 0; q < RT; q++) d[q][r] = -INFINITY;
     };
     for (uint32_t st = 0; st < 3 && st < nst; st++) issue(st);
-    if (nst > 2) wait_vm<5 * NI>();
+    if (nst > 2) wait_vm<(NW == 4 ? 5 : 2) * NI>();  // K of stage 0
     else wait_vm<0>();
     lds_bar();
     if (mine) {
-        scores(0, 0, s);
+        load_k(0, 0);
+#pragma unroll
+        for (int q = 0; q < RT; q++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[q][r] = 0.f;
+#pragma unroll
+            for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+                    s[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[q][p][k], s[q], 0, 0, 0);
+        }
+        load_k(0, 1);
         if (t0 + 32 > t1) mask(t0, s);
-        refer(s);
+        float mx[RT];
+#pragma unroll
+        for (int q = 0; q < RT; q++) mx[q] = largest(s[q]);
+        refer(mx);
     }
+    constexpr int PAIRS = 8 * RT, EARLY = 3 * PAIRS / 4;  // weights in pairs; those taken beside the scores' products
     for (uint32_t st = 0; st < nst; st++) {
-        // landed: this stage's V and the next one's K (issued K, V by stage)
-        if (st + 2 < nst) wait_vm<3 * NI>();
-        else if (st + 1 < nst) wait_vm<NI>();
-        else wait_vm<0>();
+        landed(st);
         lds_bar();
         if (st + 3 < nst) issue(st + 3);
         const uint32_t tk = t0 + st * ST_KB;
         uint8_t *vs = lds + (ST_NS + st % ST_NS) * STAGE;
         if (tk + ST_KB > t1) {  // V of the tokens past the part: zero (0 times NaN is NaN)
-            for (uint32_t i = (t1 - tk) * ROWB + tid * 16; i < STAGE; i += 256 * 16) *(u32x4 *)(vs + i) = u32x4{0, 0, 0, 0};
+            for (uint32_t i = (t1 - tk) * ROWB + tid * 16; i < STAGE; i += 64 * NW * 16) *(u32x4 *)(vs + i) = u32x4{0, 0, 0, 0};
             lds_bar();
         }
         if (!mine) continue;
 #pragma unroll
         for (uint32_t kt = 0; kt < 2; kt++) {
-            f32x16 sn[RT];
-            const bool more = kt == 0 || st + 1 < nst;
-            if (more) scores(st + kt, 1 - kt, sn);
-            half8 pf[RT][NP][2];
+            half8 pf[RT][NP][2], vf[2][DT];
+            float b[RT], mx[RT];
 #pragma unroll
             for (int q = 0; q < RT; q++) {
-                const float b = m[q] == -INFINITY ? 0.f : 4.f - m[q];
-                float ls = 0.f;
+                b[q] = m[q] == -INFINITY ? 0.f : 4.f - m[q];
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    float p = __builtin_amdgcn_exp2f(fmaf(s[q][r], c[q], b));
-                    ls += p;
+                for (int r = 0; r < 16; r++) sn[q][r] = 0.f;
+            }
+            // weights 2 i and 2 i + 1 (by 16-token product, then row tile)
+            auto weights = [&](int i) __attribute__((always_inline)) {
+                const int s2 = i / (4 * RT), q = i / 4 % RT, r0 = 2 * (i % 4);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float p = __builtin_amdgcn_exp2f(fmaf(s[q][8 * s2 + r0 + e], c[q], b[q]));
+                    l[q] += p;
 #pragma unroll
                     for (int k = 0; k < NP; k++) {
-                        pf[q][k][r / 8][r % 8] = (_Float16)p;
-                        p -= (float)pf[q][k][r / 8][r % 8];
+                        pf[q][k][s2][r0 + e] = (_Float16)p;
+                        p -= (float)pf[q][k][s2][r0 + e];
                     }
                 }
-                l[q] += ls;
-            }
-#pragma unroll
-            for (int s2 = 0; s2 < 2; s2++)
+            };
+            auto load_v = [&](int s2) __attribute__((always_inline)) {
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
                     // tokens 16 s2 + 4 h .. +3 and those 8 on (8 rows on, the piece's bit 3 flipped)
@@ -549,21 +576,58 @@ __global__ __launch_bounds__(256, 1) void k_shared_tile(SharedArgs a) {
                     uint8_t *v1 = vs + (32 * kt + 16 * s2 + 8) * ROWB + (va ^ (d * 64) ^ (PPR > 8 ? 128 : 0));
                     const tr4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)v0);
                     const tr4 y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)v1);
-                    const half8 vf = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
+                    vf[s2][d] = half8{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
                                       (_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
-#pragma unroll
-                    for (int p = NP - 1; p >= 0; p--)
-#pragma unroll
-                        for (int q = 0; q < RT; q++)
-                            o[q][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[q][p][s2], o[q][d], 0, 0, 0);
                 }
-            if (more) {
-                const uint32_t tn = tk + 32 * (kt + 1);
-                if (tn + 32 > t1) mask(tn, sn);
-                refer(sn);
+            };
+            // three runs of products, each group of them (64 cycles) with vector
+            // work that does not need it; the order is pinned by the barriers
+            load_v(0);
 #pragma unroll
-                for (int q = 0; q < RT; q++) s[q] = sn[q];
+            for (int k = 0; k < KS; k++) {
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                    for (int q = 0; q < RT; q++)
+                        sn[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[q][p][k], sn[q], 0, 0, 0);
+#pragma unroll
+                for (int i = EARLY * k / KS; i < EARLY * (k + 1) / KS; i++) weights(i);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            load_v(1);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                    for (int q = 0; q < RT; q++)
+                        o[q][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][d], pf[q][p][0], o[q][d], 0, 0, 0);
+#pragma unroll
+                for (int i = EARLY + (PAIRS - EARLY) * d / DT; i < EARLY + (PAIRS - EARLY) * (d + 1) / DT; i++) weights(i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            load_k(st + 1, kt);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                    for (int q = 0; q < RT; q++)
+                        o[q][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[1][d], pf[q][p][1], o[q][d], 0, 0, 0);
+                if (d < RT) mx[d] = largest(sn[d]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (kt == 0 || st + 1 < nst) {  // (after the last tokens the scores are of nothing)
+                const uint32_t tn = tk + 32 * (kt + 1);
+                if (tn + 32 > t1) {
+                    mask(tn, sn);
+#pragma unroll
+                    for (int q = 0; q < RT; q++) mx[q] = largest(sn[q]);
+                }
+                refer(mx);
+            }
+#pragma unroll
+            for (int q = 0; q < RT; q++) s[q] = sn[q];
         }
     }
     if (bad) atomicOr(a.err, ZH_DEVERR_KV_ROW);
@@ -734,15 +798,15 @@ extern "C" uint64_t zh_flash_decode_shared_ws(zh_ctx *c, const zh_kv_batch *kv, 
     return p.bytes ? p.bytes : 16;
 }
 
-template <int HD, int NP, int RT, typename T>
+template <int HD, int NP, int NW, typename T>
 static int tile_launch(zh_ctx *c, const SharedArgs &a, const SharedPlan &p) {
     static bool attr = false;
     if (!attr) {
-        ZH_HIP(c, hipFuncSetAttribute((const void *)k_shared_tile<HD, NP, RT, T>,
+        ZH_HIP(c, hipFuncSetAttribute((const void *)k_shared_tile<HD, NP, NW, T>,
                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)st_lds<HD>()));
         attr = true;
     }
-    hipLaunchKernelGGL((k_shared_tile<HD, NP, RT, T>), dim3(p.pre_blocks), dim3(256), st_lds<HD>(), c->stream, a);
+    hipLaunchKernelGGL((k_shared_tile<HD, NP, NW, T>), dim3(p.pre_blocks), dim3(64 * NW), st_lds<HD>(), c->stream, a);
     ZH_LAUNCH_CHECK(c);
     return ZH_OK;
 }
@@ -752,7 +816,7 @@ static int shared_launch(zh_ctx *c, const SharedArgs &a, const SharedPlan &p) {
     SharedArgs b = a;
     uint32_t blocks = p.blocks;
     if (p.n_pre && p.tile) {
-        const int rc = p.tile == 2 ? tile_launch<HD, NP, 2, T>(c, a, p) : tile_launch<HD, NP, 1, T>(c, a, p);
+        const int rc = p.tile == 2 ? tile_launch<HD, NP, 8, T>(c, a, p) : tile_launch<HD, NP, 4, T>(c, a, p);
         if (rc) return rc;
         b.pre_blocks = 0;
         blocks -= p.pre_blocks;
