@@ -337,6 +337,13 @@ constexpr uint32_t ST_KB = 64, ST_NS = 4;
 template <int HD>
 constexpr uint32_t st_lds() { return 2 * ST_NS * ST_KB * HD * 2; }
 
+// Of 16 pieces a row: rows 4 apart differ in the low bits, rows 1 apart in the
+// high ones; of 8 (two rows side by side in the banks) the same of row pairs.
+template <uint32_t PPR>
+ZH_DEV uint32_t st_swz(uint32_t row) {
+    return PPR == 16 ? (row & 3) * 4 + (row / 4 & 3) : (row / 2 & 1) * 4 + (row / 4 & 3);
+}
+
 // 16 bytes per lane from base + off to LDS at the wave-uniform address + 16 lane.
 ZH_DEV void dma16_s(const void *base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
@@ -408,7 +415,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
 #pragma unroll
     for (uint32_t i = 0; i < NI; i++) {
         const uint32_t r = i * (64 / PPR) + lane / PPR;
-        off[i] = r * ROWB + ((lane % PPR) ^ (r % PPR)) * 16;
+        off[i] = r * ROWB + ((lane % PPR) ^ st_swz<PPR>(r)) * 16;
     }
     const uint8_t *kh = (const uint8_t *)(a.kc + (size_t)kvh * a.cache_tokens * HD);
     const uint8_t *vh = (const uint8_t *)(a.vc + (size_t)kvh * a.cache_tokens * HD);
@@ -462,9 +469,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
             for (int r = 0; r < 16; r++) o[q][d][r] = 0.f;
     }
     // fragment addresses in a stage (their k-step and 32-dim tile by exclusive or)
-    const uint32_t ka = i32 * ROWB + ((h ^ (i32 % PPR)) * 16);
+    const uint32_t ka = i32 * ROWB + ((h ^ st_swz<PPR>(i32)) * 16);
     const uint32_t l16 = lane % 16, vr = 4 * h + l16 / 4, vp = 2 * (lane / 16 % 2) + l16 % 4 / 2;
-    const uint32_t va = vr * ROWB + ((vp ^ (vr % PPR)) * 16) + 8 * (l16 % 2);
+    const uint32_t va = vr * ROWB + ((vp ^ st_swz<PPR>(vr)) * 16) + 8 * (l16 % 2);
     f32x16 s[RT], sn[RT];  // scores of the current and the next 32 tokens (raw)
     half8 kf[KS];          // K fragments of the next ones
     auto load_k = [&](uint32_t st, uint32_t kt) __attribute__((always_inline)) {
@@ -571,9 +578,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
             auto load_v = [&](int s2) __attribute__((always_inline)) {
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
-                    // tokens 16 s2 + 4 h .. +3 and those 8 on (8 rows on, the piece's bit 3 flipped)
+                    // tokens 16 s2 + 4 h .. +3 and those 8 on (8 rows on, the piece's bit 1 flipped)
                     uint8_t *v0 = vs + (32 * kt + 16 * s2) * ROWB + (va ^ (d * 64));
-                    uint8_t *v1 = vs + (32 * kt + 16 * s2 + 8) * ROWB + (va ^ (d * 64) ^ (PPR > 8 ? 128 : 0));
+                    uint8_t *v1 = vs + (32 * kt + 16 * s2 + 8) * ROWB + (va ^ (d * 64) ^ 32);
                     const tr4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)v0);
                     const tr4 y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)v1);
                     vf[s2][d] = half8{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
