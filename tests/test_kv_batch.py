@@ -290,10 +290,18 @@ def test_decode_accepted():
 
 @pytest.mark.parametrize("over", [
     dict(n_heads=0), dict(n_heads=5), dict(n_heads=34), dict(max_len=0), dict(prefix_len=129), dict(q_off=16),
-    dict(q_off=4), dict(q_stride=6 * HD - 4), dict(out_stride=6 * HD + 2), dict(seq_lens=Fake(16)), dict(ws=Fake(64)),
-    dict(ws=None), dict(out=None), dict(q=None)], ids=str)
+    dict(q_off=4), dict(q_stride=6 * HD - 4), dict(out_stride=6 * HD + 2), dict(seq_lens=Fake(16)), dict(out=None),
+    dict(q=None)], ids=str)
 def test_bad_decode(over):
     assert decode_check(batch(), decode(**over)) == INVALID
+
+
+def test_bad_decode_workspace():
+    """Refused where the call works in parts; a call of one part needs none."""
+    kv = batch(table_stride=1024, tables=Fake(4 * SEQS * 1024))
+    for ws in (None, Fake(64)):
+        assert decode_check(kv, decode(max_len=16000, ws=ws)) == INVALID
+        assert decode_check(kv, decode(max_len=16000, prefix_len=0, ws=ws)) == INVALID
 
 
 def test_bad_decode_rest():

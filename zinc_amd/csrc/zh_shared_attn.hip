@@ -27,14 +27,17 @@ constexpr int SA_W = 4;           // waves of a workgroup, each on its own steps
 #ifndef SA_TILE
 #define SA_TILE 96
 #endif
+#ifndef SA_ONE
+#define SA_ONE 512
+#endif
 #ifndef SA_RT
 #define SA_RT 2
 #endif
 #ifndef SA_PRE_PER
-#define SA_PRE_PER 2
+#define SA_PRE_PER 1
 #endif
 #ifndef SA_OWN_PER
-#define SA_OWN_PER 8
+#define SA_OWN_PER 4
 #endif
 
 struct SharedArgs {
@@ -50,7 +53,7 @@ struct SharedArgs {
     uint32_t n_pre, n_own;           // parts of the prefix and of a sequence's own tokens
     uint32_t pre_tiles, pre_blocks;  // row tiles per kv head, workgroups of the prefix
     uint32_t pre_len;                // tokens of a prefix part (a multiple of SA_KB)
-    uint32_t pre_rows;               // rows of a prefix workgroup
+    uint32_t own_len;                // tokens of a sequence's own part, at least
     float scale;
 };
 
@@ -60,14 +63,29 @@ ZH_DEV uint32_t seq_len(const SharedArgs &a, uint32_t s) {
     return min(a.lens[s], a.max_len);
 }
 
-template <typename T>
-ZH_DEV float ld(const uint8_t *p, uint32_t i) {
-    return sizeof(T) == 4 ? ((const float *)p)[i] : (float)((const _Float16 *)p)[i];
+// 8 elements of a row (16-byte aligned) as floats.
+ZH_DEV void ld8(const float *p, float (&v)[8]) {
+    const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+ZH_DEV void ld8(const _Float16 *p, float (&v)[8]) {
+    const half8 a = *(const half8 *)p;
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (float)a[e];
 }
 
-// One workgroup: up to 16 QT rows of one kv head over the tokens of one part.
-// Each wave takes steps of 32 tokens by itself, K and V straight from the cache
-// into the matrix operands' registers (no LDS, no barrier before the end):
+// What a workgroup of k_shared_attn does: rows row0 .. of one kv head (numbered
+// s * G + g), tokens [t0, t1) through table row `tab`, after the tokens [0, first)
+// through table row 0 (a sequence's whole context in one workgroup).
+struct SharedPart {
+    uint32_t part, row0, nrow, t0, t1, tab, first;
+};
+
+// 16 rows of one kv head. Each wave takes steps of 32 tokens by itself, K and V
+// straight from the cache into the matrix operands' registers (no LDS, no barrier
+// before the end), the next step's K requested when the scores are done and its V
+// after the products with this one's:
 //   S^T = K q^T (tokens x rows): lane (li = lane % 16, lg = lane / 16) holds
 //   tokens 16 j + 4 lg + r of row li, so that a row's maximum is in-lane plus
 //   two lane exchanges, and its weights lie as the second product's operand
@@ -76,234 +94,247 @@ ZH_DEV float ld(const uint8_t *p, uint32_t i) {
 //   permutes; column li of the output tile n is dim HD/16 li + n.
 // NP pieces: q (scaled by a power of two to a maximum in [1, 2)) and P as sums
 // of NP fp16 values; 2 keep 22 bits of each.
-struct SharedPart {
-    uint32_t part, row0, nrow, t0, t1, tab;  // rows row0 .. (s * G + g), tokens [t0, t1) through table `tab`
-};
-
-template <int HD, int NP, int QT, typename T>
+template <int HD, int NP, typename T>
 ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, float *lds) {
     constexpr int K4 = HD / 32, ND = HD / 16;  // k-steps of the scores, dims per lane and output tiles
     constexpr int LD = HD + 4;
     float *const so = lds, *const sm = lds + SA_W * SA_ROWS * LD, *const sl = sm + SA_W * SA_ROWS;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t li = lane % 16, lg = lane / 16;
-    const uint32_t t0 = w.t0, t1 = w.t1;
-    const uint32_t ta = t0 & ~15u;  // steps start on a page; tokens before t0 are masked
-    const uint32_t nstep = t1 > t0 ? (t1 - ta + SA_KB - 1) / SA_KB : 0u;
-    // the rows' q as operand fragments: dims 32 k4 + 8 lg ..
-    half8 qf[QT][NP][K4];
-    float c[QT];  // scores in base 2
-#pragma unroll
-    for (int q = 0; q < QT; q++) {
-        const uint32_t row = w.row0 + min(16u * q + li, w.nrow - 1), rs = row / a.G, rh = kvh * a.G + row % a.G;
-        const uint8_t *qp = a.q + rs * a.q_row + (size_t)rh * HD * sizeof(T);
-        float v[K4][8], mx = 0.f;
-#pragma unroll
-        for (int k4 = 0; k4 < K4; k4++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                v[k4][e] = ld<T>(qp, 32 * k4 + 8 * lg + e);
-                mx = fmaxf(mx, fabsf(v[k4][e]));
-            }
-        float up = 1.f;
-        c[q] = a.scale * 1.44269504088896340736f;
-        if (NP > 1) {
-            mx = xor32_max(xor16_max(mx));
-            // 2^-E for a maximum in [2^E, 2^(E+1)) (not for zero, infinite or tiny rows)
-            const uint32_t E = __float_as_uint(mx) >> 23;
-            if (E >= 8 && E <= 246) {
-                up = __uint_as_float((254u - E) << 23);
-                c[q] *= __uint_as_float(E << 23);
-            }
-        }
-#pragma unroll
-        for (int k4 = 0; k4 < K4; k4++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float x = v[k4][e] * up;
-#pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    qf[q][p][k4][e] = (_Float16)x;
-                    x -= (float)qf[q][p][k4][e];
-                }
-            }
-    }
-    floatx4 o[QT][ND];
-    float m[QT], l[QT];  // the row's maximum (every lg alike), this lane's share of its sum
-#pragma unroll
-    for (int q = 0; q < QT; q++) {
-        m[q] = -INFINITY;
-        l[q] = 0.f;
-#pragma unroll
-        for (int n = 0; n < ND; n++) o[q][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
+    // steps start on a page; tokens outside their range are masked
+    const uint32_t n0 = (w.first + SA_KB - 1) / SA_KB, ta = w.t0 & ~15u;
+    const uint32_t nstep = n0 + (w.t1 > w.t0 ? (w.t1 - ta + SA_KB - 1) / SA_KB : 0u);
     const uint16_t *kh = a.kc + (size_t)kvh * a.cache_tokens * HD, *vh = a.vc + (size_t)kvh * a.cache_tokens * HD;
-    const uint32_t *tb = a.tables + (size_t)w.tab * a.stride;
     bool bad = false;
-    for (uint32_t st = wave; st < nstep; st += SA_W) {
-        const uint32_t tk = ta + st * SA_KB;
-        // the step's two pages (the second clamped to the part's last)
-        uint32_t pg[2];
+    // a step's tokens [lo, hi) from tk on, and its two pages (the second clamped to the last of the range)
+    struct Step {
+        uint32_t tk, lo, hi, pg[2];
+    };
+    auto step = [&](uint32_t st) __attribute__((always_inline)) {
+        Step x;
+        const bool f = st < n0;
+        x.tk = f ? st * SA_KB : ta + (st - n0) * SA_KB;
+        x.lo = f ? 0u : w.t0;
+        x.hi = f ? w.first : w.t1;
+        const uint32_t *tb = a.tables + (f ? (size_t)0 : (size_t)w.tab * a.stride);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            pg[j] = tb[min(tk / 16 + j, (t1 - 1) / 16)];
-            if (pg[j] >= a.cache_tokens / 16) {
+            x.pg[j] = tb[min(x.tk / 16 + j, (x.hi - 1) / 16)];
+            if (x.pg[j] >= a.cache_tokens / 16) {
                 bad = true;
-                pg[j] = 0;
+                x.pg[j] = 0;
             }
         }
-        half8 kf[2][K4];
-        uint32_t pv[2][4][ND / 2];
+        return x;
+    };
+    half8 kf[2][K4];
+    uint32_t pv[2][4][ND / 2];
+    auto load_k = [&](const Step &x) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const uint16_t *kp = kh + ((size_t)pg[j] * 16 + li) * HD + 8 * lg;
+            const uint16_t *kp = kh + ((size_t)x.pg[j] * 16 + li) * HD + 8 * lg;
 #pragma unroll
             for (int k4 = 0; k4 < K4; k4++) kf[j][k4] = *(const half8 *)(kp + 32 * k4);
-            const uint16_t *vp = vh + ((size_t)pg[j] * 16 + 4 * lg) * HD + ND * li;
+        }
+    };
+    auto load_v = [&](const Step &x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint16_t *vp = vh + ((size_t)x.pg[j] * 16 + 4 * lg) * HD + ND * li;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 if (ND == 8) *(u32x4 *)pv[j][r] = *(const u32x4 *)(vp + r * HD);
                 else *(u32x2 *)pv[j][r] = *(const u32x2 *)(vp + r * HD);
             }
         }
-        const bool whole = tk >= t0 && tk + SA_KB <= t1;
-        half8 pf[QT][NP];
-        float f[QT];
+    };
+    Step x = {};
+    if (wave < nstep) {
+        x = step(wave);
+        load_k(x);
+        load_v(x);
+    }
+    // the row's q as operand fragments: dims 32 k4 + 8 lg ..
+    half8 qf[NP][K4];
+    float c = a.scale * 1.44269504088896340736f;  // scores in base 2
+    {
+        const uint32_t row = w.row0 + min(li, w.nrow - 1), rs = row / a.G, rh = kvh * a.G + row % a.G;
+        const T *qp = (const T *)(a.q + rs * a.q_row) + (size_t)rh * HD + 8 * lg;
+        float v[K4][8], mx = 0.f;
 #pragma unroll
-        for (int q = 0; q < QT; q++) {
-            float s[2][4], mb = -INFINITY;
+        for (int k4 = 0; k4 < K4; k4++) {
+            ld8(qp + 32 * k4, v[k4]);
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                floatx4 d = {0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k4][e]));
+        }
+        float up = 1.f;
+        if (NP > 1) {
+            mx = xor32_max(xor16_max(mx));
+            // 2^-E for a maximum in [2^E, 2^(E+1)) (not for zero, infinite or tiny rows)
+            const uint32_t E = __float_as_uint(mx) >> 23;
+            if (E >= 8 && E <= 246) {
+                up = __uint_as_float((254u - E) << 23);
+                c *= __uint_as_float(E << 23);
+            }
+        }
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
+        for (int k4 = 0; k4 < K4; k4++)
 #pragma unroll
-                    for (int k4 = 0; k4 < K4; k4++)
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[j][k4], qf[q][p][k4], d, 0, 0, 0);
+            for (int e = 0; e < 8; e++) {
+                float y = v[k4][e] * up;
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    s[j][r] = d[r] * c[q];
-                    if (!whole) {
-                        const uint32_t t = tk + 16 * j + 4 * lg + r;
-                        if (t < t0 || t >= t1) s[j][r] = -INFINITY;
-                    }
-                    mb = fmaxf(mb, s[j][r]);
+                for (int p = 0; p < NP; p++) {
+                    qf[p][k4][e] = (_Float16)y;
+                    y -= (float)qf[p][k4][e];
                 }
             }
-            mb = xor32_max(xor16_max(mb));
-            // (weights up to 2^8, away from fp16's subnormals)
-            const float mn = fmaxf(m[q], mb - 8.f), ms = mn == -INFINITY ? 0.f : mn;
-            f[q] = __builtin_amdgcn_exp2f(m[q] - ms);  // (m = -inf: 0)
-            m[q] = mn;
-            float ls = 0.f;
+    }
+    floatx4 o[ND];
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+    for (int n = 0; n < ND; n++) o[n] = floatx4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;  // the row's maximum (every lg alike), this lane's share of its sum
+    for (uint32_t st = wave; st < nstep; st += SA_W) {
+        const bool more = st + SA_W < nstep;
+        Step nx = x;
+        if (more) nx = step(st + SA_W);
+        const bool whole = x.tk >= x.lo && x.tk + SA_KB <= x.hi;
+        float s[2][4], mb = -INFINITY;
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float p = __builtin_amdgcn_exp2f(s[j][r] - ms);
-                    ls += p;
+        for (int j = 0; j < 2; j++) {
+            floatx4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < NP; k++) {
-                        pf[q][k][4 * j + r] = (_Float16)p;
-                        p -= (float)pf[q][k][4 * j + r];
+            for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                for (int k4 = 0; k4 < K4; k4++)
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[j][k4], qf[p][k4], d, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                s[j][r] = d[r] * c;
+                if (!whole) {
+                    // a token outside the range: no score, and no V (0 times
+                    // what the cache holds there may be NaN)
+                    const uint32_t t = x.tk + 16 * j + 4 * lg + r;
+                    if (t < x.lo || t >= x.hi) {
+                        s[j][r] = -INFINITY;
+#pragma unroll
+                        for (int y = 0; y < ND / 2; y++) pv[j][r][y] = 0u;
                     }
                 }
-            l[q] = fmaf(l[q], f[q], ls);
+                mb = fmaxf(mb, s[j][r]);
+            }
         }
-        if (!whole) {
-            // no V of a token outside the part (0 times what the cache holds there may be NaN)
+        if (more) load_k(nx);
+        mb = xor32_max(xor16_max(mb));
+        // (weights up to 2^8, away from fp16's subnormals)
+        const float mn = fmaxf(m, mb - 8.f), ms = mn == -INFINITY ? 0.f : mn;
+        const float f = __builtin_amdgcn_exp2f(m - ms);  // (m = -inf: 0)
+        m = mn;
+        half8 pf[NP];
+        float ls = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+        for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const uint32_t t = tk + 16 * j + 4 * lg + r;
+            for (int r = 0; r < 4; r++) {
+                float p = __builtin_amdgcn_exp2f(s[j][r] - ms);
+                ls += p;
 #pragma unroll
-                    for (int x = 0; x < ND / 2; x++) pv[j][r][x] = t < t0 || t >= t1 ? 0u : pv[j][r][x];
+                for (int k = 0; k < NP; k++) {
+                    pf[k][4 * j + r] = (_Float16)p;
+                    p -= (float)pf[k][4 * j + r];
                 }
-        }
+            }
+        l = fmaf(l, f, ls);
 #pragma unroll
         for (int n = 0; n < ND; n++) {
-            uint32_t x[4];
+            uint32_t y[4];
 #pragma unroll
             for (int i = 0; i < 4; i++)  // tokens 2 i, 2 i + 1 of the operand: their halfs of dim n
-                x[i] = __builtin_amdgcn_perm(pv[i >> 1][2 * (i & 1) + 1][n >> 1], pv[i >> 1][2 * (i & 1)][n >> 1],
+                y[i] = __builtin_amdgcn_perm(pv[i >> 1][2 * (i & 1) + 1][n >> 1], pv[i >> 1][2 * (i & 1)][n >> 1],
                                              (n & 1) ? 0x07060302u : 0x05040100u);
-            const u32x4 xv = {x[0], x[1], x[2], x[3]};
-            const half8 vf = __builtin_bit_cast(half8, xv);
+            const u32x4 yv = {y[0], y[1], y[2], y[3]};
+            const half8 vf = __builtin_bit_cast(half8, yv);
 #pragma unroll
-            for (int q = 0; q < QT; q++) {
+            for (int r = 0; r < 4; r++) o[n][r] *= f;
 #pragma unroll
-                for (int r = 0; r < 4; r++) o[q][n][r] *= f[q];
-#pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
-                    o[q][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[q][p], o[q][n], 0, 0, 0);
-            }
+            for (int p = NP - 1; p >= 0; p--) o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[p], o[n], 0, 0, 0);
         }
+        if (more) load_v(nx);
+        x = nx;
     }
     if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
-    // ---- join the waves, 16 rows at a time; lane li, lg: row li, dims ND (4 lg + r) + n
+    // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
     const bool direct = a.n_pre + a.n_own == 1;
+    l = xor32_sum(xor16_sum(l));
 #pragma unroll
-    for (int q = 0; q < QT; q++) {
-        if (16u * q >= w.nrow) break;  // uniform
-        if (q) __syncthreads();
-        const float lq = xor32_sum(xor16_sum(l[q]));
+    for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int n = 0; n < ND; n += 4)
+            *(f32x4 *)(so + (wave * SA_ROWS + li) * LD + ND * (4 * lg + r) + n) =
+                f32x4{o[n][r], o[n + 1][r], o[n + 2][r], o[n + 3][r]};
+    if (lg == 0) {
+        sm[wave * SA_ROWS + li] = m;
+        sl[wave * SA_ROWS + li] = l;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < w.nrow * (HD / 4); i += 64 * SA_W) {
+        const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4, R = w.row0 + r, s = R / a.G, h = kvh * a.G + R % a.G;
+        float M = sm[r], L = 0.f;
+        f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int n = 0; n < ND; n++) so[(wave * SA_ROWS + li) * LD + ND * (4 * lg + r) + n] = o[q][n][r];
-        if (lg == 0) {
-            sm[wave * SA_ROWS + li] = m[q];
-            sl[wave * SA_ROWS + li] = lq;
+        for (int k = 1; k < SA_W; k++) M = fmaxf(M, sm[k * SA_ROWS + r]);
+        const float Ms = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int k = 0; k < SA_W; k++) {
+            const float fk = __builtin_amdgcn_exp2f(sm[k * SA_ROWS + r] - Ms);
+            const f32x4 v = *(const f32x4 *)(so + (k * SA_ROWS + r) * LD + d);
+            O.x = fmaf(v.x, fk, O.x);
+            O.y = fmaf(v.y, fk, O.y);
+            O.z = fmaf(v.z, fk, O.z);
+            O.w = fmaf(v.w, fk, O.w);
+            L = fmaf(sl[k * SA_ROWS + r], fk, L);
         }
-        __syncthreads();
-        const uint32_t nr = min(SA_ROWS, w.nrow - 16 * q);
-        for (uint32_t i = tid; i < nr * HD; i += 64 * SA_W) {
-            const uint32_t r = i / HD, d = i % HD, R = w.row0 + 16 * q + r, s = R / a.G, h = kvh * a.G + R % a.G;
-            float M = sm[r], O = 0.f, L = 0.f;
-#pragma unroll
-            for (int k = 1; k < SA_W; k++) M = fmaxf(M, sm[k * SA_ROWS + r]);
-            const float Ms = M == -INFINITY ? 0.f : M;
-#pragma unroll
-            for (int k = 0; k < SA_W; k++) {
-                const float fk = __builtin_amdgcn_exp2f(sm[k * SA_ROWS + r] - Ms);
-                O = fmaf(so[(k * SA_ROWS + r) * LD + d], fk, O);
-                L = fmaf(sl[k * SA_ROWS + r], fk, L);
-            }
-            if (direct) {
-                const float v = t1 > t0 ? O / L : 0.f;
-                uint8_t *op = a.out + s * a.out_row;
-                if (sizeof(T) == 4) ((float *)op)[h * HD + d] = v;
-                else ((_Float16 *)op)[h * HD + d] = (_Float16)v;
-            } else {
-                const size_t pr = (size_t)w.part * a.n_seq * a.nh + (size_t)s * a.nh + h;
-                a.part[pr * HD + d] = O;
-                if (d == 0) {
-                    a.stat[2 * pr] = M;
-                    a.stat[2 * pr + 1] = L;
-                }
+        if (direct) {
+            const f32x4 v = nstep ? f32x4{O.x / L, O.y / L, O.z / L, O.w / L} : f32x4{0.f, 0.f, 0.f, 0.f};
+            T *op = (T *)(a.out + s * a.out_row) + h * HD + d;
+            if constexpr (sizeof(T) == 4) *(f32x4 *)op = v;
+            else *(half4 *)op = half4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+        } else {
+            const size_t pr = (size_t)w.part * a.n_seq * a.nh + (size_t)s * a.nh + h;
+            *(f32x4 *)(a.part + pr * HD + d) = O;
+            if (d == 0) {
+                a.stat[2 * pr] = M;
+                a.stat[2 * pr + 1] = L;
             }
         }
     }
 }
 
-// The prefix's workgroups (16 QT rows each), then the sequences' own (16 rows).
-template <int HD, int NP, int QT, typename T>
-__global__ __launch_bounds__(64 * SA_W, QT * NP >= 4 ? 1 : 2) void k_shared_attn(SharedArgs a) {
-    __shared__ float lds[SA_W * SA_ROWS * (HD + 6)];
+// The tokens of a sequence that are its own (from `b` on; a sequence shorter than
+// the prefix, or a call without parts of the prefix: all), in parts of `c`.
+ZH_DEV uint32_t own_tokens(const SharedArgs &a, uint32_t len, uint32_t &b, uint32_t &c) {
+    b = len < a.prefix || !a.n_pre ? 0u : a.prefix;
+    const uint32_t least = (len - b + a.n_own - 1) / a.n_own;
+    c = max(a.own_len, (least + SA_KB - 1) / SA_KB * SA_KB);
+    return (len - b + c - 1) / c;  // parts
+}
+
+// The prefix's workgroups, then the sequences' own.
+template <int HD, int NP, typename T>
+__global__ __launch_bounds__(64 * SA_W, 3) void k_shared_attn(SharedArgs a) {
+    __shared__ __align__(16) float lds[SA_W * SA_ROWS * (HD + 6)];
     const bool pre = blockIdx.x < a.pre_blocks;
     // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
     const uint32_t job = pre ? blockIdx.x : blockIdx.x - a.pre_blocks, kvh = job % a.nkv;
     SharedPart w;
+    w.first = 0;
     if (pre) {
         const uint32_t tile = job / a.nkv % a.pre_tiles;
         w.part = job / a.nkv / a.pre_tiles;
-        w.row0 = tile * a.pre_rows;
-        w.nrow = min(a.pre_rows, a.n_seq * a.G - w.row0);
+        w.row0 = tile * SA_ROWS;
+        w.nrow = min(SA_ROWS, a.n_seq * a.G - w.row0);
         w.tab = 0;
         w.t0 = w.part * a.pre_len;
         w.t1 = min(w.t0 + a.pre_len, a.prefix);
-        shared_part<HD, NP, QT, T>(a, w, kvh, lds);
     } else {
         const uint32_t s = job / a.nkv % a.n_seq, p = job / a.nkv / a.n_seq;
         w.part = a.n_pre + p;
@@ -312,13 +343,14 @@ __global__ __launch_bounds__(64 * SA_W, QT * NP >= 4 ? 1 : 2) void k_shared_attn
         w.tab = s;
         const uint32_t len = seq_len(a, s);
         if (threadIdx.x == 0 && p == 0 && kvh == 0 && a.lens[s] > a.max_len) atomicOr(a.err, ZH_DEVERR_KV_ROW);
-        // a sequence shorter than the prefix: all of its tokens are its own
-        const uint32_t b = len < a.prefix ? 0u : a.prefix, n = (len - b + a.n_own - 1) / a.n_own;
-        const uint32_t c = (n + SA_KB - 1) / SA_KB * SA_KB;
-        w.t0 = min(b + p * c, len);
-        w.t1 = min(b + (p + 1) * c, len);
-        shared_part<HD, NP, 1, T>(a, w, kvh, lds);
+        uint32_t b, c;
+        const uint32_t n = own_tokens(a, len, b, c);
+        if (p >= n && a.n_pre + a.n_own > 1) return;  // (the join reads the parts there are)
+        w.t0 = b + p * c;
+        w.t1 = min(w.t0 + c, len);
+        if (!a.n_pre && a.prefix && len >= a.prefix) w.first = w.t0 = a.prefix;  // (one part: the whole context)
     }
+    shared_part<HD, NP, T>(a, w, kvh, lds);
 }
 
 // Many rows (a workgroup: 4 waves of 32 RT): K and V pass through LDS once for
@@ -370,44 +402,6 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
     const bool mine = row0 < rows;  // (uniform per wave: it has rows)
     const uint32_t t0 = part * a.pre_len, t1 = min(t0 + a.pre_len, a.prefix);
     const uint32_t nst = (t1 - t0 + ST_KB - 1) / ST_KB;
-    // ---- the rows' q: dims 16 k + 8 h ..
-    half8 qf[RT][NP][KS];
-    float c[RT];
-#pragma unroll
-    for (int q = 0; q < RT; q++) {
-        const uint32_t row = min(row0 + 32 * q + i32, rows - 1);
-        const uint8_t *qp = a.q + row / a.G * a.q_row + (size_t)(kvh * a.G + row % a.G) * HD * sizeof(T);
-        float v[KS][8], mx = 0.f;
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                v[k][e] = ld<T>(qp, 16 * k + 8 * h + e);
-                mx = fmaxf(mx, fabsf(v[k][e]));
-            }
-        // (the scale's sign goes into q: the largest product is the largest score)
-        float up = a.scale < 0.f ? -1.f : 1.f;
-        c[q] = fabsf(a.scale) * 1.44269504088896340736f;
-        if (NP > 1) {
-            mx = xor32_max(mx);
-            const uint32_t E = __float_as_uint(mx) >> 23;
-            if (E >= 8 && E <= 246) {
-                up *= __uint_as_float((254u - E) << 23);
-                c[q] *= __uint_as_float(E << 23);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float x = v[k][e] * up;
-#pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    qf[q][p][k][e] = (_Float16)x;
-                    x -= (float)qf[q][p][k][e];
-                }
-            }
-    }
     // ---- copies, 1 KB (1024 / ROWB rows) each: 4 waves a page of K and of V of a
     // stage; 8 waves a page of one of them
     const uint32_t lds0 = lds_addr(lds);
@@ -457,6 +451,45 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
             else wait_vm<0>();
         }
     };
+    // the first copies go out before the rows are read
+    for (uint32_t st = 0; st < 3 && st < nst; st++) issue(st);
+    // ---- the rows' q: dims 16 k + 8 h ..
+    half8 qf[RT][NP][KS];
+    float c[RT];
+#pragma unroll
+    for (int q = 0; q < RT; q++) {
+        const uint32_t row = min(row0 + 32 * q + i32, rows - 1);
+        const uint8_t *qp = a.q + row / a.G * a.q_row + (size_t)(kvh * a.G + row % a.G) * HD * sizeof(T);
+        float v[KS][8], mx = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            ld8((const T *)qp + 16 * k + 8 * h, v[k]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k][e]));
+        }
+        // (the scale's sign goes into q: the largest product is the largest score)
+        float up = a.scale < 0.f ? -1.f : 1.f;
+        c[q] = fabsf(a.scale) * 1.44269504088896340736f;
+        if (NP > 1) {
+            mx = xor32_max(mx);
+            const uint32_t E = __float_as_uint(mx) >> 23;
+            if (E >= 8 && E <= 246) {
+                up *= __uint_as_float((254u - E) << 23);
+                c[q] *= __uint_as_float(E << 23);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float x = v[k][e] * up;
+#pragma unroll
+                for (int p = 0; p < NP; p++) {
+                    qf[q][p][k][e] = (_Float16)x;
+                    x -= (float)qf[q][p][k][e];
+                }
+            }
+    }
     f32x16 o[RT][DT];
     float m[RT], l[RT];
 #pragma unroll
@@ -516,7 +549,6 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
 #pragma unroll
                 for (int q = 0; q < RT; q++) d[q][r] = -INFINITY;
     };
-    for (uint32_t st = 0; st < 3 && st < nst; st++) issue(st);
     if (nst > 2) wait_vm<(NW == 4 ? 5 : 2) * NI>();  // K of stage 0
     else wait_vm<0>();
     lds_bar();
@@ -658,59 +690,58 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
     }
 }
 
-// Joins the parts of a row, one wave each: the lanes take the parts' statistics,
-// 64 at a time, then every lane HD / 64 dims of all of them, 8 loads in flight.
+// Joins the parts of a row: HD / 4 lanes, of 4 dims each, take the parts'
+// statistics, as many at a time, then all of them the parts' sums, 8 loads of 16
+// bytes in flight.
 template <int HD, typename T>
 __global__ __launch_bounds__(256) void k_shared_join(SharedArgs a) {
-    constexpr int E = HD / 64, U = 8;
-    const uint32_t rows = a.n_seq * a.nh, lane = threadIdx.x & 63;
-    const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    if (row >= rows) return;
+    constexpr uint32_t N = HD / 4, U = 8;
+    const uint32_t rows = a.n_seq * a.nh, lane = threadIdx.x & 63, l = lane % N;
+    const uint32_t row = min(blockIdx.x * (256 / N) + threadIdx.x / N, rows - 1);  // (past the last: that row again)
     const uint32_t s = row / a.nh, len = seq_len(a, s);
     // (a sequence shorter than the prefix has no part in it)
-    const uint32_t p0 = len < a.prefix ? a.n_pre : 0u, p1 = a.n_pre + a.n_own;
-    float M = -INFINITY, L = 0.f, O[E];
+    uint32_t first, c;
+    const uint32_t p0 = len < a.prefix ? a.n_pre : 0u, p1 = a.n_pre + own_tokens(a, len, first, c);
+    float M = -INFINITY, L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t b = p0; b < p1; b += N) {
+        const uint32_t n = min(N, p1 - b);
+        const float2 st = *(const float2 *)(a.stat + 2 * ((size_t)(b + min(l, n - 1)) * rows + row));
+        float mx = st.x;
 #pragma unroll
-    for (int e = 0; e < E; e++) O[e] = 0.f;
-    for (uint32_t b = p0; b < p1; b += 64) {
-        const uint32_t n = min(64u, p1 - b);
-        const float2 st = *(const float2 *)(a.stat + 2 * ((size_t)(b + min(lane, n - 1)) * rows + row));
-        const float mn = fmaxf(M, wave_max(st.x)), ms = mn == -INFINITY ? 0.f : mn;
-        const float old = __builtin_amdgcn_exp2f(M - ms), w = lane < n ? __builtin_amdgcn_exp2f(st.x - ms) : 0.f;
+        for (uint32_t x = 1; x < N; x *= 2) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
+        const float mn = fmaxf(M, mx), ms = mn == -INFINITY ? 0.f : mn;
+        const float old = __builtin_amdgcn_exp2f(M - ms), w = l < n ? __builtin_amdgcn_exp2f(st.x - ms) : 0.f;
+        float ls = l < n ? st.y * w : 0.f;
+#pragma unroll
+        for (uint32_t x = 1; x < N; x *= 2) ls += __shfl_xor(ls, x, 64);
         M = mn;
-        L = fmaf(L, old, wave_sum(lane < n ? st.y * w : 0.f));
-#pragma unroll
-        for (int e = 0; e < E; e++) O[e] *= old;
+        L = fmaf(L, old, ls);
+        O *= old;
         for (uint32_t p = 0; p < n; p += U) {
-            float v[U][E];
+            f32x4 v[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const float *pp = a.part + ((size_t)(b + min(p + u, n - 1)) * rows + row) * HD + E * lane;
+            for (uint32_t u = 0; u < U; u++)
+                v[u] = *(const f32x4 *)(a.part + ((size_t)(b + min(p + u, n - 1)) * rows + row) * HD + 4 * l);
 #pragma unroll
-                for (int e = 0; e < E; e++) v[u][e] = pp[e];
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {  // (past the last part: its values again, weight 0)
-                const float f = lane_f(w, p + u);
-#pragma unroll
-                for (int e = 0; e < E; e++) O[e] = fmaf(v[u][e], f, O[e]);
+            for (uint32_t u = 0; u < U; u++) {  // (past the last part: its values again, weight 0)
+                const float f = __shfl(w, lane - l + p + u, 64);
+                O.x = fmaf(v[u].x, f, O.x);
+                O.y = fmaf(v[u].y, f, O.y);
+                O.z = fmaf(v[u].z, f, O.z);
+                O.w = fmaf(v[u].w, f, O.w);
             }
         }
     }
-    uint8_t *op = a.out + s * a.out_row;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const float v = len ? O[e] / L : 0.f;
-        const uint32_t i = row % a.nh * HD + E * lane + e;
-        if (sizeof(T) == 4) ((float *)op)[i] = v;
-        else ((_Float16 *)op)[i] = (_Float16)v;
-    }
+    const f32x4 r = len ? f32x4{O.x / L, O.y / L, O.z / L, O.w / L} : f32x4{0.f, 0.f, 0.f, 0.f};
+    T *op = (T *)(a.out + s * a.out_row) + row % a.nh * HD + 4 * l;
+    if constexpr (sizeof(T) == 4) *(f32x4 *)op = r;
+    else *(half4 *)op = half4{(_Float16)r.x, (_Float16)r.y, (_Float16)r.z, (_Float16)r.w};
 }
 
 // How a call is cut (the same for every call of these sizes).
 struct SharedPlan {
-    uint32_t n_pre, n_own, pre_tiles, pre_len, pre_blocks, blocks, qt;
-    uint32_t tile, pre_rows;
+    uint32_t n_pre, n_own, pre_tiles, pre_len, own_len, pre_blocks, blocks, tile;
     uint64_t stat_off, bytes;  // of ws
 };
 
@@ -719,27 +750,25 @@ uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); 
 bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t prefix, uint32_t max_len,
                  SharedPlan &p) {
     const uint32_t G = nh / nkv, own = max_len - prefix;
-    const uint64_t rows_kv = (uint64_t)n_seq * G;
-    // rows of a prefix workgroup: 128 or 256 on LDS tiles, or 16 or 32 streamed
-    p.tile = rows_kv >= SA_TILE ? (rows_kv > 128 && SA_RT > 1 ? 2 : 1) : 0;
-    p.qt = rows_kv <= 16 ? 1 : 2;
-    p.pre_rows = p.tile ? 128u * p.tile : p.qt * SA_ROWS;
-    p.pre_tiles = ceil_div(rows_kv, p.pre_rows);
-    // parts: `per` workgroups per CU, at least 128 tokens each
-    auto cut = [&](uint64_t jobs, uint32_t tokens, uint32_t per) {
-        const uint32_t most = ceil_div(tokens, 128), want = ceil_div((uint64_t)per * cus, jobs);
-        return want < most ? want : most;
+    const uint64_t rows_kv = (uint64_t)n_seq * G, jobs = (uint64_t)n_seq * nkv;
+    // parts for `per` workgroups per CU, of at least 128 tokens
+    auto cut = [&](uint64_t n, uint32_t tokens, uint32_t per) {
+        const uint32_t most = ceil_div(tokens, 128), want = (uint32_t)(((uint64_t)per * cus + n / 2) / n);
+        return want < 1 ? 1u : want < most ? want : most;
     };
-    p.n_pre = 0;
-    p.pre_len = 0;
-    if (prefix) {
+    p = {};
+    if (prefix && (prefix + own > SA_ONE || jobs > cus)) {
+        // rows of a prefix workgroup: 128 or 256 on LDS tiles, or 16 streamed
+        p.tile = rows_kv >= SA_TILE ? (rows_kv > 128 && SA_RT > 1 ? 2 : 1) : 0;
+        p.pre_tiles = ceil_div(rows_kv, p.tile ? 128u * p.tile : SA_ROWS);
         const uint32_t n = cut((uint64_t)p.pre_tiles * nkv, prefix, p.tile ? 1 : SA_PRE_PER);
         const uint32_t step = p.tile ? ST_KB : SA_KB;
         p.pre_len = ceil_div(ceil_div(prefix, n), step) * step;
         p.n_pre = ceil_div(prefix, p.pre_len);
     }
-    p.n_own = own || !prefix ? cut((uint64_t)n_seq * nkv, own ? own : 1, SA_OWN_PER) : 1u;
-    if (p.n_own == 0) p.n_own = 1;
+    // a sequence's own tokens (all of them where the prefix has no parts)
+    p.n_own = p.n_pre ? (own ? cut(jobs, own, SA_OWN_PER) : 1u) : prefix ? 1u : cut(jobs, own, SA_OWN_PER);
+    p.own_len = ceil_div(ceil_div(p.n_pre ? (own ? own : 1) : max_len, p.n_own), SA_KB) * SA_KB;
     const uint64_t pre = (uint64_t)p.n_pre * p.pre_tiles * nkv, all = pre + (uint64_t)p.n_own * n_seq * nkv;
     if (all > 0x7FFFFFFFull || (uint64_t)n_seq * nh > 0x7FFFFFFFull) return false;
     p.pre_blocks = (uint32_t)pre;
@@ -828,13 +857,11 @@ static int shared_launch(zh_ctx *c, const SharedArgs &a, const SharedPlan &p) {
         b.pre_blocks = 0;
         blocks -= p.pre_blocks;
     }
-#define SA_L(QT) hipLaunchKernelGGL((k_shared_attn<HD, NP, QT, T>), dim3(blocks), dim3(64 * SA_W), 0, c->stream, b)
-    if (p.qt == 1 || !b.pre_blocks) SA_L(1);
-    else SA_L(2);
-#undef SA_L
+    hipLaunchKernelGGL((k_shared_attn<HD, NP, T>), dim3(blocks), dim3(64 * SA_W), 0, c->stream, b);
     ZH_LAUNCH_CHECK(c);
     if (a.n_pre + a.n_own > 1) {
-        hipLaunchKernelGGL((k_shared_join<HD, T>), dim3((a.n_seq * a.nh + 3) / 4), dim3(256), 0, c->stream, a);
+        const uint32_t per = 256 / (HD / 4);  // rows of a workgroup
+        hipLaunchKernelGGL((k_shared_join<HD, T>), dim3((a.n_seq * a.nh + per - 1) / per), dim3(256), 0, c->stream, a);
         ZH_LAUNCH_CHECK(c);
     }
     return ZH_OK;
@@ -874,7 +901,7 @@ extern "C" int zh_flash_decode_shared(zh_ctx *c, const zh_kv_batch *kv, const zh
     a.pre_tiles = p.pre_tiles;
     a.pre_blocks = p.pre_blocks;
     a.pre_len = p.pre_len;
-    a.pre_rows = p.pre_rows;
+    a.own_len = p.own_len;
     a.scale = r->attn_scale != 0.f ? r->attn_scale : 1.0f / sqrtf((float)kv->head_dim);
     if (kv->head_dim == 128)
         return size == 4 ? shared_launch<128, 2, float>(c, a, p) : shared_launch<128, 1, _Float16>(c, a, p);
