@@ -15,20 +15,23 @@
 // ---------------------------------------------------------------------------
 namespace {
 
-constexpr uint32_t KC_CACHES = 96, KC_PAGES = 256;  // per launch: 4 KB of arguments hold both lists
+// Caches and pages per launch: 4 KB of arguments hold both lists; a call of few
+// pages (a fork) takes the small form, whose arguments the host writes sooner.
+constexpr uint32_t KC_CACHES = 96, KC_PAGES = 256, KC_FEW_CACHES = 64, KC_FEW_PAGES = 16;
+template <uint32_t NC, uint32_t NP>
 struct KvCopyArgs {
-    const uint8_t *src[KC_CACHES];
-    uint8_t *dst[KC_CACHES];
-    uint32_t pages[KC_PAGES][2];  // source, destination
+    const uint8_t *src[NC];
+    uint8_t *dst[NC];
+    uint32_t pages[NP][2];  // source, destination
     uint64_t src_head, dst_head;  // bytes of one head of a cache
     uint32_t n_caches, n_pages, n_heads, seg;  // seg: bytes of a page of one head
 };
-static_assert(sizeof(KvCopyArgs) <= 4096, "kernel arguments");
+static_assert(sizeof(KvCopyArgs<KC_CACHES, KC_PAGES>) <= 4096, "kernel arguments");
 
 // One workgroup: KC_U pages of one head and cache, all loads before the stores.
 constexpr int KC_U = 2;  // (4 and 8: the same times)
-template <bool NT, int U>
-ZH_DEV void kv_copy_pages(const KvCopyArgs &a, uint32_t p0, const uint8_t *s, uint8_t *d) {
+template <bool NT, int U, typename A>
+ZH_DEV void kv_copy_pages(const A &a, uint32_t p0, const uint8_t *s, uint8_t *d) {
     for (uint32_t i = threadIdx.x; i < a.seg / 16; i += blockDim.x) {
         u32x4 v[U];
 #pragma unroll
@@ -44,8 +47,8 @@ ZH_DEV void kv_copy_pages(const KvCopyArgs &a, uint32_t p0, const uint8_t *s, ui
         }
     }
 }
-template <bool NT>
-__global__ __launch_bounds__(256) void k_kv_copy(KvCopyArgs a) {
+template <bool NT, typename A>
+__global__ __launch_bounds__(256) void k_kv_copy(A a) {
     const uint32_t p0 = blockIdx.x * KC_U, h = blockIdx.y, c = blockIdx.z;
     const uint8_t *s = a.src[c] + h * a.src_head;
     uint8_t *d = a.dst[c] + h * a.dst_head;
@@ -54,12 +57,12 @@ __global__ __launch_bounds__(256) void k_kv_copy(KvCopyArgs a) {
         for (uint32_t p = p0; p < a.n_pages; p++) kv_copy_pages<NT, 1>(a, p, s, d);
 }
 
-}  // namespace
-
-int zhk_kv_copy(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *const *src, uint32_t dst_tokens,
-                uint32_t src_tokens, uint32_t n_kv_heads, uint32_t head_dim, const uint32_t *dst_pages,
-                const uint32_t *src_pages, uint32_t n_pages) {
-    KvCopyArgs a;
+template <uint32_t NC, uint32_t NP>
+int kv_copy_launches(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *const *src, uint32_t dst_tokens,
+                     uint32_t src_tokens, uint32_t n_kv_heads, uint32_t head_dim, const uint32_t *dst_pages,
+                     const uint32_t *src_pages, uint32_t n_pages) {
+    typedef KvCopyArgs<NC, NP> A;
+    A a;
     a.seg = 32 * head_dim;
     a.src_head = 2ull * src_tokens * head_dim;
     a.dst_head = 2ull * dst_tokens * head_dim;
@@ -68,29 +71,39 @@ int zhk_kv_copy(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *cons
     // past what the L2s hold, the pages go by them: 1024 pages of 32 caches of 8
     // heads 382 us (5.6 TB/s read + written) against 408 through them
     const bool nt = (uint64_t)n_caches * n_pages * n_kv_heads * a.seg > (32ull << 20);
-    for (uint32_t c0 = 0; c0 < n_caches; c0 += KC_CACHES) {
-        a.n_caches = n_caches - c0 < KC_CACHES ? n_caches - c0 : KC_CACHES;
+    for (uint32_t c0 = 0; c0 < n_caches; c0 += NC) {
+        a.n_caches = n_caches - c0 < NC ? n_caches - c0 : NC;
         for (uint32_t i = 0; i < a.n_caches; i++) {
             a.src[i] = (const uint8_t *)src[c0 + i];
             a.dst[i] = (uint8_t *)dst[c0 + i];
         }
-        for (uint32_t p0 = 0; p0 < n_pages; p0 += KC_PAGES) {
-            a.n_pages = n_pages - p0 < KC_PAGES ? n_pages - p0 : KC_PAGES;
+        for (uint32_t p0 = 0; p0 < n_pages; p0 += NP) {
+            a.n_pages = n_pages - p0 < NP ? n_pages - p0 : NP;
             for (uint32_t i = 0; i < a.n_pages; i++) {
                 a.pages[i][0] = src_pages[p0 + i];
                 a.pages[i][1] = dst_pages[p0 + i];
             }
             const dim3 grid((a.n_pages + KC_U - 1) / KC_U, a.n_heads, a.n_caches);
-            if (nt) hipLaunchKernelGGL(k_kv_copy<true>, grid, dim3(threads), 0, c->stream, a);
-            else hipLaunchKernelGGL(k_kv_copy<false>, grid, dim3(threads), 0, c->stream, a);
+            if (nt) hipLaunchKernelGGL((k_kv_copy<true, A>), grid, dim3(threads), 0, c->stream, a);
+            else hipLaunchKernelGGL((k_kv_copy<false, A>), grid, dim3(threads), 0, c->stream, a);
             ZH_LAUNCH_CHECK(c);
         }
     }
     return ZH_OK;
 }
 
+}  // namespace
+
+int zhk_kv_copy(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *const *src, uint32_t dst_tokens,
+                uint32_t src_tokens, uint32_t n_kv_heads, uint32_t head_dim, const uint32_t *dst_pages,
+                const uint32_t *src_pages, uint32_t n_pages) {
+    auto f = n_pages <= KC_FEW_PAGES ? kv_copy_launches<KC_FEW_CACHES, KC_FEW_PAGES> : kv_copy_launches<KC_CACHES, KC_PAGES>;
+    return f(c, n_caches, dst, src, dst_tokens, src_tokens, n_kv_heads, head_dim, dst_pages, src_pages, n_pages);
+}
+
+constexpr uint32_t KC_MAX = 256;  // caches of a call
 static bool caches_ok(const zh_kv_caches *s) {
-    if (!s || !s->caches || s->n_caches == 0 || s->n_caches > 256 || s->n_kv_heads == 0 || s->n_kv_heads > 65535 || s->head_dim == 0 ||
+    if (!s || !s->caches || s->n_caches == 0 || s->n_caches > KC_MAX || s->n_kv_heads == 0 || s->n_kv_heads > 65535 || s->head_dim == 0 ||
         s->head_dim > 1024 || s->cache_tokens == 0)
         return false;
     for (uint32_t i = 0; i < s->n_caches; i++)
@@ -102,27 +115,32 @@ static bool caches_ok(const zh_kv_caches *s) {
 // message then). `mark` and `call`: see zh_ctx::page_mark.
 extern "C" int zh_check_kv_copy_pages(zh_ctx *c, const zh_kv_caches *dst, const zh_kv_caches *src,
                                       const uint32_t *dst_pages, const uint32_t *src_pages, uint32_t n_pages) {
-    if (!caches_ok(dst) || !caches_ok(src) || dst->n_caches != src->n_caches || dst->n_kv_heads != src->n_kv_heads ||
+    const bool one = dst && src && dst->caches == src->caches && dst->n_caches == src->n_caches;
+    if (!caches_ok(dst) || !(one && dst->cache_tokens == src->cache_tokens && dst->n_kv_heads == src->n_kv_heads &&
+                             dst->head_dim == src->head_dim ? true : caches_ok(src)) || dst->n_caches != src->n_caches || dst->n_kv_heads != src->n_kv_heads ||
         dst->head_dim != src->head_dim)
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: cache sets");
     if (n_pages && (!dst_pages || !src_pages))
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: no page numbers");
-    // the caches' addresses in a small hash table (a fork copies a few pages of
-    // all layers: comparing every pair would take longer than the copy)
-    bool alias = false;
-    uint16_t tab[1024] = {};
-    auto place = [&](const void *p) {  // p's entry, or the empty one it would take
-        uint32_t i = (uint32_t)(((uint64_t)(uintptr_t)p * 0x9E3779B97F4A7C15ull) >> 54);
-        while (tab[i] && dst->caches[tab[i] - 1]->ptr != p) i = (i + 1) % 1024;
-        return i;
-    };
-    for (uint32_t i = 0; i < dst->n_caches; i++) {
-        uint16_t &e = tab[place(dst->caches[i]->ptr)];
-        if (e)
-            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: caches %u and %u of dst are one", e - 1u, i);
-        e = (uint16_t)(i + 1);
+    // one set copied within itself (a cache that it names twice gets the same
+    // bytes twice); else the caches' addresses in a small hash table (comparing
+    // every pair would take longer than the copy of a few pages)
+    bool alias = one;
+    if (!one) {
+        uint16_t tab[1024] = {};
+        auto place = [&](const void *p) {  // p's entry, or the empty one it would take
+            uint32_t i = (uint32_t)(((uint64_t)(uintptr_t)p * 0x9E3779B97F4A7C15ull) >> 54);
+            while (tab[i] && dst->caches[tab[i] - 1]->ptr != p) i = (i + 1) % 1024;
+            return i;
+        };
+        for (uint32_t i = 0; i < dst->n_caches; i++) {
+            uint16_t &e = tab[place(dst->caches[i]->ptr)];
+            if (e)
+                return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: caches %u and %u of dst are one", e - 1u, i);
+            e = (uint16_t)(i + 1);
+        }
+        for (uint32_t i = 0; i < src->n_caches && !alias; i++) alias = tab[place(src->caches[i]->ptr)] != 0;
     }
-    for (uint32_t i = 0; i < src->n_caches && !alias; i++) alias = tab[place(src->caches[i]->ptr)] != 0;
     if (alias && dst->cache_tokens != src->cache_tokens)
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: one cache in two sizes");
     const uint32_t np = dst->cache_tokens / 16;
@@ -161,20 +179,14 @@ extern "C" int zh_kv_copy_pages(zh_ctx *c, const zh_kv_caches *dst, const zh_kv_
     int rc = zh_check_kv_copy_pages(c, dst, src, dst_pages, src_pages, n_pages);
     if (rc) return rc;
     zh_device_scope dev(c);
-    // the buffers' addresses, KC_CACHES at a time
-    for (uint32_t c0 = 0; c0 < dst->n_caches; c0 += KC_CACHES) {
-        void *d[KC_CACHES];
-        const void *s[KC_CACHES];
-        const uint32_t n = dst->n_caches - c0 < KC_CACHES ? dst->n_caches - c0 : KC_CACHES;
-        for (uint32_t i = 0; i < n; i++) {
-            d[i] = dst->caches[c0 + i]->ptr;
-            s[i] = src->caches[c0 + i]->ptr;
-        }
-        rc = zhk_kv_copy(c, n, d, s, dst->cache_tokens, src->cache_tokens, dst->n_kv_heads, dst->head_dim, dst_pages,
-                         src_pages, n_pages);
-        if (rc) return rc;
+    void *d[KC_MAX];
+    const void *s[KC_MAX];
+    for (uint32_t i = 0; i < dst->n_caches; i++) {
+        d[i] = dst->caches[i]->ptr;
+        s[i] = src->caches[i]->ptr;
     }
-    return ZH_OK;
+    return zhk_kv_copy(c, dst->n_caches, d, s, dst->cache_tokens, src->cache_tokens, dst->n_kv_heads, dst->head_dim,
+                       dst_pages, src_pages, n_pages);
 }
 
 // ---------------------------------------------------------------------------

@@ -282,6 +282,23 @@ def _ptr(a):
     return C.c_void_p(a.ctypes.data)
 
 
+_U32 = np.dtype(np.uint32)
+
+
+def _u32_array(a):
+    """a as (argument, count) of a u32 list. A contiguous uint32 array goes as it
+    is: a fork copies its page in the time a conversion takes."""
+    if type(a) is np.ndarray and a.dtype is _U32 and a.ndim == 1:
+        try:
+            return C.byref(_u32.from_buffer(a)), a.size
+        except (TypeError, ValueError):  # read-only, with gaps or empty
+            pass
+    a = np.array(a, dtype=np.uint32, ndmin=1)
+    if a.ndim != 1:
+        raise ValueError("a list of page numbers")
+    return (C.byref(_u32.from_buffer(a)) if a.size else None), a.size
+
+
 class Buffer:
     """Device buffer (zh_buf): owned by its Context."""
 
@@ -459,11 +476,11 @@ class Context:
 
     def kv_copy_pages(self, dst, src, dst_pages, src_pages):
         """Page src_pages[i] of every cache of src to page dst_pages[i] of dst's (KvCaches)."""
-        d, s = np.ascontiguousarray(dst_pages, dtype=np.uint32), np.ascontiguousarray(src_pages, dtype=np.uint32)
-        if d.shape != s.shape or d.ndim != 1:
+        d, n = _u32_array(dst_pages)
+        s, ns = _u32_array(src_pages)
+        if n != ns:
             raise ValueError("one source page per destination page")
-        self.check(lib().zh_kv_copy_pages(self.h, dst.ptr, src.ptr, d.__array_interface__["data"][0],
-                                          s.__array_interface__["data"][0], d.size))
+        self.check(lib().zh_kv_copy_pages(self.h, dst.ptr, src.ptr, d, s, n))
 
     def softmax_topk(self, logits, n, k, routing):
         self.check(lib().zh_softmax_topk(self.h, logits.h, n, k, routing.h))
