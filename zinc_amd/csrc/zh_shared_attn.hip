@@ -27,6 +27,9 @@ constexpr int SA_W = 4;           // waves of a workgroup, each on its own steps
 #ifndef SA_TILE
 #define SA_TILE 96
 #endif
+#ifndef SA_TILE_OWN
+#define SA_TILE_OWN 2
+#endif
 #ifndef SA_ONE
 #define SA_ONE 512
 #endif
@@ -54,6 +57,7 @@ struct SharedArgs {
     uint32_t pre_tiles, pre_blocks;  // row tiles per kv head, workgroups of the prefix
     uint32_t pre_len;                // tokens of a prefix part (a multiple of SA_KB)
     uint32_t own_len;                // tokens of a sequence's own part, at least
+    uint32_t join;                   // the own parts' workgroups write the result (n_own == 1, the prefix's parts are there)
     float scale;
 };
 
@@ -80,6 +84,7 @@ ZH_DEV void ld8(const _Float16 *p, float (&v)[8]) {
 // through table row 0 (a sequence's whole context in one workgroup).
 struct SharedPart {
     uint32_t part, row0, nrow, t0, t1, tab, first;
+    bool pre, shares;  // a part of the prefix; of a sequence that has the prefix's parts too
 };
 
 // 16 rows of one kv head. Each wave takes steps of 32 tokens by itself, K and V
@@ -263,7 +268,7 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
     }
     if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
     // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
-    const bool direct = a.n_pre + a.n_own == 1;
+    const bool direct = !w.pre && (a.join || a.n_pre + a.n_own == 1);
     l = xor32_sum(xor16_sum(l));
 #pragma unroll
     for (int r = 0; r < 4; r++)
@@ -293,8 +298,38 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
             O.w = fmaf(v.w, fk, O.w);
             L = fmaf(sl[k * SA_ROWS + r], fk, L);
         }
+        if (!w.pre && a.join && a.n_pre) {
+            // the row's parts of the prefix, 8 at a time
+            const uint32_t np = w.shares ? a.n_pre : 0u, rows = a.n_seq * a.nh, row = s * a.nh + h;
+            for (uint32_t p0 = 0; p0 < np; p0 += 8) {
+                float2 st[8];
+                f32x4 v[8];
+#pragma unroll
+                for (uint32_t u = 0; u < 8; u++) {  // (past the last part: its values again, weight 0)
+                    const size_t pr = (size_t)min(p0 + u, np - 1) * rows + row;
+                    st[u] = *(const float2 *)(a.stat + 2 * pr);
+                    v[u] = *(const f32x4 *)(a.part + pr * HD + d);
+                }
+                float mn = M;
+#pragma unroll
+                for (uint32_t u = 0; u < 8; u++) mn = fmaxf(mn, st[u].x);
+                const float mr = mn == -INFINITY ? 0.f : mn, old = __builtin_amdgcn_exp2f(M - mr);
+                M = mn;
+                O *= old;
+                L *= old;
+#pragma unroll
+                for (uint32_t u = 0; u < 8; u++) {
+                    const float f = p0 + u < np ? __builtin_amdgcn_exp2f(st[u].x - mr) : 0.f;
+                    O.x = fmaf(v[u].x, f, O.x);
+                    O.y = fmaf(v[u].y, f, O.y);
+                    O.z = fmaf(v[u].z, f, O.z);
+                    O.w = fmaf(v[u].w, f, O.w);
+                    L = fmaf(st[u].y, f, L);
+                }
+            }
+        }
         if (direct) {
-            const f32x4 v = nstep ? f32x4{O.x / L, O.y / L, O.z / L, O.w / L} : f32x4{0.f, 0.f, 0.f, 0.f};
+            const f32x4 v = nstep || w.shares ? f32x4{O.x / L, O.y / L, O.z / L, O.w / L} : f32x4{0.f, 0.f, 0.f, 0.f};
             T *op = (T *)(a.out + s * a.out_row) + h * HD + d;
             if constexpr (sizeof(T) == 4) *(f32x4 *)op = v;
             else *(half4 *)op = half4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
@@ -327,6 +362,8 @@ __global__ __launch_bounds__(64 * SA_W, 3) void k_shared_attn(SharedArgs a) {
     const uint32_t job = pre ? blockIdx.x : blockIdx.x - a.pre_blocks, kvh = job % a.nkv;
     SharedPart w;
     w.first = 0;
+    w.pre = pre;
+    w.shares = false;
     if (pre) {
         const uint32_t tile = job / a.nkv % a.pre_tiles;
         w.part = job / a.nkv / a.pre_tiles;
@@ -345,7 +382,8 @@ __global__ __launch_bounds__(64 * SA_W, 3) void k_shared_attn(SharedArgs a) {
         if (threadIdx.x == 0 && p == 0 && kvh == 0 && a.lens[s] > a.max_len) atomicOr(a.err, ZH_DEVERR_KV_ROW);
         uint32_t b, c;
         const uint32_t n = own_tokens(a, len, b, c);
-        if (p >= n && a.n_pre + a.n_own > 1) return;  // (the join reads the parts there are)
+        if (p >= n && a.n_pre + a.n_own > 1 && !a.join) return;  // (the join reads the parts there are)
+        w.shares = a.n_pre && len >= a.prefix;
         w.t0 = b + p * c;
         w.t1 = min(w.t0 + c, len);
         if (!a.n_pre && a.prefix && len >= a.prefix) w.first = w.t0 = a.prefix;  // (one part: the whole context)
@@ -505,12 +543,20 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
     const uint32_t ka = i32 * ROWB + ((h ^ st_swz<PPR>(i32)) * 16);
     const uint32_t l16 = lane % 16, vr = 4 * h + l16 / 4, vp = 2 * (lane / 16 % 2) + l16 % 4 / 2;
     const uint32_t va = vr * ROWB + ((vp ^ st_swz<PPR>(vr)) * 16) + 8 * (l16 % 2);
+    const uint8_t *kp[KS], *vp0[DT], *vp1[DT];  // (the stage and the tokens in it: constant offsets)
+#pragma unroll
+    for (int k = 0; k < KS; k++) kp[k] = lds + (ka ^ (k * 32));
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+        // tokens 4 h .. +3 and those 8 on (8 rows on, the piece's bit 1 flipped)
+        vp0[d] = lds + ST_NS * STAGE + (va ^ (d * 64));
+        vp1[d] = lds + ST_NS * STAGE + 8 * ROWB + (va ^ (d * 64) ^ 32);
+    }
     f32x16 s[RT], sn[RT];  // scores of the current and the next 32 tokens (raw)
     half8 kf[KS];          // K fragments of the next ones
-    auto load_k = [&](uint32_t st, uint32_t kt) __attribute__((always_inline)) {
-        const uint8_t *ks = lds + st % ST_NS * STAGE + kt * 32 * ROWB;
+    auto load_k = [&](uint32_t slot, uint32_t kt) __attribute__((always_inline)) {
 #pragma unroll
-        for (int k = 0; k < KS; k++) kf[k] = *(const half8 *)(ks + (ka ^ (k * 32)));
+        for (int k = 0; k < KS; k++) kf[k] = *(const half8 *)(kp[k] + slot * STAGE + kt * 32 * ROWB);
     };
     // the reference maximum for scores d: moved, and the sums with it, where one
     // (largest: mx) passes it by 2^8
@@ -572,14 +618,17 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
         refer(mx);
     }
     constexpr int PAIRS = 8 * RT, EARLY = 3 * PAIRS / 4;  // weights in pairs; those taken beside the scores' products
-    for (uint32_t st = 0; st < nst; st++) {
+    for (uint32_t s0 = 0; s0 < nst; s0 += ST_NS)
+#pragma unroll
+    for (uint32_t slot = 0; slot < ST_NS; slot++) {
+        const uint32_t st = s0 + slot;
+        if (st >= nst) break;
         landed(st);
         lds_bar();
         if (st + 3 < nst) issue(st + 3);
         const uint32_t tk = t0 + st * ST_KB;
-        uint8_t *vs = lds + (ST_NS + st % ST_NS) * STAGE;
         if (tk + ST_KB > t1) {  // V of the tokens past the part: zero (0 times NaN is NaN)
-            for (uint32_t i = (t1 - tk) * ROWB + tid * 16; i < STAGE; i += 64 * NW * 16) *(u32x4 *)(vs + i) = u32x4{0, 0, 0, 0};
+            for (uint32_t i = (t1 - tk) * ROWB + tid * 16; i < STAGE; i += 64 * NW * 16) *(u32x4 *)(lds + (ST_NS + slot) * STAGE + i) = u32x4{0, 0, 0, 0};
             lds_bar();
         }
         if (!mine) continue;
@@ -610,11 +659,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
             auto load_v = [&](int s2) __attribute__((always_inline)) {
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
-                    // tokens 16 s2 + 4 h .. +3 and those 8 on (8 rows on, the piece's bit 1 flipped)
-                    uint8_t *v0 = vs + (32 * kt + 16 * s2) * ROWB + (va ^ (d * 64));
-                    uint8_t *v1 = vs + (32 * kt + 16 * s2 + 8) * ROWB + (va ^ (d * 64) ^ 32);
-                    const tr4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)v0);
-                    const tr4 y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)v1);
+                    const uint32_t at = slot * STAGE + (32 * kt + 16 * s2) * ROWB;
+                    const tr4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)(vp0[d] + at));
+                    const tr4 y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)(vp1[d] + at));
                     vf[s2][d] = half8{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
                                       (_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
                 }
@@ -645,7 +692,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
                 for (int i = EARLY + (PAIRS - EARLY) * d / DT; i < EARLY + (PAIRS - EARLY) * (d + 1) / DT; i++) weights(i);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            load_k(st + 1, kt);
+            load_k((slot + 1) % ST_NS, kt);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
 #pragma unroll
@@ -767,7 +814,8 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
         p.n_pre = ceil_div(prefix, p.pre_len);
     }
     // a sequence's own tokens (all of them where the prefix has no parts)
-    p.n_own = p.n_pre ? (own ? cut(jobs, own, SA_OWN_PER) : 1u) : prefix ? 1u : cut(jobs, own, SA_OWN_PER);
+    p.n_own = p.n_pre ? (own ? cut(jobs, own, p.tile ? SA_TILE_OWN : SA_OWN_PER) : 1u)
+              : prefix ? 1u : cut(jobs, own, SA_OWN_PER);
     p.own_len = ceil_div(ceil_div(p.n_pre ? (own ? own : 1) : max_len, p.n_own), SA_KB) * SA_KB;
     const uint64_t pre = (uint64_t)p.n_pre * p.pre_tiles * nkv, all = pre + (uint64_t)p.n_own * n_seq * nkv;
     if (all > 0x7FFFFFFFull || (uint64_t)n_seq * nh > 0x7FFFFFFFull) return false;
@@ -856,10 +904,11 @@ static int shared_launch(zh_ctx *c, const SharedArgs &a, const SharedPlan &p) {
         if (rc) return rc;
         b.pre_blocks = 0;
         blocks -= p.pre_blocks;
+        b.join = p.n_own == 1;
     }
     hipLaunchKernelGGL((k_shared_attn<HD, NP, T>), dim3(blocks), dim3(64 * SA_W), 0, c->stream, b);
     ZH_LAUNCH_CHECK(c);
-    if (a.n_pre + a.n_own > 1) {
+    if (a.n_pre + a.n_own > 1 && !b.join) {
         const uint32_t per = 256 / (HD / 4);  // rows of a workgroup
         hipLaunchKernelGGL((k_shared_join<HD, T>), dim3((a.n_seq * a.nh + per - 1) / per), dim3(256), 0, c->stream, a);
         ZH_LAUNCH_CHECK(c);
