@@ -24,24 +24,24 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr uint32_t SA_ROWS = 16;  // rows of an MFMA tile
 constexpr uint32_t SA_KB = 32;    // tokens of a wave's step
 constexpr int SA_W = 4;           // waves of a workgroup, each on its own steps
-#ifndef SA_TILE
-#define SA_TILE 96
-#endif
-#ifndef SA_TILE_OWN
-#define SA_TILE_OWN 2
-#endif
-#ifndef SA_ONE
-#define SA_ONE 512
-#endif
-#ifndef SA_RT
-#define SA_RT 2
-#endif
-#ifndef SA_PRE_PER
-#define SA_PRE_PER 1
-#endif
-#ifndef SA_OWN_PER
-#define SA_OWN_PER 4
-#endif
+// The host's choices (shared_plan), measured with 32 heads on 8, 64 own tokens a
+// sequence, f16, prefix 1024 / 4096 / 16384:
+//  * LDS tiles where the 16-row tiles' prefix tokens over the kv heads reach
+//    SA_TILE: below it one more reading of K and V through the L2s costs less
+//    than the tiles' longer launch. us streamed / tiled: 64 rows 10.3 / 13.0,
+//    14.6 / 16.3, 31.8 / 29.0; 128 rows 11.6 / 14.7, 19.9 / 22.5, 53.4 / 33.7;
+//    256 rows 15.1 / 19.3, 32.3 / 29.4, 97.2 / 42.6 (head_dim 64 and f32 cross
+//    at the same counts);
+//  * a whole context in one workgroup, prefix and own tokens, up to SA_ONE tokens
+//    and one workgroup a CU: 2 sequences at 240 tokens 7.7 us, in parts 5.8 +
+//    3.4 and the gap between them;
+//  * workgroups per CU that the parts are cut for: 1 of a prefix (16 sequences
+//    at 4096 f32 12.4 + 3.8 us, 2: 13.6 + 4.1), 8 of own tokens (48 sequences
+//    of 1 to 4096: 80.8 us, 4: 83.2), 2 where one own part per sequence also
+//    joins the prefix's (64 sequences of up to 512: 27 us, with two parts and a
+//    launch that joins them 22.9 + 8.6).
+constexpr uint64_t SA_TILE = 300000;
+constexpr uint32_t SA_ONE = 512, SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_OWN = 2;
 
 struct SharedArgs {
     const uint8_t *q;
@@ -79,6 +79,11 @@ ZH_DEV void ld8(const _Float16 *p, float (&v)[8]) {
     for (int e = 0; e < 8; e++) v[e] = (float)a[e];
 }
 
+template <bool ONCE, typename V>
+ZH_DEV V ld_kv(const V *p) {
+    return ONCE ? __builtin_nontemporal_load(p) : *p;
+}
+
 // What a workgroup of k_shared_attn does: rows row0 .. of one kv head (numbered
 // s * G + g), tokens [t0, t1) through table row `tab`, after the tokens [0, first)
 // through table row 0 (a sequence's whole context in one workgroup).
@@ -99,7 +104,8 @@ struct SharedPart {
 //   permutes; column li of the output tile n is dim HD/16 li + n.
 // NP pieces: q (scaled by a power of two to a maximum in [1, 2)) and P as sums
 // of NP fp16 values; 2 keep 22 bits of each.
-template <int HD, int NP, typename T>
+// ONCE: no other workgroup reads these K and V (loads that go by the L2s).
+template <int HD, int NP, bool ONCE, typename T>
 ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, float *lds) {
     constexpr int K4 = HD / 32, ND = HD / 16;  // k-steps of the scores, dims per lane and output tiles
     constexpr int LD = HD + 4;
@@ -139,7 +145,7 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
         for (int j = 0; j < 2; j++) {
             const uint16_t *kp = kh + ((size_t)x.pg[j] * 16 + li) * HD + 8 * lg;
 #pragma unroll
-            for (int k4 = 0; k4 < K4; k4++) kf[j][k4] = *(const half8 *)(kp + 32 * k4);
+            for (int k4 = 0; k4 < K4; k4++) kf[j][k4] = ld_kv<ONCE>((const half8 *)(kp + 32 * k4));
         }
     };
     auto load_v = [&](const Step &x) __attribute__((always_inline)) {
@@ -148,8 +154,8 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
             const uint16_t *vp = vh + ((size_t)x.pg[j] * 16 + 4 * lg) * HD + ND * li;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                if (ND == 8) *(u32x4 *)pv[j][r] = *(const u32x4 *)(vp + r * HD);
-                else *(u32x2 *)pv[j][r] = *(const u32x2 *)(vp + r * HD);
+                if (ND == 8) *(u32x4 *)pv[j][r] = ld_kv<ONCE>((const u32x4 *)(vp + r * HD));
+                else *(u32x2 *)pv[j][r] = ld_kv<ONCE>((const u32x2 *)(vp + r * HD));
             }
         }
     };
@@ -372,6 +378,7 @@ __global__ __launch_bounds__(64 * SA_W, 3) void k_shared_attn(SharedArgs a) {
         w.tab = 0;
         w.t0 = w.part * a.pre_len;
         w.t1 = min(w.t0 + a.pre_len, a.prefix);
+        shared_part<HD, NP, false, T>(a, w, kvh, lds);
     } else {
         const uint32_t s = job / a.nkv % a.n_seq, p = job / a.nkv / a.n_seq;
         w.part = a.n_pre + p;
@@ -387,8 +394,8 @@ __global__ __launch_bounds__(64 * SA_W, 3) void k_shared_attn(SharedArgs a) {
         w.t0 = b + p * c;
         w.t1 = min(w.t0 + c, len);
         if (!a.n_pre && a.prefix && len >= a.prefix) w.first = w.t0 = a.prefix;  // (one part: the whole context)
+        shared_part<HD, NP, true, T>(a, w, kvh, lds);
     }
-    shared_part<HD, NP, T>(a, w, kvh, lds);
 }
 
 // Many rows (a workgroup: 4 waves of 32 RT): K and V pass through LDS once for
@@ -806,7 +813,8 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
     p = {};
     if (prefix && (prefix + own > SA_ONE || jobs > cus)) {
         // rows of a prefix workgroup: 128 or 256 on LDS tiles, or 16 streamed
-        p.tile = rows_kv >= SA_TILE ? (rows_kv > 128 && SA_RT > 1 ? 2 : 1) : 0;
+        const uint64_t through = (rows_kv + SA_ROWS - 1) / SA_ROWS * prefix * nkv;
+        p.tile = rows_kv > 2 * SA_ROWS && through >= SA_TILE ? (rows_kv > 128 ? 2 : 1) : 0;
         p.pre_tiles = ceil_div(rows_kv, p.tile ? 128u * p.tile : SA_ROWS);
         const uint32_t n = cut((uint64_t)p.pre_tiles * nkv, prefix, p.tile ? 1 : SA_PRE_PER);
         const uint32_t step = p.tile ? ST_KB : SA_KB;
