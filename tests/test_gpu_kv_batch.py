@@ -259,31 +259,33 @@ def test_rope_rows_outside_are_left_out_and_reported(zh, ctx):
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
-def attend64(q, kc, vc, tables, lens, scale, t, P=0):
+def attend64(q, kc, vc, tables, lens, scale, t, P=0, only=None):
     """(out, bound) of the module's formula; q [S][nh][hd]. The first P tokens
-    of the sequences that long are read through sequence 0's table."""
+    of the sequences that long are read through sequence 0's table. only: the
+    sequences worked out."""
     S, nh, hd = q.shape
     nkv = kc.shape[0]
     G = nh // nkv
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
-    for s in range(S):
+    for s in range(S) if only is None else only:
         n = int(lens[s])
         if n == 0:
             continue
         tk = np.arange(n)
         via = np.where((tk < P) & (n >= P), 0, s)
         at = tables[via, tk // 16].astype(np.int64) * 16 + tk % 16
-        for h in range(nh):
-            k, v = kc[h // G, at].astype(np.float64), vc[h // G, at].astype(np.float64)
-            x = q[s, h].astype(np.float64)
-            sc = k @ x * scale
-            A = 1.45 * scale * (np.abs(k) @ np.abs(x)).max()
-            w = np.exp(sc - sc.max())
-            w /= w.sum()
-            out[s, h], W = w @ v, w @ np.abs(v)
-            tol[s, h] = W * (2.0 ** -17 * A + (n / 32 + 80) * 2.0 ** -23) + store_error(t, out[s, h])
+        for g in range(nkv):
+            hs = slice(g * G, g * G + G)
+            k, v = kc[g, at].astype(np.float64), vc[g, at].astype(np.float64)
+            x = q[s, hs].astype(np.float64)
+            sc = x @ k.T * scale
+            A = 1.45 * abs(scale) * (np.abs(x) @ np.abs(k).T).max(1, keepdims=True)
+            w = np.exp(sc - sc.max(1, keepdims=True))
+            w /= w.sum(1, keepdims=True)
+            out[s, hs], W = w @ v, w @ np.abs(v)
+            tol[s, hs] = W * (2.0 ** -17 * A + (n / 32 + 80) * 2.0 ** -23) + store_error(t, out[s, hs])
             if t == 1:
-                tol[s, h] += W * 2.0 ** -11
+                tol[s, hs] += W * 2.0 ** -11
     return out, tol
 
 
@@ -310,17 +312,16 @@ def make(rng, S, nkv, hd, P, lens, shared=True, spare=2, poison=True):
         tables[s, :k] = perm[:k]
         tables[s, k:k + own[s]] = perm[at:at + own[s]]
         at += own[s]
-    base = [rng.standard_normal((P, nkv, hd)).astype(np.float16) for _ in range(2)]
+    base = [rng.standard_normal((P, nkv, hd), dtype=np.float32).astype(np.float16) for _ in range(2)]
     for s in range(S):
-        n = int(lens[s])
-        if s == 0:
-            n = max(n, P)
-        t = np.arange(n)
+        n = max(int(lens[s]), P) if s == 0 else int(lens[s])
+        first = full * 16 if s and n >= P else 0  # (the shared pages are written once)
+        t = np.arange(first, n)
         slots = tables[s, t // 16].astype(np.int64) * 16 + t % 16
         for c, b in zip((kc, vc), base):
-            x = rng.standard_normal((n, nkv, hd)).astype(np.float16)
+            x = rng.standard_normal((n - first, nkv, hd), dtype=np.float32).astype(np.float16)
             if n >= P:
-                x[:P] = b
+                x[:P - first] = b[first:]
             c[:, slots] = x.transpose(1, 0, 2)
     return kc, vc, tables, total * 16, M
 
@@ -389,6 +390,53 @@ def test_attention(zh, ctx, case, t):
     got = run_attention(zh, ctx, q, kc, vc, tables, lens, P, M, t, gap=8 * (P % 2))
     want, tol = attend64(q, kc, vc, tables, lens, hd ** -0.5, t, P)
     close(got, want, tol)
+
+
+TILED = [  # many rows over a long prefix: K and V through LDS, 128 or 256 rows a workgroup
+    (64, 4, 128, 1237, [0, 1237, 5] + [1238 + 3 * i for i in range(60)]),   # 1008 rows, 4 workgroups
+    (128, 8, 128, 4701, [4701 + 17 * i for i in range(8)]),                 # 128 rows
+    (48, 8, 64, 12601, [12650, 12601, 400, 12640, 12602, 12700, 13000]),    # 42 rows
+    (16, 4, 64, 5000, [5001 + i for i in range(70)]),                       # 280 rows
+    (64, 64, 64, 4510, [4511 + i % 5 for i in range(130)]),                 # parts of more than 64 pages
+    (33, 33, 128, 7000, [7001 + 70 * i % 600 for i in range(34)]),          # own tokens in parts of their own
+]
+
+
+@pytest.mark.parametrize("t", [0, 1], ids=["f32", "f16"])
+@pytest.mark.parametrize("case", TILED, ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}-{c[3]}-{len(c[4])}x{max(c[4])}")
+def test_attention_of_many_rows(zh, ctx, case, t):
+    nh, nkv, hd, P, lens = case
+    rng = np.random.default_rng(nh * 100 + P)
+    kc, vc, tables, _, M = make(rng, len(lens), nkv, hd, P, lens)
+    q = (rng.standard_normal((len(lens), nh, hd)) * 1.5).astype(NP_TYPE[t])
+    scale = -0.11 if nh == 16 else hd ** -0.5
+    got = run_attention(zh, ctx, q, kc, vc, tables, lens, P, M, t, scale=scale)
+    assert np.isfinite(got).all()
+    only = sorted({0, 1, 2, len(lens) // 2, len(lens) - 1})
+    want, tol = attend64(q, kc, vc, tables, lens, scale, t, P, only)
+    close(got[only], want[only], tol[only])
+
+
+def test_attention_rescales_when_later_scores_are_larger(zh, ctx):
+    """Scores that grow along a prefix of 1408 tokens by about 2^15 in all, in
+    tiles and streamed: the running maximum moves again and again."""
+    rng = np.random.default_rng(21)
+    P, lens = 1408, [1410 + i for i in range(64)]
+    kc, vc, tables, _, M = make(rng, 64, 4, 128, P, lens)
+    q = rng.standard_normal((64, 64, 128)).astype(np.float16)
+    t = np.arange(P)
+    slots = tables[0, t // 16].astype(np.int64) * 16 + t % 16
+    u = rng.standard_normal(128)
+    u /= np.linalg.norm(u)
+    q = (q + 6 * u).astype(np.float16)  # every row along u, every K further along it
+    kc[:, slots] = (kc[:, slots].astype(np.float64) + (t / P * 20)[None, :, None] * u).astype(np.float16)
+    for typ in (0, 1):
+        x = q.astype(NP_TYPE[typ])
+        for n in (64, 3):  # 1024 rows a kv head, and 48
+            got = run_attention(zh, ctx, x[:n], kc, vc, tables[:n], lens[:n], P, M, typ)
+            only = [0, n - 1]
+            want, tol = attend64(x[:n], kc, vc, tables[:n], lens[:n], 128 ** -0.5, typ, P, only)
+            close(got[only], want[only], tol[only])
 
 
 @pytest.mark.parametrize("t", [0, 1], ids=["f32", "f16"])
