@@ -23,7 +23,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t SA_ROWS = 16;  // rows of an MFMA tile
 constexpr uint32_t SA_KB = 32;    // tokens of a wave's step
-constexpr int SA_W = 4;           // waves of a workgroup, each on its own steps
 // The host's choices (shared_plan), measured with 32 heads on 8, 64 own tokens a
 // sequence, f16, prefix 1024 / 4096 / 16384:
 //  * LDS tiles where the 16-row tiles' prefix tokens over the kv heads reach
@@ -32,16 +31,20 @@ constexpr int SA_W = 4;           // waves of a workgroup, each on its own steps
 //    14.6 / 16.3, 31.8 / 29.0; 128 rows 11.6 / 14.7, 19.9 / 22.5, 53.4 / 33.7;
 //    256 rows 15.1 / 19.3, 32.3 / 29.4, 97.2 / 42.6 (head_dim 64 and f32 cross
 //    at the same counts);
-//  * a whole context in one workgroup, prefix and own tokens, up to SA_ONE tokens
-//    and one workgroup a CU: 2 sequences at 240 tokens 7.7 us, in parts 5.8 +
-//    3.4 and the gap between them;
+//  * a whole context, prefix and own tokens, in one workgroup of 8 waves (4 up
+//    to 128 tokens) where there is at most one workgroup per CU: up to 512
+//    tokens, with at most a quarter of the CUs busy up to 320. us whole / in
+//    parts: 2 sequences at 240 tokens 6.6 / 7.5, at 500 8.7 / 7.7; 32 sequences
+//    at 500 13.2 / 16.9, of 1 to 1000 20.3 / 21.6;
 //  * workgroups per CU that the parts are cut for: 1 of a prefix (16 sequences
-//    at 4096 f32 12.4 + 3.8 us, 2: 13.6 + 4.1), 8 of own tokens (48 sequences
-//    of 1 to 4096: 80.8 us, 4: 83.2), 2 where one own part per sequence also
-//    joins the prefix's (64 sequences of up to 512: 27 us, with two parts and a
-//    launch that joins them 22.9 + 8.6).
+//    at 4096 f32 12.4 + 3.8 us, 2: 13.6 + 4.1), 8 of own tokens (64 sequences
+//    of 1 to 4000 106 us, 3: 113, 12: 105; all of 1000 50.9, 3: 48.2), 2 where
+//    one own part per sequence also joins the prefix's (64 sequences of up to
+//    512: 27 us, with two parts and a launch that joins them 22.9 + 8.6);
+//  * parts of at least 128 tokens, a step for each wave; own ones of 256 where
+//    the sequences alone fill the CUs (128 sequences of 1 to 200: 16.1 us, 19.9).
 constexpr uint64_t SA_TILE = 300000;
-constexpr uint32_t SA_ONE = 512, SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_OWN = 2;
+constexpr uint32_t SA_ONE = 512, SA_ONE_FEW = 320, SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_OWN = 2;
 
 struct SharedArgs {
     const uint8_t *q;
@@ -105,11 +108,11 @@ struct SharedPart {
 // NP pieces: q (scaled by a power of two to a maximum in [1, 2)) and P as sums
 // of NP fp16 values; 2 keep 22 bits of each.
 // ONCE: no other workgroup reads these K and V (loads that go by the L2s).
-template <int HD, int NP, bool ONCE, typename T>
+template <int HD, int NP, int W, bool ONCE, typename T>
 ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, float *lds) {
     constexpr int K4 = HD / 32, ND = HD / 16;  // k-steps of the scores, dims per lane and output tiles
     constexpr int LD = HD + 4;
-    float *const so = lds, *const sm = lds + SA_W * SA_ROWS * LD, *const sl = sm + SA_W * SA_ROWS;
+    float *const so = lds, *const sm = lds + W * SA_ROWS * LD, *const sl = sm + W * SA_ROWS;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t li = lane % 16, lg = lane / 16;
     // steps start on a page; tokens outside their range are masked
@@ -204,10 +207,10 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
 #pragma unroll
     for (int n = 0; n < ND; n++) o[n] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;  // the row's maximum (every lg alike), this lane's share of its sum
-    for (uint32_t st = wave; st < nstep; st += SA_W) {
-        const bool more = st + SA_W < nstep;
+    for (uint32_t st = wave; st < nstep; st += W) {
+        const bool more = st + W < nstep;
         Step nx = x;
-        if (more) nx = step(st + SA_W);
+        if (more) nx = step(st + W);
         const bool whole = x.tk >= x.lo && x.tk + SA_KB <= x.hi;
         float s[2][4], mb = -INFINITY;
 #pragma unroll
@@ -287,15 +290,15 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
         sl[wave * SA_ROWS + li] = l;
     }
     __syncthreads();
-    for (uint32_t i = tid; i < w.nrow * (HD / 4); i += 64 * SA_W) {
+    for (uint32_t i = tid; i < w.nrow * (HD / 4); i += 64 * W) {
         const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4, R = w.row0 + r, s = R / a.G, h = kvh * a.G + R % a.G;
         float M = sm[r], L = 0.f;
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 1; k < SA_W; k++) M = fmaxf(M, sm[k * SA_ROWS + r]);
+        for (int k = 1; k < W; k++) M = fmaxf(M, sm[k * SA_ROWS + r]);
         const float Ms = M == -INFINITY ? 0.f : M;
 #pragma unroll
-        for (int k = 0; k < SA_W; k++) {
+        for (int k = 0; k < W; k++) {
             const float fk = __builtin_amdgcn_exp2f(sm[k * SA_ROWS + r] - Ms);
             const f32x4 v = *(const f32x4 *)(so + (k * SA_ROWS + r) * LD + d);
             O.x = fmaf(v.x, fk, O.x);
@@ -360,9 +363,9 @@ ZH_DEV uint32_t own_tokens(const SharedArgs &a, uint32_t len, uint32_t &b, uint3
 }
 
 // The prefix's workgroups, then the sequences' own.
-template <int HD, int NP, typename T>
-__global__ __launch_bounds__(64 * SA_W, 3) void k_shared_attn(SharedArgs a) {
-    __shared__ __align__(16) float lds[SA_W * SA_ROWS * (HD + 6)];
+template <int HD, int NP, int W, typename T>
+__global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void k_shared_attn(SharedArgs a) {
+    __shared__ __align__(16) float lds[W * SA_ROWS * (HD + 6)];
     const bool pre = blockIdx.x < a.pre_blocks;
     // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
     const uint32_t job = pre ? blockIdx.x : blockIdx.x - a.pre_blocks, kvh = job % a.nkv;
@@ -378,7 +381,7 @@ __global__ __launch_bounds__(64 * SA_W, 3) void k_shared_attn(SharedArgs a) {
         w.tab = 0;
         w.t0 = w.part * a.pre_len;
         w.t1 = min(w.t0 + a.pre_len, a.prefix);
-        shared_part<HD, NP, false, T>(a, w, kvh, lds);
+        shared_part<HD, NP, W, false, T>(a, w, kvh, lds);
     } else {
         const uint32_t s = job / a.nkv % a.n_seq, p = job / a.nkv / a.n_seq;
         w.part = a.n_pre + p;
@@ -394,7 +397,7 @@ __global__ __launch_bounds__(64 * SA_W, 3) void k_shared_attn(SharedArgs a) {
         w.t0 = b + p * c;
         w.t1 = min(w.t0 + c, len);
         if (!a.n_pre && a.prefix && len >= a.prefix) w.first = w.t0 = a.prefix;  // (one part: the whole context)
-        shared_part<HD, NP, true, T>(a, w, kvh, lds);
+        shared_part<HD, NP, W, true, T>(a, w, kvh, lds);
     }
 }
 
@@ -795,7 +798,7 @@ __global__ __launch_bounds__(256) void k_shared_join(SharedArgs a) {
 
 // How a call is cut (the same for every call of these sizes).
 struct SharedPlan {
-    uint32_t n_pre, n_own, pre_tiles, pre_len, own_len, pre_blocks, blocks, tile;
+    uint32_t n_pre, n_own, pre_tiles, pre_len, own_len, pre_blocks, blocks, tile, waves;
     uint64_t stat_off, bytes;  // of ws
 };
 
@@ -805,26 +808,28 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
                  SharedPlan &p) {
     const uint32_t G = nh / nkv, own = max_len - prefix;
     const uint64_t rows_kv = (uint64_t)n_seq * G, jobs = (uint64_t)n_seq * nkv;
-    // parts for `per` workgroups per CU, of at least 128 tokens
-    auto cut = [&](uint64_t n, uint32_t tokens, uint32_t per) {
-        const uint32_t most = ceil_div(tokens, 128), want = (uint32_t)(((uint64_t)per * cus + n / 2) / n);
+    // parts for `per` workgroups per CU, of at least `least` tokens
+    auto cut = [&](uint64_t n, uint32_t tokens, uint32_t per, uint32_t least) {
+        const uint32_t most = ceil_div(tokens, least), want = (uint32_t)(((uint64_t)per * cus + n / 2) / n);
         return want < 1 ? 1u : want < most ? want : most;
     };
     p = {};
-    if (prefix && (prefix + own > SA_ONE || jobs > cus)) {
+    const bool one = jobs <= cus && max_len <= (4 * jobs <= cus ? SA_ONE_FEW : SA_ONE);
+    p.waves = one && max_len > 4 * SA_KB ? 8 : 4;
+    if (prefix && !one) {
         // rows of a prefix workgroup: 128 or 256 on LDS tiles, or 16 streamed
         const uint64_t through = (rows_kv + SA_ROWS - 1) / SA_ROWS * prefix * nkv;
         p.tile = rows_kv > 2 * SA_ROWS && through >= SA_TILE ? (rows_kv > 128 ? 2 : 1) : 0;
         p.pre_tiles = ceil_div(rows_kv, p.tile ? 128u * p.tile : SA_ROWS);
-        const uint32_t n = cut((uint64_t)p.pre_tiles * nkv, prefix, p.tile ? 1 : SA_PRE_PER);
+        const uint32_t n = cut((uint64_t)p.pre_tiles * nkv, prefix, SA_PRE_PER, 128);
         const uint32_t step = p.tile ? ST_KB : SA_KB;
         p.pre_len = ceil_div(ceil_div(prefix, n), step) * step;
         p.n_pre = ceil_div(prefix, p.pre_len);
     }
     // a sequence's own tokens (all of them where the prefix has no parts)
-    p.n_own = p.n_pre ? (own ? cut(jobs, own, p.tile ? SA_TILE_OWN : SA_OWN_PER) : 1u)
-              : prefix ? 1u : cut(jobs, own, SA_OWN_PER);
-    p.own_len = ceil_div(ceil_div(p.n_pre ? (own ? own : 1) : max_len, p.n_own), SA_KB) * SA_KB;
+    const uint32_t tokens = p.n_pre ? (own ? own : 1) : max_len;
+    p.n_own = one ? 1 : cut(jobs, tokens, p.tile ? SA_TILE_OWN : SA_OWN_PER, jobs >= cus ? 256 : 128);
+    p.own_len = ceil_div(ceil_div(tokens, p.n_own), SA_KB) * SA_KB;
     const uint64_t pre = (uint64_t)p.n_pre * p.pre_tiles * nkv, all = pre + (uint64_t)p.n_own * n_seq * nkv;
     if (all > 0x7FFFFFFFull || (uint64_t)n_seq * nh > 0x7FFFFFFFull) return false;
     p.pre_blocks = (uint32_t)pre;
@@ -914,7 +919,8 @@ static int shared_launch(zh_ctx *c, const SharedArgs &a, const SharedPlan &p) {
         blocks -= p.pre_blocks;
         b.join = p.n_own == 1;
     }
-    hipLaunchKernelGGL((k_shared_attn<HD, NP, T>), dim3(blocks), dim3(64 * SA_W), 0, c->stream, b);
+    if (p.waves == 8) hipLaunchKernelGGL((k_shared_attn<HD, NP, 8, T>), dim3(blocks), dim3(512), 0, c->stream, b);
+    else hipLaunchKernelGGL((k_shared_attn<HD, NP, 4, T>), dim3(blocks), dim3(256), 0, c->stream, b);
     ZH_LAUNCH_CHECK(c);
     if (a.n_pre + a.n_own > 1 && !b.join) {
         const uint32_t per = 256 / (HD / 4);  // rows of a workgroup
