@@ -314,7 +314,8 @@ int zh_flash_decode_shared(zh_ctx *ctx, const zh_kv_batch *kv, const zh_decode_r
 uint64_t zh_flash_decode_shared_ws(zh_ctx *ctx, const zh_kv_batch *kv, uint32_t n_heads, uint32_t prefix_len,
                                    uint32_t max_len);
 /* A set of at most 256 caches of one shape (the K and V caches of some or all
- * layers). */
+ * layers), fp16 [n_kv_heads][cache_tokens][head_dim] each, cache_tokens a
+ * multiple of 16. */
 typedef struct zh_kv_caches {
     zh_buf *const *caches;
     uint32_t n_caches, cache_tokens, n_kv_heads, head_dim;

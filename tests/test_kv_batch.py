@@ -194,6 +194,7 @@ def test_copy_refusals():
     assert copy_check(a, KvCaches(bufs[2:3], tokens, nkv, hd), [1], [1]) == INVALID
     assert copy_check(a, KvCaches(bufs[2:], tokens, 1, hd), [1], [1]) == INVALID
     assert copy_check(KvCaches(bufs[:2], tokens + 16, nkv, hd), b, [1], [1]) == INVALID  # past the buffers
+    assert copy_check(KvCaches(bufs[:2], 150, nkv, hd), KvCaches(bufs[2:], 150, nkv, hd), [1], [1]) == INVALID
     assert copy_check(KvCaches([], tokens, nkv, hd), KvCaches([], tokens, nkv, hd), [1], [1]) == INVALID
     assert copy_check(KvCaches(bufs[:2], tokens // 2, nkv, hd), a, [1], [2]) == INVALID  # one cache in two sizes
     many = [Fake(4096) for _ in range(256)]
@@ -269,6 +270,19 @@ def test_bad_rows_types_and_overlaps():
     assert rows_check(batch(), qkv(v=q, q_out=q)) == INVALID
 
 
+def test_bad_rows_written_inputs():
+    kv = batch()
+    bufs = {n: Fake(1 << 20) for n in ("pos", "seq", "inv_freq", "q_norm_w", "k_norm_w")}
+    for n, b in bufs.items():
+        assert rows_check(kv, qkv(**{n: b})) == OK and rows_check(kv, qkv(**{n: b, "q_out": b})) == INVALID
+    cache, tables = Fake(1 << 20), Fake(1 << 20)
+    assert rows_check(batch(k_cache=cache, v_cache=cache), qkv()) == INVALID
+    for n in ("q", "k", "v", "q_out", "pos"):
+        assert rows_check(batch(k_cache=cache), qkv(**{n: cache})) == INVALID
+        assert rows_check(batch(v_cache=cache), qkv(**{n: cache})) == INVALID
+    assert rows_check(batch(tables=tables), qkv(q_out=tables)) == INVALID
+
+
 def decode(nh=6, **over):
     f = dict(q=Fake(4 * SEQS * nh * HD), out=Fake(4 * SEQS * nh * HD), seq_lens=Fake(4 * SEQS), ws=Fake(1 << 24),
              n_heads=nh, prefix_len=40, max_len=128)
@@ -308,6 +322,19 @@ def test_bad_decode_rest():
     assert decode_check(batch(), decode(max_len=129)) == TOO_LONG
     assert decode_check(batch(), decode(type=8)) == UNSUPPORTED
     assert decode_check(batch(head_dim=96), decode()) == INVALID
+    wide = dict(table_stride=1 << 27, tables=Fake(4 * SEQS << 27))
+    assert decode_check(batch(**wide), decode(max_len=(1 << 30) + 1, ws=Fake(1 << 40))) == INVALID
+    one = Fake(1 << 30)
+    for n in ("k_cache", "v_cache", "tables"):
+        assert decode_check(batch(**{n: one}), decode(out=one)) == INVALID
+        kv = dict(table_stride=1024, tables=Fake(4 * SEQS * 1024))
+        kv[n] = one
+        assert decode_check(batch(**kv), decode(max_len=16000, ws=Fake(1 << 30))) == OK
+        assert decode_check(batch(**kv), decode(max_len=16000, ws=one)) == INVALID
+    for n in ("q", "out", "seq_lens"):
+        kv = batch(table_stride=1024, tables=Fake(4 * SEQS * 1024))
+        assert decode_check(kv, decode(max_len=16000, ws=one, **{n: one})) == INVALID
+    assert decode_check(batch(), decode(seq_lens=one, out=one)) == INVALID
     q = Fake(4 * SEQS * 8 * HD)
     assert decode_check(batch(), decode(q=q, out=q, out_off=4 * HD)) == INVALID
 

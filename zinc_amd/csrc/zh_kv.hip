@@ -104,15 +104,15 @@ int zhk_kv_copy(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *cons
 constexpr uint32_t KC_MAX = 256;  // caches of a call
 static bool caches_ok(const zh_kv_caches *s) {
     if (!s || !s->caches || s->n_caches == 0 || s->n_caches > KC_MAX || s->n_kv_heads == 0 || s->n_kv_heads > 65535 || s->head_dim == 0 ||
-        s->head_dim > 1024 || s->cache_tokens == 0)
+        s->head_dim > 1024 || s->cache_tokens == 0 || s->cache_tokens % 16)
         return false;
     for (uint32_t i = 0; i < s->n_caches; i++)
         if (!kv_in_range(s->caches[i], 0, 2ull * s->n_kv_heads * s->cache_tokens * s->head_dim)) return false;
     return true;
 }
 
-// The checks of zh_kv_copy_pages, of host data only (c may be null: no
-// message then). `mark` and `call`: see zh_ctx::page_mark.
+// The checks of zh_kv_copy_pages, of host data only (exported for the tests; c
+// may be null: no message then). `mark` and `call`: see zh_ctx::page_mark.
 extern "C" int zh_check_kv_copy_pages(zh_ctx *c, const zh_kv_caches *dst, const zh_kv_caches *src,
                                       const uint32_t *dst_pages, const uint32_t *src_pages, uint32_t n_pages) {
     const bool one = dst && src && dst->caches == src->caches && dst->n_caches == src->n_caches;
@@ -395,7 +395,7 @@ bool kv_batch_ok(const zh_kv_batch *kv) {
            kv->n_kv_heads <= 65535 && kv->head_dim && kv->head_dim <= 512 &&
            kv_in_range(kv->k_cache, 0, 2ull * kv->n_kv_heads * kv->cache_tokens * kv->head_dim) &&
            kv_in_range(kv->v_cache, 0, 2ull * kv->n_kv_heads * kv->cache_tokens * kv->head_dim) &&
-           kv_in_range(kv->tables, 0, 4ull * kv->n_seq * kv->table_stride);
+           kv_in_range(kv->tables, 0, 4ull * kv->n_seq * kv->table_stride) && kv->k_cache->ptr != kv->v_cache->ptr;
 }
 
 bool kv_rows_overlap(const zh_buf *a, uint64_t a0, uint64_t an, const zh_buf *b, uint64_t b0, uint64_t bn) {
@@ -413,7 +413,8 @@ static zh_qkv_rows with_strides(const zh_kv_batch *kv, const zh_qkv_rows *r) {
     return x;
 }
 
-// The checks of zh_qk_norm_rope_kv_write_batched, of host data only.
+// The checks of zh_qk_norm_rope_kv_write_batched, of host data only (exported
+// for the tests; c may be null: no message then).
 extern "C" int zh_check_qkv_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_qkv_rows *rows) {
     if (!kv_batch_ok(kv) || !rows) return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: cache or tables");
     const zh_qkv_rows x = with_strides(kv, rows), *r = &x;
@@ -439,7 +440,16 @@ extern "C" int zh_check_qkv_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_qkv_
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: range");
     if (r->q_off % si || r->k_off % si || r->v_off % si || r->q_out_off % so)
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: offset alignment");
-    // q_out: q's own rows, or apart from everything that is read
+    // q_out and the caches: written; q_out q's own rows, or apart from everything
+    // that is read
+    const zh_buf *const read[] = {kv->tables, r->pos, r->seq, r->q_norm_w, r->k_norm_w, r->rope_dim ? r->inv_freq : nullptr};
+    for (const zh_buf *b : read)
+        if (b && (b->ptr == r->q_out->ptr || b->ptr == kv->k_cache->ptr || b->ptr == kv->v_cache->ptr))
+            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: an input is written");
+    const zh_buf *const rows4[] = {r->q, r->k, r->v, r->q_out};
+    for (const zh_buf *b : rows4)
+        if (b->ptr == kv->k_cache->ptr || b->ptr == kv->v_cache->ptr)
+            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: rows in a cache");
     const bool same = r->q_out->ptr == r->q->ptr && r->q_out_off == r->q_off && r->q_out_type == r->type &&
                       (r->q_out_stride == r->q_stride || n == 1);
     if ((!same && kv_rows_overlap(r->q_out, r->q_out_off, ob, r->q, r->q_off, qb) &&

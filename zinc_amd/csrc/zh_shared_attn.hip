@@ -12,6 +12,8 @@
 // result itself.
 #include <math.h>
 
+#include <atomic>
+
 #include "zh_device.h"
 #include "zh_internal.h"
 #include "zh_kv.h"
@@ -401,18 +403,25 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void k_shared_attn(SharedAr
     }
 }
 
-// Many rows (a workgroup: 4 waves of 32 RT): K and V pass through LDS once for
-// all of them, in stages of 64 tokens copied there four ahead without passing
-// registers (each wave one page of a stage).
+// Many rows (a workgroup: 8 or 4 waves of 32): K and V pass through LDS once for
+// all of them, in stages of 64 tokens copied there three ahead without passing
+// registers.
 //   S^T = K q^T by v_mfma_f32_32x32x16_f16: lane (i = lane % 32, h = lane / 32)
 //   holds tokens 8 (r / 4) + 4 h + r % 4 of row i in register r; registers
 //   8 s .. 8 s + 7 are the weights' operand of the s-th 16-token product
 //   O^T += V^T P^T. V stays row-major in LDS, its transposed fragments come from
-//   ds_read_b64_tr_b16. 16-byte pieces of a row lie at piece ^ (row % pieces),
-//   so that 32 rows' reads of one piece hit every bank alike.
+//   ds_read_b64_tr_b16. 16-byte piece p of a row lies at p ^ st_swz(row), so that
+//   16 rows' reads of one piece hit every bank once and the transposing reads
+//   (4 pieces of 8 rows) every bank twice.
 // The products of the next 32 tokens' scores run while the current ones' weights
 // are computed. The reference maximum moves only when a score passes it by 2^8
 // (the weights then reach 2^12 in fp16 at most), so the output is rarely rescaled.
+// Bound by the matrix units: 2000 rows a kv head over 8192 tokens (34 GFLOP)
+// 48 us, of which 6 before the first product, 6 for the parts' stores (33 MB)
+// and 26 the products alone (1.3 PFLOP/s, a large library product's rate); the
+// rest is the softmax (4), the copies and the LDS reads (4) where they do not
+// hide. 4 waves of 64 rows, each K and V fragment for two products: 70 us (past
+// 256 registers the accumulators move between the two register files).
 constexpr uint32_t ST_KB = 64, ST_NS = 4;
 template <int HD>
 constexpr uint32_t st_lds() { return 2 * ST_NS * ST_KB * HD * 2; }
@@ -433,8 +442,7 @@ ZH_DEV void dma16_s(const void *base, uint32_t off, uint32_t lds) {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <int HD, int NP, int NW, typename T>
-__global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
-    constexpr int RT = 1;
+__global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) void k_shared_tile(SharedArgs a) {
     constexpr int KS = HD / 16, DT = HD / 32;       // k-steps of the scores, 32-dim tiles of the output
     constexpr uint32_t ROWB = HD * 2, PPR = HD / 8;  // bytes and 16-byte pieces of a row
     constexpr uint32_t STAGE = ST_KB * ROWB, NI = 16 * ROWB / 1024;  // bytes of a stage, copies of a page
@@ -446,7 +454,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
     // (the row tiles of one part and kv head on one XCD: they read the same K and V)
     const uint32_t per = a.nkv * a.n_pre, tile = blockIdx.x / per, kvh = blockIdx.x % per % a.nkv;
     const uint32_t part = blockIdx.x % per / a.nkv;
-    const uint32_t rows = a.n_seq * a.G, row0 = tile * (32 * RT * NW) + wave * (32 * RT);
+    const uint32_t rows = a.n_seq * a.G, row0 = (tile * NW + wave) * 32;
     const bool mine = row0 < rows;  // (uniform per wave: it has rows)
     const uint32_t t0 = part * a.pre_len, t1 = min(t0 + a.pre_len, a.prefix);
     const uint32_t nst = (t1 - t0 + ST_KB - 1) / ST_KB;
@@ -501,29 +509,27 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
     };
     // the first copies go out before the rows are read
     for (uint32_t st = 0; st < 3 && st < nst; st++) issue(st);
-    // ---- the rows' q: dims 16 k + 8 h ..
-    half8 qf[RT][NP][KS];
-    float c[RT];
-#pragma unroll
-    for (int q = 0; q < RT; q++) {
-        const uint32_t row = min(row0 + 32 * q + i32, rows - 1);
-        const uint8_t *qp = a.q + row / a.G * a.q_row + (size_t)(kvh * a.G + row % a.G) * HD * sizeof(T);
+    // ---- the row's q: dims 16 k + 8 h ..
+    half8 qf[NP][KS];
+    float c = fabsf(a.scale) * 1.44269504088896340736f;  // raw scores to base 2
+    {
+        const uint32_t row = min(row0 + i32, rows - 1);
+        const T *qp = (const T *)(a.q + row / a.G * a.q_row) + (size_t)(kvh * a.G + row % a.G) * HD + 8 * h;
         float v[KS][8], mx = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            ld8((const T *)qp + 16 * k + 8 * h, v[k]);
+            ld8(qp + 16 * k, v[k]);
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k][e]));
         }
         // (the scale's sign goes into q: the largest product is the largest score)
         float up = a.scale < 0.f ? -1.f : 1.f;
-        c[q] = fabsf(a.scale) * 1.44269504088896340736f;
         if (NP > 1) {
             mx = xor32_max(mx);
             const uint32_t E = __float_as_uint(mx) >> 23;
             if (E >= 8 && E <= 246) {
                 up *= __uint_as_float((254u - E) << 23);
-                c[q] *= __uint_as_float(E << 23);
+                c *= __uint_as_float(E << 23);
             }
         }
 #pragma unroll
@@ -533,22 +539,17 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
                 float x = v[k][e] * up;
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
-                    qf[q][p][k][e] = (_Float16)x;
-                    x -= (float)qf[q][p][k][e];
+                    qf[p][k][e] = (_Float16)x;
+                    x -= (float)qf[p][k][e];
                 }
             }
     }
-    f32x16 o[RT][DT];
-    float m[RT], l[RT];
+    f32x16 o[DT];
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int q = 0; q < RT; q++) {
-        m[q] = -INFINITY;
-        l[q] = 0.f;
+    for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[q][d][r] = 0.f;
-    }
+        for (int r = 0; r < 16; r++) o[d][r] = 0.f;
     // fragment addresses in a stage (their k-step and 32-dim tile by exclusive or)
     const uint32_t ka = i32 * ROWB + ((h ^ st_swz<PPR>(i32)) * 16);
     const uint32_t l16 = lane % 16, vr = 4 * h + l16 / 4, vp = 2 * (lane / 16 % 2) + l16 % 4 / 2;
@@ -562,33 +563,24 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
         vp0[d] = lds + ST_NS * STAGE + (va ^ (d * 64));
         vp1[d] = lds + ST_NS * STAGE + 8 * ROWB + (va ^ (d * 64) ^ 32);
     }
-    f32x16 s[RT], sn[RT];  // scores of the current and the next 32 tokens (raw)
-    half8 kf[KS];          // K fragments of the next ones
+    f32x16 s, sn;  // scores of the current and the next 32 tokens (raw)
+    half8 kf[KS];  // K fragments of the next ones
     auto load_k = [&](uint32_t slot, uint32_t kt) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < KS; k++) kf[k] = *(const half8 *)(kp[k] + slot * STAGE + kt * 32 * ROWB);
     };
-    // the reference maximum for scores d: moved, and the sums with it, where one
-    // (largest: mx) passes it by 2^8
-    auto refer = [&](float (&mx)[RT]) __attribute__((always_inline)) {
-        bool up = false;
+    // the reference maximum, for scores up to mx: moved, and the sums with it,
+    // where one passes it by 2^8
+    auto refer = [&](float mx) __attribute__((always_inline)) {
+        mx = xor32_max(mx) * c;
+        if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= f;
 #pragma unroll
-        for (int q = 0; q < RT; q++) {
-            mx[q] = xor32_max(mx[q]) * c[q];
-            up = up || mx[q] > m[q] + 8.f;
-        }
-        if (__builtin_amdgcn_ballot_w64(up)) {
+            for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int q = 0; q < RT; q++) {
-                const float mn = fmaxf(m[q], mx[q]);
-                const float f = __builtin_amdgcn_exp2f(m[q] - (mn == -INFINITY ? 0.f : mn));
-                m[q] = mn;
-                l[q] *= f;
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) o[q][d][r] *= f;
-            }
+                for (int r = 0; r < 16; r++) o[d][r] *= f;
         }
     };
     auto largest = [&](const f32x16 &d) __attribute__((always_inline)) {
@@ -598,12 +590,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
         return x;
     };
     // tokens past the part: no score
-    auto mask = [&](uint32_t t, f32x16 (&d)[RT]) __attribute__((always_inline)) {
+    auto mask = [&](uint32_t t, f32x16 &d) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < 16; r++)
-            if (t + 8 * (r / 4) + 4 * h + r % 4 >= t1)
-#pragma unroll
-                for (int q = 0; q < RT; q++) d[q][r] = -INFINITY;
+            if (t + 8 * (r / 4) + 4 * h + r % 4 >= t1) d[r] = -INFINITY;
     };
     if (nst > 2) wait_vm<(NW == 4 ? 5 : 2) * NI>();  // K of stage 0
     else wait_vm<0>();
@@ -611,58 +601,47 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
     if (mine) {
         load_k(0, 0);
 #pragma unroll
-        for (int q = 0; q < RT; q++) {
+        for (int r = 0; r < 16; r++) s[r] = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[q][r] = 0.f;
+        for (int p = NP - 1; p >= 0; p--)
 #pragma unroll
-            for (int p = NP - 1; p >= 0; p--)
-#pragma unroll
-                for (int k = 0; k < KS; k++)
-                    s[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[q][p][k], s[q], 0, 0, 0);
-        }
+            for (int k = 0; k < KS; k++) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[p][k], s, 0, 0, 0);
         load_k(0, 1);
         if (t0 + 32 > t1) mask(t0, s);
-        float mx[RT];
-#pragma unroll
-        for (int q = 0; q < RT; q++) mx[q] = largest(s[q]);
-        refer(mx);
+        refer(largest(s));
     }
-    constexpr int PAIRS = 8 * RT, EARLY = 3 * PAIRS / 4;  // weights in pairs; those taken beside the scores' products
-    for (uint32_t s0 = 0; s0 < nst; s0 += ST_NS)
+    constexpr int PAIRS = 8, EARLY = 6;  // weights in pairs; those taken beside the scores' products
+    for (uint32_t s0 = 0; s0 < nst; s0 += ST_NS)  // (the ring's slots unrolled: constant LDS offsets)
 #pragma unroll
     for (uint32_t slot = 0; slot < ST_NS; slot++) {
         const uint32_t st = s0 + slot;
-        if (st >= nst) break;
+        if (st >= nst) break;  // uniform
         landed(st);
         lds_bar();
         if (st + 3 < nst) issue(st + 3);
         const uint32_t tk = t0 + st * ST_KB;
         if (tk + ST_KB > t1) {  // V of the tokens past the part: zero (0 times NaN is NaN)
-            for (uint32_t i = (t1 - tk) * ROWB + tid * 16; i < STAGE; i += 64 * NW * 16) *(u32x4 *)(lds + (ST_NS + slot) * STAGE + i) = u32x4{0, 0, 0, 0};
+            for (uint32_t i = (t1 - tk) * ROWB + tid * 16; i < STAGE; i += 64 * NW * 16)
+                *(u32x4 *)(lds + (ST_NS + slot) * STAGE + i) = u32x4{0, 0, 0, 0};
             lds_bar();
         }
         if (!mine) continue;
 #pragma unroll
         for (uint32_t kt = 0; kt < 2; kt++) {
-            half8 pf[RT][NP][2], vf[2][DT];
-            float b[RT], mx[RT];
+            half8 pf[NP][2], vf[2][DT];
+            const float b = m == -INFINITY ? 0.f : 4.f - m;
+            float mx = 0.f;
 #pragma unroll
-            for (int q = 0; q < RT; q++) {
-                b[q] = m[q] == -INFINITY ? 0.f : 4.f - m[q];
+            for (int r = 0; r < 16; r++) sn[r] = 0.f;
+            auto weights = [&](int i) __attribute__((always_inline)) {  // 2 i and 2 i + 1
 #pragma unroll
-                for (int r = 0; r < 16; r++) sn[q][r] = 0.f;
-            }
-            // weights 2 i and 2 i + 1 (by 16-token product, then row tile)
-            auto weights = [&](int i) __attribute__((always_inline)) {
-                const int s2 = i / (4 * RT), q = i / 4 % RT, r0 = 2 * (i % 4);
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float p = __builtin_amdgcn_exp2f(fmaf(s[q][8 * s2 + r0 + e], c[q], b[q]));
-                    l[q] += p;
+                for (int r = 2 * i; r < 2 * i + 2; r++) {
+                    float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, b));
+                    l += p;
 #pragma unroll
                     for (int k = 0; k < NP; k++) {
-                        pf[q][k][s2][r0 + e] = (_Float16)p;
-                        p -= (float)pf[q][k][s2][r0 + e];
+                        pf[k][r / 8][r % 8] = (_Float16)p;
+                        p -= (float)pf[k][r / 8][r % 8];
                     }
                 }
             };
@@ -682,10 +661,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
 #pragma unroll
             for (int k = 0; k < KS; k++) {
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
-#pragma unroll
-                    for (int q = 0; q < RT; q++)
-                        sn[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[q][p][k], sn[q], 0, 0, 0);
+                for (int p = NP - 1; p >= 0; p--) sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[p][k], sn, 0, 0, 0);
 #pragma unroll
                 for (int i = EARLY * k / KS; i < EARLY * (k + 1) / KS; i++) weights(i);
                 __builtin_amdgcn_sched_barrier(0);
@@ -695,9 +671,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
             for (int d = 0; d < DT; d++) {
 #pragma unroll
                 for (int p = NP - 1; p >= 0; p--)
-#pragma unroll
-                    for (int q = 0; q < RT; q++)
-                        o[q][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][d], pf[q][p][0], o[q][d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][d], pf[p][0], o[d], 0, 0, 0);
 #pragma unroll
                 for (int i = EARLY + (PAIRS - EARLY) * d / DT; i < EARLY + (PAIRS - EARLY) * (d + 1) / DT; i++) weights(i);
                 __builtin_amdgcn_sched_barrier(0);
@@ -707,43 +681,35 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_shared_tile(SharedArgs a) {
             for (int d = 0; d < DT; d++) {
 #pragma unroll
                 for (int p = NP - 1; p >= 0; p--)
-#pragma unroll
-                    for (int q = 0; q < RT; q++)
-                        o[q][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[1][d], pf[q][p][1], o[q][d], 0, 0, 0);
-                if (d < RT) mx[d] = largest(sn[d]);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[1][d], pf[p][1], o[d], 0, 0, 0);
+                if (d == 0) mx = largest(sn);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (kt == 0 || st + 1 < nst) {  // (after the last tokens the scores are of nothing)
                 const uint32_t tn = tk + 32 * (kt + 1);
                 if (tn + 32 > t1) {
                     mask(tn, sn);
-#pragma unroll
-                    for (int q = 0; q < RT; q++) mx[q] = largest(sn[q]);
+                    mx = largest(sn);
                 }
                 refer(mx);
             }
-#pragma unroll
-            for (int q = 0; q < RT; q++) s[q] = sn[q];
+            s = sn;
         }
     }
     if (bad) atomicOr(a.err, ZH_DEVERR_KV_ROW);
-    if (!mine) return;
+    const uint32_t row = row0 + i32;
+    l = xor32_sum(l);
+    if (row >= rows) return;
+    const size_t pr = (size_t)part * a.n_seq * a.nh + (size_t)(row / a.G) * a.nh + kvh * a.G + row % a.G;
 #pragma unroll
-    for (int q = 0; q < RT; q++) {
-        const uint32_t row = row0 + 32 * q + i32;
-        const float lq = xor32_sum(l[q]);
-        if (row >= rows) continue;
-        const size_t pr = (size_t)part * a.n_seq * a.nh + (size_t)(row / a.G) * a.nh + kvh * a.G + row % a.G;
+    for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int g = 0; g < 4; g++)
-                *(f32x4 *)(a.part + pr * HD + 32 * d + 8 * g + 4 * h) =
-                    f32x4{o[q][d][4 * g], o[q][d][4 * g + 1], o[q][d][4 * g + 2], o[q][d][4 * g + 3]};
-        if (h == 0) {
-            a.stat[2 * pr] = m[q] - 4.f;
-            a.stat[2 * pr + 1] = lq;
-        }
+        for (int g = 0; g < 4; g++)
+            *(f32x4 *)(a.part + pr * HD + 32 * d + 8 * g + 4 * h) =
+                f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+    if (h == 0) {
+        a.stat[2 * pr] = m - 4.f;
+        a.stat[2 * pr + 1] = l;
     }
 }
 
@@ -842,7 +808,7 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
 
 bool shared_shape_ok(const zh_kv_batch *kv, uint32_t nh, uint32_t prefix, uint32_t max_len) {
     return kv_batch_ok(kv) && (kv->head_dim == 64 || kv->head_dim == 128) && nh && nh % kv->n_kv_heads == 0 &&
-           nh / kv->n_kv_heads <= SA_ROWS && max_len && prefix <= max_len;
+           nh / kv->n_kv_heads <= SA_ROWS && max_len && max_len <= 1u << 30 && prefix <= max_len;
 }
 
 }  // namespace
@@ -855,7 +821,8 @@ static zh_decode_rows with_strides(const zh_kv_batch *kv, const zh_decode_rows *
     return x;
 }
 
-// The checks of zh_flash_decode_shared, of host data only; cus: the device's CUs.
+// The checks of zh_flash_decode_shared, of host data only (exported for the
+// tests; c may be null: no message then). cus: the device's CUs.
 extern "C" int zh_check_decode_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_decode_rows *rows, uint32_t cus) {
     if (!rows || !shared_shape_ok(kv, rows->n_heads, rows->prefix_len, rows->max_len))
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "flash_decode_shared: cache, heads, head_dim or lengths");
@@ -876,6 +843,13 @@ extern "C" int zh_check_decode_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_d
         (p.bytes && !kv_in_range(r->ws, 0, p.bytes)))
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "flash_decode_shared: range (ws: %llu bytes)",
                           (unsigned long long)p.bytes);
+    // out and ws: not what the call reads besides q
+    const zh_buf *const read[] = {kv->k_cache, kv->v_cache, kv->tables, r->seq_lens};
+    for (const zh_buf *b : read)
+        if (b->ptr == r->out->ptr || (p.bytes && b->ptr == r->ws->ptr))
+            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "flash_decode_shared: out or ws is an input");
+    if (p.bytes && (r->ws->ptr == r->out->ptr || r->ws->ptr == r->q->ptr))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "flash_decode_shared: ws holds q or out");
     if (r->q_off % 16 || r->out_off % 16 || (n > 1 && (r->q_stride * size % 16 || r->out_stride * size % 16)))
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "flash_decode_shared: rows not 16-byte aligned");
     const bool same = r->q->ptr == r->out->ptr && r->q_off == r->out_off && (n == 1 || r->q_stride == r->out_stride);
@@ -897,11 +871,11 @@ extern "C" uint64_t zh_flash_decode_shared_ws(zh_ctx *c, const zh_kv_batch *kv, 
 
 template <int HD, int NP, int NW, typename T>
 static int tile_launch(zh_ctx *c, const SharedArgs &a, const SharedPlan &p) {
-    static bool attr = false;
-    if (!attr) {
+    static std::atomic<bool> attr[64];  // by device
+    if (c->device >= 64 || !attr[c->device].load(std::memory_order_relaxed)) {
         ZH_HIP(c, hipFuncSetAttribute((const void *)k_shared_tile<HD, NP, NW, T>,
                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)st_lds<HD>()));
-        attr = true;
+        if (c->device < 64) attr[c->device].store(true, std::memory_order_relaxed);
     }
     hipLaunchKernelGGL((k_shared_tile<HD, NP, NW, T>), dim3(p.pre_blocks), dim3(64 * NW), st_lds<HD>(), c->stream, a);
     ZH_LAUNCH_CHECK(c);
