@@ -394,6 +394,7 @@ def test_attention(zh, ctx, case, t):
 
 TILED = [  # many rows over a long prefix: K and V through LDS, 128 or 256 rows a workgroup
     (64, 4, 128, 1237, [0, 1237, 5] + [1238 + 3 * i for i in range(60)]),   # 1008 rows, 4 workgroups
+    (64, 4, 128, 1907, [1907, 3] + [1908 + i % 90 for i in range(60)]),     # 992 rows, f32 too
     (128, 8, 128, 4701, [4701 + 17 * i for i in range(8)]),                 # 128 rows
     (48, 8, 64, 12601, [12650, 12601, 400, 12640, 12602, 12700, 13000]),    # 42 rows
     (16, 4, 64, 5000, [5001 + i for i in range(70)]),                       # 280 rows
@@ -537,6 +538,42 @@ def test_attention_like_one_sequence_at_a_time(zh, ctx):
         ctx.flash_decode(u(q[s]), K, V, u(tables[s]), tables.shape[1], tokens, out, 32, 8, 128, n)
         one = out.download(np.float32, 32 * 128).reshape(32, 128)
         assert (np.abs(got[s] - one) <= 2 * tol[s]).all()
+
+
+def test_two_contexts_at_once(zh, ctx):
+    """Two contexts (streams), driven by two host threads over the same caches,
+    tables and queries, each with its own workspace and results."""
+    import threading
+    rng = np.random.default_rng(31)
+    P, lens = 700, [701 + 40 * i for i in range(12)]
+    kc, vc, tables, tokens, M = make(rng, 12, 4, 128, P, lens)
+    q = rng.standard_normal((12, 16, 128)).astype(np.float32)
+    want, tol = attend64(q, kc, vc, tables, lens, 128 ** -0.5, 0, P, [0, 5, 11])
+    u = ctx.upload
+    K, V, T, Q, L = u(kc), u(vc), u(tables), u(q), u(np.array(lens, np.uint32))
+    got, failed = [None, None], []
+
+    def work(i):
+        try:
+            with zh.Context(0) as c:
+                kv = zh.KvBatch(K, V, T, 12, tables.shape[1], tokens, 4, 128)
+                out, ws = c.alloc(q.nbytes), c.alloc(c.flash_decode_shared_ws(kv, 16, P, M))
+                rows = zh.DecodeRows(q=Q, out=out, seq_lens=L, ws=ws, n_heads=16, prefix_len=P, max_len=M)
+                for _ in range(50):
+                    c.flash_decode_shared(kv, rows)
+                c.sync()
+                got[i] = out.download(np.float32, q.size).reshape(q.shape)
+        except Exception as e:  # noqa: BLE001 (shown by the assertion)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    assert np.array_equal(got[0], got[1])
+    close(got[0][[0, 5, 11]].astype(np.float64), want[[0, 5, 11]], tol[[0, 5, 11]])
 
 
 # ---------------------------------------------------------------------------

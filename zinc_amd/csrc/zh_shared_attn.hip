@@ -28,11 +28,16 @@ constexpr uint32_t SA_KB = 32;    // tokens of a wave's step
 // The host's choices (shared_plan), measured with 32 heads on 8, 64 own tokens a
 // sequence, f16, prefix 1024 / 4096 / 16384:
 //  * LDS tiles where the 16-row tiles' prefix tokens over the kv heads reach
-//    SA_TILE: below it one more reading of K and V through the L2s costs less
-//    than the tiles' longer launch. us streamed / tiled: 64 rows 10.3 / 13.0,
-//    14.6 / 16.3, 31.8 / 29.0; 128 rows 11.6 / 14.7, 19.9 / 22.5, 53.4 / 33.7;
-//    256 rows 15.1 / 19.3, 32.3 / 29.4, 97.2 / 42.6 (head_dim 64 and f32 cross
-//    at the same counts);
+//    sa_tile: below it one more reading of K and V through the L2s costs less
+//    than the tiles' longer launch. us tiled / streamed, f16 at head_dim 128: 96
+//    rows over 4096 tokens (196K) 18.0 / 17.5, 6144 (294K) 21.8 / 22.4, 12288
+//    25.9 / 36.2; 256 rows over 1024 19.3 / 15.1, 8192 34.8 / 54.6. f32 128 rows
+//    over 6144 (393K) 29.1 / 27.3, 8192 (524K) 31.7 / 33.5; f16 at 64 48 rows
+//    over 4096 (98K) 11.7 / 11.3, 96 over 4096 (196K) 12.9 / 13.2; f32 at 64 96
+//    over 4096 14.5 / 13.6, 6144 (294K) 15.8 / 16.4;
+//  * a tile launch's parts: those that fill 1 to 4 rounds of one workgroup per CU
+//    best, a round's start and end counted as SA_TILE_FIX stages (180 sequences at
+//    8192 58.5 us, in the nearest number of parts 73.9);
 //  * a whole context, prefix and own tokens, in one workgroup of 8 waves (4 up
 //    to 128 tokens) where there is at most one workgroup per CU: up to 512
 //    tokens, with at most a quarter of the CUs busy up to 320. us whole / in
@@ -45,8 +50,10 @@ constexpr uint32_t SA_KB = 32;    // tokens of a wave's step
 //    512: 27 us, with two parts and a launch that joins them 22.9 + 8.6);
 //  * parts of at least 128 tokens, a step for each wave; own ones of 256 where
 //    the sequences alone fill the CUs (128 sequences of 1 to 200: 16.1 us, 19.9).
-constexpr uint64_t SA_TILE = 300000;
-constexpr uint32_t SA_ONE = 512, SA_ONE_FEW = 320, SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_OWN = 2;
+constexpr uint64_t sa_tile(uint32_t hd, bool f32) {
+    return hd == 64 ? (f32 ? 270000 : 180000) : (f32 ? 450000 : 280000);
+}
+constexpr uint32_t SA_ONE = 512, SA_ONE_FEW = 320, SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_OWN = 2, SA_TILE_FIX = 5;
 
 struct SharedArgs {
     const uint8_t *q;
@@ -771,7 +778,7 @@ struct SharedPlan {
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t prefix, uint32_t max_len,
-                 SharedPlan &p) {
+                 bool f32, SharedPlan &p) {
     const uint32_t G = nh / nkv, own = max_len - prefix;
     const uint64_t rows_kv = (uint64_t)n_seq * G, jobs = (uint64_t)n_seq * nkv;
     // parts for `per` workgroups per CU, of at least `least` tokens
@@ -785,10 +792,25 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
     if (prefix && !one) {
         // rows of a prefix workgroup: 128 or 256 on LDS tiles, or 16 streamed
         const uint64_t through = (rows_kv + SA_ROWS - 1) / SA_ROWS * prefix * nkv;
-        p.tile = rows_kv > 2 * SA_ROWS && through >= SA_TILE ? (rows_kv > 128 ? 2 : 1) : 0;
+        p.tile = rows_kv > 2 * SA_ROWS && through >= sa_tile(hd, f32) ? (rows_kv > 128 ? 2 : 1) : 0;
         p.pre_tiles = ceil_div(rows_kv, p.tile ? 128u * p.tile : SA_ROWS);
-        const uint32_t n = cut((uint64_t)p.pre_tiles * nkv, prefix, SA_PRE_PER, 128);
+        const uint64_t pj = (uint64_t)p.pre_tiles * nkv;
         const uint32_t step = p.tile ? ST_KB : SA_KB;
+        uint32_t n = cut(pj, prefix, SA_PRE_PER, 128);
+        if (p.tile) {
+            // one workgroup per CU: the parts that fill 1 to 4 rounds of them,
+            // by the rounds' stages and SA_TILE_FIX of their start and end
+            uint64_t best = ~0ull;
+            for (uint64_t r = 1; r <= 4; r++) {
+                const uint32_t most = ceil_div(prefix, 128), fit = (uint32_t)(r * cus / pj);
+                const uint32_t k = fit < 1 ? 1u : fit < most ? fit : most;
+                const uint64_t cost = ceil_div(pj * k, cus) * (uint64_t)(ceil_div(ceil_div(prefix, k), ST_KB) + SA_TILE_FIX);
+                if (cost < best) {
+                    best = cost;
+                    n = k;
+                }
+            }
+        }
         p.pre_len = ceil_div(ceil_div(prefix, n), step) * step;
         p.n_pre = ceil_div(prefix, p.pre_len);
     }
@@ -837,7 +859,8 @@ extern "C" int zh_check_decode_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_d
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "flash_decode_shared: rows overlap");
     const uint64_t qb = ((n - 1) * r->q_stride + w) * size, ob = ((n - 1) * r->out_stride + w) * size;
     SharedPlan p;
-    if (!shared_plan(cus, kv->n_seq, r->n_heads, kv->n_kv_heads, kv->head_dim, r->prefix_len, r->max_len, p))
+    if (!shared_plan(cus, kv->n_seq, r->n_heads, kv->n_kv_heads, kv->head_dim, r->prefix_len, r->max_len,
+                     r->type == ZH_F32, p))
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "flash_decode_shared: too large");
     if (!kv_in_range(r->q, r->q_off, qb) || !kv_in_range(r->out, r->out_off, ob) || !kv_in_range(r->seq_lens, 0, 4 * n) ||
         (p.bytes && !kv_in_range(r->ws, 0, p.bytes)))
@@ -862,11 +885,16 @@ extern "C" int zh_check_decode_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_d
 
 extern "C" uint64_t zh_flash_decode_shared_ws(zh_ctx *c, const zh_kv_batch *kv, uint32_t n_heads, uint32_t prefix_len,
                                               uint32_t max_len) {
-    SharedPlan p;
-    if (!c || !shared_shape_ok(kv, n_heads, prefix_len, max_len) ||
-        !shared_plan((uint32_t)c->cu_count, kv->n_seq, n_heads, kv->n_kv_heads, kv->head_dim, prefix_len, max_len, p))
-        return 0;
-    return p.bytes ? p.bytes : 16;
+    if (!c || !shared_shape_ok(kv, n_heads, prefix_len, max_len)) return 0;
+    uint64_t most = 16;  // (of either type)
+    for (int f32 = 0; f32 < 2; f32++) {
+        SharedPlan p;
+        if (!shared_plan((uint32_t)c->cu_count, kv->n_seq, n_heads, kv->n_kv_heads, kv->head_dim, prefix_len, max_len,
+                         f32 != 0, p))
+            return 0;
+        if (p.bytes > most) most = p.bytes;
+    }
+    return most;
 }
 
 template <int HD, int NP, int NW, typename T>
@@ -911,7 +939,8 @@ extern "C" int zh_flash_decode_shared(zh_ctx *c, const zh_kv_batch *kv, const zh
     const zh_decode_rows x = with_strides(kv, rows), *r = &x;
     zh_device_scope dev(c);
     SharedPlan p;
-    shared_plan((uint32_t)c->cu_count, kv->n_seq, r->n_heads, kv->n_kv_heads, kv->head_dim, r->prefix_len, r->max_len, p);
+    shared_plan((uint32_t)c->cu_count, kv->n_seq, r->n_heads, kv->n_kv_heads, kv->head_dim, r->prefix_len, r->max_len,
+                r->type == ZH_F32, p);
     SharedArgs a = {};
     const uint64_t size = r->type == ZH_F32 ? 4 : 2;
     a.q = (const uint8_t *)r->q->ptr + r->q_off;
