@@ -65,7 +65,8 @@ def copied(caches, dst, src, nkv, hd):
 
 @pytest.mark.parametrize("n_caches,nkv,hd,pool,n", [
     (1, 1, 64, 4, 1), (2, 8, 128, 40, 13), (97, 2, 64, 9, 3), (3, 3, 80, 700, 300), (2, 1, 2, 30, 11), (4, 5, 6, 20, 9),
-    (2, 2, 512, 12, 5), (2, 4, 128, 1100, 513)])
+    (2, 2, 512, 12, 5), (2, 4, 128, 1100, 513), (4, 1, 2, 4000, 1990),
+    (64, 1, 2, 3100, 1445), (65, 1, 2, 1500, 700), (3, 1, 2, 65536 + 40, 270), (1, 1, 64, 65536, 30)])
 def test_copy_pages(zh, ctx, n_caches, nkv, hd, pool, n):
     rng = np.random.default_rng(pool + n)
     caches = [rng.integers(0, 1 << 16, nkv * pool * 16 * hd).astype(np.uint16) for _ in range(n_caches)]

@@ -15,18 +15,17 @@
 // ---------------------------------------------------------------------------
 namespace {
 
-// Caches and pages per launch: 4 KB of arguments hold both lists; a call of few
-// pages (a fork) takes the small form, whose arguments the host writes sooner.
-constexpr uint32_t KC_CACHES = 96, KC_PAGES = 256, KC_FEW_CACHES = 64, KC_FEW_PAGES = 16;
-template <uint32_t NC, uint32_t NP>
+// NC caches and NP pages (numbers of type P) per launch, in 4 KB of arguments.
+template <typename P, uint32_t NC, uint32_t NP>
 struct KvCopyArgs {
+    typedef P Page;
+    static constexpr uint32_t caches = NC, n = NP;
     const uint8_t *src[NC];
     uint8_t *dst[NC];
-    uint32_t pages[NP][2];  // source, destination
     uint64_t src_head, dst_head;  // bytes of one head of a cache
-    uint32_t n_caches, n_pages, n_heads, seg;  // seg: bytes of a page of one head
+    uint32_t n_pages, seg;        // seg: bytes of a page of one head
+    P pages[NP][2];               // source, destination
 };
-static_assert(sizeof(KvCopyArgs<KC_CACHES, KC_PAGES>) <= 4096, "kernel arguments");
 
 // One workgroup: KC_U pages of one head and cache, all loads before the stores.
 constexpr int KC_U = 2;  // (4 and 8: the same times)
@@ -57,33 +56,32 @@ __global__ __launch_bounds__(256) void k_kv_copy(A a) {
         for (uint32_t p = p0; p < a.n_pages; p++) kv_copy_pages<NT, 1>(a, p, s, d);
 }
 
-template <uint32_t NC, uint32_t NP>
+template <typename A>
 int kv_copy_launches(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *const *src, uint32_t dst_tokens,
                      uint32_t src_tokens, uint32_t n_kv_heads, uint32_t head_dim, const uint32_t *dst_pages,
                      const uint32_t *src_pages, uint32_t n_pages) {
-    typedef KvCopyArgs<NC, NP> A;
+    static_assert(sizeof(A) <= 4096, "kernel arguments");
     A a;
     a.seg = 32 * head_dim;
     a.src_head = 2ull * src_tokens * head_dim;
     a.dst_head = 2ull * dst_tokens * head_dim;
-    a.n_heads = n_kv_heads;
     const uint32_t threads = a.seg >= 4096 ? 256u : (a.seg / 16 + 63) / 64 * 64;
     // past what the L2s hold, the pages go by them: 1024 pages of 32 caches of 8
     // heads 382 us (5.6 TB/s read + written) against 408 through them
     const bool nt = (uint64_t)n_caches * n_pages * n_kv_heads * a.seg > (32ull << 20);
-    for (uint32_t c0 = 0; c0 < n_caches; c0 += NC) {
-        a.n_caches = n_caches - c0 < NC ? n_caches - c0 : NC;
-        for (uint32_t i = 0; i < a.n_caches; i++) {
+    for (uint32_t c0 = 0; c0 < n_caches; c0 += A::caches) {
+        const uint32_t nc = n_caches - c0 < A::caches ? n_caches - c0 : A::caches;
+        for (uint32_t i = 0; i < nc; i++) {
             a.src[i] = (const uint8_t *)src[c0 + i];
             a.dst[i] = (uint8_t *)dst[c0 + i];
         }
-        for (uint32_t p0 = 0; p0 < n_pages; p0 += NP) {
-            a.n_pages = n_pages - p0 < NP ? n_pages - p0 : NP;
+        for (uint32_t p0 = 0; p0 < n_pages; p0 += A::n) {
+            a.n_pages = n_pages - p0 < A::n ? n_pages - p0 : A::n;
             for (uint32_t i = 0; i < a.n_pages; i++) {
-                a.pages[i][0] = src_pages[p0 + i];
-                a.pages[i][1] = dst_pages[p0 + i];
+                a.pages[i][0] = (typename A::Page)src_pages[p0 + i];
+                a.pages[i][1] = (typename A::Page)dst_pages[p0 + i];
             }
-            const dim3 grid((a.n_pages + KC_U - 1) / KC_U, a.n_heads, a.n_caches);
+            const dim3 grid((a.n_pages + KC_U - 1) / KC_U, n_kv_heads, nc);
             if (nt) hipLaunchKernelGGL((k_kv_copy<true, A>), grid, dim3(threads), 0, c->stream, a);
             else hipLaunchKernelGGL((k_kv_copy<false, A>), grid, dim3(threads), 0, c->stream, a);
             ZH_LAUNCH_CHECK(c);
@@ -97,7 +95,15 @@ int kv_copy_launches(zh_ctx *c, uint32_t n_caches, void *const *dst, const void 
 int zhk_kv_copy(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *const *src, uint32_t dst_tokens,
                 uint32_t src_tokens, uint32_t n_kv_heads, uint32_t head_dim, const uint32_t *dst_pages,
                 const uint32_t *src_pages, uint32_t n_pages) {
-    auto f = n_pages <= KC_FEW_PAGES ? kv_copy_launches<KC_FEW_CACHES, KC_FEW_PAGES> : kv_copy_launches<KC_CACHES, KC_PAGES>;
+    // the lists that fit the call in the fewest launches: 2400 pages of two caches
+    // of one head 16.7 us in three, 50.8 in ten of 256 pages; few pages take short
+    // arguments, which the host writes sooner (one page of 64 caches 4.8 us, 6.0)
+    auto f = kv_copy_launches<KvCopyArgs<uint32_t, 96, 256>>;
+    if (n_pages <= 16) f = kv_copy_launches<KvCopyArgs<uint32_t, 64, 16>>;
+    else if (dst_tokens > 16u << 16 || src_tokens > 16u << 16) {}  // (page numbers past 16 bits)
+    else if (n_caches <= 4) f = kv_copy_launches<KvCopyArgs<uint16_t, 4, 960>>;
+    else if (n_caches <= 64) f = kv_copy_launches<KvCopyArgs<uint16_t, 64, 720>>;
+    else f = kv_copy_launches<KvCopyArgs<uint16_t, 96, 592>>;
     return f(c, n_caches, dst, src, dst_tokens, src_tokens, n_kv_heads, head_dim, dst_pages, src_pages, n_pages);
 }
 
