@@ -481,11 +481,11 @@ int      zh_kv_pool_compact(zh_kv_pool *pool, uint32_t *src, uint32_t *dst, uint
 int zh_engine_read_kv(zh_engine *eng, uint32_t layer, uint32_t which, uint32_t t0, uint32_t n,
                       uint16_t *dst);
 /* Copies the K and V of the first n_tokens positions of src's sequence into
- * dst's (whole pages through both page tables, in dst's stream after src's work
- * so far; nothing of dst's other positions): a prompt is prefilled once and
- * continued by several engines (zh_engine_generate_batch). Same layers, kv
- * heads and head dims; n_tokens within both capacities. The page of dst in
- * which n_tokens ends is copied whole. */
+ * dst's (whole pages through both page tables, after both engines' work so far;
+ * the page in which n_tokens ends is copied whole): a prompt is prefilled once
+ * and continued by several engines (zh_engine_generate_batch). Same device,
+ * layers, kv heads and head dims, no page twice in dst's table
+ * (ZH_ERR_INVALID_ARGUMENT otherwise); n_tokens within both capacities. */
 int zh_engine_fork_kv(zh_engine *dst, zh_engine *src, uint32_t n_tokens);
 /* Model bytes touched per decoded token at context length L (weights + fp16
  * KV + activations), the numerator of the bandwidth roofline. */

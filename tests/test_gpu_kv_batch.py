@@ -736,3 +736,28 @@ def test_rope_of_more_rows_than_a_grid_is_high(zh, ctx):
     v64[slot] = x[:, 2].astype(np.float16)
     close(kc.download(np.float16, k64.size).reshape(k64.shape), k64, 2.0 ** -19 * 2 * np.abs(k64).max() + store_error(1, k64))
     assert np.array_equal(vc.download(np.float16, v64.size).reshape(v64.shape).astype(np.float64), v64)
+
+
+def test_engine_fork_kv_then_a_batch(zh, ctx):
+    """A prompt prefilled once and forked into the engines of a decode batch
+    gives each the tokens of its own continuation; a page table that names a
+    page twice is refused."""
+    cfg = dict(n_layers=2, hidden=512, n_heads=4, n_kv_heads=2, head_dim=128, ffn=1024, vocab=1000, n_experts=0,
+               n_experts_used=0, expert_ffn=0, max_ctx=128, type_attn=12, type_ffn_gate_up=12, type_ffn_down=14,
+               type_lm_head=14, type_embd=12, type_router=8, rope_base=1e6, eps=1e-6, seed=5)
+    prompt = np.random.default_rng(4).integers(0, 1000, 50)
+    base = zh.InferenceEngine(ctx, cfg)
+    engines = [base] + [base.share(ctx) for _ in range(3)]
+    base.prefill(prompt)
+    for e in engines[1:]:
+        e.fork_kv(base, 50)
+    starts = [[3], [500], [77], [999]]
+    want = [e.generate(p, 5, start_pos=50) for e, p in zip(engines, starts)]
+    assert zh.InferenceEngine.generate_batch(engines, starts, 5, start_pos=50) == want
+    engines[3].set_pages(np.zeros(8, dtype=np.uint32))
+    with pytest.raises(zh.ZincError) as err:
+        engines[3].fork_kv(base, 50)
+    assert err.value.name == "InvalidArgument"
+    engines[3].fork_kv(base, 16)
+    for e in reversed(engines):
+        e.deinit()

@@ -1824,9 +1824,9 @@ extern "C" int zh_engine_read_kv(zh_engine *e, uint32_t layer, uint32_t which, u
 }
 
 // The prompt's K and V of one engine into another's cache: page copies of every
-// layer (zhk_kv_copy). Engines of one context are ordered by its stream; of two,
-// the call waits for src's work before it and for the copies after it, so that
-// src may go on at once.
+// layer (zhk_kv_copy), after the work of both engines so far (their page tables
+// are read back). Of two contexts, the call waits for the copies too, so that src
+// may go on at once.
 extern "C" int zh_engine_fork_kv(zh_engine *dst, zh_engine *src, uint32_t n_tokens) {
     if (!dst || !src) return ZH_ERR_INVALID_ARGUMENT;
     const zh_model_config &a = dst->c, &b = src->c;
@@ -1840,11 +1840,15 @@ extern "C" int zh_engine_fork_kv(zh_engine *dst, zh_engine *src, uint32_t n_toke
     const uint32_t n = (n_tokens + 15) / 16;
     try {
         std::vector<uint32_t> dp(n), sp(n), seen(dst->n_pages, 0);
-        EHIP(dst, hipMemcpy(dp.data(), dst->pages, 4ull * n, hipMemcpyDeviceToHost));
-        EHIP(dst, hipMemcpy(sp.data(), src->pages, 4ull * n, hipMemcpyDeviceToHost));
+        // the tables, after what their streams still do to them (and src's work)
+        EHIP(dst, hipMemcpyAsync(dp.data(), dst->pages, 4ull * n, hipMemcpyDeviceToHost, dst->ctx->stream));
+        EHIP(dst, hipMemcpyAsync(sp.data(), src->pages, 4ull * n, hipMemcpyDeviceToHost, src->ctx->stream));
+        EHIP(dst, hipStreamSynchronize(dst->ctx->stream));
+        EHIP(dst, hipStreamSynchronize(src->ctx->stream));
         for (uint32_t i = 0; i < n; i++)
-            if (seen[dp[i]]++)
-                return zh_set_err(dst->ctx, ZH_ERR_INVALID_ARGUMENT, "fork: page %u twice in the page table", dp[i]);
+            if (dp[i] >= dst->n_pages || sp[i] >= src->n_pages || seen[dp[i]]++)
+                return zh_set_err(dst->ctx, ZH_ERR_INVALID_ARGUMENT, "fork: page %u twice in the page table or outside the cache",
+                                  dp[i]);
         std::vector<void *> d;
         std::vector<const void *> s;
         for (uint32_t l = 0; l < a.n_layers; l++) {
@@ -1853,7 +1857,6 @@ extern "C" int zh_engine_fork_kv(zh_engine *dst, zh_engine *src, uint32_t n_toke
             s.push_back(src->L[l].kc);
             s.push_back(src->L[l].vc);
         }
-        if (src->ctx != dst->ctx) EHIP(dst, hipStreamSynchronize(src->ctx->stream));
         ERC(zhk_kv_copy(dst->ctx, (uint32_t)d.size(), d.data(), s.data(), a.max_ctx, b.max_ctx, a.n_kv_heads,
                         a.head_dim, dp.data(), sp.data(), n));
         if (src->ctx != dst->ctx) EHIP(dst, hipStreamSynchronize(dst->ctx->stream));
