@@ -316,7 +316,9 @@ ZH_DEV void st8(_Float16 *p, const float (&v)[8]) {
 // Head dims of 8 L (L = 8, 16, 32 lanes of 8 dims), rope_dim / 16 zero or a
 // power of two, 16-byte aligned rows: a workgroup takes R x 256 / L heads of one
 // row (blockIdx.x) and works the row's angles out once, in LDS. The rotation's
-// partner dims lie rope_dim / 16 lanes away.
+// partner dims lie rope_dim / 16 lanes away. Bound by HBM: 8192 rows of 32 + 16
+// heads in fp16 (201 MB) 42 us, 4.8 TB/s, with R = 4 (3 / 2 / 1: 43.8 / 44.9 /
+// 48.4; one wave per head vector, each with its own angles: 190).
 template <typename TI, typename TQ, int L, int R>
 __global__ __launch_bounds__(256) void k_qkv_rows8(QkvArgs a) {
     constexpr uint32_t HD = 8 * L, NS = 256 / L;

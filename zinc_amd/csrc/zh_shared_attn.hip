@@ -45,15 +45,16 @@ constexpr uint32_t SA_KB = 32;    // tokens of a wave's step
 //    at 500 13.2 / 16.9, of 1 to 1000 20.3 / 21.6;
 //  * workgroups per CU that the parts are cut for: 1 of a prefix (16 sequences
 //    at 4096 f32 12.4 + 3.8 us, 2: 13.6 + 4.1), 8 of own tokens (64 sequences
-//    of 1 to 4000 106 us, 3: 113, 12: 105; all of 1000 50.9, 3: 48.2), 2 where
-//    one own part per sequence also joins the prefix's (64 sequences of up to
-//    512: 27 us, with two parts and a launch that joins them 22.9 + 8.6);
+//    of 1 to 4000 106 us, 3: 113, 12: 105; all of 1000 50.9, 3: 48.2);
 //  * parts of at least 128 tokens, a step for each wave; own ones of 256 where
-//    the sequences alone fill the CUs (128 sequences of 1 to 200: 16.1 us, 19.9).
+//    the sequences alone fill the CUs (128 sequences of 1 to 200: 16.1 us, 19.9),
+//    and of 512 after a tile launch, where a single own part of a sequence also
+//    joins the prefix's (64 sequences of up to 512: 27 us, in two parts and a
+//    launch that joins them 22.9 + 8.6; up to 4000 139 us, in one part 171).
 constexpr uint64_t sa_tile(uint32_t hd, bool f32) {
     return hd == 64 ? (f32 ? 270000 : 180000) : (f32 ? 450000 : 280000);
 }
-constexpr uint32_t SA_ONE = 512, SA_ONE_FEW = 320, SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_OWN = 2, SA_TILE_FIX = 5;
+constexpr uint32_t SA_ONE = 512, SA_ONE_FEW = 320, SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_FIX = 5;
 
 struct SharedArgs {
     const uint8_t *q;
@@ -116,6 +117,10 @@ struct SharedPart {
 //   permutes; column li of the output tile n is dim HD/16 li + n.
 // NP pieces: q (scaled by a power of two to a maximum in [1, 2)) and P as sums
 // of NP fp16 values; 2 keep 22 bits of each.
+// Bound by the reads: 3 workgroups of 4 waves a CU (168 registers), each wave's
+// step 16 KB; 48 sequences of 1 to 4096 tokens (400 MB) 80 us, 4.8 TB/s. Two or
+// four row tiles a wave, or a workgroup on the same tokens, read less from the
+// L2s but hold fewer steps in flight: 16 sequences at 4096 20 and 29 us, 16.3.
 // ONCE: no other workgroup reads these K and V (loads that go by the L2s).
 template <int HD, int NP, int W, bool ONCE, typename T>
 ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, float *lds) {
@@ -720,6 +725,8 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
     }
 }
 
+// (A launch of its own, 4 us for 35 parts of 512 rows: the workgroup that finishes
+// a row last would have to take the parts from past the L2s, 1.6 us more.)
 // Joins the parts of a row: HD / 4 lanes, of 4 dims each, take the parts'
 // statistics, as many at a time, then all of them the parts' sums, 8 loads of 16
 // bytes in flight.
@@ -816,7 +823,7 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
     }
     // a sequence's own tokens (all of them where the prefix has no parts)
     const uint32_t tokens = p.n_pre ? (own ? own : 1) : max_len;
-    p.n_own = one ? 1 : cut(jobs, tokens, p.tile ? SA_TILE_OWN : SA_OWN_PER, jobs >= cus ? 256 : 128);
+    p.n_own = one ? 1 : cut(jobs, tokens, SA_OWN_PER, p.tile ? 512 : jobs >= cus ? 256 : 128);
     p.own_len = ceil_div(ceil_div(tokens, p.n_own), SA_KB) * SA_KB;
     const uint64_t pre = (uint64_t)p.n_pre * p.pre_tiles * nkv, all = pre + (uint64_t)p.n_own * n_seq * nkv;
     if (all > 0x7FFFFFFFull || (uint64_t)n_seq * nh > 0x7FFFFFFFull) return false;
