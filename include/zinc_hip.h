@@ -300,7 +300,8 @@ typedef struct zh_decode_rows {
  * prefix_len tokens: out[s] = softmax(scale q[s] K^T) V over the tokens
  * t < seq_lens[s] of sequence s (its new token's K and V are in the cache).
  * K and V of the tokens below prefix_len are read once for all sequences,
- * through sequence 0's table; a sequence shorter than prefix_len attends
+ * through sequence 0's table (which names the prefix's pages even where
+ * sequence 0 is shorter or empty); a sequence shorter than prefix_len attends
  * through its own table alone. prefix_len 0: nothing shared. seq_lens[s] == 0:
  * the row is zero. A length past max_len or the table is cut there, a page
  * outside the cache reads as page 0, and the next zh_sync then returns

@@ -738,6 +738,43 @@ def test_rope_of_more_rows_than_a_grid_is_high(zh, ctx):
     assert np.array_equal(vc.download(np.float16, v64.size).reshape(v64.shape).astype(np.float64), v64)
 
 
+def test_rope_of_more_rows_than_a_launch_has(zh, ctx):
+    """2^23 + 5 rows of head_dim 64 (a launch takes 2^23), all but the first and
+    the last three padded, without a sequence list and with one."""
+    rng = np.random.default_rng(14)
+    T, hd, w = (1 << 23) + 5, 64, 192
+    at = [0, T - 3, T - 2, T - 1]
+    x = rng.standard_normal((4, 3, hd)).astype(np.float16)
+    pos = np.full(T, NONE, np.uint32)
+    pos[at] = [3, 15, 0, 7]
+    u = ctx.upload
+    X, P = ctx.alloc(2 * T * w), u(pos)
+    seq = np.zeros(T, np.uint32)
+    seq[at] = [0, 1, 2, 3]
+    S = u(seq)
+    for listed in (False, True):
+        n_seq, of = (4, [0, 1, 2, 3]) if listed else (T, at)
+        table = np.full(n_seq, 4, np.uint32)  # (outside the cache)
+        table[of] = [2, 0, 3, 1]
+        kc, vc = (u(np.zeros((64, hd), np.float16)) for _ in range(2))
+        for r, row in zip(at, x):
+            X.upload(row, 2 * r * w)
+        kv = zh.KvBatch(kc, vc, u(table), n_seq, 1, 64, 1, hd)
+        ctx.qk_norm_rope_kv_write_batched(kv, zh.QkvRows(
+            q=X, k=X, v=X, k_off=2 * hd, v_off=4 * hd, q_stride=w, k_stride=w, v_stride=w, q_out=X, q_out_stride=w,
+            pos=P, seq=S if listed else None, n_rows=T, n_q_heads=1, type=1, rope_dim=hd, inv_freq=u(np.ones(hd // 2, np.float32))))
+        ctx.sync()
+        want, mag = rope64(x[:, :2].astype(np.float64), None, np.ones(hd // 2, np.float32), pos[at], 1e-6, hd)
+        got = np.stack([X.download(np.float16, hd, 2 * r * w) for r in at])
+        close(got, want[:, 0], mag[:, 0] * 2.0 ** -19 + store_error(1, want[:, 0]))
+        k64, v64, tol = np.zeros((64, hd)), np.zeros((64, hd)), np.zeros((64, hd))
+        slot = np.array([2, 0, 3, 1]) * 16 + pos[at]
+        k64[slot], v64[slot] = want[:, 1], x[:, 2]
+        tol[slot] = mag[:, 1] * 2.0 ** -19
+        close(kc.download(np.float16, k64.size).reshape(k64.shape), k64, tol + store_error(1, k64))
+        assert np.array_equal(vc.download(np.float16, v64.size).reshape(v64.shape).astype(np.float64), v64)
+
+
 def test_engine_fork_kv_then_a_batch(zh, ctx):
     """A prompt prefilled once and forked into the engines of a decode batch
     gives each the tokens of its own continuation; a page table that names a

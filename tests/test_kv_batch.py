@@ -339,6 +339,26 @@ def test_bad_decode_rest():
     assert decode_check(batch(), decode(q=q, out=q, out_off=4 * HD)) == INVALID
 
 
+def test_decode_of_more_workgroups_than_a_launch_has():
+    n = 1 << 22  # 2^23 workgroups: a launch of 2^31 threads and more
+    kv = batch(n_seq=n, table_stride=1, tables=Fake(4 * n))
+    big = dict(q=Fake(1 << 40), out=Fake(1 << 40), seq_lens=Fake(4 * n), ws=Fake(1 << 45), max_len=16)
+    assert decode_check(kv, decode(prefix_len=0, **big)) == INVALID
+    kv = batch(n_seq=n - 1, table_stride=1, tables=Fake(4 * n))
+    assert decode_check(kv, decode(prefix_len=0, **big)) == OK
+
+
+def test_page_numbers_are_integers_of_32_bits():
+    for bad in ([-1], [1 << 32], np.array([-1]), np.array([1 << 32]), np.array([1.5]), [[1]], ["a"]):
+        with pytest.raises((ValueError, OverflowError, TypeError)):
+            zinc_amd.hip._u32_array(bad)
+    for good in ([7], np.array([7]), np.array([3, 7], dtype=np.uint32)[1:], np.arange(9, dtype=np.uint32)[7::9],
+                 np.array([7], dtype=np.uint8)):
+        p, n = zinc_amd.hip._u32_array(good)
+        assert n == 1 and p._obj.value == 7
+    assert zinc_amd.hip._u32_array([])[1] == 0 and zinc_amd.hip._u32_array(np.zeros(0, np.uint32))[1] == 0
+
+
 def test_entries_refuse_a_null_context():
     L = zinc_amd.lib()
     assert L.zh_qk_norm_rope_kv_write_batched(None, batch().ptr, qkv().ptr) == INVALID

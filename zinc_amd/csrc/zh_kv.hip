@@ -215,7 +215,7 @@ struct QkvArgs {
     const uint32_t *tables, *seq, *pos;
     uint32_t *err;
     uint32_t n_seq, stride, cache_tokens, nq, nkv, hd, rd;
-    uint32_t t0;  // rows before this launch's (k_qkv_rows)
+    uint32_t t0;  // rows before this launch's
     float eps;
 };
 
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(256) void k_qkv_rows8(QkvArgs a) {
     uint32_t slot = 0;
     bool ok = true;
     if (h0 + R * NS > a.nq) {  // (uniform: some k or v head)
-        ok = kv_slot(a.tables, a.n_seq, a.stride, a.cache_tokens, a.seq ? a.seq[t] : t, pos, slot);
+        ok = kv_slot(a.tables, a.n_seq, a.stride, a.cache_tokens, a.seq ? a.seq[t] : a.t0 + t, pos, slot);
         if (!ok && tid == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
     }
     const uint32_t h2 = a.rd / 2;
@@ -487,15 +487,11 @@ static int qkv_launch(zh_ctx *c, const QkvArgs &a, uint32_t n) {
     const uint32_t p2 = a.rd / 16;
     const bool rows16 = (((uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v |
                           (uint64_t)(uintptr_t)a.q_out | a.q_row | a.k_row | a.v_row | a.out_row) % 16) == 0;
-    if (rows16 && a.rd % 16 == 0 && (p2 & (p2 - 1)) == 0 && (a.hd == 64 || a.hd == 128 || a.hd == 256)) {
-        if (a.hd == 64) qkv_launch8<TI, TQ, 8>(c, a, n);
-        else if (a.hd == 128) qkv_launch8<TI, TQ, 16>(c, a, n);
-        else qkv_launch8<TI, TQ, 32>(c, a, n);
-        ZH_LAUNCH_CHECK(c);
-        return ZH_OK;
-    }
-    // (at most 65535 rows a launch: the grid's y)
-    for (uint32_t t0 = 0; t0 < n; t0 += 65535) {
+    const bool by8 = rows16 && a.rd % 16 == 0 && (p2 & (p2 - 1)) == 0 && (a.hd == 64 || a.hd == 128 || a.hd == 256);
+    // rows of a launch: fewer than 2^32 threads in x, at most 65535 workgroups in y
+    const uint32_t most = by8 ? 1u << 23 : 65535u;
+    for (uint64_t t0 = 0; t0 < n; t0 += most) {
+        const uint32_t m = n - t0 < most ? (uint32_t)(n - t0) : most;
         QkvArgs b = a;
         b.q += t0 * a.q_row;
         b.k += t0 * a.k_row;
@@ -503,9 +499,12 @@ static int qkv_launch(zh_ctx *c, const QkvArgs &a, uint32_t n) {
         b.q_out += t0 * a.out_row;
         b.pos += t0;
         if (b.seq) b.seq += t0;
-        b.t0 = t0;
-        hipLaunchKernelGGL((k_qkv_rows<TI, TQ>), dim3(a.nq + 2 * a.nkv, n - t0 < 65535 ? n - t0 : 65535), dim3(64), 0,
-                           c->stream, b);
+        b.t0 = (uint32_t)t0;
+        if (!by8)
+            hipLaunchKernelGGL((k_qkv_rows<TI, TQ>), dim3(a.nq + 2 * a.nkv, m), dim3(64), 0, c->stream, b);
+        else if (a.hd == 64) qkv_launch8<TI, TQ, 8>(c, b, m);
+        else if (a.hd == 128) qkv_launch8<TI, TQ, 16>(c, b, m);
+        else qkv_launch8<TI, TQ, 32>(c, b, m);
         ZH_LAUNCH_CHECK(c);
     }
     return ZH_OK;

@@ -826,7 +826,8 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
     p.n_own = one ? 1 : cut(jobs, tokens, SA_OWN_PER, p.tile ? 512 : jobs >= cus ? 256 : 128);
     p.own_len = ceil_div(ceil_div(tokens, p.n_own), SA_KB) * SA_KB;
     const uint64_t pre = (uint64_t)p.n_pre * p.pre_tiles * nkv, all = pre + (uint64_t)p.n_own * n_seq * nkv;
-    if (all > 0x7FFFFFFFull || (uint64_t)n_seq * nh > 0x7FFFFFFFull) return false;
+    // (a launch has fewer than 2^32 threads: workgroups of up to 512, rows of 32 lanes)
+    if (all >= 1ull << 23 || (uint64_t)n_seq * nh >= 1ull << 27) return false;
     p.pre_blocks = (uint32_t)pre;
     p.blocks = (uint32_t)all;
     const uint64_t parts = p.n_pre + p.n_own, rows = (uint64_t)n_seq * nh;

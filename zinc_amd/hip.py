@@ -293,9 +293,10 @@ def _u32_array(a):
             return C.byref(_u32.from_buffer(a)), a.size
         except (TypeError, ValueError):  # read-only, with gaps or empty
             pass
-    a = np.array(a, dtype=np.uint32, ndmin=1)
-    if a.ndim != 1:
-        raise ValueError("a list of page numbers")
+    x = np.array(a, ndmin=1)
+    if x.ndim != 1 or x.size and (x.dtype.kind not in "iu" or x.min() < 0 or x.max() >= 1 << 32):
+        raise ValueError("page numbers: a list of integers of 32 bits")
+    a = x.astype(np.uint32)
     return (C.byref(_u32.from_buffer(a)) if a.size else None), a.size
 
 
