@@ -13,6 +13,7 @@
 #include <math.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "zh_device.h"
 #include "zh_internal.h"
@@ -22,6 +23,7 @@ namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(4))) uint32_t const_u32;  // what no kernel writes while it runs
 
 constexpr uint32_t SA_ROWS = 16;  // rows of an MFMA tile
 constexpr uint32_t SA_KB = 32;    // tokens of a wave's step
@@ -144,7 +146,8 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
         x.tk = f ? st * SA_KB : ta + (st - n0) * SA_KB;
         x.lo = f ? 0u : w.t0;
         x.hi = f ? w.first : w.t1;
-        const uint32_t *tb = a.tables + (f ? (size_t)0 : (size_t)w.tab * a.stride);
+        // (scalar loads: a wait for them does not wait for K and V)
+        const const_u32 *tb = (const const_u32 *)(a.tables + (f ? (size_t)0 : (size_t)w.tab * a.stride));
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             x.pg[j] = tb[min(x.tk / 16 + j, (x.hi - 1) / 16)];
@@ -176,11 +179,12 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
             }
         }
     };
-    Step x = {};
+    Step x = {}, nx = {};  // this step and the next, whose pages are looked up one step ahead
     if (wave < nstep) {
         x = step(wave);
         load_k(x);
         load_v(x);
+        if (wave + W < nstep) nx = step(wave + W);
     }
     // the row's q as operand fragments: dims 32 k4 + 8 lg ..
     half8 qf[NP][K4];
@@ -221,37 +225,43 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
 #pragma unroll
     for (int n = 0; n < ND; n++) o[n] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;  // the row's maximum (every lg alike), this lane's share of its sum
-    for (uint32_t st = wave; st < nstep; st += W) {
-        const bool more = st + W < nstep;
-        Step nx = x;
-        if (more) nx = step(st + W);
+    // the weights and products of step x; `more`: the next step's loads on the way.
+    // (The last step is code of its own: a load that may not be there would make
+    // the compiler wait for V before the scores.)
+    auto work = [&](auto more) __attribute__((always_inline)) {
         const bool whole = x.tk >= x.lo && x.tk + SA_KB <= x.hi;
+        floatx4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+            for (int k4 = 0; k4 < K4; k4++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    d[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[j][k4], qf[p][k4], d[j], 0, 0, 0);
+        if constexpr (more) load_k(nx);
         float s[2][4], mb = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            floatx4 d = {0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int p = NP - 1; p >= 0; p--)
+            for (int r = 0; r < 4; r++) s[j][r] = d[j][r] * c;
+        if (!whole) {
+            // a token outside the range: no score, and no V (0 times what the
+            // cache holds there may be NaN)
 #pragma unroll
-                for (int k4 = 0; k4 < K4; k4++)
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[j][k4], qf[p][k4], d, 0, 0, 0);
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                s[j][r] = d[r] * c;
-                if (!whole) {
-                    // a token outside the range: no score, and no V (0 times
-                    // what the cache holds there may be NaN)
+                for (int r = 0; r < 4; r++) {
                     const uint32_t t = x.tk + 16 * j + 4 * lg + r;
-                    if (t < x.lo || t >= x.hi) {
-                        s[j][r] = -INFINITY;
+                    const bool out = t < x.lo || t >= x.hi;
+                    s[j][r] = out ? -INFINITY : s[j][r];
 #pragma unroll
-                        for (int y = 0; y < ND / 2; y++) pv[j][r][y] = 0u;
-                    }
+                    for (int y = 0; y < ND / 2; y++) pv[j][r][y] = out ? 0u : pv[j][r][y];
                 }
-                mb = fmaxf(mb, s[j][r]);
-            }
         }
-        if (more) load_k(nx);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) mb = fmaxf(mb, s[j][r]);
         mb = xor32_max(xor16_max(mb));
         // (weights up to 2^8, away from fp16's subnormals)
         const float mn = fmaxf(m, mb - 8.f), ms = mn == -INFINITY ? 0.f : mn;
@@ -286,8 +296,16 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
 #pragma unroll
             for (int p = NP - 1; p >= 0; p--) o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[p], o[n], 0, 0, 0);
         }
-        if (more) load_v(nx);
-        x = nx;
+        if constexpr (more) load_v(nx);
+    };
+    if (wave < nstep) {
+        for (uint32_t st = wave + W; st < nstep; st += W) {
+            const Step nn = st + W < nstep ? step(st + W) : nx;
+            work(std::true_type{});
+            x = nx;
+            nx = nn;
+        }
+        work(std::false_type{});
     }
     if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
     // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
@@ -795,7 +813,7 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
     };
     p = {};
     const bool one = jobs <= cus && max_len <= (4 * jobs <= cus ? SA_ONE_FEW : SA_ONE);
-    p.waves = one && max_len > 4 * SA_KB ? 8 : 4;
+    p.waves = one && max_len > 8 * SA_KB ? 8 : 4;
     if (prefix && !one) {
         // rows of a prefix workgroup: 128 or 256 on LDS tiles, or 16 streamed
         const uint64_t through = (rows_kv + SA_ROWS - 1) / SA_ROWS * prefix * nkv;
