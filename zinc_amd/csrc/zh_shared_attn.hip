@@ -27,6 +27,7 @@ typedef __attribute__((address_space(4))) uint32_t const_u32;  // what no kernel
 
 constexpr uint32_t SA_ROWS = 16;  // rows of an MFMA tile
 constexpr uint32_t SA_KB = 32;    // tokens of a wave's step
+constexpr int W = 4;              // waves of a workgroup
 // The host's choices (shared_plan), measured with 32 heads on 8, 64 own tokens a
 // sequence, f16, prefix 1024 / 4096 / 16384:
 //  * LDS tiles where the 16-row tiles' prefix tokens over the kv heads reach
@@ -40,23 +41,27 @@ constexpr uint32_t SA_KB = 32;    // tokens of a wave's step
 //  * a tile launch's parts: those that fill 1 to 4 rounds of one workgroup per CU
 //    best, a round's start and end counted as SA_TILE_FIX stages (180 sequences at
 //    8192 58.5 us, in the nearest number of parts 73.9);
-//  * a whole context, prefix and own tokens, in one workgroup of 8 waves (4 up
-//    to 128 tokens) where there is at most one workgroup per CU: up to 512
-//    tokens, with at most a quarter of the CUs busy up to 320. us whole / in
-//    parts: 2 sequences at 240 tokens 6.6 / 7.5, at 500 8.7 / 7.7; 32 sequences
-//    at 500 13.2 / 16.9, of 1 to 1000 20.3 / 21.6;
+//  * a whole context, prefix and own tokens, in one workgroup where there is at
+//    most one per CU, the more of them the longer (sa_one tokens for few, twice
+//    that for one per CU), a prefix past sa_one excepted. us whole / in parts, f16
+//    at 128: 2 sequences at 512 tokens 7.6 / 8.5; 16 at 700 13.4 / 13.9, at 1000
+//    18.4 / 15.3; 32 at 1000 22.4 / 26.1, of 1 to 1400 24.6 / 23.0, with a prefix
+//    of 500 18.4 / 18.8, of 900 12.9 / 11.2; at 64: 8 at 760 7.2 / 7.8, 16 at
+//    1500 14.4 / 13.0, 32 at 1400 16.1 / 19.4;
 //  * workgroups per CU that the parts are cut for: 1 of a prefix (16 sequences
-//    at 4096 f32 12.4 + 3.8 us, 2: 13.6 + 4.1), 8 of own tokens (64 sequences
-//    of 1 to 4000 106 us, 3: 113, 12: 105; all of 1000 50.9, 3: 48.2);
-//  * parts of at least 128 tokens, a step for each wave; own ones of 256 where
-//    the sequences alone fill the CUs (128 sequences of 1 to 200: 16.1 us, 19.9),
-//    and of 512 after a tile launch, where a single own part of a sequence also
-//    joins the prefix's (64 sequences of up to 512: 27 us, in two parts and a
-//    launch that joins them 22.9 + 8.6; up to 4000 139 us, in one part 171).
+//    at 4096 f32 14.2 us, 2: 17.6), 4 of own tokens (64 sequences at 1000 tokens
+//    47.9 us, 8: 50.4; 8 at 4000 26.8, 31.2; 64 of 1 to 4000 105, 102), 8 after a
+//    tile launch (64 of up to 2000 90.6, 4: 95.9; 128 of up to 4000 221, 251);
+//  * parts of at least 128 tokens, a step for each wave; own ones of 256 (16
+//    sequences at 4096 of up to 300 own 15.9 us, 128: 17.0), and of 512 after a
+//    tile launch, where a single own part of a sequence also joins the prefix's
+//    (32 sequences of up to 512: 38 us, in two parts and a launch that joins them
+//    40.7; up to 1000 48.8, 45.9; 64 of up to 4000 139 us, in one part 171).
 constexpr uint64_t sa_tile(uint32_t hd, bool f32) {
     return hd == 64 ? (f32 ? 270000 : 180000) : (f32 ? 450000 : 280000);
 }
-constexpr uint32_t SA_ONE = 512, SA_ONE_FEW = 320, SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_FIX = 5;
+constexpr uint32_t sa_one(uint32_t hd) { return hd == 64 ? 768 : 512; }
+constexpr uint32_t SA_PRE_PER = 1, SA_OWN_PER = 4, SA_TILE_OWN_PER = 8, SA_TILE_FIX = 5;
 
 struct SharedArgs {
     const uint8_t *q;
@@ -124,7 +129,7 @@ struct SharedPart {
 // four row tiles a wave, or a workgroup on the same tokens, read less from the
 // L2s but hold fewer steps in flight: 16 sequences at 4096 20 and 29 us, 16.3.
 // ONCE: no other workgroup reads these K and V (loads that go by the L2s).
-template <int HD, int NP, int W, bool ONCE, typename T>
+template <int HD, int NP, bool ONCE, typename T>
 ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, float *lds) {
     constexpr int K4 = HD / 32, ND = HD / 16;  // k-steps of the scores, dims per lane and output tiles
     constexpr int LD = HD + 4;
@@ -395,8 +400,8 @@ ZH_DEV uint32_t own_tokens(const SharedArgs &a, uint32_t len, uint32_t &b, uint3
 }
 
 // The prefix's workgroups, then the sequences' own.
-template <int HD, int NP, int W, typename T>
-__global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void k_shared_attn(SharedArgs a) {
+template <int HD, int NP, typename T>
+__global__ __launch_bounds__(64 * W, 3) void k_shared_attn(SharedArgs a) {
     __shared__ __align__(16) float lds[W * SA_ROWS * (HD + 6)];
     const bool pre = blockIdx.x < a.pre_blocks;
     // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
@@ -413,7 +418,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void k_shared_attn(SharedAr
         w.tab = 0;
         w.t0 = w.part * a.pre_len;
         w.t1 = min(w.t0 + a.pre_len, a.prefix);
-        shared_part<HD, NP, W, false, T>(a, w, kvh, lds);
+        shared_part<HD, NP, false, T>(a, w, kvh, lds);
     } else {
         const uint32_t s = job / a.nkv % a.n_seq, p = job / a.nkv / a.n_seq;
         w.part = a.n_pre + p;
@@ -429,7 +434,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void k_shared_attn(SharedAr
         w.t0 = b + p * c;
         w.t1 = min(w.t0 + c, len);
         if (!a.n_pre && a.prefix && len >= a.prefix) w.first = w.t0 = a.prefix;  // (one part: the whole context)
-        shared_part<HD, NP, W, true, T>(a, w, kvh, lds);
+        shared_part<HD, NP, true, T>(a, w, kvh, lds);
     }
 }
 
@@ -796,7 +801,7 @@ __global__ __launch_bounds__(256) void k_shared_join(SharedArgs a) {
 
 // How a call is cut (the same for every call of these sizes).
 struct SharedPlan {
-    uint32_t n_pre, n_own, pre_tiles, pre_len, own_len, pre_blocks, blocks, tile, waves;
+    uint32_t n_pre, n_own, pre_tiles, pre_len, own_len, pre_blocks, blocks, tile;
     uint64_t stat_off, bytes;  // of ws
 };
 
@@ -812,8 +817,7 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
         return want < 1 ? 1u : want < most ? want : most;
     };
     p = {};
-    const bool one = jobs <= cus && max_len <= (4 * jobs <= cus ? SA_ONE_FEW : SA_ONE);
-    p.waves = one && max_len > 8 * SA_KB ? 8 : 4;
+    const bool one = jobs <= cus && prefix <= sa_one(hd) && max_len <= sa_one(hd) + sa_one(hd) * jobs / cus;
     if (prefix && !one) {
         // rows of a prefix workgroup: 128 or 256 on LDS tiles, or 16 streamed
         const uint64_t through = (rows_kv + SA_ROWS - 1) / SA_ROWS * prefix * nkv;
@@ -841,7 +845,7 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
     }
     // a sequence's own tokens (all of them where the prefix has no parts)
     const uint32_t tokens = p.n_pre ? (own ? own : 1) : max_len;
-    p.n_own = one ? 1 : cut(jobs, tokens, SA_OWN_PER, p.tile ? 512 : jobs >= cus ? 256 : 128);
+    p.n_own = one ? 1 : cut(jobs, tokens, p.tile ? SA_TILE_OWN_PER : SA_OWN_PER, p.tile ? 512 : 256);
     p.own_len = ceil_div(ceil_div(tokens, p.n_own), SA_KB) * SA_KB;
     const uint64_t pre = (uint64_t)p.n_pre * p.pre_tiles * nkv, all = pre + (uint64_t)p.n_own * n_seq * nkv;
     // (a launch has fewer than 2^32 threads: workgroups of up to 512, rows of 32 lanes)
@@ -947,8 +951,7 @@ static int shared_launch(zh_ctx *c, const SharedArgs &a, const SharedPlan &p) {
         blocks -= p.pre_blocks;
         b.join = p.n_own == 1;
     }
-    if (p.waves == 8) hipLaunchKernelGGL((k_shared_attn<HD, NP, 8, T>), dim3(blocks), dim3(512), 0, c->stream, b);
-    else hipLaunchKernelGGL((k_shared_attn<HD, NP, 4, T>), dim3(blocks), dim3(256), 0, c->stream, b);
+    hipLaunchKernelGGL((k_shared_attn<HD, NP, T>), dim3(blocks), dim3(64 * W), 0, c->stream, b);
     ZH_LAUNCH_CHECK(c);
     if (a.n_pre + a.n_own > 1 && !b.join) {
         const uint32_t per = 256 / (HD / 4);  // rows of a workgroup
