@@ -49,9 +49,9 @@ constexpr int W = 4;              // waves of a workgroup
 //    of 500 18.4 / 18.8, of 900 12.9 / 11.2; at 64: 8 at 760 7.2 / 7.8, 16 at
 //    1500 14.4 / 13.0, 32 at 1400 16.1 / 19.4;
 //  * workgroups per CU that the parts are cut for: 1 of a prefix (16 sequences
-//    at 4096 f32 14.2 us, 2: 17.6), 4 of own tokens (64 sequences at 1000 tokens
-//    47.9 us, 8: 50.4; 8 at 4000 26.8, 31.2; 64 of 1 to 4000 105, 102), 8 after a
-//    tile launch (64 of up to 2000 90.6, 4: 95.9; 128 of up to 4000 221, 251);
+//    at 4096 f32 14.2 us, 2: 17.6), 8 of own tokens (100 sequences of 1 to 4000
+//    167 us, 4: 197, 12: 164; 128 of up to 4000 after a tile launch 221, 251, 215;
+//    64 of 4000 173, 163, 177; of 1000 49.8, 48.0, 49.8);
 //  * parts of at least 128 tokens, a step for each wave; own ones of 256 (16
 //    sequences at 4096 of up to 300 own 15.9 us, 128: 17.0), and of 512 after a
 //    tile launch, where a single own part of a sequence also joins the prefix's
@@ -61,7 +61,7 @@ constexpr uint64_t sa_tile(uint32_t hd, bool f32) {
     return hd == 64 ? (f32 ? 270000 : 180000) : (f32 ? 450000 : 280000);
 }
 constexpr uint32_t sa_one(uint32_t hd) { return hd == 64 ? 768 : 512; }
-constexpr uint32_t SA_PRE_PER = 1, SA_OWN_PER = 4, SA_TILE_OWN_PER = 8, SA_TILE_FIX = 5;
+constexpr uint32_t SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_FIX = 5;
 
 struct SharedArgs {
     const uint8_t *q;
@@ -845,7 +845,7 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
     }
     // a sequence's own tokens (all of them where the prefix has no parts)
     const uint32_t tokens = p.n_pre ? (own ? own : 1) : max_len;
-    p.n_own = one ? 1 : cut(jobs, tokens, p.tile ? SA_TILE_OWN_PER : SA_OWN_PER, p.tile ? 512 : 256);
+    p.n_own = one ? 1 : cut(jobs, tokens, SA_OWN_PER, p.tile ? 512 : 256);
     p.own_len = ceil_div(ceil_div(tokens, p.n_own), SA_KB) * SA_KB;
     const uint64_t pre = (uint64_t)p.n_pre * p.pre_tiles * nkv, all = pre + (uint64_t)p.n_own * n_seq * nkv;
     // (a launch has fewer than 2^32 threads: workgroups of up to 512, rows of 32 lanes)
