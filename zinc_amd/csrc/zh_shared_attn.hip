@@ -504,17 +504,17 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
     }
     const uint8_t *kh = (const uint8_t *)(a.kc + (size_t)kvh * a.cache_tokens * HD);
     const uint8_t *vh = (const uint8_t *)(a.vc + (size_t)kvh * a.cache_tokens * HD);
-    uint32_t pages = 0;  // lane l: page 64 (stage / 16) + l of the part
+    // the page that this wave copies of a stage, looked up (by a scalar load, which
+    // the copies' order does not wait for) before the barrier ahead of its copy
     bool bad = false;
-    auto issue = [&](uint32_t st) __attribute__((always_inline)) {
-        if (st % 16 == 0) {
-            pages = a.tables[min(t0 / 16 + st * 4 + lane, (t1 - 1) / 16)];
-            if (pages >= a.cache_tokens / 16) {
-                bad = true;
-                pages = 0;
-            }
+    auto page = [&](uint32_t st) __attribute__((always_inline)) {
+        return ((const const_u32 *)a.tables)[min(t0 / 16 + st * 4 + wave % 4, (t1 - 1) / 16)];
+    };
+    auto issue = [&](uint32_t st, uint32_t pg) __attribute__((always_inline)) {
+        if (pg >= a.cache_tokens / 16) {
+            bad = true;
+            pg = 0;
         }
-        const uint32_t pg = __builtin_amdgcn_readlane(pages, st % 16 * 4 + wave % 4);
         const uint64_t at = (uint64_t)pg * (16 * ROWB);
         const uint32_t to = lds0 + st % ST_NS * STAGE + wave % 4 * (16 * ROWB);
         if (NW == 4 || wave < 4) {
@@ -543,7 +543,11 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
         }
     };
     // the first copies go out before the rows are read
-    for (uint32_t st = 0; st < 3 && st < nst; st++) issue(st);
+    const uint32_t pg0 = page(0), pg1 = page(1), pg2 = page(2);
+    uint32_t pg = page(3);
+    issue(0, pg0);
+    if (nst > 1) issue(1, pg1);
+    if (nst > 2) issue(2, pg2);
     // ---- the row's q: dims 16 k + 8 h ..
     half8 qf[NP][KS];
     float c = fabsf(a.scale) * 1.44269504088896340736f;  // raw scores to base 2
@@ -653,14 +657,17 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
         if (st >= nst) break;  // uniform
         landed(st);
         lds_bar();
-        if (st + 3 < nst) issue(st + 3);
+        if (st + 3 < nst) issue(st + 3, pg);
         const uint32_t tk = t0 + st * ST_KB;
         if (tk + ST_KB > t1) {  // V of the tokens past the part: zero (0 times NaN is NaN)
             for (uint32_t i = (t1 - tk) * ROWB + tid * 16; i < STAGE; i += 64 * NW * 16)
                 *(u32x4 *)(lds + (ST_NS + slot) * STAGE + i) = u32x4{0, 0, 0, 0};
             lds_bar();
         }
-        if (!mine) continue;
+        if (!mine) {
+            pg = page(st + 4);
+            continue;
+        }
 #pragma unroll
         for (uint32_t kt = 0; kt < 2; kt++) {
             half8 pf[NP][2], vf[2][DT];
@@ -712,6 +719,7 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
                 __builtin_amdgcn_sched_barrier(0);
             }
             load_k((slot + 1) % ST_NS, kt);
+            if (kt == 1) pg = page(st + 4);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
 #pragma unroll
@@ -731,7 +739,7 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
             s = sn;
         }
     }
-    if (bad) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+    if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
     const uint32_t row = row0 + i32;
     l = xor32_sum(l);
     if (row >= rows) return;
