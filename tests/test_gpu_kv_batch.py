@@ -401,6 +401,11 @@ TILED = [  # many rows over a long prefix: K and V through LDS, 128 or 256 rows 
     (16, 4, 64, 5000, [5001 + i for i in range(70)]),                       # 280 rows
     (64, 64, 64, 4510, [4511 + i % 5 for i in range(130)]),                 # parts of more than 64 pages
     (33, 33, 128, 7000, [7001 + 70 * i % 600 for i in range(34)]),          # own tokens in parts of their own
+    # long enough for tiles in f32 too
+    (128, 8, 128, 12001, [12001 + 17 * i for i in range(8)]),
+    (64, 4, 128, 3137, [3137, 3] + [3138 + i % 90 for i in range(60)]),
+    (48, 8, 64, 24001, [24050, 24001, 400, 24040, 24002, 24100, 24400]),
+    (33, 33, 128, 7741, [7742 + 90 * i % 1300 for i in range(34)]),
 ]
 
 
@@ -419,11 +424,34 @@ def test_attention_of_many_rows(zh, ctx, case, t):
     close(got[only], want[only], tol[only])
 
 
-def test_attention_rescales_when_later_scores_are_larger(zh, ctx):
-    """Scores that grow along a prefix of 1408 tokens by about 2^15 in all, in
-    tiles and streamed: the running maximum moves again and again."""
+@pytest.mark.parametrize("t", [0, 1], ids=["f32", "f16"])
+def test_attention_in_tiles_of_odd_queries_and_a_bad_page(zh, ctx, t):
+    """992 rows over a prefix of 3137 tokens: a query of f16's smallest values, one
+    with a NaN (no other row's), and a page of the prefix outside the cache."""
+    rng = np.random.default_rng(22)
+    P, lens = 3137, [3138 + i % 40 for i in range(62)]
+    kc, vc, tables, _, M = make(rng, 62, 4, 128, P, lens, poison=False)
+    q = rng.standard_normal((62, 64, 128)).astype(NP_TYPE[t])
+    q[5] *= NP_TYPE[t](2.0 ** -20)
+    x = q.copy()
+    x[7, 9, 3] = np.nan
+    tables[0, 100] = 0xFFFFFFFF
+    got = run_attention(zh, ctx, x, kc, vc, tables, lens, P, M, t, expect_error=True)
+    tables[0, 100] = 0
+    only = [0, 5, 7, 61]
+    want, tol = attend64(q, kc, vc, tables, lens, 128 ** -0.5, t, P, only)
+    ok = np.ones(got.shape, bool)
+    ok[7, 9] = False
+    assert np.isnan(got[7, 9]).all()
+    close(got[only], want[only], tol[only], ok[only])
+
+
+@pytest.mark.parametrize("P", [1408, 2944])  # (f16 in tiles, f32 too)
+def test_attention_rescales_when_later_scores_are_larger(zh, ctx, P):
+    """Scores that grow along a prefix by about 2^15 in all, in tiles and
+    streamed: the running maximum moves again and again."""
     rng = np.random.default_rng(21)
-    P, lens = 1408, [1410 + i for i in range(64)]
+    lens = [P + 2 + i for i in range(64)]
     kc, vc, tables, _, M = make(rng, 64, 4, 128, P, lens)
     q = rng.standard_normal((64, 64, 128)).astype(np.float16)
     t = np.arange(P)

@@ -348,6 +348,25 @@ def test_decode_of_more_workgroups_than_a_launch_has():
     assert decode_check(kv, decode(prefix_len=0, **big)) == OK
 
 
+@pytest.mark.parametrize("n_seq,prefix", [(1, 0), (3, 300), (16, 0), (16, 4096), (40, 700), (64, 9000), (200, 8192)])
+def test_workspace_for_a_length_serves_the_shorter_ones(n_seq, prefix):
+    """A workspace is made for the largest max_len of a serving loop."""
+    kv = batch(n_seq=n_seq, table_stride=4096, tables=Fake(4 * n_seq * 4096))
+    q, out, lens = Fake(1 << 30), Fake(1 << 30), Fake(4 * n_seq)
+
+    def need(max_len, t):
+        lo, hi = 0, 1 << 40
+        while lo < hi:
+            mid = (lo + hi) // 2
+            r = decode(q=q, out=out, seq_lens=lens, ws=Fake(mid), prefix_len=prefix, max_len=max_len, type=t)
+            lo, hi = (lo, mid) if decode_check(kv, r) == OK else (mid + 1, hi)
+        return lo
+
+    for t in (0, F16):
+        sizes = [need(max(prefix, 1) + own, t) for own in (0, 1, 16, 100, 130, 300, 500, 513, 700, 1100, 2000, 5000, 30000)]
+        assert sizes == sorted(sizes)
+
+
 def test_page_numbers_are_integers_of_32_bits():
     for bad in ([-1], [1 << 32], np.array([-1]), np.array([1 << 32]), np.array([1.5]), [[1]], ["a"]):
         with pytest.raises((ValueError, OverflowError, TypeError)):

@@ -33,11 +33,10 @@ constexpr int W = 4;              // waves of a workgroup
 //  * LDS tiles where the 16-row tiles' prefix tokens over the kv heads reach
 //    sa_tile: below it one more reading of K and V through the L2s costs less
 //    than the tiles' longer launch. us tiled / streamed, f16 at head_dim 128: 96
-//    rows over 4096 tokens (196K) 18.0 / 17.5, 6144 (294K) 21.8 / 22.4, 12288
-//    25.9 / 36.2; 256 rows over 1024 19.3 / 15.1, 8192 34.8 / 54.6. f32 128 rows
-//    over 6144 (393K) 29.1 / 27.3, 8192 (524K) 31.7 / 33.5; f16 at 64 48 rows
-//    over 4096 (98K) 11.7 / 11.3, 96 over 4096 (196K) 12.9 / 13.2; f32 at 64 96
-//    over 4096 14.5 / 13.6, 6144 (294K) 15.8 / 16.4;
+//    rows over 6144 tokens (294K) 21.0 / 19.9, 8192 (393K) 22.5 / 23.7, 128 over
+//    8192 (524K) 24.5 / 27.3; f32 128 over 8192 30.2 / 27.6, 12288 (786K) 34.6 /
+//    36.2; f16 at 64 128 over 4096 (262K) 13.2 / 12.4, 96 over 8192 14.2 / 15.4;
+//    f32 at 64 128 over 6144 (393K) 16.3 / 15.2, 96 over 12288 (589K) 19.7 / 20.1;
 //  * a tile launch's parts: those that fill 1 to 4 rounds of one workgroup per CU
 //    best, a round's start and end counted as SA_TILE_FIX stages (180 sequences at
 //    8192 58.5 us, in the nearest number of parts 73.9);
@@ -58,7 +57,7 @@ constexpr int W = 4;              // waves of a workgroup
 //    (32 sequences of up to 512: 38 us, in two parts and a launch that joins them
 //    40.7; up to 1000 48.8, 45.9; 64 of up to 4000 139 us, in one part 171).
 constexpr uint64_t sa_tile(uint32_t hd, bool f32) {
-    return hd == 64 ? (f32 ? 270000 : 180000) : (f32 ? 450000 : 280000);
+    return hd == 64 ? (f32 ? 560000 : 290000) : (f32 ? 750000 : 350000);
 }
 constexpr uint32_t sa_one(uint32_t hd) { return hd == 64 ? 768 : 512; }
 constexpr uint32_t SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_FIX = 5;
@@ -834,7 +833,9 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
         p.pre_tiles = ceil_div(rows_kv, p.tile ? 128u * p.tile : SA_ROWS);
         const uint64_t pj = (uint64_t)p.pre_tiles * nkv;
         const uint32_t step = p.tile ? ST_KB : SA_KB;
-        uint32_t n = cut(pj, prefix, SA_PRE_PER, 128);
+        // (at most that many: a CU with two of them would end last)
+        const uint64_t want = SA_PRE_PER * cus / pj;
+        uint32_t n = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(want, 1), ceil_div(prefix, 128));
         if (p.tile) {
             // one workgroup per CU: the parts that fill 1 to 4 rounds of them,
             // by the rounds' stages and SA_TILE_FIX of their start and end
