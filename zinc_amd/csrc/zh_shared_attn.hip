@@ -37,9 +37,11 @@ constexpr int W = 4;              // waves of a workgroup
 //    8192 (524K) 24.5 / 27.3; f32 128 over 8192 30.2 / 27.6, 12288 (786K) 34.6 /
 //    36.2; f16 at 64 128 over 4096 (262K) 13.2 / 12.4, 96 over 8192 14.2 / 15.4;
 //    f32 at 64 128 over 6144 (393K) 16.3 / 15.2, 96 over 12288 (589K) 19.7 / 20.1;
-//  * a tile launch's parts: those that fill 1 to 4 rounds of one workgroup per CU
-//    best, a round's start and end counted as SA_TILE_FIX stages (180 sequences at
-//    8192 58.5 us, in the nearest number of parts 73.9);
+//  * a prefix's parts: those that fill 1 to 4 rounds of one workgroup per CU best,
+//    a round's start and end counted as SA_TILE_FIX stages, streamed SA_FIX steps
+//    (180 sequences at 8192 in tiles 58.5 us, in the nearest number of parts 73.9;
+//    streamed 48 rows at 12288 20.5, in the nearest number 27.5, 384 at 8192 68.3,
+//    with one round 81.9; 16 sequences at 4096 f32 14.2, with two rounds 17.6);
 //  * a whole context, prefix and own tokens, in one workgroup where there is at
 //    most one per CU, the more of them the longer (sa_one tokens for few, twice
 //    that for one per CU), a prefix past sa_one excepted. us whole / in parts, f16
@@ -47,10 +49,9 @@ constexpr int W = 4;              // waves of a workgroup
 //    18.4 / 15.3; 32 at 1000 22.4 / 26.1, of 1 to 1400 24.6 / 23.0, with a prefix
 //    of 500 18.4 / 18.8, of 900 12.9 / 11.2; at 64: 8 at 760 7.2 / 7.8, 16 at
 //    1500 14.4 / 13.0, 32 at 1400 16.1 / 19.4;
-//  * workgroups per CU that the parts are cut for: 1 of a prefix (16 sequences
-//    at 4096 f32 14.2 us, 2: 17.6), 8 of own tokens (100 sequences of 1 to 4000
-//    167 us, 4: 197, 12: 164; 128 of up to 4000 after a tile launch 221, 251, 215;
-//    64 of 4000 173, 163, 177; of 1000 49.8, 48.0, 49.8);
+//  * workgroups per CU that the own tokens' parts are cut for: 8 (100 sequences
+//    of 1 to 4000 167 us, 4: 197, 12: 164; 128 of up to 4000 after a tile launch
+//    221, 251, 215; 64 of 4000 173, 163, 177; of 1000 49.8, 48.0, 49.8);
 //  * parts of at least 128 tokens, a step for each wave; own ones of 256 (16
 //    sequences at 4096 of up to 300 own 15.9 us, 128: 17.0), and of 512 after a
 //    tile launch, where a single own part of a sequence also joins the prefix's
@@ -60,7 +61,7 @@ constexpr uint64_t sa_tile(uint32_t hd, bool f32) {
     return hd == 64 ? (f32 ? 560000 : 290000) : (f32 ? 750000 : 350000);
 }
 constexpr uint32_t sa_one(uint32_t hd) { return hd == 64 ? 768 : 512; }
-constexpr uint32_t SA_PRE_PER = 1, SA_OWN_PER = 8, SA_TILE_FIX = 5;
+constexpr uint32_t SA_OWN_PER = 8, SA_FIX = 3, SA_TILE_FIX = 5;
 
 struct SharedArgs {
     const uint8_t *q;
@@ -819,11 +820,6 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
                  bool f32, SharedPlan &p) {
     const uint32_t G = nh / nkv, own = max_len - prefix;
     const uint64_t rows_kv = (uint64_t)n_seq * G, jobs = (uint64_t)n_seq * nkv;
-    // parts for `per` workgroups per CU, of at least `least` tokens
-    auto cut = [&](uint64_t n, uint32_t tokens, uint32_t per, uint32_t least) {
-        const uint32_t most = ceil_div(tokens, least), want = (uint32_t)(((uint64_t)per * cus + n / 2) / n);
-        return want < 1 ? 1u : want < most ? want : most;
-    };
     p = {};
     const bool one = jobs <= cus && prefix <= sa_one(hd) && max_len <= sa_one(hd) + sa_one(hd) * jobs / cus;
     if (prefix && !one) {
@@ -832,22 +828,18 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
         p.tile = rows_kv > 2 * SA_ROWS && through >= sa_tile(hd, f32) ? (rows_kv > 128 ? 2 : 1) : 0;
         p.pre_tiles = ceil_div(rows_kv, p.tile ? 128u * p.tile : SA_ROWS);
         const uint64_t pj = (uint64_t)p.pre_tiles * nkv;
-        const uint32_t step = p.tile ? ST_KB : SA_KB;
-        // (at most that many: a CU with two of them would end last)
-        const uint64_t want = SA_PRE_PER * cus / pj;
-        uint32_t n = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(want, 1), ceil_div(prefix, 128));
-        if (p.tile) {
-            // one workgroup per CU: the parts that fill 1 to 4 rounds of them,
-            // by the rounds' stages and SA_TILE_FIX of their start and end
-            uint64_t best = ~0ull;
-            for (uint64_t r = 1; r <= 4; r++) {
-                const uint32_t most = ceil_div(prefix, 128), fit = (uint32_t)(r * cus / pj);
-                const uint32_t k = fit < 1 ? 1u : fit < most ? fit : most;
-                const uint64_t cost = ceil_div(pj * k, cus) * (uint64_t)(ceil_div(ceil_div(prefix, k), ST_KB) + SA_TILE_FIX);
-                if (cost < best) {
-                    best = cost;
-                    n = k;
-                }
+        // the parts that fill 1 to 4 rounds of one workgroup per CU, by the rounds'
+        // stages (steps of all waves) and SA_FIX of their start and end
+        const uint32_t fix = p.tile ? SA_TILE_FIX : SA_FIX;
+        const uint32_t step = p.tile ? ST_KB : SA_KB, unit = p.tile ? ST_KB : W * SA_KB, most = ceil_div(prefix, 128);
+        uint32_t n = 1;
+        uint64_t best = ~0ull;
+        for (uint64_t r = 1; r <= 4; r++) {
+            const uint32_t fit = (uint32_t)(r * cus / pj), k = fit < 1 ? 1u : fit < most ? fit : most;
+            const uint64_t cost = ceil_div(pj * k, cus) * (uint64_t)(ceil_div(ceil_div(prefix, k), unit) + fix);
+            if (cost < best) {
+                best = cost;
+                n = k;
             }
         }
         p.pre_len = ceil_div(ceil_div(prefix, n), step) * step;
@@ -855,7 +847,9 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
     }
     // a sequence's own tokens (all of them where the prefix has no parts)
     const uint32_t tokens = p.n_pre ? (own ? own : 1) : max_len;
-    p.n_own = one ? 1 : cut(jobs, tokens, SA_OWN_PER, p.tile ? 512 : 256);
+    const uint32_t most = one ? 1 : ceil_div(tokens, p.tile ? 512 : 256);
+    const uint32_t want = (uint32_t)(((uint64_t)SA_OWN_PER * cus + jobs / 2) / jobs);
+    p.n_own = want < 1 ? 1u : want < most ? want : most;
     p.own_len = ceil_div(ceil_div(tokens, p.n_own), SA_KB) * SA_KB;
     const uint64_t pre = (uint64_t)p.n_pre * p.pre_tiles * nkv, all = pre + (uint64_t)p.n_own * n_seq * nkv;
     // (a launch has fewer than 2^32 threads: workgroups of up to 512, rows of 32 lanes)
