@@ -125,7 +125,7 @@ struct SharedPart {
 // NP pieces: q (scaled by a power of two to a maximum in [1, 2)) and P as sums
 // of NP fp16 values; 2 keep 22 bits of each.
 // Bound by the reads: 3 workgroups of 4 waves a CU (168 registers), each wave's
-// step 16 KB; 64 sequences of 4000 tokens (1.05 GB) 163 us, 6.4 TB/s, 48 of 1 to
+// step 16 KB; 64 sequences of 4000 tokens (1.05 GB) 167 us, 6.3 TB/s, 48 of 1 to
 // 4096 (400 MB) 79 us, 5 TB/s. Two or four row tiles a wave, or a workgroup on the
 // same tokens, read less from the L2s but hold fewer steps in flight: 16
 // sequences at 4096 20 and 29 us, 16.3 with one.
