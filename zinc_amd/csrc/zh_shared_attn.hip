@@ -78,8 +78,19 @@ struct SharedArgs {
     uint32_t pre_len;                // tokens of a prefix part (a multiple of SA_KB)
     uint32_t own_len;                // tokens of a sequence's own part, at least
     uint32_t join;                   // the own parts' workgroups write the result (n_own == 1, the prefix's parts are there)
-    float scale;
+    float scale;        // |attn_scale| log2 e = scale * 2^scale_exp, with attn_scale's sign
+    int32_t scale_exp;
 };
+
+// What takes the products of a row's q, scaled by 2^-e, to base-2 scores: the
+// scale's magnitude times 2^e, kept in [2^-120, 2^80]. Products lie below 2^39 in
+// steps of 2^-48 at least, so below that range every weight is 1 and above it all
+// but a row's largest are 0, as without the bounds; within it no score is
+// infinite, and none that is masked (-inf) meets a factor of 0.
+ZH_DEV float score_factor(const SharedArgs &a, int e) {
+    const float f = fabsf(ldexpf(a.scale, a.scale_exp + e));
+    return f < 0x1p-120f ? 0x1p-120f : f > 0x1p80f ? 0x1p80f : f;  // (NaN stays)
+}
 
 // The sequence's length as the kernels take it: cut at max_len (the host has
 // checked that the table holds that many tokens).
@@ -123,7 +134,8 @@ struct SharedPart {
 //   V's rows are read whole (lane li: dims HD/16 li ..), transposed by byte
 //   permutes; column li of the output tile n is dim HD/16 li + n.
 // NP pieces: q (scaled by a power of two to a maximum in [1, 2)) and P as sums
-// of NP fp16 values; 2 keep 22 bits of each.
+// of NP fp16 values; 2 keep 22 bits of each. The scale's and q's powers of two meet
+// in score_factor, for queries and scales of any size.
 // Bound by the reads: 3 workgroups of 4 waves a CU (168 registers), each wave's
 // step 16 KB; 64 sequences of 4000 tokens (1.05 GB) 167 us, 6.3 TB/s, 48 of 1 to
 // 4096 (400 MB) 79 us, 5 TB/s. Two or four row tiles a wave, or a workgroup on the
@@ -194,7 +206,7 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
     }
     // the row's q as operand fragments: dims 32 k4 + 8 lg ..
     half8 qf[NP][K4];
-    float c = a.scale * 1.44269504088896340736f;  // scores in base 2
+    int e = 0;  // q is scaled by 2^-e
     {
         const uint32_t row = w.row0 + min(li, w.nrow - 1), rs = row / a.G, rh = kvh * a.G + row % a.G;
         const T *qp = (const T *)(a.q + rs * a.q_row) + (size_t)rh * HD + 8 * lg;
@@ -205,28 +217,24 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k4][e]));
         }
-        float up = 1.f;
         if (NP > 1) {
             mx = xor32_max(xor16_max(mx));
-            // 2^-E for a maximum in [2^E, 2^(E+1)) (not for zero, infinite or tiny rows)
             const uint32_t E = __float_as_uint(mx) >> 23;
-            if (E >= 8 && E <= 246) {
-                up = __uint_as_float((254u - E) << 23);
-                c *= __uint_as_float(E << 23);
-            }
+            if (E < 255) e = (int)E - 127;  // a maximum in [2^e, 2^(e+1)), or a smaller one in 2^-127 steps
         }
 #pragma unroll
         for (int k4 = 0; k4 < K4; k4++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float y = v[k4][e] * up;
+            for (int i = 0; i < 8; i++) {
+                float y = NP > 1 ? ldexpf(v[k4][i], -e) : v[k4][i];
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
-                    qf[p][k4][e] = (_Float16)y;
-                    y -= (float)qf[p][k4][e];
+                    qf[p][k4][i] = (_Float16)y;
+                    y -= (float)qf[p][k4][i];
                 }
             }
     }
+    const float c = copysignf(score_factor(a, e), a.scale);
     floatx4 o[ND];
 #pragma unroll
     for (int n = 0; n < ND; n++) o[n] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -551,7 +559,7 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
     if (nst > 2) issue(2, pg2);
     // ---- the row's q: dims 16 k + 8 h ..
     half8 qf[NP][KS];
-    float c = fabsf(a.scale) * 1.44269504088896340736f;  // raw scores to base 2
+    int qe = 0;  // q is scaled by 2^-qe
     {
         const uint32_t row = min(row0 + i32, rows - 1);
         const T *qp = (const T *)(a.q + row / a.G * a.q_row) + (size_t)(kvh * a.G + row % a.G) * HD + 8 * h;
@@ -562,21 +570,18 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k][e]));
         }
-        // (the scale's sign goes into q: the largest product is the largest score)
-        float up = a.scale < 0.f ? -1.f : 1.f;
         if (NP > 1) {
             mx = xor32_max(mx);
             const uint32_t E = __float_as_uint(mx) >> 23;
-            if (E >= 8 && E <= 246) {
-                up *= __uint_as_float((254u - E) << 23);
-                c *= __uint_as_float(E << 23);
-            }
+            if (E < 255) qe = (int)E - 127;
         }
+        // (the scale's sign goes into q: the largest product is the largest score)
+        const float sign = copysignf(1.f, a.scale);
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                float x = v[k][e] * up;
+                float x = (NP > 1 ? ldexpf(v[k][e], -qe) : v[k][e]) * sign;
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
                     qf[p][k][e] = (_Float16)x;
@@ -584,6 +589,7 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
                 }
             }
     }
+    const float c = score_factor(a, qe);  // raw scores to base 2
     f32x16 o[DT];
     float m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -1001,7 +1007,12 @@ extern "C" int zh_flash_decode_shared(zh_ctx *c, const zh_kv_batch *kv, const zh
     a.pre_blocks = p.pre_blocks;
     a.pre_len = p.pre_len;
     a.own_len = p.own_len;
-    a.scale = r->attn_scale != 0.f ? r->attn_scale : 1.0f / sqrtf((float)kv->head_dim);
+    // (64 bits: a scale of any size times log2 e)
+    const double scale = (double)(r->attn_scale != 0.f ? r->attn_scale : 1.0f / sqrtf((float)kv->head_dim)) *
+                         1.44269504088896340736f;
+    int scale_exp = 0;
+    a.scale = isfinite(scale) ? (float)frexp(scale, &scale_exp) : NAN;
+    a.scale_exp = scale_exp;
     if (kv->head_dim == 128)
         return size == 4 ? shared_launch<128, 2, float>(c, a, p) : shared_launch<128, 1, _Float16>(c, a, p);
     return size == 4 ? shared_launch<64, 2, float>(c, a, p) : shared_launch<64, 1, _Float16>(c, a, p);
