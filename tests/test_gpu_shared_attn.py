@@ -41,6 +41,20 @@ def test_f32_queries_of_the_type_s_whole_range(zh, ctx, case, size):  # noqa: F8
 
 
 @FORMS
+def test_f32_queries_with_one_large_dim(zh, ctx, case):  # noqa: F811
+    """A dim of the queries 2^16 times the others, where K is zero: the scores are the
+    others' (q's smaller dims keep 2^-39 of the largest: here 2^-23 of a typical one)."""
+    q, kc, vc, tables, lens, P, M = inputs(case, 9)
+    q[:, :, 5] = 2.0 ** 16 * np.where(np.arange(case[0]) % 2, 1, -1)
+    kc[:, :, 5] = 0
+    q = q.astype(np.float32)
+    got = run_attention(zh, ctx, q, kc, vc, tables, lens, P, M, 0)
+    only = checked(lens)
+    want, tol = attend64(q, kc, vc, tables, lens, case[2] ** -0.5, 0, P, only)
+    close(got[only], want[only], tol[only])
+
+
+@FORMS
 @pytest.mark.parametrize("t,size,scale", [(0, 1e-30, 1e-30), (0, 1e-38, -1e-38), (0, 1.0, 1e-44), (1, 1.0, -1e-44)])
 def test_scores_too_small_to_tell_tokens_apart(zh, ctx, case, t, size, scale):  # noqa: F811
     """Scores below 2^-60: every weight alike, nothing masked among them (scale *

@@ -133,9 +133,11 @@ struct SharedPart {
 //   wants them: O^T += V^T P^T, k = (token 4 lg + r of tile 0, then of tile 1).
 //   V's rows are read whole (lane li: dims HD/16 li ..), transposed by byte
 //   permutes; column li of the output tile n is dim HD/16 li + n.
-// NP pieces: q (scaled by a power of two to a maximum in [1, 2)) and P as sums
-// of NP fp16 values; 2 keep 22 bits of each. The scale's and q's powers of two meet
-// in score_factor, for queries and scales of any size.
+// NP pieces: q (scaled by a power of two to a maximum in [2^14, 2^15)) and P as
+// sums of NP fp16 values; 2 keep 22 bits of each, of q's dims down to 2^-14 of the
+// row's largest (below that they lie in fp16's subnormals: 2^-39 of the largest).
+// The scale's and q's powers of two meet in score_factor, for queries and scales of
+// any size.
 // Bound by the reads: 3 workgroups of 4 waves a CU (168 registers), each wave's
 // step 16 KB; 64 sequences of 4000 tokens (1.05 GB) 167 us, 6.3 TB/s, 48 of 1 to
 // 4096 (400 MB) 79 us, 5 TB/s. Two or four row tiles a wave, or a workgroup on the
@@ -220,7 +222,7 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
         if (NP > 1) {
             mx = xor32_max(xor16_max(mx));
             const uint32_t E = __float_as_uint(mx) >> 23;
-            if (E < 255) e = (int)E - 127;  // a maximum in [2^e, 2^(e+1)), or a smaller one in 2^-127 steps
+            if (E < 255) e = (int)E - 141;  // (E == 0, subnormal or zero rows: a smaller maximum)
         }
 #pragma unroll
         for (int k4 = 0; k4 < K4; k4++)
@@ -573,7 +575,7 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
         if (NP > 1) {
             mx = xor32_max(mx);
             const uint32_t E = __float_as_uint(mx) >> 23;
-            if (E < 255) qe = (int)E - 127;
+            if (E < 255) qe = (int)E - 141;
         }
         // (the scale's sign goes into q: the largest product is the largest score)
         const float sign = copysignf(1.f, a.scale);
