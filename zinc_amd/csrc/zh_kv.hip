@@ -393,9 +393,11 @@ __global__ __launch_bounds__(256) void k_qkv_rows8(QkvArgs a) {
 
 }  // namespace
 
-// Bytes from the first to past the last element of `rows` rows of `width`.
+// Bytes from the first to past the last element of `rows` rows of `width` (past 64
+// bits: more than any buffer has).
 static uint64_t rows_bytes(uint32_t rows, uint32_t stride, uint64_t width, uint32_t size) {
-    return ((uint64_t)(rows - 1) * stride + width) * size;
+    const uint64_t n = (uint64_t)(rows - 1) * stride + width;
+    return n > ~0ull / size ? ~0ull : n * size;
 }
 
 bool kv_batch_ok(const zh_kv_batch *kv) {
@@ -403,7 +405,7 @@ bool kv_batch_ok(const zh_kv_batch *kv) {
            kv->n_kv_heads <= 65535 && kv->head_dim && kv->head_dim <= 512 &&
            kv_in_range(kv->k_cache, 0, 2ull * kv->n_kv_heads * kv->cache_tokens * kv->head_dim) &&
            kv_in_range(kv->v_cache, 0, 2ull * kv->n_kv_heads * kv->cache_tokens * kv->head_dim) &&
-           kv_in_range(kv->tables, 0, 4ull * kv->n_seq * kv->table_stride) && kv->k_cache->ptr != kv->v_cache->ptr;
+           kv->tables && (uint64_t)kv->n_seq * kv->table_stride <= kv->tables->size / 4 && kv->k_cache->ptr != kv->v_cache->ptr;
 }
 
 bool kv_rows_overlap(const zh_buf *a, uint64_t a0, uint64_t an, const zh_buf *b, uint64_t b0, uint64_t bn) {
