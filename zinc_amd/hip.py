@@ -7,6 +7,7 @@ missing, importing this module's `lib()` raises.
 """
 import ctypes as C
 import os
+import weakref
 
 import numpy as np
 
@@ -185,17 +186,27 @@ SIGNATURES = {
 
 class _Plan:
     """A struct of the C ABI that a caller fills once and passes to many
-    calls: the buffers it names are kept alive with it."""
+    calls. It keeps its Buffer objects, and a buffer that is freed takes the
+    plan with it: calls with it are refused from then on."""
 
     def _set(self, **fields):
         self.c = self.Struct()
         self._held = []
         for name, v in fields.items():
             if isinstance(v, Buffer):
-                self._held.append(v)
+                self._hold(v)
                 v = v.h
             setattr(self.c, name, v)
         self.ptr = C.byref(self.c)
+
+    def _hold(self, buf):
+        self._held.append(buf)
+        if buf._plans is None:
+            buf._plans = weakref.WeakSet()
+        buf._plans.add(self)
+
+    def _drop(self):
+        self.c = self.ptr = None
 
 
 class KvBatch(_Plan):
@@ -257,7 +268,8 @@ class KvCaches(_Plan):
         self._array = (_P * max(len(caches), 1))(*[b.h for b in caches])
         self._set(caches=C.cast(self._array, C.POINTER(_P)), n_caches=len(caches), cache_tokens=cache_tokens,
                   n_kv_heads=n_kv_heads, head_dim=head_dim)
-        self._held = list(caches)
+        for b in caches:
+            self._hold(b)
 
 
 _lib = None
@@ -302,6 +314,7 @@ def _u32_array(a):
 
 class Buffer:
     """Device buffer (zh_buf): owned by its Context."""
+    _plans = None  # the plans that name it
 
     def __init__(self, ctx, size):
         self.ctx = ctx
@@ -312,6 +325,8 @@ class Buffer:
 
     def free(self):
         if self.h:
+            for plan in list(self._plans or ()):
+                plan._drop()
             lib().zh_buf_free(self.ctx.h, self.h)
             self.h = None
 
