@@ -312,7 +312,9 @@ typedef struct zh_decode_rows {
  * Finite queries and scales of any size. Allocates nothing and adds in a fixed order; calls that
  * may overlap (other contexts, replayed graphs) need a ws each. */
 int zh_flash_decode_shared(zh_ctx *ctx, const zh_kv_batch *kv, const zh_decode_rows *rows);
-/* Bytes of ws for a call of these sizes (0: refused sizes). */
+/* Bytes of ws for a call of these sizes and for every call of fewer sequences, a
+ * shorter prefix (none included) or a smaller max_len, of either type (0: refused
+ * sizes). A call is checked for what it needs itself, which may be less. */
 uint64_t zh_flash_decode_shared_ws(zh_ctx *ctx, const zh_kv_batch *kv, uint32_t n_heads, uint32_t prefix_len,
                                    uint32_t max_len);
 /* A set of at most 256 caches of one shape (the K and V caches of some or all

@@ -824,6 +824,12 @@ struct SharedPlan {
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
+// Whether the prefix of rows_kv rows a kv head goes through LDS tiles.
+bool shared_tiled(uint64_t rows_kv, uint32_t nkv, uint32_t hd, uint32_t prefix, bool f32) {
+    const uint64_t through = (rows_kv + SA_ROWS - 1) / SA_ROWS * prefix * nkv;
+    return rows_kv > 2 * SA_ROWS && through >= sa_tile(hd, f32);
+}
+
 bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t prefix, uint32_t max_len,
                  bool f32, SharedPlan &p) {
     const uint32_t G = nh / nkv, own = max_len - prefix;
@@ -832,8 +838,7 @@ bool shared_plan(uint32_t cus, uint32_t n_seq, uint32_t nh, uint32_t nkv, uint32
     const bool one = jobs <= cus && prefix <= sa_one(hd) && max_len <= sa_one(hd) + sa_one(hd) * jobs / cus;
     if (prefix && !one) {
         // rows of a prefix workgroup: 128 or 256 on LDS tiles, or 16 streamed
-        const uint64_t through = (rows_kv + SA_ROWS - 1) / SA_ROWS * prefix * nkv;
-        p.tile = rows_kv > 2 * SA_ROWS && through >= sa_tile(hd, f32) ? (rows_kv > 128 ? 2 : 1) : 0;
+        p.tile = !shared_tiled(rows_kv, nkv, hd, prefix, f32) ? 0 : rows_kv > 128 ? 2 : 1;
         p.pre_tiles = ceil_div(rows_kv, p.tile ? 128u * p.tile : SA_ROWS);
         const uint64_t pj = (uint64_t)p.pre_tiles * nkv;
         // the parts that fill 1 to 4 rounds of one workgroup per CU, by the rounds'
@@ -925,18 +930,52 @@ extern "C" int zh_check_decode_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_d
     return ZH_OK;
 }
 
+// How a call of these sizes and type is cut: out = {rows of a prefix workgroup / 128
+// where it goes through LDS tiles (0: streamed), parts of the prefix, parts of a
+// sequence's own tokens, bytes of ws}. Exported for the tests.
+extern "C" int zh_check_shared_plan(const zh_kv_batch *kv, uint32_t n_heads, uint32_t prefix_len, uint32_t max_len,
+                                    uint32_t type, uint32_t cus, uint64_t *out) {
+    SharedPlan p;
+    if (!shared_shape_ok(kv, n_heads, prefix_len, max_len) ||
+        !shared_plan(cus, kv->n_seq, n_heads, kv->n_kv_heads, kv->head_dim, prefix_len, max_len, type == ZH_F32, p))
+        return ZH_ERR_INVALID_ARGUMENT;
+    out[0] = p.tile;
+    out[1] = p.n_pre;
+    out[2] = p.n_own;
+    out[3] = p.bytes;
+    return ZH_OK;
+}
+
+// zh_flash_decode_shared_ws of a device of `cus` CUs (exported for the tests): an
+// upper bound for every smaller n_seq, prefix_len and max_len and both types, since
+// one call's bytes (shared_plan) fall and rise with each of them. Its rows of parts,
+// n_seq (n_pre + n_own) of them per head, are
+//  * own ones: n_own is 1 or at most SA_OWN_PER cus / (n_seq nkv) + 1/2, and at most
+//    one per 256 tokens;
+//  * the prefix's: n_pre is 1 or at most 4 cus / (nkv pre_tiles), where pre_tiles
+//    holds n_seq heads / nkv rows in tiles of 16, 128 or 256, and at most one per 128
+//    tokens.
+extern "C" uint64_t zh_check_shared_ws(const zh_kv_batch *kv, uint32_t n_heads, uint32_t prefix_len, uint32_t max_len,
+                                       uint32_t cus) {
+    SharedPlan p;
+    if (!shared_shape_ok(kv, n_heads, prefix_len, max_len)) return 0;
+    const uint32_t nkv = kv->n_kv_heads, hd = kv->head_dim;
+    const uint64_t n = kv->n_seq, rows_kv = n * (n_heads / nkv);
+    if (!shared_plan(cus, kv->n_seq, n_heads, nkv, hd, prefix_len, max_len, false, p) ||
+        !shared_plan(cus, kv->n_seq, n_heads, nkv, hd, prefix_len, max_len, true, p))
+        return 0;
+    const uint64_t own = std::min(n * ceil_div(max_len, 256),
+                                  std::max<uint64_t>(n, (uint64_t)SA_OWN_PER * cus / nkv + n / 2 + 1));
+    // (f16 takes the tiles first)
+    const uint64_t tile = !shared_tiled(rows_kv, nkv, hd, prefix_len, false) ? SA_ROWS : rows_kv > 128 ? 256 : 128;
+    const uint64_t pre =
+        !prefix_len ? 0 : std::min(n * ceil_div(prefix_len, 128), std::max<uint64_t>(n, 4ull * cus * tile / n_heads));
+    return std::max<uint64_t>(16, (own + pre) * n_heads * (4ull * hd + 8));
+}
+
 extern "C" uint64_t zh_flash_decode_shared_ws(zh_ctx *c, const zh_kv_batch *kv, uint32_t n_heads, uint32_t prefix_len,
                                               uint32_t max_len) {
-    if (!c || !shared_shape_ok(kv, n_heads, prefix_len, max_len)) return 0;
-    uint64_t most = 16;  // (of either type)
-    for (int f32 = 0; f32 < 2; f32++) {
-        SharedPlan p;
-        if (!shared_plan((uint32_t)c->cu_count, kv->n_seq, n_heads, kv->n_kv_heads, kv->head_dim, prefix_len, max_len,
-                         f32 != 0, p))
-            return 0;
-        if (p.bytes > most) most = p.bytes;
-    }
-    return most;
+    return c ? zh_check_shared_ws(kv, n_heads, prefix_len, max_len, (uint32_t)c->cu_count) : 0;
 }
 
 template <int HD, int NP, int NW, typename T>

@@ -487,7 +487,8 @@ class Context:
         self.check(lib().zh_flash_decode_shared(self.h, kv.ptr, rows.ptr))
 
     def flash_decode_shared_ws(self, kv, n_heads, prefix_len, max_len):
-        """Bytes of the workspace of such a call (0: refused sizes)."""
+        """Bytes of a workspace for such a call and every one of fewer sequences, a shorter
+        prefix or a smaller max_len (0: refused sizes)."""
         return lib().zh_flash_decode_shared_ws(self.h, kv.ptr, n_heads, prefix_len, max_len)
 
     def kv_copy_pages(self, dst, src, dst_pages, src_pages):
