@@ -804,7 +804,9 @@ extern "C" int zh_kv_pool_alloc(zh_kv_pool *p, uint64_t request_id, uint32_t cou
     if (count == 0) return ZH_OK;
     try {
         std::vector<uint32_t> &own = p->pages[request_id];
-        own.reserve(own.size() + count);
+        // (room for what is pushed below, twice as much each time: a request that
+        // grows by a page at a time would copy its list for each)
+        if (own.capacity() - own.size() < count) own.reserve(std::max(own.size() + count, 2 * own.capacity()));
         for (uint32_t i = 0; i < count; i++) {
             const uint32_t id = p->free_list.back();
             p->free_list.pop_back();
