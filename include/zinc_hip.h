@@ -276,7 +276,8 @@ typedef struct zh_qkv_rows {
  * pos[t] == ZH_POS_NONE: a padded row, nothing of it is read or written. A row
  * whose sequence, page entry or page lies outside has its q_out written and no
  * cache slot, and the next zh_sync returns ZH_ERR_INVALID_ARGUMENT. Where rows
- * of one call name the same slot it holds, head by head, one of them. head_dim
+ * of one call name the same slot, every element of it is one of theirs, not
+ * always of the same row: name each slot once. head_dim
  * even and at most 512, rope_dim even and at most head_dim (0: no rotation). */
 #define ZH_POS_NONE 0xFFFFFFFFu
 int zh_qk_norm_rope_kv_write_batched(zh_ctx *ctx, const zh_kv_batch *kv, const zh_qkv_rows *rows);
