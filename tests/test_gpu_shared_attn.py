@@ -5,6 +5,8 @@ import numpy as np
 import pytest
 from test_gpu_kv_batch import NP_TYPE, attend64, close, ctx, make, run_attention, store_error, zh  # noqa: F401
 
+from test_shared_attn_plan import plan
+
 pytestmark = pytest.mark.gpu
 
 # q heads, kv heads, head_dim, prefix, lengths: streamed, and through LDS tiles (f32 too)
@@ -89,3 +91,46 @@ def test_scores_too_large_for_f32(zh, ctx, case, t, size, scale):  # noqa: F811
                 assert (np.abs(got[s, h] - want) <= np.abs(want) * 2.0 ** -20 + store_error(t, want)).all(), (s, h)
                 rows += 1
     assert rows > len(checked(lens)) * case[0] // 2
+
+
+# Through LDS tiles in both types: q heads, kv heads, head_dim, prefix, lengths, scale, rows of a
+# workgroup / 128. The prefixes end 1 to 61 tokens into a stage of 64.
+TILED = [
+    (128, 8, 128, 1527, [0, 1527, 5] + [1528 + 3 * i % 31 for i in range(59)], 0.09, 2),  # 992 rows
+    (128, 8, 64, 1153, [1153, 3] + [1154 + i % 19 for i in range(60)], -0.11, 2),
+    (512, 32, 128, 3361, [3361 + 17 * i for i in range(7)], -0.09, 1),                   # 112 rows
+    (512, 32, 64, 2506, [2507, 40, 2506, 2600, 2510, 2511, 2512], 0.125, 1),
+    (128, 8, 128, 1527, [1528 + 19 * i % 1100 for i in range(62)], 0.09, 2),             # own tokens in parts
+    (24, 8, 128, 5221, [5222 + i % 40 for i in range(91)], 0.09, 2),                     # 273 rows, 3 a sequence
+]
+
+
+def relative_rms(got, want):
+    return np.sqrt(np.square(got - want).sum() / np.square(want).sum())
+
+
+# Beside the bound of every element, one of their root mean square: rounding errors of many tokens
+# and dims are as often up as down. f32: a score of up to 8 within 2^-22 of itself moves a weight by
+# 2^-19, the weights' two pieces and exp2 by 2^-21, some hundred sums by 10 2^-24: below 2^-18, and
+# the limit is 2^-17. One fp16 piece of q or of the weights alone is 2^-13 (test_shared_attn_bound).
+# f16: the weights' one piece and the store's rounding, 2^-11 / 12^(1/2) of a value on its average
+# octave each: below 2^-11.
+RMS = {0: 2.0 ** -17, 1: 2.0 ** -11}
+
+
+@pytest.mark.parametrize("t", [0, 1], ids=["f32", "f16"])
+@pytest.mark.parametrize("case", TILED + [(*STREAMED, 0.09, 0)],
+                         ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}-{c[3]}-{len(c[4])}x{max(c[4])}")
+def test_attention_in_the_form_it_is_meant_for(zh, ctx, case, t):  # noqa: F811
+    """Rows of every wave (32 rows) of a workgroup."""
+    nh, nkv, hd, P, lens, scale, tile = case
+    q, kc, vc, tables, _, _, M = inputs(case[:5], nh + P)
+    q = (q * 1.5).astype(NP_TYPE[t])
+    way = plan(len(lens), nh, nkv, hd, P, M, t, ctx.info()[1])
+    assert way[0] == tile and (tile == 0 or way[2] == (3 if max(lens) > P + 1000 else 1))
+    got = run_attention(zh, ctx, q, kc, vc, tables, lens, P, M, t, scale=scale)
+    G = nh // nkv
+    only = [s for s in range(len(lens)) if s == 0 or s * G // 32 != (s - 1) * G // 32 or s == len(lens) - 1]
+    want, tol = attend64(q, kc, vc, tables, lens, scale, t, P, only)
+    close(got[only], want[only], tol[only])
+    assert relative_rms(got[only], want[only]) < RMS[t]
