@@ -200,9 +200,10 @@ extern "C" int zh_kv_copy_pages(zh_ctx *c, const zh_kv_caches *dst, const zh_kv_
 //   h = w (x / sqrt(mean x^2 + eps)) over a head (or x), then dims i and
 //   i + r/2 (i < r/2, r = rope_dim): (a cos - b sin, a sin + b cos) with the
 //   angle pos * inv_freq[i].
-// The angle is a 64-bit product (exact: 32 + 24 bits), reduced in 64 bits to a
-// fraction of a turn: in 32 bits a position of 2^17 alone would leave an error
-// of 2^-8 radians. Everything else is 32-bit and rounded once, at the store.
+// The angle is a 64-bit product (exact below position 2^29: 29 + 24 bits), taken
+// and reduced in 64 bits to a fraction of a turn; at the last positions before 2^32
+// it is off by less than 2^-19 radians. In 32 bits a position of 2^17 alone would
+// leave an error of 2^-8. Everything else is 32-bit and rounded once, at the store.
 // ---------------------------------------------------------------------------
 namespace {
 
@@ -479,7 +480,11 @@ template <typename TI, typename TQ, int L>
 static void qkv_launch8(zh_ctx *c, const QkvArgs &a, uint32_t n) {
     constexpr uint32_t NS = 256 / L;
     const uint32_t H = a.nq + 2 * a.nkv;
-    // few rows: every workgroup one round of heads, for the most workgroups
+    // few rows: every workgroup one round of heads, for the most workgroups. us at 1 /
+    // 4 rounds, 32 + 16 heads of 128 f32 to f16: 64 rows 3.2 / 4.2, 256 3.9 / 4.5, 512
+    // 5.2 / 5.3, 768 6.7 / 6.6, 1024 8.1 / 7.9; f16 of as many heads 512 5.2 / 5.3, 1024
+    // 8.0 / 7.4; 32 heads of 64 f32 512 3.5 / 3.7, 2048 6.4 / 7.4 (one round better);
+    // 56 of 256 f16 128 5.0 / 5.3, 256 7.0 / 5.6 (four better)
     if (n < 512) hipLaunchKernelGGL((k_qkv_rows8<TI, TQ, L, 1>), dim3(n, (H + NS - 1) / NS), dim3(256), 0, c->stream, a);
     else hipLaunchKernelGGL((k_qkv_rows8<TI, TQ, L, 4>), dim3(n, (H + 4 * NS - 1) / (4 * NS)), dim3(256), 0, c->stream, a);
 }
