@@ -309,7 +309,8 @@ typedef struct zh_decode_rows {
  * ZH_ERR_INVALID_ARGUMENT. Nothing past a sequence's end enters its result,
  * whatever the cache holds there. head_dim 64 or 128. ZH_F32: q and the
  * probabilities in two fp16 pieces each (22 bits; of a row's dims below 2^-14 of
- * its largest, 2^-39 of that); ZH_F16: in one; sums and softmax in 32 bits.
+ * its largest, 2^-39 of that); ZH_F16: the probabilities in two, those of a long
+ * prefix of many rows (more than 32 a kv head) in one; sums and softmax in 32 bits.
  * Finite queries and scales of any size. Allocates nothing and adds in a fixed order; calls that
  * may overlap (other contexts, replayed graphs) need a ws each. */
 int zh_flash_decode_shared(zh_ctx *ctx, const zh_kv_batch *kv, const zh_decode_rows *rows);

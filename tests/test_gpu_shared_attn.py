@@ -134,3 +134,22 @@ def test_attention_in_the_form_it_is_meant_for(zh, ctx, case, t):  # noqa: F811
     want, tol = attend64(q, kc, vc, tables, lens, scale, t, P, only)
     close(got[only], want[only], tol[only])
     assert relative_rms(got[only], want[only]) < RMS[t]
+
+
+@pytest.mark.parametrize("case", [STREAMED, (32, 8, 128, 300, [400, 500, 301, 7]), (16, 2, 64, 0, [900, 1, 33, 1300]),
+                                  (64, 4, 128, 1237, [1238 + i for i in range(60)])],
+                         ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}-{c[3]}-{len(c[4])}x{max(c[4])}")
+def test_f16_results_are_rounded_once_where_the_prefix_is_streamed(zh, ctx, case):  # noqa: F811
+    """Against the formula's results rounded to fp16. What is within 2^-18 before that
+    rounding is off by a step (2^-10 at most) in one of 2^8 at most: a root mean square
+    below (2^-18 2^-10)^(1/2) = 2^-14. With weights of 11 bits most results are off by
+    2^-13 before it: (2^-13 2^-10)^(1/2) = 2^-11.5. The limit is 2^-13."""
+    nh, nkv, hd, P, lens = case
+    q, kc, vc, tables, _, _, M = inputs(case, 51)
+    q = (q * 1.5).astype(np.float16)
+    assert plan(len(lens), nh, nkv, hd, P, M, 1, ctx.info()[1])[0] == 0
+    got = run_attention(zh, ctx, q, kc, vc, tables, lens, P, M, 1)
+    only = checked(lens)
+    want, tol = attend64(q, kc, vc, tables, lens, hd ** -0.5, 1, P, only)
+    close(got[only], want[only], tol[only])
+    assert relative_rms(got[only], want[only].astype(np.float16).astype(np.float64)) < 2.0 ** -13

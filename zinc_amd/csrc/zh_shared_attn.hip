@@ -36,7 +36,11 @@ constexpr int W = 4;              // waves of a workgroup
 //    rows over 6144 tokens (294K) 21.0 / 19.9, 8192 (393K) 22.5 / 23.7, 128 over
 //    8192 (524K) 24.5 / 27.3; f32 128 over 8192 30.2 / 27.6, 12288 (786K) 34.6 /
 //    36.2; f16 at 64 128 over 4096 (262K) 13.2 / 12.4, 96 over 8192 14.2 / 15.4;
-//    f32 at 64 128 over 6144 (393K) 16.3 / 15.2, 96 over 12288 (589K) 19.7 / 20.1;
+//    f32 at 64 128 over 6144 (393K) 16.3 / 15.2, 96 over 12288 (589K) 19.7 / 20.1 no
+//    tiles for 32 rows and fewer, of which a workgroup of four waves uses one: 32
+//    rows, f16 at 128, over 32768 tokens of 8 heads 32.0 / 29.0, 65536 of 8 51.7 /
+//    47.6, 16384 of 32 47.5 / 50.1, 131072 of 4 52.7 / 82.5; f32 65536 of 8 80.9 /
+//    50.4; f16 at 64 over 65536 of 8 34.9 / 30.1;
 //  * a prefix's parts: those that fill 1 to 4 rounds of one workgroup per CU best,
 //    a round's start and end counted as SA_TILE_FIX stages, streamed SA_FIX steps
 //    (180 sequences at 8192 in tiles 58.5 us, in the nearest number of parts 73.9;
@@ -52,9 +56,10 @@ constexpr int W = 4;              // waves of a workgroup
 //  * workgroups per CU that the own tokens' parts are cut for: 8 (100 sequences
 //    of 1 to 4000 167 us, 4: 197, 12: 164; 128 of up to 4000 after a tile launch
 //    221, 251, 215; 64 of 4000 173, 163, 177; of 1000 49.8, 48.0, 49.8);
-//  * parts of at least 128 tokens, a step for each wave; own ones of 256 (16
-//    sequences at 4096 of up to 300 own 15.9 us, 128: 17.0), and of 512 after a
-//    tile launch, where a single own part of a sequence also joins the prefix's
+//  * a prefix's parts of at least 128 tokens, a step for each wave; of own tokens at
+//    most one for each 256 begun, all of a length (300 tokens: two of 160; 16
+//    sequences at 4096 of up to 300 own 15.9 us, one for each 128: 17.0), and for
+//    each 512 after a tile launch, where a single own part of a sequence also joins the prefix's
 //    (32 sequences of up to 512: 38 us, in two parts and a launch that joins them
 //    40.7; up to 1000 48.8, 45.9; 64 of up to 4000 139 us, in one part 171).
 constexpr uint64_t sa_tile(uint32_t hd, bool f32) {
@@ -138,6 +143,9 @@ struct SharedPart {
 // row's largest (below that they lie in fp16's subnormals: 2^-39 of the largest).
 // The scale's and q's powers of two meet in score_factor, for queries and scales of
 // any size.
+// An f16 query is one piece; its weights take 2 too, which cost at most 2% here (48
+// sequences of 1 to 4096 tokens 86.5 us against 85.9, 16 over 4096 15.1 / 14.8, 32 of
+// 500 11.8 / 11.7) and leave the store's rounding as the only one to fp16.
 // Bound by the reads: 3 workgroups of 4 waves a CU (168 registers), each wave's
 // step 16 KB; 64 sequences of 4000 tokens (1.05 GB) 167 us, 6.3 TB/s, 48 of 1 to
 // 4096 (400 MB) 79 us, 5 TB/s. Two or four row tiles a wave, or a workgroup on the
@@ -147,7 +155,7 @@ struct SharedPart {
 template <int HD, int NP, bool ONCE, typename T>
 ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, float *lds) {
     constexpr int K4 = HD / 32, ND = HD / 16;  // k-steps of the scores, dims per lane and output tiles
-    constexpr int LD = HD + 4;
+    constexpr int LD = HD + 4, NQ = sizeof(T) == 2 ? 1 : NP;  // (an f16 query is one piece)
     float *const so = lds, *const sm = lds + W * SA_ROWS * LD, *const sl = sm + W * SA_ROWS;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t li = lane % 16, lg = lane / 16;
@@ -207,7 +215,7 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
         if (wave + W < nstep) nx = step(wave + W);
     }
     // the row's q as operand fragments: dims 32 k4 + 8 lg ..
-    half8 qf[NP][K4];
+    half8 qf[NQ][K4];
     int e = 0;  // q is scaled by 2^-e
     {
         const uint32_t row = w.row0 + min(li, w.nrow - 1), rs = row / a.G, rh = kvh * a.G + row % a.G;
@@ -219,7 +227,7 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k4][e]));
         }
-        if (NP > 1) {
+        if (NQ > 1) {
             mx = xor32_max(xor16_max(mx));
             const uint32_t E = __float_as_uint(mx) >> 23;
             if (E < 255) e = (int)E - 141;  // (E == 0, subnormal or zero rows: a smaller maximum)
@@ -228,9 +236,9 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
         for (int k4 = 0; k4 < K4; k4++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                float y = NP > 1 ? ldexpf(v[k4][i], -e) : v[k4][i];
+                float y = NQ > 1 ? ldexpf(v[k4][i], -e) : v[k4][i];
 #pragma unroll
-                for (int p = 0; p < NP; p++) {
+                for (int p = 0; p < NQ; p++) {
                     qf[p][k4][i] = (_Float16)y;
                     y -= (float)qf[p][k4][i];
                 }
@@ -248,7 +256,7 @@ ZH_DEV void shared_part(const SharedArgs &a, const SharedPart &w, uint32_t kvh, 
         const bool whole = x.tk >= x.lo && x.tk + SA_KB <= x.hi;
         floatx4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int p = NP - 1; p >= 0; p--)
+        for (int p = NQ - 1; p >= 0; p--)
 #pragma unroll
             for (int k4 = 0; k4 < K4; k4++)
 #pragma unroll
@@ -468,6 +476,10 @@ __global__ __launch_bounds__(64 * W, 3) void k_shared_attn(SharedArgs a) {
 // rest is the softmax (4), the copies and the LDS reads (4) where they do not
 // hide. 4 waves of 64 rows, each K and V fragment for two products: 70 us (past
 // 256 registers the accumulators move between the two register files).
+// NP pieces as in k_shared_attn, but f16 weights in 1: their second products would
+// take 106 us for 75 (64 sequences over 32768 tokens) and 100 for 72 (250 over 8192);
+// the rounding adds to the store's, 2.8e-4 of the output's root mean square over 1550
+// tokens for 2.07e-4.
 constexpr uint32_t ST_KB = 64, ST_NS = 4;
 template <int HD>
 constexpr uint32_t st_lds() { return 2 * ST_NS * ST_KB * HD * 2; }
@@ -1002,7 +1014,7 @@ static int shared_launch(zh_ctx *c, const SharedArgs &a, const SharedPlan &p) {
         blocks -= p.pre_blocks;
         b.join = p.n_own == 1;
     }
-    hipLaunchKernelGGL((k_shared_attn<HD, NP, T>), dim3(blocks), dim3(64 * W), 0, c->stream, b);
+    hipLaunchKernelGGL((k_shared_attn<HD, 2, T>), dim3(blocks), dim3(64 * W), 0, c->stream, b);
     ZH_LAUNCH_CHECK(c);
     if (a.n_pre + a.n_own > 1 && !b.join) {
         const uint32_t per = 256 / (HD / 4);  // rows of a workgroup
