@@ -36,11 +36,11 @@ constexpr int W = 4;              // waves of a workgroup
 //    rows over 6144 tokens (294K) 21.0 / 19.9, 8192 (393K) 22.5 / 23.7, 128 over
 //    8192 (524K) 24.5 / 27.3; f32 128 over 8192 30.2 / 27.6, 12288 (786K) 34.6 /
 //    36.2; f16 at 64 128 over 4096 (262K) 13.2 / 12.4, 96 over 8192 14.2 / 15.4;
-//    f32 at 64 128 over 6144 (393K) 16.3 / 15.2, 96 over 12288 (589K) 19.7 / 20.1 no
-//    tiles for 32 rows and fewer, of which a workgroup of four waves uses one: 32
-//    rows, f16 at 128, over 32768 tokens of 8 heads 32.0 / 29.0, 65536 of 8 51.7 /
-//    47.6, 16384 of 32 47.5 / 50.1, 131072 of 4 52.7 / 82.5; f32 65536 of 8 80.9 /
-//    50.4; f16 at 64 over 65536 of 8 34.9 / 30.1;
+//    f32 at 64 128 over 6144 (393K) 16.3 / 15.2, 96 over 12288 (589K) 19.7 / 20.1;
+//    none for 32 rows and fewer, which keep one wave of a workgroup busy: 32 rows,
+//    f16 at 128, over 32768 tokens of 8 heads 32.0 / 29.0, 65536 of 8 51.7 / 47.6,
+//    16384 of 32 47.5 / 50.1, 131072 of 4 52.7 / 82.5; f32 65536 of 8 80.9 / 50.4;
+//    f16 at 64 over 65536 of 8 34.9 / 30.1;
 //  * a prefix's parts: those that fill 1 to 4 rounds of one workgroup per CU best,
 //    a round's start and end counted as SA_TILE_FIX stages, streamed SA_FIX steps
 //    (180 sequences at 8192 in tiles 58.5 us, in the nearest number of parts 73.9;
@@ -59,9 +59,9 @@ constexpr int W = 4;              // waves of a workgroup
 //  * a prefix's parts of at least 128 tokens, a step for each wave; of own tokens at
 //    most one for each 256 begun, all of a length (300 tokens: two of 160; 16
 //    sequences at 4096 of up to 300 own 15.9 us, one for each 128: 17.0), and for
-//    each 512 after a tile launch, where a single own part of a sequence also joins the prefix's
-//    (32 sequences of up to 512: 38 us, in two parts and a launch that joins them
-//    40.7; up to 1000 48.8, 45.9; 64 of up to 4000 139 us, in one part 171).
+//    each 512 after a tile launch, where a single own part of a sequence also joins
+//    the prefix's (32 sequences of up to 512: 38 us, in two parts and a launch that
+//    joins them 40.7; up to 1000 48.8, 45.9; 64 of up to 4000 139 us, in one part 171).
 constexpr uint64_t sa_tile(uint32_t hd, bool f32) {
     return hd == 64 ? (f32 ? 560000 : 290000) : (f32 ? 750000 : 350000);
 }
