@@ -1,6 +1,7 @@
 """Decode attention with a shared prefix (zh_flash_decode_shared): queries and
-scales of any size, against the module's formula in 64 bits (the bounds are
-test_gpu_kv_batch's, the same for both forms of the prefix)."""
+scales of any size, the form that a case is meant for, f16 results rounded once,
+against the formula in 64 bits (the bounds are test_gpu_kv_batch's, the same for
+both forms of the prefix)."""
 import numpy as np
 import pytest
 from test_gpu_kv_batch import NP_TYPE, attend64, close, ctx, make, run_attention, store_error, zh  # noqa: F401
