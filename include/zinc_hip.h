@@ -336,6 +336,98 @@ typedef struct zh_kv_caches {
 int zh_kv_copy_pages(zh_ctx *ctx, const zh_kv_caches *dst, const zh_kv_caches *src, const uint32_t *dst_pages,
                      const uint32_t *src_pages, uint32_t n_pages);
 
+/* ---- the same batches over a cache in 8 bits --------------------------- */
+/* A cache of codes, 8-bit [n_kv_heads][cache_tokens][head_dim], and its scales,
+ * f32 [cache_tokens / 16][n_kv_heads]: one for each block, the 16 tokens of a
+ * page and one head. A code stands for its number times its block's scale:
+ *   ZH_I8    two's complement, written as -127 .. 127
+ *   ZH_E4M3  4 exponent and 3 mantissa bits, up to 448, no infinities; 0x7F and
+ *            0xFF (not a number) are never written
+ * Scales are written as powers of two from 2^-64 on, the least under which no
+ * value of the block passes the format's largest; any scale in [2^-64, 2^64] is
+ * read. A block with another scale reads as NaN: so does one that was given an
+ * infinity, a NaN or a value past 2^64 times the largest (its scale is NaN). */
+enum { ZH_I8 = 24, ZH_E4M3 = 256 };
+/* One layer's caches, the page tables of a batch (as in zh_kv_batch) and the
+ * batch's rows: sequence s has the rows row_start[s] .. row_start[s + 1] - 1 of
+ * the call (u32 [n_seq + 1], ascending; NULL: row s alone, or none where
+ * seq_lens[s] is 0) and, these among them, seq_lens[s] tokens; its rows are its
+ * last ones, in order. A sequence may have no rows; rows outside every sequence
+ * are left as they were. Tables, row_start and seq_lens are read on the device:
+ * where row_start falls or passes the call's rows, a sequence has more rows than
+ * tokens (the first ones are left out) or more tokens than its table holds, or a
+ * page lies outside the cache, the next zh_sync returns ZH_ERR_INVALID_ARGUMENT.
+ * head_dim 64 or 128. */
+typedef struct zh_kv8_batch {
+    zh_buf *k_cache, *v_cache, *k_scale, *v_scale;
+    const zh_buf *tables, *row_start, *seq_lens;
+    uint32_t n_seq, table_stride, cache_tokens, n_kv_heads, head_dim, type;
+} zh_kv8_batch;
+/* zh_qk_norm_rope_kv_write_batched into such a cache: the same q_out (rows->seq
+ * and rows->pos are NULL, the batch says where the rows stand; rows 16-byte
+ * aligned, rope_dim a multiple of 8), k and v quantised as they are written. A
+ * page that the rows reach keeps its earlier tokens: its scale rises, where the
+ * rows need that, and what it holds is rounded again to the new one. A page whose
+ * first token is among the rows begins anew: its other slots become 0. k is
+ * computed in 64 bits, so the codes are those of the exact values. A row without a
+ * place in the cache still has its q_out written. Each page that is written
+ * belongs to one sequence of the batch (zh_kv_pool_unshare). */
+int zh_qk_norm_rope_kv8_write_batched(zh_ctx *ctx, const zh_kv8_batch *kv, const zh_qkv_rows *rows);
+/* A batch's query rows and where their results go (strides in elements, 0: rows
+ * without gaps; offsets in bytes; rows 16-byte aligned; out may be q's own rows). */
+typedef struct zh_attn_rows {
+    const zh_buf *q;
+    zh_buf *out;
+    uint64_t q_off, out_off;
+    uint32_t q_stride, out_stride;
+    uint32_t type;                   /* of q and out: ZH_F32 or ZH_F16 */
+    uint32_t n_heads;                /* a multiple of n_kv_heads */
+    zh_buf *ws;                      /* zh_flash_attn_kv8_ws bytes */
+    uint32_t n_rows;                 /* of q and out */
+    uint32_t max_rows, max_len;      /* the most rows and tokens of a sequence */
+    float attn_scale;                /* 0: 1/sqrt(head_dim) */
+} zh_attn_rows;
+/* Causal paged attention of a batch over such a cache (its rows' K and V are
+ * written): out = softmax(scale q K^T) V over the tokens of the row's sequence up
+ * to its own. One row a sequence is a decode step, a few are drafted tokens, many
+ * a chunk of a prompt; a batch may mix them. Rows past max_rows of a sequence are
+ * left as they were, a length past max_len or the table is cut there, a page
+ * outside the cache reads as page 0, and the next zh_sync then returns
+ * ZH_ERR_INVALID_ARGUMENT. A row of a sequence without tokens is zero. What a row
+ * may not see does not enter its result, whatever the cache holds there (NaN codes
+ * of tokens of the same call excepted). ZH_F32: q and the probabilities in two fp16 pieces each
+ * (22 bits); ZH_F16: the probabilities in two, those of many rows (more than 32
+ * of a sequence and kv head) in one; sums and softmax in 32 bits. Allocates
+ * nothing and adds in a fixed order; calls that may overlap (other contexts,
+ * replayed graphs) need a ws each. attn_scale finite. */
+int zh_flash_attn_kv8(zh_ctx *ctx, const zh_kv8_batch *kv, const zh_attn_rows *rows);
+/* Bytes of ws for a call of these sizes and for every call of fewer sequences or
+ * rows, a smaller max_rows or max_len, of either type (0: refused sizes). A call is
+ * checked for what it needs itself, which may be less. */
+uint64_t zh_flash_attn_kv8_ws(zh_ctx *ctx, const zh_kv8_batch *kv, uint32_t n_heads, uint32_t n_rows,
+                              uint32_t max_rows, uint32_t max_len);
+/* A set of at most 256 such caches of one shape, each with its scales. */
+typedef struct zh_kv8_caches {
+    zh_buf *const *caches, *const *scales;
+    uint32_t n_caches, cache_tokens, n_kv_heads, head_dim, type, reserved;
+} zh_kv8_caches;
+/* Pages between sets of caches with as many caches, heads and dims: page
+ * src_pages[i] of every cache of src to page dst_pages[i] of the same cache of
+ * dst (page numbers are host memory, read before the call returns; the work is
+ * enqueued). Refused with ZH_ERR_INVALID_ARGUMENT and nothing done: a page
+ * outside its caches, two copies to one page, a buffer in two places (but for a
+ * set copied within itself, where no page is both read and written).
+ *  pack:   fp16 quantised; n_tokens of ceil(n_tokens / 16) pages, the slots of
+ *          the last page past them become 0 whatever src holds there
+ *  unpack: codes times scale, rounded to fp16
+ *  copy:   codes and scales as they are, of one type */
+int zh_kv8_pack_pages(zh_ctx *ctx, const zh_kv8_caches *dst, const zh_kv_caches *src, const uint32_t *dst_pages,
+                      const uint32_t *src_pages, uint32_t n_tokens);
+int zh_kv8_unpack_pages(zh_ctx *ctx, const zh_kv_caches *dst, const zh_kv8_caches *src, const uint32_t *dst_pages,
+                        const uint32_t *src_pages, uint32_t n_pages);
+int zh_kv8_copy_pages(zh_ctx *ctx, const zh_kv8_caches *dst, const zh_kv8_caches *src, const uint32_t *dst_pages,
+                      const uint32_t *src_pages, uint32_t n_pages);
+
 /* ---- engine: InferenceEngine surface (forward.zig:1226-10983) ---------- */
 /* Batched prefill projection (dispatchProjectionBatched, forward.zig:8147-8216;
  * recordMulMmQ4K dmmv.zig:1045-1094 / mul_mm_q4k.comp): Y[n][m] (+= when

@@ -9,6 +9,20 @@ static inline bool kv_in_range(const zh_buf *b, uint64_t off, uint64_t n) {
     return b && off <= b->size && n <= b->size - off;
 }
 bool kv_batch_ok(const zh_kv_batch *kv);
+// The rows' strides (0: rows without gaps) filled in.
+zh_qkv_rows kv_with_strides(const zh_qkv_rows *r, uint32_t n_kv_heads, uint32_t head_dim);
+// The checks of q, k and v rows (strides filled in): heads, types, ranges, and
+// that nothing which the call reads (`read`, NULLs left out) is a buffer that it
+// writes (`written`) or lies in q_out, but for q's own rows. `who` names the
+// operator in messages.
+int kv_check_rows(zh_ctx *c, const char *who, const zh_qkv_rows *r, uint32_t n_kv_heads, uint32_t head_dim,
+                  const zh_buf *const *written, uint32_t n_written, const zh_buf *const *read, uint32_t n_read);
+// The checks of a list of page copies; `alias`: source and destination are the
+// same caches.
+int kv_check_pages(zh_ctx *c, const char *who, const uint32_t *dst_pages, const uint32_t *src_pages, uint32_t n_pages,
+                   uint32_t dst_cache_pages, uint32_t src_cache_pages, bool alias);
+bool kv_caches_ok(const zh_kv_caches *s);
+constexpr uint32_t KC_MAX = 256;  // caches of a call that copies pages
 // Byte ranges [a0, a0 + an) of a and [b0, b0 + bn) of b share a byte.
 bool kv_rows_overlap(const zh_buf *a, uint64_t a0, uint64_t an, const zh_buf *b, uint64_t b0, uint64_t bn);
 // Two sets of rows of one stride (elements of `size` bytes) whose byte ranges

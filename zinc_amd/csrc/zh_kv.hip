@@ -107,8 +107,7 @@ int zhk_kv_copy(zh_ctx *c, uint32_t n_caches, void *const *dst, const void *cons
     return f(c, n_caches, dst, src, dst_tokens, src_tokens, n_kv_heads, head_dim, dst_pages, src_pages, n_pages);
 }
 
-constexpr uint32_t KC_MAX = 256;  // caches of a call
-static bool caches_ok(const zh_kv_caches *s) {
+bool kv_caches_ok(const zh_kv_caches *s) {
     if (!s || !s->caches || s->n_caches == 0 || s->n_caches > KC_MAX || s->n_kv_heads == 0 || s->n_kv_heads > 65535 || s->head_dim == 0 ||
         s->head_dim > 1024 || s->cache_tokens == 0 || s->cache_tokens % 16)
         return false;
@@ -117,13 +116,45 @@ static bool caches_ok(const zh_kv_caches *s) {
     return true;
 }
 
+// `mark` and `call`: see zh_ctx::page_mark.
+int kv_check_pages(zh_ctx *c, const char *who, const uint32_t *dst_pages, const uint32_t *src_pages, uint32_t n_pages,
+                   uint32_t dst_cache_pages, uint32_t src_cache_pages, bool alias) {
+    const uint32_t np = dst_cache_pages;
+    for (uint32_t i = 0; i < n_pages; i++)
+        if (dst_pages[i] >= np || src_pages[i] >= src_cache_pages)
+            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: copy %u, page %u to %u, outside the cache", who, i,
+                              src_pages[i], dst_pages[i]);
+    try {
+        std::vector<uint32_t> own;
+        std::vector<uint32_t> &mark = c ? c->page_mark : own;
+        if (mark.size() < np) mark.resize(np, 0);
+        uint32_t one = 0, &call = c ? c->page_call : one;
+        if (++call == 0) {  // (wrapped: the old marks go)
+            std::fill(mark.begin(), mark.end(), 0u);
+            call = 1;
+        }
+        for (uint32_t i = 0; i < n_pages; i++) {
+            if (mark[dst_pages[i]] == call)
+                return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: two copies to page %u", who, dst_pages[i]);
+            mark[dst_pages[i]] = call;
+        }
+        if (alias)
+            for (uint32_t i = 0; i < n_pages; i++)
+                if (mark[src_pages[i]] == call)
+                    return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: page %u is read and written", who, src_pages[i]);
+    } catch (const std::bad_alloc &) {
+        return zh_set_err(c, ZH_ERR_OUT_OF_MEMORY, "%s: host memory", who);
+    }
+    return ZH_OK;
+}
+
 // The checks of zh_kv_copy_pages, of host data only (exported for the tests; c
-// may be null: no message then). `mark` and `call`: see zh_ctx::page_mark.
+// may be null: no message then).
 extern "C" int zh_check_kv_copy_pages(zh_ctx *c, const zh_kv_caches *dst, const zh_kv_caches *src,
                                       const uint32_t *dst_pages, const uint32_t *src_pages, uint32_t n_pages) {
     const bool one = dst && src && dst->caches == src->caches && dst->n_caches == src->n_caches;
-    if (!caches_ok(dst) || !(one && dst->cache_tokens == src->cache_tokens && dst->n_kv_heads == src->n_kv_heads &&
-                             dst->head_dim == src->head_dim ? true : caches_ok(src)) || dst->n_caches != src->n_caches || dst->n_kv_heads != src->n_kv_heads ||
+    if (!kv_caches_ok(dst) || !(one && dst->cache_tokens == src->cache_tokens && dst->n_kv_heads == src->n_kv_heads &&
+                             dst->head_dim == src->head_dim ? true : kv_caches_ok(src)) || dst->n_caches != src->n_caches || dst->n_kv_heads != src->n_kv_heads ||
         dst->head_dim != src->head_dim)
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: cache sets");
     if (n_pages && (!dst_pages || !src_pages))
@@ -149,34 +180,8 @@ extern "C" int zh_check_kv_copy_pages(zh_ctx *c, const zh_kv_caches *dst, const 
     }
     if (alias && dst->cache_tokens != src->cache_tokens)
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: one cache in two sizes");
-    const uint32_t np = dst->cache_tokens / 16;
-    for (uint32_t i = 0; i < n_pages; i++)
-        if (dst_pages[i] >= np || src_pages[i] >= src->cache_tokens / 16)
-            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: copy %u, page %u to %u, outside the cache", i,
-                              src_pages[i], dst_pages[i]);
-    try {
-        std::vector<uint32_t> own;
-        std::vector<uint32_t> &mark = c ? c->page_mark : own;
-        if (mark.size() < np) mark.resize(np, 0);
-        uint32_t one = 0, &call = c ? c->page_call : one;
-        if (++call == 0) {  // (wrapped: the old marks go)
-            std::fill(mark.begin(), mark.end(), 0u);
-            call = 1;
-        }
-        for (uint32_t i = 0; i < n_pages; i++) {
-            if (mark[dst_pages[i]] == call)
-                return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: two copies to page %u", dst_pages[i]);
-            mark[dst_pages[i]] = call;
-        }
-        if (alias)
-            for (uint32_t i = 0; i < n_pages; i++)
-                if (mark[src_pages[i]] == call)
-                    return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "kv_copy_pages: page %u is read and written",
-                                      src_pages[i]);
-    } catch (const std::bad_alloc &) {
-        return zh_set_err(c, ZH_ERR_OUT_OF_MEMORY, "kv_copy_pages: host memory");
-    }
-    return ZH_OK;
+    return kv_check_pages(c, "kv_copy_pages", dst_pages, src_pages, n_pages, dst->cache_tokens / 16,
+                          src->cache_tokens / 16, alias);
 }
 
 extern "C" int zh_kv_copy_pages(zh_ctx *c, const zh_kv_caches *dst, const zh_kv_caches *src, const uint32_t *dst_pages,
@@ -414,53 +419,54 @@ bool kv_rows_overlap(const zh_buf *a, uint64_t a0, uint64_t an, const zh_buf *b,
     return pa < pb + bn && pb < pa + an;
 }
 
-// The rows with their strides (0: rows without gaps).
-static zh_qkv_rows with_strides(const zh_kv_batch *kv, const zh_qkv_rows *r) {
+zh_qkv_rows kv_with_strides(const zh_qkv_rows *r, uint32_t n_kv_heads, uint32_t head_dim) {
     zh_qkv_rows x = *r;
-    if (!x.q_stride) x.q_stride = x.n_q_heads * kv->head_dim;
-    if (!x.q_out_stride) x.q_out_stride = x.n_q_heads * kv->head_dim;
-    if (!x.k_stride) x.k_stride = kv->n_kv_heads * kv->head_dim;
-    if (!x.v_stride) x.v_stride = kv->n_kv_heads * kv->head_dim;
+    if (!x.q_stride) x.q_stride = x.n_q_heads * head_dim;
+    if (!x.q_out_stride) x.q_out_stride = x.n_q_heads * head_dim;
+    if (!x.k_stride) x.k_stride = n_kv_heads * head_dim;
+    if (!x.v_stride) x.v_stride = n_kv_heads * head_dim;
     return x;
 }
 
-// The checks of zh_qk_norm_rope_kv_write_batched, of host data only (exported
-// for the tests; c may be null: no message then).
-extern "C" int zh_check_qkv_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_qkv_rows *rows) {
-    if (!kv_batch_ok(kv) || !rows) return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: cache or tables");
-    const zh_qkv_rows x = with_strides(kv, rows), *r = &x;
-    const uint32_t nkv = kv->n_kv_heads, hd = kv->head_dim, nq = r->n_q_heads, n = r->n_rows;
+int kv_check_rows(zh_ctx *c, const char *who, const zh_qkv_rows *r, uint32_t nkv, uint32_t hd,
+                  const zh_buf *const *written, uint32_t n_written, const zh_buf *const *read, uint32_t n_read) {
+    const uint32_t nq = r->n_q_heads, n = r->n_rows;
     if (hd % 2 || nq == 0 || nq > 65535 || nq % nkv || (uint64_t)nq + 2ull * nkv > 65535)
-        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: heads %u / %u of %u", nq, nkv, hd);
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: heads %u / %u of %u", who, nq, nkv, hd);
     if (r->rope_dim % 2 || r->rope_dim > hd)
-        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: rope_dim %u of %u", r->rope_dim, hd);
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: rope_dim %u of %u", who, r->rope_dim, hd);
     if ((r->type != ZH_F32 && r->type != ZH_F16) || (r->q_out_type != ZH_F32 && r->q_out_type != ZH_F16))
-        return zh_set_err(c, ZH_ERR_UNSUPPORTED_QUANT_TYPE, "qk_norm_rope_kv batch: types %u, %u", r->type, r->q_out_type);
+        return zh_set_err(c, ZH_ERR_UNSUPPORTED_QUANT_TYPE, "%s: types %u, %u", who, r->type, r->q_out_type);
     if (n == 0) return ZH_OK;
     const uint32_t si = r->type == ZH_F32 ? 4 : 2, so = r->q_out_type == ZH_F32 ? 4 : 2;
     const uint64_t qw = (uint64_t)nq * hd, kw = (uint64_t)nkv * hd;
     if (n > 1 && (r->q_stride < qw || r->k_stride < kw || r->v_stride < kw || r->q_out_stride < qw))
-        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: rows overlap");
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: rows overlap", who);
     const uint64_t qb = rows_bytes(n, r->q_stride, qw, si), ob = rows_bytes(n, r->q_out_stride, qw, so);
     if (!kv_in_range(r->q, r->q_off, qb) || !kv_in_range(r->k, r->k_off, rows_bytes(n, r->k_stride, kw, si)) ||
         !kv_in_range(r->v, r->v_off, rows_bytes(n, r->v_stride, kw, si)) || !kv_in_range(r->q_out, r->q_out_off, ob) ||
-        !kv_in_range(r->pos, 0, 4ull * n) || (r->seq && !kv_in_range(r->seq, 0, 4ull * n)) ||
-        (!r->seq && n > kv->n_seq) || (r->q_norm_w && !kv_in_range(r->q_norm_w, 0, 4ull * hd)) ||
+        (r->q_norm_w && !kv_in_range(r->q_norm_w, 0, 4ull * hd)) ||
         (r->k_norm_w && !kv_in_range(r->k_norm_w, 0, 4ull * hd)) ||
         (r->rope_dim && !kv_in_range(r->inv_freq, 0, 2ull * r->rope_dim)))
-        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: range");
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: range", who);
     if (r->q_off % si || r->k_off % si || r->v_off % si || r->q_out_off % so)
-        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: offset alignment");
-    // q_out and the caches: written; q_out q's own rows, or apart from everything
-    // that is read
-    const zh_buf *const read[] = {kv->tables, r->pos, r->seq, r->q_norm_w, r->k_norm_w, r->rope_dim ? r->inv_freq : nullptr};
-    for (const zh_buf *b : read)
-        if (b && (b->ptr == r->q_out->ptr || b->ptr == kv->k_cache->ptr || b->ptr == kv->v_cache->ptr))
-            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: an input is written");
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: offset alignment", who);
+    // what is written: not what is read; q_out q's own rows, or apart from them too
+    const zh_buf *const mine[] = {r->q_norm_w, r->k_norm_w, r->rope_dim ? r->inv_freq : nullptr};
     const zh_buf *const rows4[] = {r->q, r->k, r->v, r->q_out};
+    auto is_written = [&](const zh_buf *b) {
+        if (!b) return false;
+        if (b->ptr == r->q_out->ptr) return true;
+        for (uint32_t i = 0; i < n_written; i++)
+            if (b->ptr == written[i]->ptr) return true;
+        return false;
+    };
+    for (uint32_t i = 0; i < n_read + 3; i++)
+        if (is_written(i < n_read ? read[i] : mine[i - n_read]))
+            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: an input is written", who);
     for (const zh_buf *b : rows4)
-        if (b->ptr == kv->k_cache->ptr || b->ptr == kv->v_cache->ptr)
-            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: rows in a cache");
+        for (uint32_t i = 0; i < n_written; i++)
+            if (b->ptr == written[i]->ptr) return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: rows in a cache", who);
     const bool same = r->q_out->ptr == r->q->ptr && r->q_out_off == r->q_off && r->q_out_type == r->type &&
                       (r->q_out_stride == r->q_stride || n == 1);
     if ((!same && kv_rows_overlap(r->q_out, r->q_out_off, ob, r->q, r->q_off, qb) &&
@@ -472,8 +478,22 @@ extern "C" int zh_check_qkv_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_qkv_
         (kv_rows_overlap(r->q_out, r->q_out_off, ob, r->v, r->v_off, rows_bytes(n, r->v_stride, kw, si)) &&
          !(r->q_out_type == r->type && r->q_out_stride == r->v_stride &&
            kv_columns_apart(r->q_out, r->q_out_off, r->v, r->v_off, r->v_stride, qw, kw, si))))
-        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "qk_norm_rope_kv batch: q_out overlaps rows that are read");
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: q_out overlaps rows that are read", who);
     return ZH_OK;
+}
+
+// The checks of zh_qk_norm_rope_kv_write_batched, of host data only (exported
+// for the tests; c may be null: no message then).
+extern "C" int zh_check_qkv_rows(zh_ctx *c, const zh_kv_batch *kv, const zh_qkv_rows *rows) {
+    const char *who = "qk_norm_rope_kv batch";
+    if (!kv_batch_ok(kv) || !rows) return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: cache or tables", who);
+    const zh_qkv_rows x = kv_with_strides(rows, kv->n_kv_heads, kv->head_dim), *r = &x;
+    const uint64_t n = r->n_rows;
+    const zh_buf *const written[] = {kv->k_cache, kv->v_cache}, *const read[] = {kv->tables, r->pos, r->seq};
+    const int rc = kv_check_rows(c, who, r, kv->n_kv_heads, kv->head_dim, written, 2, read, 3);
+    if (rc == ZH_OK && n && (!kv_in_range(r->pos, 0, 4 * n) || (r->seq ? !kv_in_range(r->seq, 0, 4 * n) : n > kv->n_seq)))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: range of pos or seq", who);
+    return rc;
 }
 
 template <typename TI, typename TQ, int L>
@@ -521,7 +541,7 @@ extern "C" int zh_qk_norm_rope_kv_write_batched(zh_ctx *c, const zh_kv_batch *kv
     if (!c) return ZH_ERR_INVALID_ARGUMENT;
     const int rc = zh_check_qkv_rows(c, kv, rows);
     if (rc || rows->n_rows == 0) return rc;
-    const zh_qkv_rows x = with_strides(kv, rows), *r = &x;
+    const zh_qkv_rows x = kv_with_strides(rows, kv->n_kv_heads, kv->head_dim), *r = &x;
     zh_device_scope dev(c);
     const uint32_t si = r->type == ZH_F32 ? 4 : 2, so = r->q_out_type == ZH_F32 ? 4 : 2;
     QkvArgs a = {};

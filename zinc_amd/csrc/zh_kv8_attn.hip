@@ -1,0 +1,703 @@
+// zh_kv8_attn.hip — causal paged attention of a batch over a cache held in 8 bits
+// (zh_flash_attn_kv8).
+//
+// For row i of sequence s and query head h of kv head k, over the tokens t that it
+// may see, with codes Kc, Vc and block scales a_t, b_t:
+//   out = sum_t w_t Vc[t] / sum_t w_t / b_t,  w_t = 2^(x_t + log2 b_t - m),
+//   x_t = log2 e scale a_t q . Kc[t]
+// The scales never meet the codes: a_t multiplies a score, b_t goes into the weight,
+// whose reference m is the largest x_t + log2 b_t. Weights of products with V are
+// then relative to the largest contribution whatever the blocks' scales are, and fit
+// fp16. Codes become fp16 exactly (i8 as its value times 2^-10).
+#include <math.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "zh_kv8.h"
+
+namespace {
+
+constexpr int W = 4;         // waves of a streaming workgroup
+constexpr uint32_t CUT = 64;  // parts are whole numbers of so many tokens
+
+struct Kv8Attn {
+    const uint8_t *q;
+    uint8_t *out;
+    uint64_t q_row, out_row;  // bytes between rows
+    const uint8_t *kc, *vc;
+    const float *ks, *vs;
+    const uint32_t *tables, *row_start, *seq_lens;
+    float *part, *stat;  // a part's unnormalised sums; maximum (base 2) and sum of weights
+    uint32_t *err;
+    uint32_t n_seq, stride, cache_tokens, nh, nkv, G, n_rows, max_rows, max_len;
+    uint32_t tiles;           // row tiles of a sequence and kv head
+    uint32_t n_own, own_len;  // parts of a sequence's tokens, their length at least
+    float scale;              // |attn_scale| log2 e = scale * 2^scale_exp, with attn_scale's sign
+    int32_t scale_exp;
+};
+
+// A sequence's rows: [row, row + n), row i over the tokens below lim(i).
+struct AttnSeq {
+    uint32_t row, n, all, len, cut;  // all: rows before the cut at max_rows; len, cut at `cut`
+    ZH_DEVM uint32_t lim(uint32_t i) const {
+        const uint64_t e = (uint64_t)len + i + 1;
+        return e > all ? (uint32_t)min(e - all, (uint64_t)cut) : 0u;
+    }
+};
+ZH_DEV AttnSeq attn_seq(const Kv8Attn &a, uint32_t s, bool &bad) {
+    AttnSeq x;
+    uint32_t first = s, end = min(s + 1, a.n_rows);
+    if (a.row_start) {
+        first = a.row_start[s];
+        end = a.row_start[s + 1];
+        if (first > end || end > a.n_rows) bad = true;
+        end = min(end, a.n_rows);
+    }
+    x.len = a.seq_lens[s];
+    x.row = first;
+    x.all = end > first ? end - first : 0u;
+    x.n = min(x.all, a.max_rows);
+    x.cut = min(x.len, a.max_len);
+    if (x.all > a.max_rows || x.len > a.max_len || (a.row_start && x.all > x.len)) bad = true;
+    return x;
+}
+
+// What takes the products of a row's q, scaled by 2^-e, times a block's scale to
+// base-2 scores. Kept in [2^-120, 2^80]: products lie below 2^32 in steps of 2^-48 at
+// least, so below that range every weight is 1 and above it all but a row's largest
+// are 0, as without the bounds; within it no score is infinite, and none that is
+// masked (-inf) meets a factor of 0.
+ZH_DEV float score_factor(float c, float scale) { return fminf(fmaxf(c * scale, 0x1p-120f), 0x1p80f); }
+
+// A block's scales as the kernels take them: the scores' factor, the weights'
+// exponent and what takes a weight to its share of the sum; `ok` false: it reads as NaN
+// (and the others are harmless).
+template <uint32_t F>
+struct Block {
+    float ks, lv, iv;
+    bool ok;
+    ZH_DEVM void set(uint32_t k, uint32_t v) {
+        constexpr float unit = F == ZH_I8 ? 1024.f : 1.f;
+        ok = kv8_scale_ok(k) && kv8_scale_ok(v);
+        const uint32_t kb = ok ? k : 0x3F800000u, vb = ok ? v : 0x3F800000u;
+        // (exact for powers of two; for others the exponent's fraction is within 2^-21)
+        const float mant = __uint_as_float((vb & 0x7FFFFFu) | 0x3F800000u);
+        ks = __uint_as_float(kb) * unit;
+        lv = (float)((int)(vb >> 23) - 127) + __builtin_amdgcn_logf(mant);
+        iv = __builtin_amdgcn_rcpf(mant) * __uint_as_float((254u - (vb >> 23)) << 23) * (1.f / unit);
+    }
+};
+
+// ---- codes to fp16 (i8: the code plus 128 is an fp16 subnormal's bits, 2^-24 each)
+ZH_DEV half2v i8_pair(uint32_t biased, uint32_t sel) {
+    return __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0u, biased, sel)) * (_Float16)16384.f - (_Float16)0.125f;
+}
+// eight codes of a row
+template <uint32_t F>
+ZH_DEV half8 row8(uint32_t lo, uint32_t hi) {
+    half2v h[4];
+    if (F == ZH_I8) {
+        lo ^= 0x80808080u;
+        hi ^= 0x80808080u;
+        h[0] = i8_pair(lo, 0x0C010C00u);
+        h[1] = i8_pair(lo, 0x0C030C02u);
+        h[2] = i8_pair(hi, 0x0C010C00u);
+        h[3] = i8_pair(hi, 0x0C030C02u);
+    } else {
+        h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+        h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+        h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+        h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+    }
+    return half8{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
+}
+// the codes of dims n and n + 1 (n even, of a dword) of tokens a and b: (a, b) of n, (a, b) of n + 1
+template <uint32_t F>
+ZH_DEV void pair2(uint32_t a, uint32_t b, int n, half2v &x, half2v &y) {
+    if (F == ZH_I8) {  // (a and b biased)
+        const uint32_t sel = n % 4 == 0 ? 0x0C040C00u : 0x0C060C02u;
+        x = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(b, a, sel)) * (_Float16)16384.f - (_Float16)0.125f;
+        y = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(b, a, sel + 0x00010001u)) * (_Float16)16384.f - (_Float16)0.125f;
+    } else {
+        const uint32_t p = __builtin_amdgcn_perm(b, a, n % 4 == 0 ? 0x05010400u : 0x07030602u);
+        x = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(p, 1.0f, false);
+        y = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(p, 1.0f, true);
+    }
+}
+
+ZH_DEV void ld8(const float *p, float (&v)[8]) {
+    const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+ZH_DEV void ld8(const _Float16 *p, float (&v)[8]) {
+    const half8 a = *(const half8 *)p;
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (float)a[e];
+}
+template <typename T>
+ZH_DEV void st_out(const Kv8Attn &a, uint32_t row, uint32_t h, uint32_t d, uint32_t hd, const f32x4 &v) {
+    T *op = (T *)(a.out + row * a.out_row) + (size_t)h * hd + d;
+    if constexpr (sizeof(T) == 4) *(f32x4 *)op = v;
+    else *(half4 *)op = half4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+}
+
+// The parts of `len` tokens, of `c` each.
+ZH_DEV uint32_t own_parts(const Kv8Attn &a, uint32_t len, uint32_t &c) {
+    const uint32_t least = (len + a.n_own - 1) / a.n_own;
+    c = max(a.own_len, (least + CUT - 1) / CUT * CUT);
+    return (len + c - 1) / c;
+}
+
+// 16 RT rows of one sequence and kv head over a part of its tokens. Each wave takes
+// steps of NJ pages by itself, K and V straight from the cache into registers (no
+// LDS, no barrier before the end), the next step's K requested when the scores are
+// done and its V after the products with this one's:
+//   S^T = K q^T (tokens x rows): lane (li = lane % 16, lg = lane / 16) reads 16
+//   codes of token li, dims 64 u + 16 lg .., which are two fragments (the dims'
+//   order within a product is free, q's fragments follow it), and holds the scores
+//   of tokens 4 lg + r of row li;
+//   O^T += V^T P^T, k = (token 4 lg + r of a page, then of the next): lane li reads
+//   dims HD/16 li .. of its 4 tokens, and pairs of tokens are put side by side by byte
+//   permutes before they become fp16; column li of output tile n is dim HD/16 li + n.
+// NP pieces of q (scaled by a power of two to a maximum in [2^14, 2^15)) as sums of
+// fp16 values, 2 of the weights: 22 bits of each.
+template <int HD, int NP, int RT, uint32_t NJ, uint32_t F, typename T>
+__global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a) {
+    constexpr uint32_t KB = 16 * NJ;
+    constexpr int U = HD / 64, ND = HD / 16, VD = ND / 4;  // 16-code pieces of a K row, dims and dwords of V per lane
+    constexpr int LD = HD + 4, NQ = sizeof(T) == 2 ? 1 : NP, PV = 2;
+    constexpr uint32_t ROWS = 16 * RT;
+    __shared__ __align__(16) float so[W * 16 * LD];
+    __shared__ float sm[W * 16], sl[W * 16];
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const uint32_t li = lane % 16, lg = lane / 16;
+    // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
+    const uint32_t kvh = blockIdx.x % a.nkv, job = blockIdx.x / a.nkv, tile = job % a.tiles;
+    const uint32_t s = job / a.tiles % a.n_seq, part = job / a.tiles / a.n_seq;
+    bool bad = false;
+    const AttnSeq seq = attn_seq(a, s, bad);
+    if (tid == 0 && part == 0 && kvh == 0 && tile == 0 && bad) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+    bad = false;
+    const uint32_t all_rows = seq.n * a.G, row0 = tile * ROWS;
+    if (row0 >= all_rows) return;
+    const uint32_t nrow = min(ROWS, all_rows - row0);
+    // the tokens that some row sees, and those that every row sees
+    const uint32_t end = seq.lim((row0 + nrow - 1) / a.G), every = seq.lim(row0 / a.G);
+    uint32_t c;
+    const uint32_t parts = own_parts(a, end, c);
+    if (part && part >= parts) return;  // (a row without tokens: part 0 writes its zeros)
+    const uint32_t t0 = part * c, t1 = min(t0 + c, end);
+    const uint32_t nstep = t1 > t0 ? (t1 - t0 + KB - 1) / KB : 0u;
+    const uint8_t *kh = a.kc + (size_t)kvh * a.cache_tokens * HD, *vh = a.vc + (size_t)kvh * a.cache_tokens * HD;
+    const const_u32 *tab = (const const_u32 *)(a.tables + (size_t)s * a.stride);
+    const const_u32 *ksc = (const const_u32 *)(a.ks + kvh), *vsc = (const const_u32 *)(a.vs + kvh);
+    // a step's pages (clamped to the last of the part), looked up a step ahead by
+    // scalar loads, whose wait does not wait for K and V
+    struct Step {
+        uint32_t tk, pg[NJ];
+    };
+    auto step = [&](uint32_t st) __attribute__((always_inline)) {
+        Step x;
+        x.tk = t0 + st * KB;
+#pragma unroll
+        for (uint32_t j = 0; j < NJ; j++) {
+            x.pg[j] = tab[min(x.tk / 16 + j, (t1 - 1) / 16)];
+            if (x.pg[j] >= a.cache_tokens / 16) {
+                bad = true;
+                x.pg[j] = 0;
+            }
+        }
+        return x;
+    };
+    u32x4 kr[NJ][U];
+    uint32_t vr[NJ][4][VD];
+    auto load_k = [&](const Step &x) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t j = 0; j < NJ; j++) {
+            const uint8_t *p = kh + ((size_t)x.pg[j] * 16 + li) * HD + 16 * lg;
+#pragma unroll
+            for (int u = 0; u < U; u++) kr[j][u] = __builtin_nontemporal_load((const u32x4 *)(p + 64 * u));
+        }
+    };
+    auto load_v = [&](const Step &x) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t j = 0; j < NJ; j++) {
+            const uint8_t *p = vh + ((size_t)x.pg[j] * 16 + 4 * lg) * HD + ND * li;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                if (VD == 2) *(u32x2 *)vr[j][r] = __builtin_nontemporal_load((const u32x2 *)(p + r * HD));
+                else vr[j][r][0] = __builtin_nontemporal_load((const uint32_t *)(p + r * HD));
+            }
+        }
+    };
+    uint32_t ksb[NJ], vsb[NJ];  // this step's scales
+    auto load_s = [&](const Step &x) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t j = 0; j < NJ; j++) {
+            ksb[j] = ksc[(size_t)x.pg[j] * a.nkv];
+            vsb[j] = vsc[(size_t)x.pg[j] * a.nkv];
+        }
+    };
+    Step x = {}, nx = {};
+    if (wave < nstep) {
+        x = step(wave);
+        load_k(x);
+        load_v(x);
+        load_s(x);
+        if (wave + W < nstep) nx = step(wave + W);
+    }
+    // the rows' q as operand fragments: dims 64 u + 16 lg + 8 h .. (the scale's sign in them)
+    half8 qf[RT][NQ][2 * U];
+    float cf[RT];  // products to base-2 scores, but for the block's scale
+    uint32_t lim[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const uint32_t r = row0 + min(16 * rt + li, nrow - 1), i = r / a.G;
+        lim[rt] = min(seq.lim(i), t1);
+        const T *qp = (const T *)(a.q + (uint64_t)(seq.row + i) * a.q_row) + (size_t)(kvh * a.G + r % a.G) * HD + 16 * lg;
+        float v[2 * U][8], mx = 0.f;
+#pragma unroll
+        for (int k = 0; k < 2 * U; k++) {
+            ld8(qp + 64 * (k / 2) + 8 * (k % 2), v[k]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k][e]));
+        }
+        int e = 0;  // q is scaled by 2^-e
+        if (NQ > 1) {
+            mx = xor32_max(xor16_max(mx));
+            const uint32_t E = __float_as_uint(mx) >> 23;
+            if (E < 255) e = (int)E - 141;  // (E == 0, subnormal or zero rows: a smaller maximum)
+        }
+        const float sign = copysignf(1.f, a.scale);
+#pragma unroll
+        for (int k = 0; k < 2 * U; k++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                float y = (NQ > 1 ? ldexpf(v[k][i], -e) : v[k][i]) * sign;
+#pragma unroll
+                for (int p = 0; p < NQ; p++) {
+                    qf[rt][p][k][i] = (_Float16)y;
+                    y -= (float)qf[rt][p][k][i];
+                }
+            }
+        cf[rt] = fabsf(ldexpf(a.scale, a.scale_exp + e));
+    }
+    floatx4 o[RT][ND];
+    float m[RT], l[RT];  // the row's reference (every lg alike), this lane's share of its sum
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.f;
+#pragma unroll
+        for (int n = 0; n < ND; n++) o[rt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    // the weights and products of step x; `more`: the next step's loads on the way.
+    // (The last step is code of its own: a load that may not be there would make
+    // the compiler wait for V before the scores.)
+    auto work = [&](auto more) __attribute__((always_inline)) {
+        Block<F> b[NJ];
+        bool ok = true;
+#pragma unroll
+        for (uint32_t j = 0; j < NJ; j++) {
+            b[j].set(ksb[j], vsb[j]);
+            ok = ok && b[j].ok;
+        }
+        floatx4 d[RT][NJ];
+#pragma unroll
+        for (uint32_t j = 0; j < NJ; j++) {
+            half8 kf[2 * U];
+#pragma unroll
+            for (int k = 0; k < 2 * U; k++)
+                kf[k] = row8<F>(kr[j][k / 2][2 * (k % 2)], kr[j][k / 2][2 * (k % 2) + 1]);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                d[rt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int p = NQ - 1; p >= 0; p--)
+#pragma unroll
+                    for (int k = 0; k < 2 * U; k++)
+                        d[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], qf[rt][p][k], d[rt][j], 0, 0, 0);
+            }
+        }
+        if constexpr (more) {
+            load_k(nx);
+            load_s(nx);
+        }
+        const bool whole = ok && x.tk + KB <= min(every, t1);
+        half8 pf[RT][PV][NJ / 2];
+        float f[RT];
+        if (!whole) {
+            // V of tokens past the part: zero (0 times what the cache holds there may be NaN)
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int y = 0; y < VD; y++) vr[j][r][y] = x.tk + 16 * j + 4 * lg + r >= t1 ? 0u : vr[j][r][y];
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            float sc[NJ][4], mb = -INFINITY;
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; j++) {
+                const float ck = score_factor(cf[rt], b[j].ks);
+#pragma unroll
+                for (int r = 0; r < 4; r++) sc[j][r] = fmaf(d[rt][j][r], ck, b[j].lv);
+            }
+            if (!whole) {
+#pragma unroll
+                for (uint32_t j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const bool out = x.tk + 16 * j + 4 * lg + r >= lim[rt];
+                        sc[j][r] = out ? -INFINITY : b[j].ok ? sc[j][r] : NAN;
+                    }
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) mb = fmaxf(mb, sc[j][r]);
+            mb = xor32_max(xor16_max(mb));
+            // (the largest weight is 2^14: what fp16's subnormals lose of the others is 2^-39 of it)
+            const float mn = fmaxf(m[rt], mb - 14.f), ms = mn == -INFINITY ? 0.f : mn;
+            f[rt] = __builtin_amdgcn_exp2f(m[rt] - ms);  // (m = -inf: 0)
+            m[rt] = mn;
+            float ls = 0.f;
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float p = __builtin_amdgcn_exp2f(sc[j][r] - ms);
+                    ls = fmaf(p, b[j].iv, ls);
+#pragma unroll
+                    for (int k = 0; k < PV; k++) {
+                        pf[rt][k][j / 2][4 * (j % 2) + r] = (_Float16)p;
+                        p -= (float)pf[rt][k][j / 2][4 * (j % 2) + r];
+                    }
+                }
+            l[rt] = fmaf(l[rt], f[rt], ls);
+        }
+        if (F == ZH_I8) {
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int y = 0; y < VD; y++) vr[j][r][y] ^= 0x80808080u;
+        }
+#pragma unroll
+        for (int n = 0; n < ND; n += 2) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    o[rt][n][r] *= f[rt];
+                    o[rt][n + 1][r] *= f[rt];
+                }
+#pragma unroll
+            for (uint32_t jj = 0; jj < NJ / 2; jj++) {
+                half2v e[2][4];  // dims n and n + 1: token pairs of the two pages
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    pair2<F>(vr[2 * jj + i / 2][2 * (i % 2)][n / 4], vr[2 * jj + i / 2][2 * (i % 2) + 1][n / 4], n, e[0][i],
+                             e[1][i]);
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    const half8 vf = {e[y][0].x, e[y][0].y, e[y][1].x, e[y][1].y, e[y][2].x, e[y][2].y, e[y][3].x, e[y][3].y};
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                        for (int p = PV - 1; p >= 0; p--)
+                            o[rt][n + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][p][jj], o[rt][n + y], 0, 0, 0);
+                }
+            }
+        }
+        if constexpr (more) load_v(nx);
+    };
+    if (wave < nstep) {
+        for (uint32_t st = wave + W; st < nstep; st += W) {
+            const Step nn = st + W < nstep ? step(st + W) : nx;
+            work(std::true_type{});
+            x = nx;
+            nx = nn;
+        }
+        work(std::false_type{});
+    }
+    if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+    // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
+    const size_t p0 = ((((size_t)s * a.nkv + kvh) * a.tiles + tile) * a.n_own + part) * ROWS;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        if (rt) __syncthreads();
+        const float ls = xor32_sum(xor16_sum(l[rt]));
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int n = 0; n < ND; n += 4)
+                *(f32x4 *)(so + (wave * 16 + li) * LD + ND * (4 * lg + r) + n) =
+                    f32x4{o[rt][n][r], o[rt][n + 1][r], o[rt][n + 2][r], o[rt][n + 3][r]};
+        if (lg == 0) {
+            sm[wave * 16 + li] = m[rt];
+            sl[wave * 16 + li] = ls;
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < 16 * (HD / 4); i += 64 * W) {
+            const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
+            if (16 * rt + r >= nrow) break;
+            const uint32_t R = row0 + 16 * rt + r, qi = R / a.G, h = kvh * a.G + R % a.G;
+            float M = sm[r], L = 0.f;
+            f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 1; k < W; k++) M = fmaxf(M, sm[k * 16 + r]);
+            const float Ms = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int k = 0; k < W; k++) {
+                const float fk = __builtin_amdgcn_exp2f(sm[k * 16 + r] - Ms);
+                const f32x4 v = *(const f32x4 *)(so + (k * 16 + r) * LD + d);
+                O.x = fmaf(v.x, fk, O.x);
+                O.y = fmaf(v.y, fk, O.y);
+                O.z = fmaf(v.z, fk, O.z);
+                O.w = fmaf(v.w, fk, O.w);
+                L = fmaf(sl[k * 16 + r], fk, L);
+            }
+            if (parts <= 1) {
+                const f32x4 v = seq.lim(qi) ? f32x4{O.x / L, O.y / L, O.z / L, O.w / L} : f32x4{0.f, 0.f, 0.f, 0.f};
+                st_out<T>(a, seq.row + qi, h, d, HD, v);
+            } else {
+                const size_t pr = p0 + 16 * rt + r;
+                *(f32x4 *)(a.part + pr * HD + d) = O;
+                if (d == 0) {
+                    a.stat[2 * pr] = M;
+                    a.stat[2 * pr + 1] = L;
+                }
+            }
+        }
+    }
+}
+
+// Joins the parts of a row: HD / 4 lanes, of 4 dims each, take the parts'
+// statistics, as many at a time, then all of them the parts' sums, 8 loads of 16
+// bytes in flight. Parts stand `apart` rows from each other.
+template <int HD>
+ZH_DEV f32x4 join_row(const Kv8Attn &a, size_t first, uint32_t parts, uint32_t apart) {
+    constexpr uint32_t N = HD / 4, U = 8;
+    const uint32_t lane = threadIdx.x & 63, l = lane % N;
+    float M = -INFINITY, L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t b = 0; b < parts; b += N) {
+        const uint32_t n = min(N, parts - b);
+        const float2 st = *(const float2 *)(a.stat + 2 * (first + (size_t)(b + min(l, n - 1)) * apart));
+        float mx = st.x;
+#pragma unroll
+        for (uint32_t x = 1; x < N; x *= 2) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
+        const float mn = fmaxf(M, mx), ms = mn == -INFINITY ? 0.f : mn;
+        const float old = __builtin_amdgcn_exp2f(M - ms), w = l < n ? __builtin_amdgcn_exp2f(st.x - ms) : 0.f;
+        float ls = l < n ? st.y * w : 0.f;
+#pragma unroll
+        for (uint32_t x = 1; x < N; x *= 2) ls += __shfl_xor(ls, x, 64);
+        M = mn;
+        L = fmaf(L, old, ls);
+        O *= old;
+        for (uint32_t p = 0; p < n; p += U) {
+            f32x4 v[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++)
+                v[u] = *(const f32x4 *)(a.part + (first + (size_t)(b + min(p + u, n - 1)) * apart) * HD + 4 * l);
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++) {  // (past the last part: its values again, weight 0)
+                const float f = __shfl(w, lane - l + min(p + u, N - 1), 64);
+                O.x = fmaf(v[u].x, p + u < n ? f : 0.f, O.x);
+                O.y = fmaf(v[u].y, p + u < n ? f : 0.f, O.y);
+                O.z = fmaf(v[u].z, p + u < n ? f : 0.f, O.z);
+                O.w = fmaf(v[u].w, p + u < n ? f : 0.f, O.w);
+            }
+        }
+    }
+    return f32x4{O.x / L, O.y / L, O.z / L, O.w / L};
+}
+
+template <int HD, int RT, typename T>
+__global__ __launch_bounds__(256) void k_kv8_join(Kv8Attn a) {
+    constexpr uint32_t N = HD / 4, PER = 256 / N, ROWS = 16 * RT;  // rows of a workgroup, of a tile
+    const uint32_t item = blockIdx.x / (ROWS / PER), r = blockIdx.x % (ROWS / PER) * PER + threadIdx.x / N;
+    const uint32_t tile = item % a.tiles, kvh = item / a.tiles % a.nkv, s = item / a.tiles / a.nkv;
+    bool bad = false;
+    const AttnSeq seq = attn_seq(a, s, bad);
+    const uint32_t all_rows = seq.n * a.G, row0 = tile * ROWS;
+    if (row0 >= all_rows) return;
+    const uint32_t nrow = min(ROWS, all_rows - row0);
+    uint32_t c;
+    const uint32_t parts = own_parts(a, seq.lim((row0 + nrow - 1) / a.G), c);
+    if (parts <= 1 || r / (64 / N) * (64 / N) >= nrow) return;  // (uniform per wave)
+    const uint32_t R = row0 + min(r, nrow - 1), qi = R / a.G, h = kvh * a.G + R % a.G;
+    const f32x4 v = join_row<HD>(a, (size_t)item * a.n_own * ROWS + (R - row0), parts, ROWS);
+    if (r < nrow) st_out<T>(a, seq.row + qi, h, threadIdx.x % N * 4, HD, seq.lim(qi) ? v : f32x4{0.f, 0.f, 0.f, 0.f});
+}
+
+// How a call is cut (the same for every call of these sizes).
+struct Kv8Plan {
+    uint32_t rt, tiles, n_own, own_len, blocks;
+    uint64_t stat_off, bytes;  // of ws
+};
+constexpr uint32_t PER_CU = 8;  // workgroups per CU that the parts are cut for
+
+uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t max_rows, uint32_t max_len, Kv8Plan &p) {
+    const uint32_t G = nh / kv->n_kv_heads;
+    const uint64_t rows = (uint64_t)max_rows * G;
+    p = {};
+    p.rt = rows <= 16 ? 1 : 2;
+    if (rows > 1ull << 31) return false;
+    p.tiles = ceil_div(rows, 16 * p.rt);
+    const uint64_t jobs = (uint64_t)kv->n_seq * kv->n_kv_heads * p.tiles;
+    const uint32_t most = ceil_div(max_len, 256);
+    const uint64_t want = ((uint64_t)PER_CU * cus + jobs / 2) / jobs;
+    p.n_own = (uint32_t)(want < 1 ? 1u : want < most ? want : most);
+    p.own_len = ceil_div(ceil_div(max_len, p.n_own), CUT) * CUT;
+    // (a launch has fewer than 2^32 threads)
+    if (jobs * p.n_own >= 1ull << 23) return false;
+    p.blocks = (uint32_t)(jobs * p.n_own);
+    const uint64_t parts = p.n_own == 1 ? 0 : jobs * p.n_own * 16 * p.rt;
+    p.stat_off = parts * kv->head_dim * 4;
+    p.bytes = p.stat_off + parts * 8;
+    return true;
+}
+
+bool kv8_shape_ok(const zh_kv8_batch *kv, uint32_t nh, uint32_t n_rows, uint32_t max_rows, uint32_t max_len) {
+    return kv8_batch_ok(kv, n_rows) && nh && nh % kv->n_kv_heads == 0 && n_rows && n_rows < 1u << 30 && max_rows &&
+           max_rows <= n_rows && max_len && max_len <= 1u << 30;
+}
+
+}  // namespace
+
+static zh_attn_rows with_strides(const zh_kv8_batch *kv, const zh_attn_rows *r) {
+    zh_attn_rows x = *r;
+    if (!x.q_stride) x.q_stride = x.n_heads * kv->head_dim;
+    if (!x.out_stride) x.out_stride = x.n_heads * kv->head_dim;
+    return x;
+}
+
+// The checks of zh_flash_attn_kv8, of host data only (exported for the tests; c may
+// be null: no message then). cus: the device's CUs.
+extern "C" int zh_check_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_attn_rows *rows, uint32_t cus) {
+    const char *const who = "flash_attn_kv8";
+    if (!rows || !kv8_shape_ok(kv, rows->n_heads, rows->n_rows, rows->max_rows, rows->max_len))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: caches, heads, rows or lengths", who);
+    if (!kv8_type_ok(kv->type)) return zh_set_err(c, ZH_ERR_UNSUPPORTED_QUANT_TYPE, "%s: cache type %u", who, kv->type);
+    const zh_attn_rows x = with_strides(kv, rows), *r = &x;
+    if ((uint64_t)r->max_len > 16ull * kv->table_stride)
+        return zh_set_err(c, ZH_ERR_CONTEXT_LENGTH_EXCEEDED, "%s: max_len %u in tables of %u pages", who, r->max_len,
+                          kv->table_stride);
+    if (r->type != ZH_F32 && r->type != ZH_F16)
+        return zh_set_err(c, ZH_ERR_UNSUPPORTED_QUANT_TYPE, "%s: type %u", who, r->type);
+    if (!isfinite(r->attn_scale)) return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: attn_scale", who);
+    const uint64_t size = r->type == ZH_F32 ? 4 : 2, w = (uint64_t)r->n_heads * kv->head_dim, n = r->n_rows;
+    if (w > 0xFFFFFFFFull || (n > 1 && (r->q_stride < w || r->out_stride < w)))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: rows overlap", who);
+    const uint64_t qb = ((n - 1) * r->q_stride + w) * size, ob = ((n - 1) * r->out_stride + w) * size;
+    Kv8Plan p;
+    if (!kv8_plan(cus, kv, r->n_heads, r->max_rows, r->max_len, p))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: too large", who);
+    if (!kv_in_range(r->q, r->q_off, qb) || !kv_in_range(r->out, r->out_off, ob) ||
+        (p.bytes && !kv_in_range(r->ws, 0, p.bytes)))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: range (ws: %llu bytes)", who, (unsigned long long)p.bytes);
+    // out and ws: not what the call reads besides q
+    const zh_buf *const read[] = {kv->k_cache, kv->v_cache, kv->k_scale, kv->v_scale, kv->tables, kv->row_start, kv->seq_lens};
+    for (const zh_buf *b : read)
+        if (b && (b->ptr == r->out->ptr || (p.bytes && b->ptr == r->ws->ptr)))
+            return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: out or ws is an input", who);
+    if (p.bytes && (r->ws->ptr == r->out->ptr || r->ws->ptr == r->q->ptr))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: ws holds q or out", who);
+    if (r->q_off % 16 || r->out_off % 16 || (n > 1 && (r->q_stride * size % 16 || r->out_stride * size % 16)))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: rows not 16-byte aligned", who);
+    const bool same = r->q->ptr == r->out->ptr && r->q_off == r->out_off && (n == 1 || r->q_stride == r->out_stride);
+    if (!same && kv_rows_overlap(r->q, r->q_off, qb, r->out, r->out_off, ob) &&
+        !(r->q_stride == r->out_stride &&
+          kv_columns_apart(r->out, r->out_off, r->q, r->q_off, r->q_stride, w, w, (uint32_t)size)))
+        return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: out overlaps q", who);
+    return ZH_OK;
+}
+
+// zh_flash_attn_kv8_ws of a device of `cus` CUs (exported for the tests).
+extern "C" uint64_t zh_check_attn_kv8_ws(const zh_kv8_batch *kv, uint32_t n_heads, uint32_t n_rows, uint32_t max_rows,
+                                         uint32_t max_len, uint32_t cus) {
+    Kv8Plan p;
+    if (!kv8_shape_ok(kv, n_heads, n_rows, max_rows, max_len) || !kv8_plan(cus, kv, n_heads, max_rows, max_len, p)) return 0;
+    return std::max<uint64_t>(16, p.bytes);
+}
+
+extern "C" uint64_t zh_flash_attn_kv8_ws(zh_ctx *c, const zh_kv8_batch *kv, uint32_t n_heads, uint32_t n_rows,
+                                         uint32_t max_rows, uint32_t max_len) {
+    return c ? zh_check_attn_kv8_ws(kv, n_heads, n_rows, max_rows, max_len, (uint32_t)c->cu_count) : 0;
+}
+
+template <int HD, int NP, int RT, uint32_t F, typename T>
+static int attn_launch(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p) {
+    constexpr uint32_t NJ = NP == 2 && HD == 128 ? 2 : 4;
+    hipLaunchKernelGGL((k_kv8_attn<HD, NP, RT, NJ, F, T>), dim3(p.blocks), dim3(64 * W), 0, c->stream, a);
+    ZH_LAUNCH_CHECK(c);
+    if (p.n_own > 1) {
+        const uint32_t per = 256 / (HD / 4), items = a.n_seq * a.nkv * a.tiles;
+        hipLaunchKernelGGL((k_kv8_join<HD, RT, T>), dim3(items * (16 * RT / per)), dim3(256), 0, c->stream, a);
+        ZH_LAUNCH_CHECK(c);
+    }
+    return ZH_OK;
+}
+template <int HD, int NP, uint32_t F, typename T>
+static int attn_rt(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p) {
+    return p.rt == 1 ? attn_launch<HD, NP, 1, F, T>(c, a, p) : attn_launch<HD, NP, 2, F, T>(c, a, p);
+}
+template <int HD, uint32_t F>
+static int attn_type(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p, uint32_t type) {
+    return type == ZH_F32 ? attn_rt<HD, 2, F, float>(c, a, p) : attn_rt<HD, 1, F, _Float16>(c, a, p);
+}
+
+extern "C" int zh_flash_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_attn_rows *rows) {
+    if (!c) return ZH_ERR_INVALID_ARGUMENT;
+    const int rc = zh_check_attn_kv8(c, kv, rows, (uint32_t)c->cu_count);
+    if (rc) return rc;
+    const zh_attn_rows x = with_strides(kv, rows), *r = &x;
+    zh_device_scope dev(c);
+    Kv8Plan p;
+    kv8_plan((uint32_t)c->cu_count, kv, r->n_heads, r->max_rows, r->max_len, p);
+    Kv8Attn a = {};
+    const uint64_t size = r->type == ZH_F32 ? 4 : 2;
+    a.q = (const uint8_t *)r->q->ptr + r->q_off;
+    a.out = (uint8_t *)r->out->ptr + r->out_off;
+    a.q_row = r->q_stride * size;
+    a.out_row = r->out_stride * size;
+    a.kc = (const uint8_t *)kv->k_cache->ptr;
+    a.vc = (const uint8_t *)kv->v_cache->ptr;
+    a.ks = (const float *)kv->k_scale->ptr;
+    a.vs = (const float *)kv->v_scale->ptr;
+    a.tables = (const uint32_t *)kv->tables->ptr;
+    a.row_start = kv->row_start ? (const uint32_t *)kv->row_start->ptr : nullptr;
+    a.seq_lens = (const uint32_t *)kv->seq_lens->ptr;
+    a.part = p.bytes ? (float *)r->ws->ptr : nullptr;
+    a.stat = p.bytes ? (float *)((char *)r->ws->ptr + p.stat_off) : nullptr;
+    a.err = c->err_dev;
+    a.n_seq = kv->n_seq;
+    a.stride = kv->table_stride;
+    a.cache_tokens = kv->cache_tokens;
+    a.nh = r->n_heads;
+    a.nkv = kv->n_kv_heads;
+    a.G = a.nh / a.nkv;
+    a.n_rows = r->n_rows;
+    a.max_rows = r->max_rows;
+    a.max_len = r->max_len;
+    a.tiles = p.tiles;
+    a.n_own = p.n_own;
+    a.own_len = p.own_len;
+    // (64 bits: a scale of any size times log2 e)
+    const double scale = (double)(r->attn_scale != 0.f ? r->attn_scale : 1.0f / sqrtf((float)kv->head_dim)) *
+                         1.44269504088896340736f;
+    int scale_exp = 0;
+    a.scale = (float)frexp(scale, &scale_exp);
+    a.scale_exp = scale_exp;
+    if (kv->head_dim == 128)
+        return kv->type == ZH_I8 ? attn_type<128, ZH_I8>(c, a, p, r->type) : attn_type<128, ZH_E4M3>(c, a, p, r->type);
+    return kv->type == ZH_I8 ? attn_type<64, ZH_I8>(c, a, p, r->type) : attn_type<64, ZH_E4M3>(c, a, p, r->type);
+}

@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("ZH_LIB_PATH") or os.path.join(HERE, "libzinc_hip.so")
 
 F32, F16, Q8_0, Q4_K, Q5_K, Q6_K, MXFP4 = 0, 1, 8, 12, 13, 14, 39
+I8, E4M3 = 24, 256  # codes of an 8-bit KV cache
 OK = 0
 STATUS = {1: "UnsupportedQuantType", 2: "InvalidArgument", 3: "HipError",
           4: "ContextLengthExceeded", 5: "OutOfMemory", 6: "TensorNotFound", 7: "InvalidMagic",
@@ -113,6 +114,12 @@ SIGNATURES = {
     "zh_flash_decode_shared": (_i32, [_P, _P, _P]),
     "zh_flash_decode_shared_ws": (_u64, [_P, _P, _u32, _u32, _u32]),
     "zh_kv_copy_pages": (_i32, [_P, _P, _P, _P, _P, _u32]),
+    "zh_qk_norm_rope_kv8_write_batched": (_i32, [_P, _P, _P]),
+    "zh_flash_attn_kv8": (_i32, [_P, _P, _P]),
+    "zh_flash_attn_kv8_ws": (_u64, [_P, _P, _u32, _u32, _u32, _u32]),
+    "zh_kv8_pack_pages": (_i32, [_P, _P, _P, _P, _P, _u32]),
+    "zh_kv8_unpack_pages": (_i32, [_P, _P, _P, _P, _P, _u32]),
+    "zh_kv8_copy_pages": (_i32, [_P, _P, _P, _P, _P, _u32]),
     "zh_softmax_topk": (_i32, [_P, _P, _u32, _u32, _P]),
     "zh_moe_weighted_acc": (_i32, [_P, _P, _P, _P, _u32, _u32, _u32]),
     "zh_argmax": (_i32, [_P, _P, _u32, _P, _u64]),
@@ -269,6 +276,53 @@ class KvCaches(_Plan):
         self._set(caches=C.cast(self._array, C.POINTER(_P)), n_caches=len(caches), cache_tokens=cache_tokens,
                   n_kv_heads=n_kv_heads, head_dim=head_dim)
         for b in caches:
+            self._hold(b)
+
+
+class Kv8Batch(_Plan):
+    """zh_kv8_batch: one layer's paged caches in 8 bits with their scales, the
+    page tables of a batch and which rows of a call are each sequence's."""
+
+    class Struct(C.Structure):
+        _fields_ = [(n, _P) for n in ("k_cache", "v_cache", "k_scale", "v_scale", "tables", "row_start",
+                                      "seq_lens")] + [(n, _u32) for n in (
+            "n_seq", "table_stride", "cache_tokens", "n_kv_heads", "head_dim", "type")]
+
+    def __init__(self, k_cache, v_cache, k_scale, v_scale, tables, seq_lens, n_seq, table_stride, cache_tokens,
+                 n_kv_heads, head_dim, type, row_start=None):
+        self._set(k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, tables=tables,
+                  row_start=row_start, seq_lens=seq_lens, n_seq=n_seq, table_stride=table_stride,
+                  cache_tokens=cache_tokens, n_kv_heads=n_kv_heads, head_dim=head_dim, type=type)
+
+
+class AttnRows(_Plan):
+    """zh_attn_rows: the query rows of a batch and where their results go."""
+
+    class Struct(C.Structure):
+        _fields_ = [("q", _P), ("out", _P), ("q_off", _u64), ("out_off", _u64), ("q_stride", _u32),
+                    ("out_stride", _u32), ("type", _u32), ("n_heads", _u32), ("ws", _P), ("n_rows", _u32),
+                    ("max_rows", _u32), ("max_len", _u32), ("attn_scale", _f32)]
+
+    def __init__(self, q, out, ws, n_rows, max_rows, max_len, n_heads, type=F32, q_off=0, out_off=0, q_stride=0,
+                 out_stride=0, attn_scale=0.0):
+        self._set(q=q, out=out, q_off=q_off, out_off=out_off, q_stride=q_stride, out_stride=out_stride, type=type,
+                  n_heads=n_heads, ws=ws, n_rows=n_rows, max_rows=max_rows, max_len=max_len, attn_scale=attn_scale)
+
+
+class Kv8Caches(_Plan):
+    """zh_kv8_caches: caches in 8 bits of one shape, with their scales."""
+
+    class Struct(C.Structure):
+        _fields_ = [("caches", C.POINTER(_P)), ("scales", C.POINTER(_P))] + [(n, _u32) for n in (
+            "n_caches", "cache_tokens", "n_kv_heads", "head_dim", "type", "reserved")]
+
+    def __init__(self, caches, scales, cache_tokens, n_kv_heads, head_dim, type):
+        if len(caches) != len(scales):
+            raise ValueError("one buffer of scales per cache")
+        self._arrays = [(_P * max(len(x), 1))(*[b.h for b in x]) for x in (caches, scales)]
+        self._set(caches=C.cast(self._arrays[0], C.POINTER(_P)), scales=C.cast(self._arrays[1], C.POINTER(_P)),
+                  n_caches=len(caches), cache_tokens=cache_tokens, n_kv_heads=n_kv_heads, head_dim=head_dim, type=type)
+        for b in [*caches, *scales]:
             self._hold(b)
 
 
@@ -498,6 +552,42 @@ class Context:
         if n != ns:
             raise ValueError("one source page per destination page")
         self.check(lib().zh_kv_copy_pages(self.h, dst.ptr, src.ptr, d, s, n))
+
+    def qk_norm_rope_kv8_write_batched(self, kv, rows):
+        """q/k norm, rotation and quantised KV write of a batch (Kv8Batch, QkvRows)."""
+        self.check(lib().zh_qk_norm_rope_kv8_write_batched(self.h, kv.ptr, rows.ptr))
+
+    def flash_attn_kv8(self, kv, rows):
+        """Causal attention of a batch over a cache in 8 bits (Kv8Batch, AttnRows)."""
+        self.check(lib().zh_flash_attn_kv8(self.h, kv.ptr, rows.ptr))
+
+    def flash_attn_kv8_ws(self, kv, n_heads, n_rows, max_rows, max_len):
+        """Bytes of a workspace for such a call and every one of fewer sequences or rows or a
+        smaller max_rows or max_len (0: refused sizes)."""
+        return lib().zh_flash_attn_kv8_ws(self.h, kv.ptr, n_heads, n_rows, max_rows, max_len)
+
+    def kv8_pack_pages(self, dst, src, dst_pages, src_pages, n_tokens):
+        """n_tokens tokens in pages of src (KvCaches) quantised into pages of dst (Kv8Caches)."""
+        d, n = _u32_array(dst_pages)
+        s, ns = _u32_array(src_pages)
+        if n != ns or n != -(-n_tokens // 16):
+            raise ValueError("one source and one destination page per 16 tokens")
+        self.check(lib().zh_kv8_pack_pages(self.h, dst.ptr, src.ptr, d, s, n_tokens))
+
+    def _kv8_pages(self, entry, dst, src, dst_pages, src_pages):
+        d, n = _u32_array(dst_pages)
+        s, ns = _u32_array(src_pages)
+        if n != ns:
+            raise ValueError("one source page per destination page")
+        self.check(entry(self.h, dst.ptr, src.ptr, d, s, n))
+
+    def kv8_unpack_pages(self, dst, src, dst_pages, src_pages):
+        """Pages of src (Kv8Caches) read back into pages of dst (KvCaches)."""
+        self._kv8_pages(lib().zh_kv8_unpack_pages, dst, src, dst_pages, src_pages)
+
+    def kv8_copy_pages(self, dst, src, dst_pages, src_pages):
+        """Pages of src with their scales to pages of dst (Kv8Caches)."""
+        self._kv8_pages(lib().zh_kv8_copy_pages, dst, src, dst_pages, src_pages)
 
     def softmax_topk(self, logits, n, k, routing):
         self.check(lib().zh_softmax_topk(self.h, logits.h, n, k, routing.h))
