@@ -11,8 +11,8 @@ value within 2^-45 of the border of two codes is not met by chance.
     more, and a scale that is no power of two adds 2^-20 (its exponent's fraction,
     its reciprocal): |error| <= W (2^-17 A + (n / 32 + 84 + 2 E) 2^-23 [+ 2^-19]),
     W = sum w |v|. Pieces of weights end at fp16's least subnormal, 2^-24: a weight is
-    off by 2^-25 where the row's largest w b is 2^14, which adds 2^-39 max(w b)
-    sum |Vc|. ZH_F16 adds 2^-11 W where the
+    off by 2^-25 where the row's largest w b is 2^14 (on LDS tiles 2^4 at least),
+    which adds 2^-39 (2^-29) max(w b) sum |Vc|. ZH_F16 adds 2^-11 W where the
     weights are one piece, and the store's rounding.
 """
 import kv8_ref as ref
@@ -240,4 +240,5 @@ def test_attention(zh, ctx, fmt, t, case):
     starts = None if all(c == 1 for c in counts) else np.concatenate([[0], np.cumsum(counts)])
     q, got = attend(zh, ctx, rng, cache, tables, counts, lens, G, t, starts)
     want, *terms = expect(cache, tables, q, counts, lens, hd ** -0.5)
-    close(got, want, tolerance(cache, t, want, *terms, lens))
+    tiled = max(counts) * G > 32
+    close(got, want, tolerance(cache, t, want, *terms, lens, floor=-29 if tiled else -39))

@@ -31,8 +31,10 @@ struct Kv8Attn {
     float *part, *stat;  // a part's unnormalised sums; maximum (base 2) and sum of weights
     uint32_t *err;
     uint32_t n_seq, stride, cache_tokens, nh, nkv, G, n_rows, max_rows, max_len;
-    uint32_t tiles;           // row tiles of a sequence and kv head
-    uint32_t n_own, own_len;  // parts of a sequence's tokens, their length at least
+    uint32_t few;             // rows of a sequence and kv head that are streamed; more go through LDS tiles
+    uint32_t n_own, own_len;  // parts of a streamed sequence's tokens, their length at least
+    float *tpart, *tstat;     // parts of LDS tiles
+    uint32_t items, tparts;   // LDS tiles of a kv head (as many at most), parts of each one's tokens
     float scale;              // |attn_scale| log2 e = scale * 2^scale_exp, with attn_scale's sign
     int32_t scale_exp;
 };
@@ -174,17 +176,15 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t li = lane % 16, lg = lane / 16;
     // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
-    const uint32_t kvh = blockIdx.x % a.nkv, job = blockIdx.x / a.nkv, tile = job % a.tiles;
-    const uint32_t s = job / a.tiles % a.n_seq, part = job / a.tiles / a.n_seq;
+    const uint32_t kvh = blockIdx.x % a.nkv, s = blockIdx.x / a.nkv % a.n_seq, part = blockIdx.x / a.nkv / a.n_seq;
     bool bad = false;
     const AttnSeq seq = attn_seq(a, s, bad);
-    if (tid == 0 && part == 0 && kvh == 0 && tile == 0 && bad) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+    if (tid == 0 && part == 0 && kvh == 0 && bad) atomicOr(a.err, ZH_DEVERR_KV_ROW);
     bad = false;
-    const uint32_t all_rows = seq.n * a.G, row0 = tile * ROWS;
-    if (row0 >= all_rows) return;
-    const uint32_t nrow = min(ROWS, all_rows - row0);
+    const uint32_t nrow = seq.n * a.G;
+    if (nrow == 0 || nrow > a.few) return;
     // the tokens that some row sees, and those that every row sees
-    const uint32_t end = seq.lim((row0 + nrow - 1) / a.G), every = seq.lim(row0 / a.G);
+    const uint32_t end = seq.lim(seq.n - 1), every = seq.lim(0);
     uint32_t c;
     const uint32_t parts = own_parts(a, end, c);
     if (part && part >= parts) return;  // (a row without tokens: part 0 writes its zeros)
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
     uint32_t lim[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const uint32_t r = row0 + min(16 * rt + li, nrow - 1), i = r / a.G;
+        const uint32_t r = min(16 * rt + li, nrow - 1), i = r / a.G;
         lim[rt] = min(seq.lim(i), t1);
         const T *qp = (const T *)(a.q + (uint64_t)(seq.row + i) * a.q_row) + (size_t)(kvh * a.G + r % a.G) * HD + 16 * lg;
         float v[2 * U][8], mx = 0.f;
@@ -427,7 +427,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
     }
     if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
     // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
-    const size_t p0 = ((((size_t)s * a.nkv + kvh) * a.tiles + tile) * a.n_own + part) * ROWS;
+    const size_t p0 = (((size_t)s * a.nkv + kvh) * a.n_own + part) * ROWS;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         if (rt) __syncthreads();
@@ -446,7 +446,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
         for (uint32_t i = tid; i < 16 * (HD / 4); i += 64 * W) {
             const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
             if (16 * rt + r >= nrow) break;
-            const uint32_t R = row0 + 16 * rt + r, qi = R / a.G, h = kvh * a.G + R % a.G;
+            const uint32_t R = 16 * rt + r, qi = R / a.G, h = kvh * a.G + R % a.G;
             float M = sm[r], L = 0.f;
             f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -477,18 +477,404 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
     }
 }
 
+// Many rows: a workgroup takes NW x 32 of them (rows of a kv head in the order query,
+// head), each wave 32, over K and V that pass through LDS once for all of them, in
+// stages of 64 tokens, as fp16: every thread converts its pieces on the way there, so
+// a code becomes fp16 once a workgroup and not once a wave.
+//   S^T = K q^T by v_mfma_f32_32x32x16_f16: lane (i = lane % 32, h = lane / 32)
+//   holds tokens 8 (r / 4) + 4 h + r % 4 of row i in register r: registers 0 .. 7 are
+//   one page's, 8 .. 15 the next one's, each with its block's scales; registers
+//   8 s .. 8 s + 7 are the weights' operand of the s-th 16-token product
+//   O^T += V^T P^T. V stays row-major in LDS, its transposed fragments come from
+//   ds_read_b64_tr_b16. 16-byte piece p of a row lies at p ^ t_swz(row), so that
+//   16 rows' reads of one piece hit every bank once and the transposing reads
+//   (4 pieces of 8 rows) every bank twice.
+// The products of the next 32 tokens' scores run while the current ones' weights
+// are computed. The reference moves only when a score passes it by 2^8 (the weights
+// then reach 2^12 in fp16 at most), so the output is rarely rescaled. A wave stops at
+// the last token that one of its rows sees.
+constexpr uint32_t TK = 64, TS = 3;  // tokens of a stage, stages in LDS
+template <int HD>
+constexpr uint32_t t_lds() { return 2 * TS * TK * HD * 2 + TS * 64; }
+
+// Of 16 pieces a row: rows 4 apart differ in the low bits, rows 1 apart in the
+// high ones; of 8 (two rows side by side in the banks) the same of row pairs.
+template <uint32_t PPR>
+ZH_DEV uint32_t t_swz(uint32_t row) {
+    return PPR == 16 ? (row & 3) * 4 + (row / 4 & 3) : (row / 2 & 1) * 4 + (row / 4 & 3);
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// The LDS tile `u` of a kv head: its sequence, and which of the sequence's tiles (the
+// last ones, which see the most tokens, first).
+ZH_DEV bool tile_of(const Kv8Attn &a, uint32_t rows, uint32_t u, uint32_t &s, uint32_t &tile, AttnSeq &seq) {
+    bool bad = false;
+    auto count = [&](uint32_t i) {
+        const uint64_t n = (uint64_t)attn_seq(a, i, bad).n * a.G;
+        return n > a.few ? (uint32_t)((n + rows - 1) / rows) : 0u;
+    };
+    uint32_t item;
+    if (!kv8_find(a.n_seq, u, count, s, item)) return false;
+    seq = attn_seq(a, s, bad);
+    tile = (uint32_t)((uint64_t)seq.n * a.G + rows - 1) / rows - 1 - item;
+    return true;
+}
+// The parts of a tile's `end` tokens, of `c` each.
+ZH_DEV uint32_t tile_parts(const Kv8Attn &a, uint32_t end, uint32_t &c) {
+    c = max((end + a.tparts - 1) / a.tparts, 1u);
+    c = (c + TK - 1) / TK * TK;
+    return (end + c - 1) / c;
+}
+
+template <int HD, int NP, int NW, uint32_t F, typename T>
+__global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) void k_kv8_tile(Kv8Attn a) {
+    constexpr int KS = HD / 16, DT = HD / 32;        // k-steps of the scores, 32-dim tiles of the output
+    constexpr uint32_t ROWB = HD * 2, PPR = HD / 8;  // bytes and 16-byte pieces of an fp16 row
+    constexpr uint32_t STAGE = TK * ROWB, ROWS = 32 * NW, NT = 64 * NW;
+    constexpr uint32_t CPR = HD / 16, PC = TK * CPR;  // 16-code pieces of a row and of a stage's K (or V)
+    constexpr uint32_t NPC = 2 * PC / NT, NL = PC > NT ? PC / NT : 1;  // a thread's pieces, rows
+    extern __shared__ __align__(16) uint8_t lds[];
+    typedef __fp16 tr4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) tr4 lds_tr4;
+    float *const scl = (float *)(lds + 2 * TS * STAGE);  // [stage][page]: Block's ks, lv, iv and ok
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const uint32_t i32 = lane % 32, h = lane / 32;
+    // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
+    const uint32_t kvh = blockIdx.x % a.nkv, part = blockIdx.x / a.nkv % a.tparts, u = blockIdx.x / a.nkv / a.tparts;
+    uint32_t s, tile;
+    AttnSeq seq;
+    if (!tile_of(a, ROWS, u, s, tile, seq)) return;
+    const uint32_t rows = seq.n * a.G, r0 = tile * ROWS, w0 = r0 + wave * 32;
+    const uint32_t end = seq.lim((min(r0 + ROWS, rows) - 1) / a.G);
+    uint32_t c;
+    const uint32_t parts = tile_parts(a, end, c);
+    if (part && part >= parts) return;  // (rows without tokens: part 0 writes their zeros)
+    const uint32_t t0 = part * c, t1 = min(t0 + c, end), nst = t1 > t0 ? (t1 - t0 + TK - 1) / TK : 0u;
+    // the wave's rows: the stages that it takes, the tokens that all of them see
+    const bool mine = w0 < rows;
+    const uint32_t wend = mine ? min(seq.lim((min(w0 + 32, rows) - 1) / a.G), t1) : 0u;
+    const uint32_t wst = wend > t0 ? (wend - t0 + TK - 1) / TK : 0u, every = mine ? min(seq.lim(w0 / a.G), t1) : 0u;
+    const uint32_t row = min(w0 + i32, rows - 1), qi = row / a.G, lim = min(seq.lim(qi), t1);
+    // ---- a thread's pieces of a stage: 16 codes of a token each
+    const uint8_t *kh = a.kc + (size_t)kvh * a.cache_tokens * HD, *vh = a.vc + (size_t)kvh * a.cache_tokens * HD;
+    const uint32_t *tab = a.tables + (size_t)s * a.stride;
+    bool bad = false;
+    auto trow = [&](uint32_t i) { return (i * NT + tid) % PC / CPR; };  // piece i's token of the stage
+    const uint32_t col = tid % CPR;
+    const bool kfirst = PC >= NT || tid < PC;  // piece 0 is one of K
+    struct Raw {
+        u32x4 x[NPC];
+        uint32_t k[NL], v[NL];  // scales (of the threads that have a page's first piece of K)
+    };
+    uint32_t pg[NL];
+    auto look = [&](uint32_t st) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t i = 0; i < NL; i++) pg[i] = tab[min((t0 + st * TK + trow(i)) / 16, (t1 - 1) / 16)];
+    };
+    auto fetch = [&](Raw &r) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t i = 0; i < NL; i++)
+            if (pg[i] >= a.cache_tokens / 16) {
+                bad = true;
+                pg[i] = 0;
+            }
+#pragma unroll
+        for (uint32_t i = 0; i < NPC; i++) {
+            const uint8_t *base = (PC >= NT ? i < PC / NT : kfirst) ? kh : vh;
+            r.x[i] = *(const u32x4 *)(base + ((size_t)pg[i % NL] * 16 + trow(i) % 16) * HD + col * 16);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < NL; i++)
+            if (kfirst && col == 0 && trow(i) % 16 == 0) {
+                r.k[i] = ((const uint32_t *)a.ks)[(size_t)pg[i] * a.nkv + kvh];
+                r.v[i] = ((const uint32_t *)a.vs)[(size_t)pg[i] * a.nkv + kvh];
+            }
+    };
+    auto put = [&](uint32_t st, const Raw &r) __attribute__((always_inline)) {
+        const uint32_t slot = st % TS;
+#pragma unroll
+        for (uint32_t i = 0; i < NPC; i++) {
+            const uint32_t t = trow(i);
+            const bool isk = PC >= NT ? i < PC / NT : kfirst;
+            u32x4 x = r.x[i];
+            // V past the part: zero (0 times what the cache holds there may be NaN)
+            if (!isk && t0 + st * TK + t >= t1) x = F == ZH_I8 ? u32x4{} : u32x4{0, 0, 0, 0};
+            uint8_t *to = lds + (isk ? 0u : TS * STAGE) + slot * STAGE + t * ROWB;
+            *(half8 *)(to + ((2 * col) ^ t_swz<PPR>(t)) * 16) = row8<F>(x.x, x.y);
+            *(half8 *)(to + ((2 * col + 1) ^ t_swz<PPR>(t)) * 16) = row8<F>(x.z, x.w);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < NL; i++)
+            if (kfirst && col == 0 && trow(i) % 16 == 0) {
+                Block<F> b;
+                b.set(r.k[i], r.v[i]);
+                *(f32x4 *)(scl + (slot * 4 + trow(i) / 16) * 4) = f32x4{b.ks, b.lv, b.iv, b.ok ? 1.f : 0.f};
+            }
+    };
+    Raw raw;
+    if (nst) {
+        Raw raw1;
+        look(0);
+        fetch(raw);
+        look(1);
+        fetch(raw1);
+        look(2);
+        put(0, raw);
+        if (nst > 1) put(1, raw1);
+        fetch(raw);
+        look(3);
+    }
+    // ---- the row's q: dims 16 k + 8 h ..
+    half8 qf[NP][KS];
+    float cf;  // products to base-2 scores, but for the block's scale
+    {
+        const T *qp = (const T *)(a.q + (uint64_t)(seq.row + qi) * a.q_row) + (size_t)(kvh * a.G + row % a.G) * HD + 8 * h;
+        float v[KS][8], mx = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            ld8(qp + 16 * k, v[k]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k][e]));
+        }
+        int qe = 0;  // q is scaled by 2^-qe
+        if (NP > 1) {
+            mx = xor32_max(mx);
+            const uint32_t E = __float_as_uint(mx) >> 23;
+            if (E < 255) qe = (int)E - 141;
+        }
+        // (the scale's sign goes into q: the largest product is the largest score)
+        const float sign = copysignf(1.f, a.scale);
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float x = (NP > 1 ? ldexpf(v[k][e], -qe) : v[k][e]) * sign;
+#pragma unroll
+                for (int p = 0; p < NP; p++) {
+                    qf[p][k][e] = (_Float16)x;
+                    x -= (float)qf[p][k][e];
+                }
+            }
+        cf = fabsf(ldexpf(a.scale, a.scale_exp + qe));
+    }
+    f32x16 o[DT];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.f;
+    // fragment addresses in a stage (their k-step and 32-dim tile by exclusive or)
+    const uint32_t ka = i32 * ROWB + ((h ^ t_swz<PPR>(i32)) * 16);
+    const uint32_t l16 = lane % 16, vr = 4 * h + l16 / 4, vp = 2 * (lane / 16 % 2) + l16 % 4 / 2;
+    const uint32_t va = vr * ROWB + ((vp ^ t_swz<PPR>(vr)) * 16) + 8 * (l16 % 2);
+    const uint8_t *kp[KS], *vp0[DT], *vp1[DT];  // (the stage and the tokens in it: constant offsets)
+#pragma unroll
+    for (int k = 0; k < KS; k++) kp[k] = lds + (ka ^ (k * 32));
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+        // tokens 4 h .. +3 and those 8 on (8 rows on, the piece's bit 1 flipped)
+        vp0[d] = lds + TS * STAGE + (va ^ (d * 64));
+        vp1[d] = lds + TS * STAGE + 8 * ROWB + (va ^ (d * 64) ^ 32);
+    }
+    f32x16 sc, sn;  // products of the current and the next 32 tokens
+    half8 kf[KS];   // K fragments of the next ones
+    struct Half {   // of 32 tokens' two pages: scores' factors, weights' exponents and shares
+        float ck[2], lv[2], iv[2];
+        bool ok;
+    };
+    Half hc, hn;
+    auto load_k = [&](uint32_t slot, uint32_t kt) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < KS; k++) kf[k] = *(const half8 *)(kp[k] + slot * STAGE + kt * 32 * ROWB);
+    };
+    auto load_h = [&](Half &x, uint32_t slot, uint32_t kt) __attribute__((always_inline)) {
+        float ok = 1.f;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const f32x4 b = *(const f32x4 *)(scl + (slot * 4 + 2 * kt + j) * 4);
+            x.ck[j] = score_factor(cf, b.x);
+            x.lv[j] = b.y;
+            x.iv[j] = b.z;
+            ok *= b.w;
+        }
+        x.ok = __builtin_amdgcn_readfirstlane(__float_as_uint(ok)) != 0;
+    };
+    // the reference, for scores up to mx: moved, and the sums with it, where one
+    // passes it by 2^8
+    auto refer = [&](float mx) __attribute__((always_inline)) {
+        mx = xor32_max(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[d][r] *= f;
+        }
+    };
+    auto largest = [&](const f32x16 &d, const Half &x) __attribute__((always_inline)) {
+        float y = d[0], z = d[8];
+#pragma unroll
+        for (int r = 1; r < 8; r++) {
+            y = fmaxf(y, d[r]);
+            z = fmaxf(z, d[8 + r]);
+        }
+        return fmaxf(fmaf(y, x.ck[0], x.lv[0]), fmaf(z, x.ck[1], x.lv[1]));
+    };
+    // tokens from t on that the row does not see: no score; blocks that read as NaN
+    // (their factors are harmless)
+    auto mask = [&](uint32_t t, f32x16 &d, const Half &x, uint32_t slot, uint32_t kt) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const bool ok = scl[(slot * 4 + 2 * kt + j) * 4 + 3] != 0.f;
+#pragma unroll
+            for (int r = 8 * j; r < 8 * j + 8; r++)
+                d[r] = t + 8 * (r / 4) + 4 * h + r % 4 >= lim ? -INFINITY : ok ? d[r] : NAN;
+        }
+    };
+    lds_bar();
+    if (wst) {
+        load_k(0, 0);
+        load_h(hc, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 16; r++) sc[r] = 0.f;
+#pragma unroll
+        for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+            for (int k = 0; k < KS; k++) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[p][k], sc, 0, 0, 0);
+        load_k(0, 1);
+        if (t0 + 32 > every || !hc.ok) mask(t0, sc, hc, 0, 0);
+        refer(largest(sc, hc));
+    }
+    constexpr int PAIRS = 8, EARLY = 6;  // weights in pairs; those taken beside the scores' products
+    for (uint32_t s0 = 0; s0 < nst; s0 += TS)  // (the ring's slots unrolled: constant LDS offsets)
+#pragma unroll
+    for (uint32_t slot = 0; slot < TS; slot++) {
+        const uint32_t st = s0 + slot;
+        if (st >= nst) break;  // uniform
+        lds_bar();
+        if (st + 2 < nst) put(st + 2, raw);
+        if (st + 3 < nst) {
+            fetch(raw);
+            look(st + 4);
+        }
+        if (st >= wst) continue;  // uniform per wave
+        const uint32_t tk = t0 + st * TK;
+#pragma unroll
+        for (uint32_t kt = 0; kt < 2; kt++) {
+            half8 pf[NP][2], vf[2][DT];
+            const float b = m == -INFINITY ? 0.f : 4.f - m;
+            const float bl[2] = {hc.lv[0] + b, hc.lv[1] + b};
+            float mx = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) sn[r] = 0.f;
+            auto weights = [&](int i) __attribute__((always_inline)) {  // 2 i and 2 i + 1
+#pragma unroll
+                for (int r = 2 * i; r < 2 * i + 2; r++) {
+                    float p = __builtin_amdgcn_exp2f(fmaf(sc[r], hc.ck[r / 8], bl[r / 8]));
+                    l = fmaf(p, hc.iv[r / 8], l);
+#pragma unroll
+                    for (int k = 0; k < NP; k++) {
+                        pf[k][r / 8][r % 8] = (_Float16)p;
+                        p -= (float)pf[k][r / 8][r % 8];
+                    }
+                }
+            };
+            auto load_v = [&](int s2) __attribute__((always_inline)) {
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const uint32_t at = slot * STAGE + (32 * kt + 16 * s2) * ROWB;
+                    const tr4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)(vp0[d] + at));
+                    const tr4 y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)(vp1[d] + at));
+                    vf[s2][d] = half8{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
+                                      (_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+                }
+            };
+            // three runs of products, each group of them (64 cycles) with vector
+            // work that does not need it; the order is pinned by the barriers
+            load_v(0);
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--) sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[p][k], sn, 0, 0, 0);
+#pragma unroll
+                for (int i = EARLY * k / KS; i < EARLY * (k + 1) / KS; i++) weights(i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            load_v(1);
+            load_h(hn, kt == 0 ? slot : (slot + 1) % TS, 1 - kt);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][d], pf[p][0], o[d], 0, 0, 0);
+#pragma unroll
+                for (int i = EARLY + (PAIRS - EARLY) * d / DT; i < EARLY + (PAIRS - EARLY) * (d + 1) / DT; i++) weights(i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            load_k((slot + 1) % TS, kt);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[1][d], pf[p][1], o[d], 0, 0, 0);
+                if (d == 0) mx = largest(sn, hn);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (kt == 0 || st + 1 < wst) {  // (after the wave's last tokens the products are of nothing)
+                const uint32_t tn = tk + 32 * (kt + 1);
+                if (tn + 32 > every || !hn.ok) {
+                    mask(tn, sn, hn, kt == 0 ? slot : (slot + 1) % TS, 1 - kt);
+                    mx = largest(sn, hn);
+                }
+                refer(mx);
+            }
+            sc = sn;
+            hc = hn;
+        }
+    }
+    if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+    l = xor32_sum(l);
+    if (w0 + i32 >= rows) return;
+    if (parts <= 1) {
+        const bool none = seq.lim(qi) == 0;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                if (!none) v = f32x4{o[d][4 * g] / l, o[d][4 * g + 1] / l, o[d][4 * g + 2] / l, o[d][4 * g + 3] / l};
+                st_out<T>(a, seq.row + qi, kvh * a.G + row % a.G, 32 * d + 8 * g + 4 * h, HD, v);
+            }
+        return;
+    }
+    const size_t pr = (((size_t)u * a.nkv + kvh) * a.tparts + part) * ROWS + (row - r0);
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *(f32x4 *)(a.tpart + pr * HD + 32 * d + 8 * g + 4 * h) =
+                f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+    if (h == 0) {
+        a.tstat[2 * pr] = m - 4.f;
+        a.tstat[2 * pr + 1] = l;
+    }
+}
+
 // Joins the parts of a row: HD / 4 lanes, of 4 dims each, take the parts'
 // statistics, as many at a time, then all of them the parts' sums, 8 loads of 16
 // bytes in flight. Parts stand `apart` rows from each other.
 template <int HD>
-ZH_DEV f32x4 join_row(const Kv8Attn &a, size_t first, uint32_t parts, uint32_t apart) {
+ZH_DEV f32x4 join_row(const float *part, const float *stat, size_t first, uint32_t parts, uint32_t apart) {
     constexpr uint32_t N = HD / 4, U = 8;
     const uint32_t lane = threadIdx.x & 63, l = lane % N;
     float M = -INFINITY, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t b = 0; b < parts; b += N) {
         const uint32_t n = min(N, parts - b);
-        const float2 st = *(const float2 *)(a.stat + 2 * (first + (size_t)(b + min(l, n - 1)) * apart));
+        const float2 st = *(const float2 *)(stat + 2 * (first + (size_t)(b + min(l, n - 1)) * apart));
         float mx = st.x;
 #pragma unroll
         for (uint32_t x = 1; x < N; x *= 2) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
@@ -504,7 +890,7 @@ ZH_DEV f32x4 join_row(const Kv8Attn &a, size_t first, uint32_t parts, uint32_t a
             f32x4 v[U];
 #pragma unroll
             for (uint32_t u = 0; u < U; u++)
-                v[u] = *(const f32x4 *)(a.part + (first + (size_t)(b + min(p + u, n - 1)) * apart) * HD + 4 * l);
+                v[u] = *(const f32x4 *)(part + (first + (size_t)(b + min(p + u, n - 1)) * apart) * HD + 4 * l);
 #pragma unroll
             for (uint32_t u = 0; u < U; u++) {  // (past the last part: its values again, weight 0)
                 const float f = __shfl(w, lane - l + min(p + u, N - 1), 64);
@@ -522,37 +908,56 @@ template <int HD, int RT, typename T>
 __global__ __launch_bounds__(256) void k_kv8_join(Kv8Attn a) {
     constexpr uint32_t N = HD / 4, PER = 256 / N, ROWS = 16 * RT;  // rows of a workgroup, of a tile
     const uint32_t item = blockIdx.x / (ROWS / PER), r = blockIdx.x % (ROWS / PER) * PER + threadIdx.x / N;
-    const uint32_t tile = item % a.tiles, kvh = item / a.tiles % a.nkv, s = item / a.tiles / a.nkv;
+    const uint32_t kvh = item % a.nkv, s = item / a.nkv;
     bool bad = false;
     const AttnSeq seq = attn_seq(a, s, bad);
-    const uint32_t all_rows = seq.n * a.G, row0 = tile * ROWS;
-    if (row0 >= all_rows) return;
-    const uint32_t nrow = min(ROWS, all_rows - row0);
+    const uint32_t nrow = seq.n * a.G;
+    if (nrow == 0 || nrow > a.few) return;
     uint32_t c;
-    const uint32_t parts = own_parts(a, seq.lim((row0 + nrow - 1) / a.G), c);
+    const uint32_t parts = own_parts(a, seq.lim(seq.n - 1), c);
     if (parts <= 1 || r / (64 / N) * (64 / N) >= nrow) return;  // (uniform per wave)
-    const uint32_t R = row0 + min(r, nrow - 1), qi = R / a.G, h = kvh * a.G + R % a.G;
-    const f32x4 v = join_row<HD>(a, (size_t)item * a.n_own * ROWS + (R - row0), parts, ROWS);
+    const uint32_t R = min(r, nrow - 1), qi = R / a.G, h = kvh * a.G + R % a.G;
+    const f32x4 v = join_row<HD>(a.part, a.stat, (size_t)item * a.n_own * ROWS + R, parts, ROWS);
+    if (r < nrow) st_out<T>(a, seq.row + qi, h, threadIdx.x % N * 4, HD, seq.lim(qi) ? v : f32x4{0.f, 0.f, 0.f, 0.f});
+}
+
+template <int HD, int NW, typename T>
+__global__ __launch_bounds__(256) void k_kv8_tile_join(Kv8Attn a) {
+    constexpr uint32_t N = HD / 4, PER = 256 / N, ROWS = 32 * NW;
+    const uint32_t item = blockIdx.x / (ROWS / PER), r = blockIdx.x % (ROWS / PER) * PER + threadIdx.x / N;
+    const uint32_t kvh = item % a.nkv, u = item / a.nkv;
+    uint32_t s, tile;
+    AttnSeq seq;
+    if (!tile_of(a, ROWS, u, s, tile, seq)) return;
+    const uint32_t r0 = tile * ROWS, nrow = min(ROWS, seq.n * a.G - r0);
+    uint32_t c;
+    const uint32_t parts = tile_parts(a, seq.lim((r0 + nrow - 1) / a.G), c);
+    if (parts <= 1 || r / (64 / N) * (64 / N) >= nrow) return;  // (uniform per wave)
+    const uint32_t R = r0 + min(r, nrow - 1), qi = R / a.G, h = kvh * a.G + R % a.G;
+    const f32x4 v = join_row<HD>(a.tpart, a.tstat, (size_t)item * a.tparts * ROWS + (R - r0), parts, ROWS);
     if (r < nrow) st_out<T>(a, seq.row + qi, h, threadIdx.x % N * 4, HD, seq.lim(qi) ? v : f32x4{0.f, 0.f, 0.f, 0.f});
 }
 
 // How a call is cut (the same for every call of these sizes).
 struct Kv8Plan {
-    uint32_t rt, tiles, n_own, own_len, blocks;
-    uint64_t stat_off, bytes;  // of ws
+    uint32_t rt, few, n_own, own_len, blocks;  // streamed
+    uint32_t nw, items, tparts, tblocks;       // LDS tiles (nw 0: none)
+    uint64_t stat_off, tpart_off, tstat_off, bytes;  // of ws
 };
-constexpr uint32_t PER_CU = 8;  // workgroups per CU that the parts are cut for
+constexpr uint32_t PER_CU = 8;   // workgroups per CU that the streamed parts are cut for
+constexpr uint32_t FEW = 32;     // rows that are streamed
+constexpr uint32_t TILE_FIX = 5; // a tile launch's start and end, in stages
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
-bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t max_rows, uint32_t max_len, Kv8Plan &p) {
-    const uint32_t G = nh / kv->n_kv_heads;
-    const uint64_t rows = (uint64_t)max_rows * G;
+bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t n_rows, uint32_t max_rows, uint32_t max_len,
+              Kv8Plan &p) {
+    const uint64_t G = nh / kv->n_kv_heads, rows = max_rows * G, nkv = kv->n_kv_heads, hd = kv->head_dim;
     p = {};
+    if (n_rows * G >= 1ull << 31) return false;
     p.rt = rows <= 16 ? 1 : 2;
-    if (rows > 1ull << 31) return false;
-    p.tiles = ceil_div(rows, 16 * p.rt);
-    const uint64_t jobs = (uint64_t)kv->n_seq * kv->n_kv_heads * p.tiles;
+    p.few = 16 * p.rt;
+    const uint64_t jobs = kv->n_seq * nkv;
     const uint32_t most = ceil_div(max_len, 256);
     const uint64_t want = ((uint64_t)PER_CU * cus + jobs / 2) / jobs;
     p.n_own = (uint32_t)(want < 1 ? 1u : want < most ? want : most);
@@ -561,8 +966,35 @@ bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t max_ro
     if (jobs * p.n_own >= 1ull << 23) return false;
     p.blocks = (uint32_t)(jobs * p.n_own);
     const uint64_t parts = p.n_own == 1 ? 0 : jobs * p.n_own * 16 * p.rt;
-    p.stat_off = parts * kv->head_dim * 4;
-    p.bytes = p.stat_off + parts * 8;
+    uint64_t tparts = 0;
+    if (rows > p.few) {
+        p.nw = rows > 128 ? 8 : 4;
+        const uint64_t tr = 32 * p.nw;
+        // a sequence of n rows takes at most (n + tr - 1) / tr tiles, and n / (few + 1) sequences take any
+        const uint64_t seqs = std::min<uint64_t>(kv->n_seq, n_rows * G / (p.few + 1));
+        const uint64_t items = (n_rows * G + seqs * (tr - 1)) / tr, tj = items * nkv;
+        // the parts that fill 1 to 4 rounds of one workgroup per CU, by the rounds' stages
+        const uint32_t top = ceil_div(max_len, 256);
+        uint32_t n = 1;
+        uint64_t best = ~0ull;
+        for (uint64_t r = 1; r <= 4; r++) {
+            const uint32_t fit = (uint32_t)(r * cus / tj), k = fit < 1 ? 1u : fit < top ? fit : top;
+            const uint64_t cost = ceil_div(tj * k, cus) * (uint64_t)(ceil_div(ceil_div(max_len, k), TK) + TILE_FIX);
+            if (cost < best) {
+                best = cost;
+                n = k;
+            }
+        }
+        p.items = (uint32_t)items;
+        p.tparts = n;
+        if (tj * n >= 1ull << 22 || items * nkv * tr >= 1ull << 27) return false;
+        p.tblocks = (uint32_t)(tj * n);
+        tparts = n == 1 ? 0 : tj * n * tr;
+    }
+    p.stat_off = parts * hd * 4;
+    p.tpart_off = p.stat_off + parts * 8;
+    p.tstat_off = p.tpart_off + tparts * hd * 4;
+    p.bytes = p.tstat_off + tparts * 8;
     return true;
 }
 
@@ -599,7 +1031,7 @@ extern "C" int zh_check_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: rows overlap", who);
     const uint64_t qb = ((n - 1) * r->q_stride + w) * size, ob = ((n - 1) * r->out_stride + w) * size;
     Kv8Plan p;
-    if (!kv8_plan(cus, kv, r->n_heads, r->max_rows, r->max_len, p))
+    if (!kv8_plan(cus, kv, r->n_heads, r->n_rows, r->max_rows, r->max_len, p))
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: too large", who);
     if (!kv_in_range(r->q, r->q_off, qb) || !kv_in_range(r->out, r->out_off, ob) ||
         (p.bytes && !kv_in_range(r->ws, 0, p.bytes)))
@@ -625,7 +1057,8 @@ extern "C" int zh_check_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
 extern "C" uint64_t zh_check_attn_kv8_ws(const zh_kv8_batch *kv, uint32_t n_heads, uint32_t n_rows, uint32_t max_rows,
                                          uint32_t max_len, uint32_t cus) {
     Kv8Plan p;
-    if (!kv8_shape_ok(kv, n_heads, n_rows, max_rows, max_len) || !kv8_plan(cus, kv, n_heads, max_rows, max_len, p)) return 0;
+    if (!kv8_shape_ok(kv, n_heads, n_rows, max_rows, max_len) || !kv8_plan(cus, kv, n_heads, n_rows, max_rows, max_len, p))
+        return 0;
     return std::max<uint64_t>(16, p.bytes);
 }
 
@@ -640,15 +1073,36 @@ static int attn_launch(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p) {
     hipLaunchKernelGGL((k_kv8_attn<HD, NP, RT, NJ, F, T>), dim3(p.blocks), dim3(64 * W), 0, c->stream, a);
     ZH_LAUNCH_CHECK(c);
     if (p.n_own > 1) {
-        const uint32_t per = 256 / (HD / 4), items = a.n_seq * a.nkv * a.tiles;
-        hipLaunchKernelGGL((k_kv8_join<HD, RT, T>), dim3(items * (16 * RT / per)), dim3(256), 0, c->stream, a);
+        const uint32_t per = 256 / (HD / 4);
+        hipLaunchKernelGGL((k_kv8_join<HD, RT, T>), dim3(a.n_seq * a.nkv * (16 * RT / per)), dim3(256), 0, c->stream, a);
         ZH_LAUNCH_CHECK(c);
     }
     return ZH_OK;
 }
+
+template <int HD, int NP, int NW, uint32_t F, typename T>
+static int tile_launch(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p) {
+    static std::atomic<bool> attr[64];  // by device
+    if (c->device >= 64 || !attr[c->device].load(std::memory_order_relaxed)) {
+        ZH_HIP(c, hipFuncSetAttribute((const void *)k_kv8_tile<HD, NP, NW, F, T>,
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)t_lds<HD>()));
+        if (c->device < 64) attr[c->device].store(true, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL((k_kv8_tile<HD, NP, NW, F, T>), dim3(p.tblocks), dim3(64 * NW), t_lds<HD>(), c->stream, a);
+    ZH_LAUNCH_CHECK(c);
+    if (p.tparts > 1) {
+        const uint32_t per = 256 / (HD / 4);
+        hipLaunchKernelGGL((k_kv8_tile_join<HD, NW, T>), dim3(p.items * a.nkv * (32 * NW / per)), dim3(256), 0, c->stream, a);
+        ZH_LAUNCH_CHECK(c);
+    }
+    return ZH_OK;
+}
+
 template <int HD, int NP, uint32_t F, typename T>
 static int attn_rt(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p) {
-    return p.rt == 1 ? attn_launch<HD, NP, 1, F, T>(c, a, p) : attn_launch<HD, NP, 2, F, T>(c, a, p);
+    const int rc = p.rt == 1 ? attn_launch<HD, NP, 1, F, T>(c, a, p) : attn_launch<HD, NP, 2, F, T>(c, a, p);
+    if (rc || !p.nw) return rc;
+    return p.nw == 8 ? tile_launch<HD, NP, 8, F, T>(c, a, p) : tile_launch<HD, NP, 4, F, T>(c, a, p);
 }
 template <int HD, uint32_t F>
 static int attn_type(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p, uint32_t type) {
@@ -662,7 +1116,7 @@ extern "C" int zh_flash_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
     const zh_attn_rows x = with_strides(kv, rows), *r = &x;
     zh_device_scope dev(c);
     Kv8Plan p;
-    kv8_plan((uint32_t)c->cu_count, kv, r->n_heads, r->max_rows, r->max_len, p);
+    kv8_plan((uint32_t)c->cu_count, kv, r->n_heads, r->n_rows, r->max_rows, r->max_len, p);
     Kv8Attn a = {};
     const uint64_t size = r->type == ZH_F32 ? 4 : 2;
     a.q = (const uint8_t *)r->q->ptr + r->q_off;
@@ -688,7 +1142,11 @@ extern "C" int zh_flash_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
     a.n_rows = r->n_rows;
     a.max_rows = r->max_rows;
     a.max_len = r->max_len;
-    a.tiles = p.tiles;
+    a.tpart = p.bytes ? (float *)((char *)r->ws->ptr + p.tpart_off) : nullptr;
+    a.tstat = p.bytes ? (float *)((char *)r->ws->ptr + p.tstat_off) : nullptr;
+    a.few = p.few;
+    a.items = p.items;
+    a.tparts = p.tparts;
     a.n_own = p.n_own;
     a.own_len = p.own_len;
     // (64 bits: a scale of any size times log2 e)
