@@ -10,6 +10,8 @@
 // scale that makes the block's largest value the largest code, the step is up to
 // twice as long.
 #pragma once
+#include <type_traits>
+
 #include "zh_device.h"
 #include "zh_internal.h"
 #include "zh_kv.h"
@@ -113,20 +115,30 @@ ZH_DEV Kv8Seq kv8_seq(const uint32_t *row_start, const uint32_t *seq_lens, uint3
     x.pos = x.len - x.n;
     return x;
 }
-// Item `u` of those that the sequences have (count(s) each, in order): its
-// sequence, and u counted from the sequence's first. Every wave by itself, 64
-// sequences at a time; false: there are fewer.
+// Sums over the lanes up to each one (row shifts, then the rows' totals passed on).
+ZH_DEV uint32_t wave_scan(uint32_t v) {
+    auto step = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    };
+    typedef std::integral_constant<int, 0xF> all;
+    step(std::integral_constant<int, 0x111>{}, all{});  // row_shr 1, 2, 4, 8
+    step(std::integral_constant<int, 0x112>{}, all{});
+    step(std::integral_constant<int, 0x114>{}, all{});
+    step(std::integral_constant<int, 0x118>{}, all{});
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast 15 to rows 1 and 3
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast 31 to rows 2 and 3
+    return v;
+}
+ZH_DEV uint32_t wave_total(uint32_t v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
+// Item `u` of those that the sequences have (n(s) each, in order): its sequence, and u
+// counted from the sequence's first. Every wave by itself, 64 sequences at a time;
+// false: there are fewer.
 template <typename C>
 ZH_DEV bool kv8_find(uint32_t n_seq, uint32_t u, C count, uint32_t &s, uint32_t &item) {
     const uint32_t lane = threadIdx.x & 63;
     for (uint32_t s0 = 0; s0 < n_seq; s0 += 64) {
-        const uint32_t n = s0 + lane < n_seq ? count(s0 + lane) : 0u;
-        uint32_t sum = n;
-#pragma unroll
-        for (uint32_t d = 1; d < 64; d *= 2) {
-            const uint32_t x = __shfl_up(sum, d, 64);
-            if (lane >= d) sum += x;
-        }
+        const uint32_t n = s0 + lane < n_seq ? count(s0 + lane) : 0u, sum = wave_scan(n);
         const uint64_t past = __builtin_amdgcn_ballot_w64(sum > u);
         if (past) {
             const uint32_t k = __builtin_ctzll(past);

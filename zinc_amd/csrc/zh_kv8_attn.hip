@@ -19,7 +19,8 @@
 namespace {
 
 constexpr int W = 4;         // waves of a streaming workgroup
-constexpr uint32_t CUT = 64;  // parts are whole numbers of so many tokens
+constexpr uint32_t NJ = 2;   // pages of a wave's step
+constexpr uint32_t CUT = 64;  // tokens of a unit, of which a streaming workgroup takes whole ones
 
 struct Kv8Attn {
     const uint8_t *q;
@@ -32,7 +33,7 @@ struct Kv8Attn {
     uint32_t *err;
     uint32_t n_seq, stride, cache_tokens, nh, nkv, G, n_rows, max_rows, max_len;
     uint32_t few;             // rows of a sequence and kv head that are streamed; more go through LDS tiles
-    uint32_t n_own, own_len;  // parts of a streamed sequence's tokens, their length at least
+    uint32_t groups, least;   // streaming workgroups of a kv head, units of each at least (0: one takes one sequence)
     float *tpart, *tstat;     // parts of LDS tiles
     uint32_t items, tparts;   // LDS tiles of a kv head (as many at most), parts of each one's tokens
     float scale;              // |attn_scale| log2 e = scale * 2^scale_exp, with attn_scale's sign
@@ -145,14 +146,45 @@ ZH_DEV void st_out(const Kv8Attn &a, uint32_t row, uint32_t h, uint32_t d, uint3
     else *(half4 *)op = half4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
 }
 
-// The parts of `len` tokens, of `c` each.
-ZH_DEV uint32_t own_parts(const Kv8Attn &a, uint32_t len, uint32_t &c) {
-    const uint32_t least = (len + a.n_own - 1) / a.n_own;
-    c = max(a.own_len, (least + CUT - 1) / CUT * CUT);
-    return (len + c - 1) / c;
+// The units of tokens that sequence s has for the streaming workgroups (one at
+// least, for rows without tokens).
+ZH_DEV uint32_t units_of(const Kv8Attn &a, uint32_t s, bool &bad) {
+    const AttnSeq x = attn_seq(a, s, bad);
+    const uint64_t n = (uint64_t)x.n * a.G;
+    return n && n <= a.few ? max((x.lim(x.n - 1) + CUT - 1) / CUT, 1u) : 0u;
+}
+// How the units of the streamed sequences are dealt out to the workgroups of a kv
+// head. Shares of q units, whatever sequences they are of, so that ragged lengths even
+// out; or, where no more workgroups than there are take parts of at most q units that
+// each lie in one sequence, those: sequences of one length (16 of 4096 tokens 27 us; in
+// shares, whose second sequence begins with loads that nothing hides, 32). Every wave by
+// itself.
+struct Share {
+    uint32_t q, total;
+    bool parts;
+    // the workgroups (parts) or units of a sequence of so many units
+    ZH_DEVM uint32_t items(uint32_t units) const { return parts ? (units + q - 1) / q : units; }
+};
+// u0: the lane's sequence's units (of the first 64)
+ZH_DEV Share share(const Kv8Attn &a, uint32_t u0, bool &bad) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t n = u0;
+    for (uint32_t s = lane + 64; s < a.n_seq; s += 64) n += units_of(a, s, bad);
+    Share x;
+    x.total = wave_total(n);
+    x.q = max((x.total + a.groups - 1) / a.groups, a.least);
+    x.parts = true;
+    n = x.items(u0);
+    for (uint32_t s = lane + 64; s < a.n_seq; s += 64) n += x.items(units_of(a, s, bad));
+    x.parts = wave_total(n) <= a.groups;
+    return x;
 }
 
-// 16 RT rows of one sequence and kv head over a part of its tokens. Each wave takes
+// A share of units of one kv head: in each sequence that it reaches into, up to 16 RT
+// rows over some of its tokens. A sequence that lies in one share is finished there;
+// of the others, each share leaves its unnormalised sum, maximum and sum of weights for
+// k_kv8_join: in slot 0 of the workgroup if it begins inside the sequence, else in slot
+// 1, so that a workgroup needs two however many sequences there are. Each wave takes
 // steps of NJ pages by itself, K and V straight from the cache into registers (no
 // LDS, no barrier before the end), the next step's K requested when the scores are
 // done and its V after the products with this one's:
@@ -165,7 +197,7 @@ ZH_DEV uint32_t own_parts(const Kv8Attn &a, uint32_t len, uint32_t &c) {
 //   permutes before they become fp16; column li of output tile n is dim HD/16 li + n.
 // NP pieces of q (scaled by a power of two to a maximum in [2^14, 2^15)) as sums of
 // fp16 values, 2 of the weights: 22 bits of each.
-template <int HD, int NP, int RT, uint32_t NJ, uint32_t F, typename T>
+template <int HD, int NP, int RT, uint32_t F, typename T>
 __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a) {
     constexpr uint32_t KB = 16 * NJ;
     constexpr int U = HD / 64, ND = HD / 16, VD = ND / 4;  // 16-code pieces of a K row, dims and dwords of V per lane
@@ -176,19 +208,41 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t li = lane % 16, lg = lane / 16;
     // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
-    const uint32_t kvh = blockIdx.x % a.nkv, s = blockIdx.x / a.nkv % a.n_seq, part = blockIdx.x / a.nkv / a.n_seq;
+    const uint32_t kvh = blockIdx.x % a.nkv, group = blockIdx.x / a.nkv;
+    uint32_t s = group, unit = 0, left = ~0u;  // the sequence, the unit in it, units to take from there
     bool bad = false;
+    if (a.least) {
+        const uint32_t u0 = lane < a.n_seq ? units_of(a, lane, bad) : 0u;
+        const Share x = share(a, u0, bad);
+        if (__builtin_amdgcn_ballot_w64(bad) && blockIdx.x == 0 && tid == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+        auto count = [&](uint32_t i) { return x.items(i < 64 ? u0 : units_of(a, i, bad)); };
+        if (!kv8_find(a.n_seq, x.parts ? group : group * x.q, count, s, unit)) return;
+        left = x.q;
+        if (x.parts) {  // (all of a length)
+            const uint32_t n = s < 64 ? __builtin_amdgcn_readlane(u0, s) : units_of(a, s, bad), p = x.items(n), c = (n + p - 1) / p;
+            unit *= c;
+            left = n > unit ? min(c, n - unit) : 0u;
+        }
+    } else {
+        units_of(a, s, bad);
+        if (bad && kvh == 0 && tid == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+    }
+    for (; left && s < a.n_seq; s++) {
+    bad = false;
     const AttnSeq seq = attn_seq(a, s, bad);
-    if (tid == 0 && part == 0 && kvh == 0 && bad) atomicOr(a.err, ZH_DEVERR_KV_ROW);
     bad = false;
     const uint32_t nrow = seq.n * a.G;
-    if (nrow == 0 || nrow > a.few) return;
+    if (nrow == 0 || nrow > a.few) {
+        if (!a.least) return;
+        continue;
+    }
     // the tokens that some row sees, and those that every row sees
-    const uint32_t end = seq.lim(seq.n - 1), every = seq.lim(0);
-    uint32_t c;
-    const uint32_t parts = own_parts(a, end, c);
-    if (part && part >= parts) return;  // (a row without tokens: part 0 writes its zeros)
-    const uint32_t t0 = part * c, t1 = min(t0 + c, end);
+    const uint32_t end = seq.lim(seq.n - 1), every = seq.lim(0), units = max((end + CUT - 1) / CUT, 1u);
+    const uint32_t take = min(left, units - unit), t0 = unit * CUT, t1 = min(t0 + take * CUT, end);
+    const bool direct = take == units;
+    const uint32_t slot = unit ? 0u : 1u;
+    left = a.least ? left - take : 0u;
+    unit = 0;
     const uint32_t nstep = t1 > t0 ? (t1 - t0 + KB - 1) / KB : 0u;
     const uint8_t *kh = a.kc + (size_t)kvh * a.cache_tokens * HD, *vh = a.vc + (size_t)kvh * a.cache_tokens * HD;
     const const_u32 *tab = (const const_u32 *)(a.tables + (size_t)s * a.stride);
@@ -427,10 +481,10 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
     }
     if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
     // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
-    const size_t p0 = (((size_t)s * a.nkv + kvh) * a.n_own + part) * ROWS;
+    const size_t p0 = ((size_t)blockIdx.x * 2 + slot) * ROWS;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        if (rt) __syncthreads();
+        __syncthreads();  // (the words below have been read)
         const float ls = xor32_sum(xor16_sum(l[rt]));
 #pragma unroll
         for (int r = 0; r < 4; r++)
@@ -462,7 +516,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
                 O.w = fmaf(v.w, fk, O.w);
                 L = fmaf(sl[k * 16 + r], fk, L);
             }
-            if (parts <= 1) {
+            if (direct) {
                 const f32x4 v = seq.lim(qi) ? f32x4{O.x / L, O.y / L, O.z / L, O.w / L} : f32x4{0.f, 0.f, 0.f, 0.f};
                 st_out<T>(a, seq.row + qi, h, d, HD, v);
             } else {
@@ -474,6 +528,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
                 }
             }
         }
+    }
     }
 }
 
@@ -865,16 +920,19 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
 
 // Joins the parts of a row: HD / 4 lanes, of 4 dims each, take the parts'
 // statistics, as many at a time, then all of them the parts' sums, 8 loads of 16
-// bytes in flight. Parts stand `apart` rows from each other.
-template <int HD>
-ZH_DEV f32x4 join_row(const float *part, const float *stat, size_t first, uint32_t parts, uint32_t apart) {
+// bytes in flight. Part p is row at(p) of part and stat.
+template <int HD, typename A>
+ZH_DEV f32x4 join_row(const float *part, const float *stat, uint32_t parts, A at) {
     constexpr uint32_t N = HD / 4, U = 8;
     const uint32_t lane = threadIdx.x & 63, l = lane % N;
     float M = -INFINITY, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t b = 0; b < parts; b += N) {
         const uint32_t n = min(N, parts - b);
-        const float2 st = *(const float2 *)(stat + 2 * (first + (size_t)(b + min(l, n - 1)) * apart));
+        const float2 st = *(const float2 *)(stat + 2 * at(b + min(l, n - 1)));
+        f32x4 v[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) v[u] = *(const f32x4 *)(part + at(b + min(u, n - 1)) * HD + 4 * l);
         float mx = st.x;
 #pragma unroll
         for (uint32_t x = 1; x < N; x *= 2) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
@@ -887,10 +945,9 @@ ZH_DEV f32x4 join_row(const float *part, const float *stat, size_t first, uint32
         L = fmaf(L, old, ls);
         O *= old;
         for (uint32_t p = 0; p < n; p += U) {
-            f32x4 v[U];
+            if (p)
 #pragma unroll
-            for (uint32_t u = 0; u < U; u++)
-                v[u] = *(const f32x4 *)(part + (first + (size_t)(b + min(p + u, n - 1)) * apart) * HD + 4 * l);
+                for (uint32_t u = 0; u < U; u++) v[u] = *(const f32x4 *)(part + at(b + min(p + u, n - 1)) * HD + 4 * l);
 #pragma unroll
             for (uint32_t u = 0; u < U; u++) {  // (past the last part: its values again, weight 0)
                 const float f = __shfl(w, lane - l + min(p + u, N - 1), 64);
@@ -910,14 +967,29 @@ __global__ __launch_bounds__(256) void k_kv8_join(Kv8Attn a) {
     const uint32_t item = blockIdx.x / (ROWS / PER), r = blockIdx.x % (ROWS / PER) * PER + threadIdx.x / N;
     const uint32_t kvh = item % a.nkv, s = item / a.nkv;
     bool bad = false;
+    const uint32_t lane = threadIdx.x & 63;
     const AttnSeq seq = attn_seq(a, s, bad);
     const uint32_t nrow = seq.n * a.G;
-    if (nrow == 0 || nrow > a.few) return;
-    uint32_t c;
-    const uint32_t parts = own_parts(a, seq.lim(seq.n - 1), c);
-    if (parts <= 1 || r / (64 / N) * (64 / N) >= nrow) return;  // (uniform per wave)
+    if (nrow == 0 || nrow > a.few || r / (64 / N) * (64 / N) >= nrow) return;  // (uniform per wave)
+    const uint32_t u0 = lane < a.n_seq ? units_of(a, lane, bad) : 0u;
+    const Share x = share(a, u0, bad);
+    uint32_t before = 0;
+    for (uint32_t i = lane; i < s; i += 64) before += x.items(i < 64 ? u0 : units_of(a, i, bad));
+    before = wave_total(before);
+    const uint32_t units = units_of(a, s, bad);
+    uint32_t first = before, parts = x.items(units);
+    if (x.parts) {  // (parts of one length: the last ones may be empty)
+        const uint32_t c = (units + parts - 1) / parts;
+        parts = (units + c - 1) / c;
+    } else {
+        first = before / x.q;
+        parts = (before + units - 1) / x.q - first + 1;
+    }
+    if (parts <= 1) return;
     const uint32_t R = min(r, nrow - 1), qi = R / a.G, h = kvh * a.G + R % a.G;
-    const f32x4 v = join_row<HD>(a.part, a.stat, (size_t)item * a.n_own * ROWS + R, parts, ROWS);
+    // (the first part begins with the sequence, the others in it)
+    auto at = [&](uint32_t p) { return ((size_t)((first + p) * a.nkv + kvh) * 2 + (p ? 0u : 1u)) * ROWS + R; };
+    const f32x4 v = join_row<HD>(a.part, a.stat, parts, at);
     if (r < nrow) st_out<T>(a, seq.row + qi, h, threadIdx.x % N * 4, HD, seq.lim(qi) ? v : f32x4{0.f, 0.f, 0.f, 0.f});
 }
 
@@ -934,20 +1006,22 @@ __global__ __launch_bounds__(256) void k_kv8_tile_join(Kv8Attn a) {
     const uint32_t parts = tile_parts(a, seq.lim((r0 + nrow - 1) / a.G), c);
     if (parts <= 1 || r / (64 / N) * (64 / N) >= nrow) return;  // (uniform per wave)
     const uint32_t R = r0 + min(r, nrow - 1), qi = R / a.G, h = kvh * a.G + R % a.G;
-    const f32x4 v = join_row<HD>(a.tpart, a.tstat, (size_t)item * a.tparts * ROWS + (R - r0), parts, ROWS);
+    auto at = [&](uint32_t p) { return ((size_t)item * a.tparts + p) * ROWS + (R - r0); };
+    const f32x4 v = join_row<HD>(a.tpart, a.tstat, parts, at);
     if (r < nrow) st_out<T>(a, seq.row + qi, h, threadIdx.x % N * 4, HD, seq.lim(qi) ? v : f32x4{0.f, 0.f, 0.f, 0.f});
 }
 
 // How a call is cut (the same for every call of these sizes).
 struct Kv8Plan {
-    uint32_t rt, few, n_own, own_len, blocks;  // streamed
+    uint32_t rt, few, groups, least;           // streamed
     uint32_t nw, items, tparts, tblocks;       // LDS tiles (nw 0: none)
     uint64_t stat_off, tpart_off, tstat_off, bytes;  // of ws
 };
-constexpr uint32_t PER_CU = 8;   // workgroups per CU that the streamed parts are cut for
+constexpr uint32_t LEAST = 4;    // units of a share at least
 constexpr uint32_t FEW = 32;     // rows that are streamed
 constexpr uint32_t TILE_FIX = 5; // a tile launch's start and end, in stages
 
+constexpr uint64_t kv8_one(uint32_t hd) { return hd == 64 ? 768 : 512; }
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t n_rows, uint32_t max_rows, uint32_t max_len,
@@ -957,15 +1031,15 @@ bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t n_rows
     if (n_rows * G >= 1ull << 31) return false;
     p.rt = rows <= 16 ? 1 : 2;
     p.few = 16 * p.rt;
-    const uint64_t jobs = kv->n_seq * nkv;
-    const uint32_t most = ceil_div(max_len, 256);
-    const uint64_t want = ((uint64_t)PER_CU * cus + jobs / 2) / jobs;
-    p.n_own = (uint32_t)(want < 1 ? 1u : want < most ? want : most);
-    p.own_len = ceil_div(ceil_div(max_len, p.n_own), CUT) * CUT;
-    // (a launch has fewer than 2^32 threads)
-    if (jobs * p.n_own >= 1ull << 23) return false;
-    p.blocks = (uint32_t)(jobs * p.n_own);
-    const uint64_t parts = p.n_own == 1 ? 0 : jobs * p.n_own * 16 * p.rt;
+    const uint64_t jobs = kv->n_seq * nkv, slots = (p.rt == 1 ? 3ull : 2ull) * cus;
+    // one workgroup a sequence: few short ones, or so many that they even out by themselves
+    const bool whole = (jobs <= cus && max_len <= kv8_one(hd) + kv8_one(hd) * jobs / cus) || jobs >= 8 * slots;
+    p.least = whole ? 0 : LEAST;
+    const uint64_t units = kv->n_seq * (uint64_t)ceil_div(max_len, CUT);
+    p.groups = whole ? kv->n_seq
+                     : (uint32_t)std::min<uint64_t>(std::max<uint64_t>(slots / nkv, 1), (units + LEAST - 1) / LEAST);
+    if (units >= 1ull << 31 || p.groups * nkv >= 1ull << 23) return false;  // (a launch has fewer than 2^32 threads)
+    const uint64_t parts = whole ? 0 : 2ull * p.groups * nkv * 16 * p.rt;
     uint64_t tparts = 0;
     if (rows > p.few) {
         p.nw = rows > 128 ? 8 : 4;
@@ -1069,10 +1143,9 @@ extern "C" uint64_t zh_flash_attn_kv8_ws(zh_ctx *c, const zh_kv8_batch *kv, uint
 
 template <int HD, int NP, int RT, uint32_t F, typename T>
 static int attn_launch(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p) {
-    constexpr uint32_t NJ = NP == 2 && HD == 128 ? 2 : 4;
-    hipLaunchKernelGGL((k_kv8_attn<HD, NP, RT, NJ, F, T>), dim3(p.blocks), dim3(64 * W), 0, c->stream, a);
+    hipLaunchKernelGGL((k_kv8_attn<HD, NP, RT, F, T>), dim3(p.groups * a.nkv), dim3(64 * W), 0, c->stream, a);
     ZH_LAUNCH_CHECK(c);
-    if (p.n_own > 1) {
+    if (p.least) {
         const uint32_t per = 256 / (HD / 4);
         hipLaunchKernelGGL((k_kv8_join<HD, RT, T>), dim3(a.n_seq * a.nkv * (16 * RT / per)), dim3(256), 0, c->stream, a);
         ZH_LAUNCH_CHECK(c);
@@ -1147,8 +1220,8 @@ extern "C" int zh_flash_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
     a.few = p.few;
     a.items = p.items;
     a.tparts = p.tparts;
-    a.n_own = p.n_own;
-    a.own_len = p.own_len;
+    a.groups = p.groups;
+    a.least = p.least;
     // (64 bits: a scale of any size times log2 e)
     const double scale = (double)(r->attn_scale != 0.f ? r->attn_scale : 1.0f / sqrtf((float)kv->head_dim)) *
                          1.44269504088896340736f;
