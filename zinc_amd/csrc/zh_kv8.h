@@ -32,10 +32,12 @@ bool kv8_batch_ok(const zh_kv8_batch *kv, uint32_t n_rows);
 // The bits of a scale in [2^-64, 2^64] (positive).
 ZH_DEV bool kv8_scale_ok(uint32_t bits) { return bits - 0x1F800000u <= 0x5F800000u - 0x1F800000u; }
 
-// The least e for which |x| <= largest * 2^e (exactly: 448 = 7/8 2^9, 127 = 127/128
-// 2^7), KV8_LOW at least; KV8_NAN past KV8_HIGH and for no number.
+// The least e for which x <= largest * 2^e (exactly: 448 = 7/8 2^9, 127 = 127/128
+// 2^7), KV8_LOW at least, KV8_NAN past KV8_HIGH. x: the largest of some magnitudes, and
+// `sum` their sum, which is no number (or too large) if one of them is none, where the
+// largest would not tell.
 template <uint32_t F, typename T>
-ZH_DEV int kv8_exp(T x) {
+ZH_DEV int kv8_exp(T x, T sum) {
     int e;
     T m;
     if constexpr (sizeof(T) == 8) {
@@ -45,11 +47,37 @@ ZH_DEV int kv8_exp(T x) {
         e = __builtin_amdgcn_frexp_expf(x);
         m = __builtin_amdgcn_frexp_mantf(x);
     }
-    m = m < 0 ? -m : m;
     e = F == ZH_I8 ? e - 7 + (m > (T)0.9921875) : e - 9 + (m > (T)0.875);
     if (x == 0) e = KV8_LOW;
-    if (!(m < 1)) e = KV8_NAN;  // (an infinity's or NaN's mantissa is itself)
+    if (!(sum < (T)INFINITY)) e = KV8_NAN;
     return e > KV8_HIGH ? KV8_NAN : max(e, KV8_LOW);
+}
+// The largest of each team's (L lanes, 8 or 16) and of the wave's values, by lane
+// exchanges within rows of 16.
+template <int L>
+ZH_DEV int team_max(int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
+    return L == 16 ? max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false)) : v;
+}
+ZH_DEV int wave_max(int v) {
+    v = team_max<16>(v);
+    return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+// The sum over teams of L lanes (8 or 16) in 64 bits.
+template <int CTRL>
+ZH_DEV double dpp_add64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, false);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int L>
+ZH_DEV double team_sum64(double v) {
+    v = dpp_add64<0x141>(dpp_add64<0x4E>(dpp_add64<0xB1>(v)));
+    return L == 16 ? dpp_add64<0x140>(v) : v;
 }
 ZH_DEV float kv8_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 

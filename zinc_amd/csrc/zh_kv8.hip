@@ -33,12 +33,14 @@ bool kv8_batch_ok(const zh_kv8_batch *kv, uint32_t n_rows) {
 // same cache whatever batch they came in. That is 30 operations of half rate for
 // each element of k beside its loads, 2 us of the chip for 8192 rows of 8 heads.
 //
-// A workgroup that writes takes one page of one sequence and some heads of k or v:
-// thread (slot, l) holds slot `slot` of the page and 8 dims, so the block's largest
-// value is a reduction of exponents over the workgroup, and the page's old tokens,
-// where the scale rises, are there to be rounded again. In a decode step one slot of
-// 16 has a row; the others' threads wait, which costs nothing where latency counts.
-// q's heads are workgroups of a row each, behind these in the same launch.
+// Two forms. Sequences with several rows: a workgroup takes one page of one sequence
+// and some heads of q, k or v: thread (slot, l) holds slot `slot` of the page and 8
+// dims, the angles of its four pairs are taken once for all its heads, a block's largest
+// value is a reduction over the workgroup, and the page's old tokens, where the scale
+// rises, are there to be rounded again. One row a sequence (a decode step): 16 head
+// vectors of a row a workgroup, each on 16 (8) lanes, which reach for the page's other
+// slots themselves where the scale rises; in the first form 15 of 16 threads would idle
+// (250 rows of 8 heads 12.8 us).
 // ---------------------------------------------------------------------------
 namespace {
 
@@ -52,21 +54,31 @@ struct Kv8Write {
     const uint32_t *tables, *row_start, *seq_lens;
     uint32_t *err;
     uint32_t n_seq, stride, cache_tokens, nq, nkv, rd, n_rows;
-    uint32_t hpb, groups;    // heads of a workgroup that writes, workgroups of a page's k (and of its v)
-    uint32_t kv_blocks;      // workgroups that write
-    uint32_t q_groups;       // workgroups of a row's q
-    uint32_t unit0;          // pages (rows) before this launch's
+    uint32_t q_heads, kv_heads;    // heads of a workgroup
+    uint32_t q_groups, kv_groups;  // workgroups of a page's (a row's) q, of its k (and of its v)
+    uint32_t unit0;           // pages (rows) before this launch's
     float eps;
 };
 
-ZH_DEV void ld4(const float *p, float (&v)[4]) {
-    const f32x4 a = *(const f32x4 *)p;
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-}
-ZH_DEV void ld4(const _Float16 *p, float (&v)[4]) {
-    const half4 a = *(const half4 *)p;
-#pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = (float)a[e];
+// four elements as they are, and as floats
+template <typename T>
+struct Quad {
+    typedef T V __attribute__((ext_vector_type(4)));
+    V v;
+    ZH_DEVM void load(const T *p) { v = *(const V *)p; }
+    template <typename S>
+    ZH_DEVM void get(S (&x)[4]) const {
+        x[0] = (S)v.x;
+        x[1] = (S)v.y;
+        x[2] = (S)v.z;
+        x[3] = (S)v.w;
+    }
+};
+template <typename T>
+ZH_DEV void ld4(const T *p, float (&x)[4]) {
+    Quad<T> q;
+    q.load(p);
+    q.get(x);
 }
 ZH_DEV void st4(float *p, const float (&v)[4]) { *(f32x4 *)p = f32x4{v[0], v[1], v[2], v[3]}; }
 ZH_DEV void st4(_Float16 *p, const float (&v)[4]) {
@@ -90,238 +102,304 @@ ZH_DEV bool quads(uint32_t l, uint32_t rd, uint32_t &lo, uint32_t &hi) {
     return rot;
 }
 
-template <int L>
-ZH_DEV double team_sum64(double v) {
+enum class Part { q, k, v };
+
+// Normalises and rotates the two quads of a lane's dims of one head (k: in 64 bits).
+template <typename V, int L>
+ZH_DEV void turned(V (&x)[4], V (&y)[4], bool norm, const float (&w0)[4], const float (&w1)[4], float eps, bool rot,
+                   const V (&co)[4], const V (&sn)[4]) {
+    if (norm) {  // (uniform; all lanes take part in the sum)
+        V sq = 0;
 #pragma unroll
-    for (int d = 1; d < L; d *= 2) v += __shfl_xor(v, d, 64);
-    return v;
+        for (int e = 0; e < 4; e++) sq = fma(x[e], x[e], fma(y[e], y[e], sq));
+        V ri;
+        if constexpr (sizeof(V) == 8) ri = 1.0 / sqrt(team_sum64<L>(sq) / (8 * L) + (double)eps);
+        else ri = 1.0f / sqrtf(team_sum_dpp<L>(sq) / (float)(8 * L) + eps);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[e] = w0[e] * (x[e] * ri);
+            y[e] = w1[e] * (y[e] * ri);
+        }
+    }
+    if (rot)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const V p = x[e], q = y[e];
+            x[e] = p * co[e] - q * sn[e];
+            y[e] = p * sn[e] + q * co[e];
+        }
 }
 
-// Heads [h0, h0 + n) of k (or v) in the slots of one page.
-template <typename TI, uint32_t F, int HD, bool K>
-ZH_DEV void write_heads(const Kv8Write &a, const Kv8Seq &seq, uint32_t page, uint32_t phys, uint32_t h0, uint32_t n) {
-    constexpr int L = HD / 8, NW = L / 4;  // lanes of a row, waves
-    __shared__ int top[2][NW];
+// The larger of a block's own scale (its bits; begun: it has none) and 2^t.
+ZH_DEV float block_scale(int t, uint32_t own, bool begun) {
+    if (t == KV8_NAN || (!begun && !kv8_scale_ok(own))) return NAN;
+    const float s = kv8_pow2(t);
+    return !begun && s < __uint_as_float(own) ? __uint_as_float(own) : s;
+}
+// The largest magnitude of two quads as kv8_exp takes it.
+template <uint32_t F, typename V>
+ZH_DEV int quads_exp(const V (&x)[4], const V (&y)[4]) {
+    V most = 0, sum = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const V p = x[e] < 0 ? -x[e] : x[e], q = y[e] < 0 ? -y[e] : y[e];
+        most = fmax(most, fmax(p, q));
+        sum += p + q;
+    }
+    return kv8_exp<F>(most, sum);
+}
+template <uint32_t F, typename V>
+ZH_DEV uint32_t code4(V (&x)[4], float s, float inv) {
+    if (s != s) return 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] *= inv;
+    return kv8_encode<F>(x);
+}
+template <uint32_t F>
+ZH_DEV uint32_t recode(uint32_t c, float f) {
+    float v[4];
+    kv8_decode<F>(c, v);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] *= f;
+    return kv8_encode<F>(v);
+}
+
+// Heads [h0, h0 + n) of q, k or v in the slots of one page (phys; q: of its tokens), B
+// at a time: the next ones' loads are on the way while these are worked on (a lane's
+// loads are 8 bytes an fp16 head: with one head on the way 20 waves of a CU have 20 KB
+// in flight, a quarter of what HBM takes to stay busy), and one barrier serves B
+// reductions.
+template <typename TI, typename TQ, uint32_t F, int HD, Part P>
+ZH_DEV void page_heads(const Kv8Write &a, const Kv8Seq &seq, uint32_t page, uint32_t phys, uint32_t h0, uint32_t n) {
+    constexpr int L = HD / 8, NW = L / 4, B = P == Part::k ? 2 : 4;  // lanes of a row, waves
+    using V = typename std::conditional<P == Part::k, double, float>::type;
+    __shared__ int top[2][B][NW];
     const uint32_t tid = threadIdx.x, l = tid % L, slot = tid / L, pos = page * 16 + slot;
     const bool mine = pos >= seq.pos && pos < seq.len, begun = page * 16 >= seq.pos;
     uint32_t lo = 8 * l, hi = 8 * l + 4;
     bool rot = false;
-    if (K) rot = quads(l, a.rd, lo, hi);
+    if (P != Part::v) rot = quads(l, a.rd, lo, hi);
     const uint32_t row = seq.row + (mine ? pos - seq.pos : 0u);
-    const TI *src = (const TI *)((K ? a.k : a.v) + row * (K ? a.k_row : a.v_row)) + (size_t)h0 * HD;
-    uint8_t *dst = (K ? a.kc : a.vc) + ((size_t)h0 * a.cache_tokens + phys * 16 + slot) * HD;
-    float *scale = (K ? a.ks : a.vs) + (size_t)phys * a.nkv + h0;
-    float x0[4] = {}, x1[4] = {};
-    if (mine) {
-        ld4(src + lo, x0);
-        ld4(src + hi, x1);
-    }
-    double co[4], sn[4];
+    const uint8_t *base = P == Part::q ? a.q + row * a.q_row : P == Part::k ? a.k + row * a.k_row : a.v + row * a.v_row;
+    const TI *src = (const TI *)base + (size_t)h0 * HD;
+    Quad<TI> r0[B] = {}, r1[B] = {};
+    auto load = [&](uint32_t i) __attribute__((always_inline)) {
+        if (mine)
+#pragma unroll
+            for (uint32_t j = 0; j < B; j++)
+                if (i + j < n) {
+                    r0[j].load(src + (i + j) * HD + lo);
+                    r1[j].load(src + (i + j) * HD + hi);
+                }
+    };
+    load(0);
+    V co[4] = {}, sn[4] = {};
     float w0[4] = {1.f, 1.f, 1.f, 1.f}, w1[4] = {1.f, 1.f, 1.f, 1.f};
-    if constexpr (K) {
+    const float *w = P == Part::q ? a.qw : a.kw;
+    if constexpr (P != Part::v) {
+        if (w) {
+            ld4(w + lo, w0);
+            ld4(w + hi, w1);
+        }
         if (rot && mine) {
             float f[4];
             ld4(a.inv_freq + 4 * l, f);
 #pragma unroll
-            for (int e = 0; e < 4; e++) sincospi(2.0 * turns(pos, f[e]), &sn[e], &co[e]);
-        }
-        if (a.kw) {
-            ld4(a.kw + lo, w0);
-            ld4(a.kw + hi, w1);
+            for (int e = 0; e < 4; e++) {
+                if constexpr (P == Part::k) sincospi(2.0 * turns(pos, f[e]), &sn[e], &co[e]);
+                else sincospif(2.0f * (float)turns(pos, f[e]), &sn[e], &co[e]);
+            }
         }
     }
-    for (uint32_t i = 0; i < n; i++, src += HD, dst += (size_t)a.cache_tokens * HD, scale++) {
-        using V = typename std::conditional<K, double, float>::type;
-        V y0[4], y1[4];
-        const uint32_t old = __float_as_uint(*scale);
+    uint8_t *dst = (P == Part::k ? a.kc : a.vc) + ((size_t)h0 * a.cache_tokens + phys * 16 + slot) * HD;
+    float *scale = (P == Part::k ? a.ks : a.vs) + (size_t)phys * a.nkv + h0;
+    TQ *out = (TQ *)(a.q_out + row * a.out_row) + (size_t)h0 * HD;
+    for (uint32_t i = 0, par = 0; i < n; i += B, par ^= 1) {
+        V y0[B][4], y1[B][4];
+        uint32_t old[B];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            y0[e] = x0[e];
-            y1[e] = x1[e];
+        for (int j = 0; j < B; j++) {
+            r0[j].get(y0[j]);
+            r1[j].get(y1[j]);
+            if (P != Part::q) old[j] = __float_as_uint(scale[min(i + j, n - 1)]);
         }
-        if (mine && i + 1 < n) {
-            ld4(src + HD + lo, x0);
-            ld4(src + HD + hi, x1);
-        }
-        if constexpr (K) {
-            if (a.kw) {  // (uniform; all lanes take part in the sum)
-                double sq = 0.0;
+        load(i + B);  // (also where q_out is q: its own dims of other heads)
 #pragma unroll
-                for (int e = 0; e < 4; e++) sq = fma(y0[e], y0[e], fma(y1[e], y1[e], sq));
-                const double ri = 1.0 / sqrt(team_sum64<L>(sq) / HD + (double)a.eps);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    y0[e] = w0[e] * (y0[e] * ri);
-                    y1[e] = w1[e] * (y1[e] * ri);
+        for (int j = 0; j < B; j++) {
+            if (i + j >= n) break;  // uniform
+            if constexpr (P != Part::v) turned<V, L>(y0[j], y1[j], w != nullptr, w0, w1, a.eps, rot, co, sn);
+            if constexpr (P == Part::q) {
+                if (mine) {
+                    st4(out + (i + j) * HD + lo, y0[j]);
+                    st4(out + (i + j) * HD + hi, y1[j]);
                 }
-            }
-            if (rot && mine)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const double p = y0[e], q = y1[e];
-                    y0[e] = p * co[e] - q * sn[e];
-                    y1[e] = p * sn[e] + q * co[e];
-                }
-        }
-        int t = KV8_LOW;
-        if (mine)
-#pragma unroll
-            for (int e = 0; e < 4; e++) t = max(t, max(kv8_exp<F>(y0[e]), kv8_exp<F>(y1[e])));
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) t = max(t, __shfl_xor(t, d, 64));
-        if (tid % 64 == 0) top[i & 1][tid / 64] = t;
-        __syncthreads();  // (one a head: the next but one writes these words after every thread has passed the next)
-#pragma unroll
-        for (int j = 0; j < NW; j++) t = max(t, top[i & 1][j]);
-        // the block's scale: the larger of its own and the rows'
-        float s = t == KV8_NAN || (!begun && !kv8_scale_ok(old)) ? NAN : kv8_pow2(t);
-        if (!begun) s = s < __uint_as_float(old) ? __uint_as_float(old) : s;
-        const float inv = 1.0f / s;
-        if (mine) {
-            uint32_t c0 = 0, c1 = 0;
-            if (s == s) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    y0[e] *= inv;
-                    y1[e] *= inv;
-                }
-                c0 = kv8_encode<F>(y0);
-                c1 = kv8_encode<F>(y1);
-            }
-            *(uint32_t *)(dst + lo) = c0;
-            *(uint32_t *)(dst + hi) = c1;
-        } else if (begun) {
-            *(uint32_t *)(dst + lo) = 0;
-            *(uint32_t *)(dst + hi) = 0;
-        } else if (s != __uint_as_float(old) && s == s) {
-            const float f = __uint_as_float(old) * inv;
-            float v[4];
-            for (uint32_t d : {lo, hi}) {
-                kv8_decode<F>(*(const uint32_t *)(dst + d), v);
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] *= f;
-                *(uint32_t *)(dst + d) = kv8_encode<F>(v);
+            } else {
+                const int t = wave_max(mine ? quads_exp<F>(y0[j], y1[j]) : KV8_LOW);
+                if (tid % 64 == 0) top[par][j][tid / 64] = t;
             }
         }
-        if (tid == 0) *scale = s;
+        if constexpr (P != Part::q) {
+            lds_bar();  // (the round after the next writes these words, when all threads have passed the next one's)
+#pragma unroll
+            for (int j = 0; j < B; j++) {
+                if (i + j >= n) break;  // uniform
+                int t = top[par][j][0];
+#pragma unroll
+                for (int k = 1; k < NW; k++) t = max(t, top[par][j][k]);
+                const float own = __uint_as_float(old[j]), s = block_scale(t, old[j], begun), inv = 1.0f / s;
+                uint8_t *to = dst + (size_t)(i + j) * a.cache_tokens * HD;
+                if (mine) {
+                    *(uint32_t *)(to + lo) = code4<F>(y0[j], s, inv);
+                    *(uint32_t *)(to + hi) = code4<F>(y1[j], s, inv);
+                } else if (begun) {
+                    *(uint32_t *)(to + lo) = 0;
+                    *(uint32_t *)(to + hi) = 0;
+                } else if (s != own && s == s) {
+                    *(uint32_t *)(to + lo) = recode<F>(*(const uint32_t *)(to + lo), own * inv);
+                    *(uint32_t *)(to + hi) = recode<F>(*(const uint32_t *)(to + hi), own * inv);
+                }
+                if (tid == 0) scale[i + j] = s;
+            }
+        }
     }
 }
 
+// The rows' description, checked once a call.
+ZH_DEV void check_rows(const Kv8Write &a) {
+    if (blockIdx.x || a.unit0) return;
+    uint32_t bad = 0;
+    for (uint32_t s = threadIdx.x; s < a.n_seq; s += blockDim.x) {
+        const Kv8Seq x = kv8_seq(a.row_start, a.seq_lens, s, a.n_rows, bad);
+        if (x.n && (x.len - 1) / 16 >= a.stride) bad = 1;
+    }
+    if (bad) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+}
+
+// A page's heads.
 template <typename TI, typename TQ, uint32_t F, int HD>
 __global__ __launch_bounds__(2 * HD) void k_kv8_write(Kv8Write a) {
-    constexpr uint32_t L = HD / 8, NS = 16, T = 2 * HD;  // lanes of a head vector, vectors of a workgroup
-    const uint32_t tid = threadIdx.x;
-    if (blockIdx.x < a.kv_blocks) {
-        const uint32_t per = 2 * a.groups, u = a.unit0 + blockIdx.x / per, g = blockIdx.x % per;
-        if (blockIdx.x == 0 && a.unit0 == 0) {  // the rows' description, checked once
-            uint32_t bad = 0;
-            for (uint32_t s = tid; s < a.n_seq; s += T) {
-                const Kv8Seq x = kv8_seq(a.row_start, a.seq_lens, s, a.n_rows, bad);
-                if (x.n && (x.len - 1) / 16 >= a.stride) bad = 1;
-            }
-            if (bad) atomicOr(a.err, ZH_DEVERR_KV_ROW);
-        }
-        uint32_t s = u, page;
-        Kv8Seq seq;
-        if (!a.row_start) {
-            uint32_t bad;
-            if (u >= a.n_seq) return;
-            seq = kv8_seq(nullptr, a.seq_lens, u, a.n_rows, bad);
-            if (!seq.n) return;
-            page = 0;
-        } else {
-            uint32_t bad;
-            auto pages = [&](uint32_t i) {
-                const Kv8Seq x = kv8_seq(a.row_start, a.seq_lens, i, a.n_rows, bad);
-                return x.n ? (x.len - 1) / 16 - x.pos / 16 + 1 : 0u;
-            };
-            if (!kv8_find(a.n_seq, u, pages, s, page)) return;
-            seq = kv8_seq(a.row_start, a.seq_lens, s, a.n_rows, bad);
-        }
-        page += seq.pos / 16;
-        if (page >= a.stride) return;
-        const uint32_t phys = a.tables[(size_t)s * a.stride + page];
-        if (phys >= a.cache_tokens / 16) {
-            if (tid == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
-            return;
-        }
-        const uint32_t h0 = g % a.groups * a.hpb, n = min(a.hpb, a.nkv - h0);
-        if (g < a.groups) write_heads<TI, F, HD, true>(a, seq, page, phys, h0, n);
-        else write_heads<TI, F, HD, false>(a, seq, page, phys, h0, n);
+    const uint32_t per = a.q_groups + 2 * a.kv_groups, u = a.unit0 + blockIdx.x / per, g = blockIdx.x % per;
+    check_rows(a);
+    uint32_t s, page, bad;
+    auto pages = [&](uint32_t i) {
+        const Kv8Seq x = kv8_seq(a.row_start, a.seq_lens, i, a.n_rows, bad);
+        return x.n ? (x.len - 1) / 16 - x.pos / 16 + 1 : 0u;
+    };
+    if (!kv8_find(a.n_seq, u, pages, s, page)) return;
+    const Kv8Seq seq = kv8_seq(a.row_start, a.seq_lens, s, a.n_rows, bad);
+    page += seq.pos / 16;
+    if (g < a.q_groups) {
+        page_heads<TI, TQ, F, HD, Part::q>(a, seq, page, 0, g * a.q_heads, min(a.q_heads, a.nq - g * a.q_heads));
         return;
     }
-    // ---- q: NS heads of one row at a time
-    __shared__ float2 cs[HD / 2];
-    const uint32_t b = blockIdx.x - a.kv_blocks, t = a.unit0 + b / a.q_groups, l = tid % L;
-    Kv8Seq seq;
-    uint32_t pos = 0;
-    if (!a.row_start) {
-        uint32_t bad;
-        seq = kv8_seq(nullptr, a.seq_lens, t, a.n_rows, bad);
-        if (!seq.n) return;
-        pos = seq.pos;
-    } else {
-        bool found = false;  // the sequence with row t
-        for (uint32_t s0 = 0; s0 < a.n_seq && !found; s0 += 64) {
-            uint32_t bad = 0;
-            Kv8Seq x = {0, 0, 0, 0};
-            if (s0 + tid % 64 < a.n_seq) x = kv8_seq(a.row_start, a.seq_lens, s0 + tid % 64, a.n_rows, bad);
-            const uint64_t hit = __builtin_amdgcn_ballot_w64(t >= x.row && t - x.row < x.n);
-            if (hit) {
-                const uint32_t k = __builtin_ctzll(hit);
-                pos = __builtin_amdgcn_readlane(x.pos, k) + (t - __builtin_amdgcn_readlane(x.row, k));
-                found = true;
-            }
-        }
-        if (!found) return;
+    if (page >= a.stride) return;
+    const uint32_t phys = a.tables[(size_t)s * a.stride + page];
+    if (phys >= a.cache_tokens / 16) {
+        if (threadIdx.x == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+        return;
     }
-    uint32_t lo, hi;
-    const bool rot = quads(l, a.rd, lo, hi);
-    if (a.rd) {  // (uniform)
-        for (uint32_t i = tid; i < a.rd / 2; i += T)
-            sincospif(2.0f * (float)turns(pos, a.inv_freq[i]), &cs[i].y, &cs[i].x);
+    const uint32_t h0 = (g - a.q_groups) % a.kv_groups * a.kv_heads, n = min(a.kv_heads, a.nkv - h0);
+    if (g - a.q_groups < a.kv_groups) page_heads<TI, TQ, F, HD, Part::k>(a, seq, page, phys, h0, n);
+    else page_heads<TI, TQ, F, HD, Part::v>(a, seq, page, phys, h0, n);
+}
+
+// 16 head vectors of one row (q's heads, then k's and v's).
+template <typename TI, typename TQ, uint32_t F, int HD>
+__global__ __launch_bounds__(2 * HD) void k_kv8_rows(Kv8Write a) {
+    constexpr uint32_t L = HD / 8;
+    __shared__ double2 cs[HD / 2];
+    const uint32_t tid = threadIdx.x, l = tid % L, H = a.nq + 2 * a.nkv;
+    const uint32_t t = a.unit0 + blockIdx.x / a.q_groups, v = blockIdx.x % a.q_groups * 16 + tid / L, h = min(v, H - 1);
+    const bool is_k = h >= a.nq && h < a.nq + a.nkv, is_v = h >= a.nq + a.nkv;
+    const uint32_t hh = is_v ? h - a.nq - a.nkv : is_k ? h - a.nq : h;
+    check_rows(a);
+    uint32_t lo = 8 * l, hi = 8 * l + 4;
+    bool rot = false;
+    if (!is_v) rot = quads(l, a.rd, lo, hi);
+    const TI *src = (const TI *)(is_v ? a.v + t * a.v_row : is_k ? a.k + t * a.k_row : a.q + t * a.q_row) + (size_t)hh * HD;
+    Quad<TI> r0, r1;
+    r0.load(src + lo);
+    r1.load(src + hi);
+    const uint32_t len = a.seq_lens[t], pos = len - 1;
+    if (len == 0) return;
+    // (a vector past the last: nothing stored)
+    const bool kv = h >= a.nq && v < H;
+    uint32_t phys = 0, old = 0;
+    bool ok = kv && pos / 16 < a.stride;
+    float *scale = nullptr;
+    if (ok) {
+        phys = a.tables[(size_t)t * a.stride + pos / 16];
+        ok = phys < a.cache_tokens / 16;
+        if (!ok && l == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+    }
+    if (ok) {
+        scale = (is_v ? a.vs : a.ks) + (size_t)phys * a.nkv + hh;
+        old = __float_as_uint(*scale);
+    }
+    if (a.rd) {  // (uniform; a workgroup has a thread for each angle)
+        if (tid < a.rd / 2) sincospi(2.0 * turns(pos, a.inv_freq[tid]), &cs[tid].y, &cs[tid].x);
         __syncthreads();
     }
-    float co[4] = {}, sn[4] = {}, w0[4] = {1.f, 1.f, 1.f, 1.f}, w1[4] = {1.f, 1.f, 1.f, 1.f};
-    if (rot)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            co[e] = cs[4 * l + e].x;
-            sn[e] = cs[4 * l + e].y;
-        }
-    if (a.qw) {
-        ld4(a.qw + lo, w0);
-        ld4(a.qw + hi, w1);
+    const float *w = is_k ? a.kw : a.qw;
+    float w0[4] = {}, w1[4] = {};
+    if (w && !is_v) {
+        ld4(w + lo, w0);
+        ld4(w + hi, w1);
     }
-    const uint8_t *src = a.q + t * a.q_row;
-    uint8_t *out = a.q_out + t * a.out_row;
-    for (uint32_t h0 = b % a.q_groups * NS; h0 < a.nq; h0 += a.q_groups * NS) {
-        const uint32_t h = min(h0 + tid / L, a.nq - 1);
-        float x[4], y[4];
-        ld4((const TI *)src + h * HD + lo, x);
-        ld4((const TI *)src + h * HD + hi, y);
-        if (a.qw) {
-            float sq = 0.f;
+    int e;
+    double x[4], y[4];
+    if (h < a.nq) {
+        float p[4], q[4], co[4], sn[4];
+        r0.get(p);
+        r1.get(q);
 #pragma unroll
-            for (int e = 0; e < 4; e++) sq = fmaf(x[e], x[e], fmaf(y[e], y[e], sq));
-            const float ri = 1.0f / sqrtf(team_sum_dpp<L>(sq) / (float)HD + a.eps);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[e] = w0[e] * (x[e] * ri);
-                y[e] = w1[e] * (y[e] * ri);
-            }
+        for (int i = 0; i < 4; i++) {
+            co[i] = rot ? (float)cs[4 * l + i].x : 0.f;
+            sn[i] = rot ? (float)cs[4 * l + i].y : 0.f;
         }
-        if (rot)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float p = x[e], q = y[e];
-                x[e] = p * co[e] - q * sn[e];
-                y[e] = p * sn[e] + q * co[e];
-            }
-        if (h0 + tid / L >= a.nq) continue;
-        st4((TQ *)out + h * HD + lo, x);
-        st4((TQ *)out + h * HD + hi, y);
+        turned<float, L>(p, q, w != nullptr, w0, w1, a.eps, rot, co, sn);
+        if (v < H) {
+            TQ *out = (TQ *)(a.q_out + t * a.out_row) + (size_t)hh * HD;
+            st4(out + lo, p);
+            st4(out + hi, q);
+        }
+        return;
     }
+    r0.get(x);
+    r1.get(y);
+    if (is_k) {
+        double co[4], sn[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            co[i] = rot ? cs[4 * l + i].x : 0.0;
+            sn[i] = rot ? cs[4 * l + i].y : 0.0;
+        }
+        turned<double, L>(x, y, w != nullptr, w0, w1, a.eps, rot, co, sn);
+    }
+    e = team_max<L>(quads_exp<F>(x, y));
+    if (!ok) return;
+    const bool begun = pos % 16 == 0;
+    const float own = __uint_as_float(old), s = block_scale(e, old, begun), inv = 1.0f / s;
+    uint8_t *to = (is_v ? a.vc : a.kc) + ((size_t)hh * a.cache_tokens + phys * 16) * HD;
+    const uint32_t c0 = code4<F>(x, s, inv), c1 = code4<F>(y, s, inv), slot = pos % 16;
+    if (begun || (s != own && s == s)) {  // the page's other slots too: 0, or rounded again
+        uint32_t o[16][2] = {};
+        if (!begun)
+#pragma unroll
+            for (uint32_t i = 0; i < 16; i++) {
+                o[i][0] = *(const uint32_t *)(to + i * HD + lo);
+                o[i][1] = *(const uint32_t *)(to + i * HD + hi);
+            }
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i++)
+            if (i != slot) {
+                *(uint32_t *)(to + i * HD + lo) = begun ? 0u : recode<F>(o[i][0], own * inv);
+                *(uint32_t *)(to + i * HD + hi) = begun ? 0u : recode<F>(o[i][1], own * inv);
+            }
+    }
+    *(uint32_t *)(to + slot * HD + lo) = c0;
+    *(uint32_t *)(to + slot * HD + hi) = c1;
+    if (l == 0) *scale = s;
 }
 
 }  // namespace
@@ -350,15 +428,14 @@ extern "C" int zh_check_kv8_rows(zh_ctx *c, const zh_kv8_batch *kv, const zh_qkv
 
 template <typename TI, typename TQ, uint32_t F, int HD>
 static int kv8_write_launch(zh_ctx *c, const Kv8Write &a, uint64_t units) {
-    // the pages and rows that a launch of fewer than 2^32 threads takes
-    const uint64_t per = 2ull * a.groups + a.q_groups, most = std::max<uint64_t>((1ull << 23) / per, 1);
-    for (uint64_t u0 = 0; u0 < units || u0 < a.n_rows; u0 += most) {
+    // the pages (rows) that a launch of fewer than 2^32 threads takes
+    const uint64_t per = a.row_start ? 2ull * a.kv_groups + a.q_groups : a.q_groups, most = (1ull << 23) / per;
+    for (uint64_t u0 = 0; u0 < units; u0 += most) {  // (per is below 2^18)
         Kv8Write b = a;
         b.unit0 = (uint32_t)u0;
-        const uint64_t n = u0 < units ? std::min(units - u0, most) : 0, r = u0 < a.n_rows ? std::min(a.n_rows - u0, most) : 0;
-        b.kv_blocks = (uint32_t)(n * 2 * a.groups);
-        hipLaunchKernelGGL((k_kv8_write<TI, TQ, F, HD>), dim3((uint32_t)(b.kv_blocks + r * a.q_groups)), dim3(2 * HD), 0,
-                           c->stream, b);
+        const dim3 grid((uint32_t)(std::min(units - u0, most) * per));
+        if (a.row_start) hipLaunchKernelGGL((k_kv8_write<TI, TQ, F, HD>), grid, dim3(2 * HD), 0, c->stream, b);
+        else hipLaunchKernelGGL((k_kv8_rows<TI, TQ, F, HD>), grid, dim3(2 * HD), 0, c->stream, b);
         ZH_LAUNCH_CHECK(c);
     }
     return ZH_OK;
@@ -408,9 +485,15 @@ extern "C" int zh_qk_norm_rope_kv8_write_batched(zh_ctx *c, const zh_kv8_batch *
     a.eps = r->eps;
     // pages that rows reach: a sequence of n rows at most (n + 30) / 16, and n
     const uint64_t units = a.row_start ? std::min<uint64_t>((a.n_rows + 30ull * a.n_seq) / 16, a.n_rows) : a.n_rows;
-    a.hpb = 1;
-    a.groups = (a.nkv + a.hpb - 1) / a.hpb;
-    a.q_groups = (a.nq + 15) / 16;
+    // heads of a workgroup: the more of them, the fewer angles are taken and the more
+    // loads are on the way. us at 4 heads of q and 1 of k (of v) / 8 and 2 / 16 and 4,
+    // 32 + 16 heads of 128, f16: 100 rows 4.6 / 5.9 / 8.4, 333 6.0 / 6.8 / 8.7, 1000 11.8 /
+    // 10.2 / 12.0, 2500 21.8 / 18.8 / 16.6, 8192 71 / 51 / 46; f32 8192 80 / 70 / 75
+    const bool big = units >= 128 && si == 2;
+    a.q_heads = units < 48 ? 4 : big ? 16 : 8;
+    a.kv_heads = units < 48 ? 1 : big ? 4 : 2;
+    a.kv_groups = (a.nkv + a.kv_heads - 1) / a.kv_heads;
+    a.q_groups = a.row_start ? (a.nq + a.q_heads - 1) / a.q_heads : (a.nq + 2 * a.nkv + 15) / 16;
     if (si == 4)
         return so == 4 ? kv8_write_type<float, float>(c, a, units, kv->type, kv->head_dim)
                        : kv8_write_type<float, _Float16>(c, a, units, kv->type, kv->head_dim);
@@ -455,13 +538,16 @@ __global__ __launch_bounds__(256) void k_kv8_pack(A a) {
         for (int i = 0; i < N; i++)
             if ((64 * i + lane) * 8 / HD >= a.last) x[i] = half8{};
     }
-    int t = KV8_LOW;
+    float most = 0.f, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) t = max(t, kv8_exp<F>((float)x[i][e]));
-#pragma unroll
-    for (int k = 1; k < 64; k *= 2) t = max(t, __shfl_xor(t, k, 64));
+        for (int e = 0; e < 8; e++) {
+            const float v = fabsf((float)x[i][e]);
+            most = fmaxf(most, v);
+            sum += v;
+        }
+    const int t = wave_max(kv8_exp<F>(most, sum));
     const bool nan = t == KV8_NAN;
     const float inv = nan ? 0.f : kv8_pow2(-t);
 #pragma unroll
