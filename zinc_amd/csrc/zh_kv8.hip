@@ -532,7 +532,7 @@ __global__ __launch_bounds__(256) void k_kv8_pack(A a) {
     u32x2 *d = (u32x2 *)(a.dst[c] + (h * a.dst_tokens + (uint64_t)a.pages[p][1] * 16) * HD);
     half8 x[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) x[i] = __builtin_bit_cast(half8, __builtin_nontemporal_load(s + 64 * i + lane));
+    for (int i = 0; i < N; i++) x[i] = __builtin_bit_cast(half8, s[64 * i + lane]);  // (a prompt's pages were just written)
     if (p == a.n_pages - 1) {
 #pragma unroll
         for (int i = 0; i < N; i++)

@@ -81,7 +81,7 @@ struct Block {
     float ks, lv, iv;
     bool ok;
     ZH_DEVM void set(uint32_t k, uint32_t v) {
-        constexpr float unit = F == ZH_I8 ? 1024.f : 1.f;
+        constexpr float unit = F == ZH_I8 ? 1024.f : 1.f;  // (of the fp16 codes)
         ok = kv8_scale_ok(k) && kv8_scale_ok(v);
         const uint32_t kb = ok ? k : 0x3F800000u, vb = ok ? v : 0x3F800000u;
         // (exact for powers of two; for others the exponent's fraction is within 2^-21)
@@ -541,23 +541,22 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
 //   one page's, 8 .. 15 the next one's, each with its block's scales; registers
 //   8 s .. 8 s + 7 are the weights' operand of the s-th 16-token product
 //   O^T += V^T P^T. V stays row-major in LDS, its transposed fragments come from
-//   ds_read_b64_tr_b16. 16-byte piece p of a row lies at p ^ t_swz(row), so that
-//   16 rows' reads of one piece hit every bank once and the transposing reads
-//   (4 pieces of 8 rows) every bank twice.
+//   ds_read_b64_tr_b16. Rows are padded, K's by 16 bytes, V's by 64: 16 rows' reads of
+//   one 16-byte piece hit every bank once, the transposing reads (64 bytes of 8 rows)
+//   every bank twice, and all of a lane's fragments lie at constant offsets from one
+//   address (swizzled pieces took 24 registers of addresses, and 12 others to scratch,
+//   whose reloads wait for the loads on the way).
 // The products of the next 32 tokens' scores run while the current ones' weights
 // are computed. The reference moves only when a score passes it by 2^8 (the weights
 // then reach 2^12 in fp16 at most), so the output is rarely rescaled. A wave stops at
 // the last token that one of its rows sees.
 constexpr uint32_t TK = 64, TS = 3;  // tokens of a stage, stages in LDS
 template <int HD>
-constexpr uint32_t t_lds() { return 2 * TS * TK * HD * 2 + TS * 64; }
-
-// Of 16 pieces a row: rows 4 apart differ in the low bits, rows 1 apart in the
-// high ones; of 8 (two rows side by side in the banks) the same of row pairs.
-template <uint32_t PPR>
-ZH_DEV uint32_t t_swz(uint32_t row) {
-    return PPR == 16 ? (row & 3) * 4 + (row / 4 & 3) : (row / 2 & 1) * 4 + (row / 4 & 3);
-}
+constexpr uint32_t t_krow() { return 2 * HD + 16; }
+template <int HD>
+constexpr uint32_t t_vrow() { return 2 * HD + 64; }
+template <int HD>
+constexpr uint32_t t_lds() { return TS * TK * (t_krow<HD>() + t_vrow<HD>()) + TS * 64; }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -583,16 +582,16 @@ ZH_DEV uint32_t tile_parts(const Kv8Attn &a, uint32_t end, uint32_t &c) {
 }
 
 template <int HD, int NP, int NW, uint32_t F, typename T>
-__global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) void k_kv8_tile(Kv8Attn a) {
+__global__ __launch_bounds__(64 * NW, HD == 128 && NW == 4 ? 1 : 2) void k_kv8_tile(Kv8Attn a) {
     constexpr int KS = HD / 16, DT = HD / 32;        // k-steps of the scores, 32-dim tiles of the output
-    constexpr uint32_t ROWB = HD * 2, PPR = HD / 8;  // bytes and 16-byte pieces of an fp16 row
-    constexpr uint32_t STAGE = TK * ROWB, ROWS = 32 * NW, NT = 64 * NW;
+    constexpr uint32_t KROW = t_krow<HD>(), VROW = t_vrow<HD>(), KST = TK * KROW, VST = TK * VROW;  // of a row, a stage
+    constexpr uint32_t ROWS = 32 * NW, NT = 64 * NW;
     constexpr uint32_t CPR = HD / 16, PC = TK * CPR;  // 16-code pieces of a row and of a stage's K (or V)
     constexpr uint32_t NPC = 2 * PC / NT, NL = PC > NT ? PC / NT : 1;  // a thread's pieces, rows
     extern __shared__ __align__(16) uint8_t lds[];
     typedef __fp16 tr4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) tr4 lds_tr4;
-    float *const scl = (float *)(lds + 2 * TS * STAGE);  // [stage][page]: Block's ks, lv, iv and ok
+    float *const scl = (float *)(lds + TS * (KST + VST));  // [stage][page]: Block's ks, lv, iv and ok
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t i32 = lane % 32, h = lane / 32;
     // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
@@ -654,10 +653,10 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
             const bool isk = PC >= NT ? i < PC / NT : kfirst;
             u32x4 x = r.x[i];
             // V past the part: zero (0 times what the cache holds there may be NaN)
-            if (!isk && t0 + st * TK + t >= t1) x = F == ZH_I8 ? u32x4{} : u32x4{0, 0, 0, 0};
-            uint8_t *to = lds + (isk ? 0u : TS * STAGE) + slot * STAGE + t * ROWB;
-            *(half8 *)(to + ((2 * col) ^ t_swz<PPR>(t)) * 16) = row8<F>(x.x, x.y);
-            *(half8 *)(to + ((2 * col + 1) ^ t_swz<PPR>(t)) * 16) = row8<F>(x.z, x.w);
+            if (!isk && t0 + st * TK + t >= t1) x = u32x4{0, 0, 0, 0};
+            uint8_t *to = lds + (isk ? slot * KST + t * KROW : TS * KST + slot * VST + t * VROW) + col * 32;
+            *(half8 *)to = row8<F>(x.x, x.y);
+            *(half8 *)(to + 16) = row8<F>(x.z, x.w);
         }
 #pragma unroll
         for (uint32_t i = 0; i < NL; i++)
@@ -719,19 +718,11 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.f;
-    // fragment addresses in a stage (their k-step and 32-dim tile by exclusive or)
-    const uint32_t ka = i32 * ROWB + ((h ^ t_swz<PPR>(i32)) * 16);
-    const uint32_t l16 = lane % 16, vr = 4 * h + l16 / 4, vp = 2 * (lane / 16 % 2) + l16 % 4 / 2;
-    const uint32_t va = vr * ROWB + ((vp ^ t_swz<PPR>(vr)) * 16) + 8 * (l16 % 2);
-    const uint8_t *kp[KS], *vp0[DT], *vp1[DT];  // (the stage and the tokens in it: constant offsets)
-#pragma unroll
-    for (int k = 0; k < KS; k++) kp[k] = lds + (ka ^ (k * 32));
-#pragma unroll
-    for (int d = 0; d < DT; d++) {
-        // tokens 4 h .. +3 and those 8 on (8 rows on, the piece's bit 1 flipped)
-        vp0[d] = lds + TS * STAGE + (va ^ (d * 64));
-        vp1[d] = lds + TS * STAGE + 8 * ROWB + (va ^ (d * 64) ^ 32);
-    }
+    // a lane's fragments in a stage: K's k-step k at kp + 32 k, V's 32-dim tile d at vp +
+    // 64 d, of tokens 4 h .. +3, and of those 8 on
+    const uint32_t l16 = lane % 16;
+    const uint8_t *const kp = lds + i32 * KROW + 16 * h;
+    const uint8_t *const vp = lds + TS * KST + (4 * h + l16 / 4) * VROW + 32 * (lane / 16 % 2) + 8 * (l16 % 4);
     f32x16 sc, sn;  // products of the current and the next 32 tokens
     half8 kf[KS];   // K fragments of the next ones
     struct Half {   // of 32 tokens' two pages: scores' factors, weights' exponents and shares
@@ -739,9 +730,13 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
         bool ok;
     };
     Half hc, hn;
-    auto load_k = [&](uint32_t slot, uint32_t kt) __attribute__((always_inline)) {
+    // (two pieces of f32 leave no registers for V beside the scores' products, nor for
+    // all of K ahead of them)
+    constexpr bool LATE = NP == 2 && HD == 128 && NW == 8;
+    constexpr int AHEAD = LATE ? KS / 2 : KS;
+    auto load_k = [&](uint32_t slot, uint32_t kt, int k0, int k1) __attribute__((always_inline)) {
 #pragma unroll
-        for (int k = 0; k < KS; k++) kf[k] = *(const half8 *)(kp[k] + slot * STAGE + kt * 32 * ROWB);
+        for (int k = k0; k < k1; k++) kf[k] = *(const half8 *)(kp + slot * KST + kt * 32 * KROW + 32 * k);
     };
     auto load_h = [&](Half &x, uint32_t slot, uint32_t kt) __attribute__((always_inline)) {
         float ok = 1.f;
@@ -780,7 +775,7 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
     };
     // tokens from t on that the row does not see: no score; blocks that read as NaN
     // (their factors are harmless)
-    auto mask = [&](uint32_t t, f32x16 &d, const Half &x, uint32_t slot, uint32_t kt) __attribute__((always_inline)) {
+    auto mask = [&](uint32_t t, f32x16 &d, uint32_t slot, uint32_t kt) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const bool ok = scl[(slot * 4 + 2 * kt + j) * 4 + 3] != 0.f;
@@ -791,7 +786,7 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
     };
     lds_bar();
     if (wst) {
-        load_k(0, 0);
+        load_k(0, 0, 0, KS);
         load_h(hc, 0, 0);
 #pragma unroll
         for (int r = 0; r < 16; r++) sc[r] = 0.f;
@@ -799,8 +794,8 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
         for (int p = NP - 1; p >= 0; p--)
 #pragma unroll
             for (int k = 0; k < KS; k++) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[p][k], sc, 0, 0, 0);
-        load_k(0, 1);
-        if (t0 + 32 > every || !hc.ok) mask(t0, sc, hc, 0, 0);
+        load_k(0, 1, 0, AHEAD);
+        if (t0 + 32 > every || !hc.ok) mask(t0, sc, 0, 0);
         refer(largest(sc, hc));
     }
     constexpr int PAIRS = 8, EARLY = 6;  // weights in pairs; those taken beside the scores' products
@@ -810,12 +805,17 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
         const uint32_t st = s0 + slot;
         if (st >= nst) break;  // uniform
         lds_bar();
-        if (st + 2 < nst) put(st + 2, raw);
-        if (st + 3 < nst) {
-            fetch(raw);
-            look(st + 4);
+        auto next = [&]() __attribute__((always_inline)) {  // the stages ahead
+            if (st + 2 < nst) put(st + 2, raw);
+            if (st + 3 < nst) {
+                fetch(raw);
+                look(st + 4);
+            }
+        };
+        if (st >= wst) {  // uniform per wave
+            next();
+            continue;
         }
-        if (st >= wst) continue;  // uniform per wave
         const uint32_t tk = t0 + st * TK;
 #pragma unroll
         for (uint32_t kt = 0; kt < 2; kt++) {
@@ -840,25 +840,27 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
             auto load_v = [&](int s2) __attribute__((always_inline)) {
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
-                    const uint32_t at = slot * STAGE + (32 * kt + 16 * s2) * ROWB;
-                    const tr4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)(vp0[d] + at));
-                    const tr4 y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)(vp1[d] + at));
+                    const uint32_t at = slot * VST + (32 * kt + 16 * s2) * VROW + 64 * d;
+                    const tr4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)(vp + at));
+                    const tr4 y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4 *)(vp + at + 8 * VROW));
                     vf[s2][d] = half8{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
                                       (_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
                 }
             };
             // three runs of products, each group of them (64 cycles) with vector
             // work that does not need it; the order is pinned by the barriers
-            load_v(0);
+            if (kt == 1) next();  // (their loads have had half a stage more)
+            if (!LATE) load_v(0);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
 #pragma unroll
                 for (int p = NP - 1; p >= 0; p--) sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k], qf[p][k], sn, 0, 0, 0);
+                if (LATE && k % 2 && k < KS / 2) load_k(kt == 0 ? slot : (slot + 1) % TS, 1 - kt, KS / 2 + k - 1, KS / 2 + k + 1);
 #pragma unroll
                 for (int i = EARLY * k / KS; i < EARLY * (k + 1) / KS; i++) weights(i);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            load_v(1);
+            load_v(LATE ? 0 : 1);
             load_h(hn, kt == 0 ? slot : (slot + 1) % TS, 1 - kt);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
@@ -869,7 +871,8 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
                 for (int i = EARLY + (PAIRS - EARLY) * d / DT; i < EARLY + (PAIRS - EARLY) * (d + 1) / DT; i++) weights(i);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            load_k((slot + 1) % TS, kt);
+            if (LATE) load_v(1);
+            load_k((slot + 1) % TS, kt, 0, AHEAD);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
 #pragma unroll
@@ -881,7 +884,7 @@ __global__ __launch_bounds__(64 * NW, NP == 2 && HD == 128 && NW == 4 ? 1 : 2) v
             if (kt == 0 || st + 1 < wst) {  // (after the wave's last tokens the products are of nothing)
                 const uint32_t tn = tk + 32 * (kt + 1);
                 if (tn + 32 > every || !hn.ok) {
-                    mask(tn, sn, hn, kt == 0 ? slot : (slot + 1) % TS, 1 - kt);
+                    mask(tn, sn, kt == 0 ? slot : (slot + 1) % TS, 1 - kt);
                     mx = largest(sn, hn);
                 }
                 refer(mx);
