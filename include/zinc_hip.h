@@ -396,8 +396,8 @@ typedef struct zh_attn_rows {
  * ZH_ERR_INVALID_ARGUMENT. A row of a sequence without tokens is zero. What a row
  * may not see does not enter its result, whatever the cache holds there (NaN codes
  * of tokens of the same call excepted). ZH_F32: q and the probabilities in two fp16 pieces each
- * (22 bits); ZH_F16: the probabilities in two, those of many rows (more than 32
- * of a sequence and kv head) in one; sums and softmax in 32 bits. Allocates
+ * (22 bits); ZH_F16: the probabilities in two, or in one in a call of many rows
+ * (max_rows of more than 128 query rows of a kv head); sums and softmax in 32 bits. Allocates
  * nothing and adds in a fixed order; calls that may overlap (other contexts,
  * replayed graphs) need a ws each. attn_scale finite. */
 int zh_flash_attn_kv8(zh_ctx *ctx, const zh_kv8_batch *kv, const zh_attn_rows *rows);

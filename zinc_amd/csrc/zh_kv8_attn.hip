@@ -33,31 +33,43 @@ struct Kv8Attn {
     uint32_t *err;
     uint32_t n_seq, stride, cache_tokens, nh, nkv, G, n_rows, max_rows, max_len;
     uint32_t few;             // rows of a sequence and kv head that are streamed; more go through LDS tiles
-    uint32_t groups, least;   // streaming workgroups of a kv head, units of each at least (0: one takes one sequence)
+    uint32_t rt, tiles;       // rows of a streamed tile, tiles of a sequence at most
+    uint32_t groups, least;   // streaming workgroups of a kv head, units of each at least (0: one takes one tile)
     float *tpart, *tstat;     // parts of LDS tiles
-    uint32_t items, tparts;   // LDS tiles of a kv head (as many at most), parts of each one's tokens
+    uint32_t tslots;          // workgroups that a kv head's LDS tiles are dealt out to (0: one a tile)
     float scale;              // |attn_scale| log2 e = scale * 2^scale_exp, with attn_scale's sign
     int32_t scale_exp;
 };
 
+// A uniform value, which the compiler does not take for one behind a division.
+ZH_DEV uint32_t scalar(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// A value that the compiler knows nothing of, so that it stays the one base of addresses.
+ZH_DEV uint32_t opaque(uint32_t v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 // A sequence's rows: [row, row + n), row i over the tokens below lim(i).
 struct AttnSeq {
-    uint32_t row, n, all, len, cut;  // all: rows before the cut at max_rows; len, cut at `cut`
+    uint32_t s, row, n, all, len, cut;  // all: rows before the cut at max_rows; len, cut at `cut`
     ZH_DEVM uint32_t lim(uint32_t i) const {
-        const uint64_t e = (uint64_t)len + i + 1;
-        return e > all ? (uint32_t)min(e - all, (uint64_t)cut) : 0u;
+        const uint32_t after = all - 1 - i;
+        return len > after ? min(len - after, cut) : 0u;
     }
 };
 ZH_DEV AttnSeq attn_seq(const Kv8Attn &a, uint32_t s, bool &bad) {
     AttnSeq x;
     uint32_t first = s, end = min(s + 1, a.n_rows);
-    if (a.row_start) {
-        first = a.row_start[s];
-        end = a.row_start[s + 1];
+    const const_u32 *row_start = (const const_u32 *)a.row_start, *lens = (const const_u32 *)a.seq_lens;
+    if (row_start) {
+        first = row_start[s];
+        end = row_start[s + 1];
         if (first > end || end > a.n_rows) bad = true;
         end = min(end, a.n_rows);
     }
-    x.len = a.seq_lens[s];
+    x.s = s;
+    x.len = lens[s];
     x.row = first;
     x.all = end > first ? end - first : 0u;
     x.n = min(x.all, a.max_rows);
@@ -129,6 +141,11 @@ ZH_DEV void pair2(uint32_t a, uint32_t b, int n, half2v &x, half2v &y) {
     }
 }
 
+// (a load that goes by the L2s, where no other workgroup reads the same)
+template <bool ONCE, typename V>
+ZH_DEV V ld_once(const V *p) {
+    return ONCE ? __builtin_nontemporal_load(p) : *p;
+}
 ZH_DEV void ld8(const float *p, float (&v)[8]) {
     const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 4);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
@@ -146,13 +163,22 @@ ZH_DEV void st_out(const Kv8Attn &a, uint32_t row, uint32_t h, uint32_t d, uint3
     else *(half4 *)op = half4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
 }
 
-// The units of tokens that sequence s has for the streaming workgroups (one at
-// least, for rows without tokens).
-ZH_DEV uint32_t units_of(const Kv8Attn &a, uint32_t s, bool &bad) {
+// What sequence s has for the streaming workgroups: row tiles, and units of tokens of
+// each (one at least, for rows without tokens).
+struct UnitSeq {
+    uint32_t tiles, units;
+};
+ZH_DEV UnitSeq unit_seq(const Kv8Attn &a, uint32_t s, bool &bad) {
     const AttnSeq x = attn_seq(a, s, bad);
     const uint64_t n = (uint64_t)x.n * a.G;
-    return n && n <= a.few ? max((x.lim(x.n - 1) + CUT - 1) / CUT, 1u) : 0u;
+    UnitSeq u = {0, 1};
+    if (n && n <= a.few) {
+        u.tiles = ((uint32_t)n + a.rt - 1) / a.rt;
+        u.units = max((x.lim(x.n - 1) + CUT - 1) / CUT, 1u);
+    }
+    return u;
 }
+
 // How the units of the streamed sequences are dealt out to the workgroups of a kv
 // head. Shares of q units, whatever sequences they are of, so that ragged lengths even
 // out; or, where no more workgroups than there are take parts of at most q units that
@@ -162,22 +188,29 @@ ZH_DEV uint32_t units_of(const Kv8Attn &a, uint32_t s, bool &bad) {
 struct Share {
     uint32_t q, total;
     bool parts;
-    // the workgroups (parts) or units of a sequence of so many units
-    ZH_DEVM uint32_t items(uint32_t units) const { return parts ? (units + q - 1) / q : units; }
+    // the workgroups (parts) or units of a sequence
+    ZH_DEVM uint32_t items(const UnitSeq &u) const { return u.tiles * (parts ? (u.units + q - 1) / q : u.units); }
 };
-// u0: the lane's sequence's units (of the first 64)
-ZH_DEV Share share(const Kv8Attn &a, uint32_t u0, bool &bad) {
+// u0: the lane's sequence (of the first 64)
+ZH_DEV Share share(const Kv8Attn &a, const UnitSeq &u0, bool &bad) {
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t n = u0;
-    for (uint32_t s = lane + 64; s < a.n_seq; s += 64) n += units_of(a, s, bad);
+    uint32_t n = u0.tiles * u0.units;
+    for (uint32_t s = lane + 64; s < a.n_seq; s += 64) {
+        const UnitSeq u = unit_seq(a, s, bad);
+        n += u.tiles * u.units;
+    }
     Share x;
     x.total = wave_total(n);
     x.q = max((x.total + a.groups - 1) / a.groups, a.least);
     x.parts = true;
     n = x.items(u0);
-    for (uint32_t s = lane + 64; s < a.n_seq; s += 64) n += x.items(units_of(a, s, bad));
+    for (uint32_t s = lane + 64; s < a.n_seq; s += 64) n += x.items(unit_seq(a, s, bad));
     x.parts = wave_total(n) <= a.groups;
     return x;
+}
+ZH_DEV UnitSeq first_units(const Kv8Attn &a, bool &bad) {
+    const uint32_t lane = threadIdx.x & 63;
+    return lane < a.n_seq ? unit_seq(a, lane, bad) : UnitSeq{0, 1};
 }
 
 // A share of units of one kv head: in each sequence that it reaches into, up to 16 RT
@@ -206,333 +239,359 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
     __shared__ __align__(16) float so[W * 16 * LD];
     __shared__ float sm[W * 16], sl[W * 16];
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const uint32_t li = lane % 16, lg = lane / 16;
+    const uint32_t li = lane % 16, lg = lane / 16, koff = li * HD + 16 * lg, voff = 4 * lg * HD + ND * li;
     // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
     const uint32_t kvh = blockIdx.x % a.nkv, group = blockIdx.x / a.nkv;
-    uint32_t s = group, unit = 0, left = ~0u;  // the sequence, the unit in it, units to take from there
+    // the sequence and row tile, the unit in it, units to take from there
+    uint32_t s = group / a.tiles, tile = group % a.tiles, unit = 0, left = ~0u;
     bool bad = false;
     if (a.least) {
-        const uint32_t u0 = lane < a.n_seq ? units_of(a, lane, bad) : 0u;
+        const UnitSeq u0 = first_units(a, bad);
         const Share x = share(a, u0, bad);
         if (__builtin_amdgcn_ballot_w64(bad) && blockIdx.x == 0 && tid == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
-        auto count = [&](uint32_t i) { return x.items(i < 64 ? u0 : units_of(a, i, bad)); };
-        if (!kv8_find(a.n_seq, x.parts ? group : group * x.q, count, s, unit)) return;
+        auto count = [&](uint32_t i) { return x.items(i < 64 ? u0 : unit_seq(a, i, bad)); };
+        uint32_t item;
+        if (!kv8_find(a.n_seq, x.parts ? group : group * x.q, count, s, item)) return;
+        const UnitSeq u = unit_seq(a, s, bad);
+        const uint32_t p = x.parts ? (u.units + x.q - 1) / x.q : u.units;
+        tile = item / p;
+        unit = item % p;
         left = x.q;
         if (x.parts) {  // (all of a length)
-            const uint32_t n = s < 64 ? __builtin_amdgcn_readlane(u0, s) : units_of(a, s, bad), p = x.items(n), c = (n + p - 1) / p;
+            const uint32_t c = (u.units + p - 1) / p;
             unit *= c;
-            left = n > unit ? min(c, n - unit) : 0u;
+            left = u.units > unit ? min(c, u.units - unit) : 0u;
         }
     } else {
-        units_of(a, s, bad);
-        if (bad && kvh == 0 && tid == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+        attn_seq(a, s, bad);
+        if (bad && kvh == 0 && tile == 0 && tid == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
     }
-    for (; left && s < a.n_seq; s++) {
-    bad = false;
-    const AttnSeq seq = attn_seq(a, s, bad);
-    bad = false;
-    const uint32_t nrow = seq.n * a.G;
-    if (nrow == 0 || nrow > a.few) {
-        if (!a.least) return;
-        continue;
-    }
-    // the tokens that some row sees, and those that every row sees
-    const uint32_t end = seq.lim(seq.n - 1), every = seq.lim(0), units = max((end + CUT - 1) / CUT, 1u);
-    const uint32_t take = min(left, units - unit), t0 = unit * CUT, t1 = min(t0 + take * CUT, end);
-    const bool direct = take == units;
-    const uint32_t slot = unit ? 0u : 1u;
-    left = a.least ? left - take : 0u;
-    unit = 0;
-    const uint32_t nstep = t1 > t0 ? (t1 - t0 + KB - 1) / KB : 0u;
-    const uint8_t *kh = a.kc + (size_t)kvh * a.cache_tokens * HD, *vh = a.vc + (size_t)kvh * a.cache_tokens * HD;
-    const const_u32 *tab = (const const_u32 *)(a.tables + (size_t)s * a.stride);
-    const const_u32 *ksc = (const const_u32 *)(a.ks + kvh), *vsc = (const const_u32 *)(a.vs + kvh);
-    // a step's pages (clamped to the last of the part), looked up a step ahead by
-    // scalar loads, whose wait does not wait for K and V
-    struct Step {
-        uint32_t tk, pg[NJ];
+    // (made scalars before the loop, or, with 32 rows, in it: the other way round 16 rows
+    // of f32 spill 5 registers, 32 spill 14, and 48 ragged sequences take 56 us for 46.5)
+    auto scalars = [&]() __attribute__((always_inline)) {
+        s = scalar(s);
+        tile = RT == 1 ? 0u : scalar(tile);  // (16 rows: one tile)
+        unit = scalar(unit);
+        left = scalar(left);
     };
-    auto step = [&](uint32_t st) __attribute__((always_inline)) {
-        Step x;
-        x.tk = t0 + st * KB;
-#pragma unroll
-        for (uint32_t j = 0; j < NJ; j++) {
-            x.pg[j] = tab[min(x.tk / 16 + j, (t1 - 1) / 16)];
-            if (x.pg[j] >= a.cache_tokens / 16) {
-                bad = true;
-                x.pg[j] = 0;
-            }
+    if (RT == 1) scalars();
+    while (true) {
+        if (RT > 1) scalars();
+        if (!left || s >= a.n_seq) break;
+        bad = false;
+        const AttnSeq seq = attn_seq(a, s, bad);
+        bad = false;
+        const uint32_t all_rows = seq.n * a.G, row0 = RT == 1 ? 0u : tile * ROWS;
+        if (row0 >= all_rows || all_rows > a.few) {  // (none, or no streamed ones)
+            if (!a.least) return;
+            s++;
+            continue;
         }
-        return x;
-    };
-    u32x4 kr[NJ][U];
-    uint32_t vr[NJ][4][VD];
-    auto load_k = [&](const Step &x) __attribute__((always_inline)) {
-#pragma unroll
-        for (uint32_t j = 0; j < NJ; j++) {
-            const uint8_t *p = kh + ((size_t)x.pg[j] * 16 + li) * HD + 16 * lg;
-#pragma unroll
-            for (int u = 0; u < U; u++) kr[j][u] = __builtin_nontemporal_load((const u32x4 *)(p + 64 * u));
-        }
-    };
-    auto load_v = [&](const Step &x) __attribute__((always_inline)) {
-#pragma unroll
-        for (uint32_t j = 0; j < NJ; j++) {
-            const uint8_t *p = vh + ((size_t)x.pg[j] * 16 + 4 * lg) * HD + ND * li;
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                if (VD == 2) *(u32x2 *)vr[j][r] = __builtin_nontemporal_load((const u32x2 *)(p + r * HD));
-                else vr[j][r][0] = __builtin_nontemporal_load((const uint32_t *)(p + r * HD));
-            }
-        }
-    };
-    uint32_t ksb[NJ], vsb[NJ];  // this step's scales
-    auto load_s = [&](const Step &x) __attribute__((always_inline)) {
-#pragma unroll
-        for (uint32_t j = 0; j < NJ; j++) {
-            ksb[j] = ksc[(size_t)x.pg[j] * a.nkv];
-            vsb[j] = vsc[(size_t)x.pg[j] * a.nkv];
-        }
-    };
-    Step x = {}, nx = {};
-    if (wave < nstep) {
-        x = step(wave);
-        load_k(x);
-        load_v(x);
-        load_s(x);
-        if (wave + W < nstep) nx = step(wave + W);
-    }
-    // the rows' q as operand fragments: dims 64 u + 16 lg + 8 h .. (the scale's sign in them)
-    half8 qf[RT][NQ][2 * U];
-    float cf[RT];  // products to base-2 scores, but for the block's scale
-    uint32_t lim[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const uint32_t r = min(16 * rt + li, nrow - 1), i = r / a.G;
-        lim[rt] = min(seq.lim(i), t1);
-        const T *qp = (const T *)(a.q + (uint64_t)(seq.row + i) * a.q_row) + (size_t)(kvh * a.G + r % a.G) * HD + 16 * lg;
-        float v[2 * U][8], mx = 0.f;
-#pragma unroll
-        for (int k = 0; k < 2 * U; k++) {
-            ld8(qp + 64 * (k / 2) + 8 * (k % 2), v[k]);
-#pragma unroll
-            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k][e]));
-        }
-        int e = 0;  // q is scaled by 2^-e
-        if (NQ > 1) {
-            mx = xor32_max(xor16_max(mx));
-            const uint32_t E = __float_as_uint(mx) >> 23;
-            if (E < 255) e = (int)E - 141;  // (E == 0, subnormal or zero rows: a smaller maximum)
-        }
-        const float sign = copysignf(1.f, a.scale);
-#pragma unroll
-        for (int k = 0; k < 2 * U; k++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float y = (NQ > 1 ? ldexpf(v[k][i], -e) : v[k][i]) * sign;
-#pragma unroll
-                for (int p = 0; p < NQ; p++) {
-                    qf[rt][p][k][i] = (_Float16)y;
-                    y -= (float)qf[rt][p][k][i];
-                }
-            }
-        cf[rt] = fabsf(ldexpf(a.scale, a.scale_exp + e));
-    }
-    floatx4 o[RT][ND];
-    float m[RT], l[RT];  // the row's reference (every lg alike), this lane's share of its sum
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        m[rt] = -INFINITY;
-        l[rt] = 0.f;
-#pragma unroll
-        for (int n = 0; n < ND; n++) o[rt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
-    // the weights and products of step x; `more`: the next step's loads on the way.
-    // (The last step is code of its own: a load that may not be there would make
-    // the compiler wait for V before the scores.)
-    auto work = [&](auto more) __attribute__((always_inline)) {
-        Block<F> b[NJ];
-        bool ok = true;
-#pragma unroll
-        for (uint32_t j = 0; j < NJ; j++) {
-            b[j].set(ksb[j], vsb[j]);
-            ok = ok && b[j].ok;
-        }
-        floatx4 d[RT][NJ];
-#pragma unroll
-        for (uint32_t j = 0; j < NJ; j++) {
-            half8 kf[2 * U];
-#pragma unroll
-            for (int k = 0; k < 2 * U; k++)
-                kf[k] = row8<F>(kr[j][k / 2][2 * (k % 2)], kr[j][k / 2][2 * (k % 2) + 1]);
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                d[rt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int p = NQ - 1; p >= 0; p--)
-#pragma unroll
-                    for (int k = 0; k < 2 * U; k++)
-                        d[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], qf[rt][p][k], d[rt][j], 0, 0, 0);
-            }
-        }
-        if constexpr (more) {
-            load_k(nx);
-            load_s(nx);
-        }
-        const bool whole = ok && x.tk + KB <= min(every, t1);
-        half8 pf[RT][PV][NJ / 2];
-        float f[RT];
-        if (!whole) {
-            // V of tokens past the part: zero (0 times what the cache holds there may be NaN)
-#pragma unroll
-            for (uint32_t j = 0; j < NJ; j++)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int y = 0; y < VD; y++) vr[j][r][y] = x.tk + 16 * j + 4 * lg + r >= t1 ? 0u : vr[j][r][y];
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            float sc[NJ][4], mb = -INFINITY;
+        const uint32_t nrow = min(ROWS, all_rows - row0);
+        // the tokens that some row of the sequence sees, of the tile, and those that all of
+        // the tile see
+        const uint32_t far = scalar(seq.lim(seq.n - 1)), end = RT == 1 ? far : scalar(seq.lim((row0 + nrow - 1) / a.G));
+        const uint32_t every = scalar(seq.lim(row0 / a.G));
+        const uint32_t units = max((far + CUT - 1) / CUT, 1u);
+        const uint32_t take = min(left, units - unit), t0 = min(unit * CUT, end), t1 = min(t0 + take * CUT, end);
+        const bool direct = take == units;
+        const uint32_t slot = unit ? 0u : 1u;
+        left = a.least ? left - take : 0u;
+        unit = 0;
+        // (where the next one begins, if there is one)
+        const bool last = RT == 1 || row0 + ROWS >= all_rows;
+        tile = last ? 0u : tile + 1;
+        s += last;
+        const uint32_t nstep = t1 > t0 ? (t1 - t0 + KB - 1) / KB : 0u;
+        const uint8_t *kh = a.kc + (size_t)kvh * a.cache_tokens * HD, *vh = a.vc + (size_t)kvh * a.cache_tokens * HD;
+        const const_u32 *tab = (const const_u32 *)(a.tables + (size_t)seq.s * a.stride);
+        const const_u32 *ksc = (const const_u32 *)(a.ks + kvh), *vsc = (const const_u32 *)(a.vs + kvh);
+        // a step's pages (clamped to the last of the part), looked up a step ahead by
+        // scalar loads, whose wait does not wait for K and V
+        struct Step {
+            uint32_t tk, pg[NJ];
+        };
+        auto step = [&](uint32_t st) __attribute__((always_inline)) {
+            Step x;
+            x.tk = t0 + st * KB;
 #pragma unroll
             for (uint32_t j = 0; j < NJ; j++) {
-                const float ck = score_factor(cf[rt], b[j].ks);
-#pragma unroll
-                for (int r = 0; r < 4; r++) sc[j][r] = fmaf(d[rt][j][r], ck, b[j].lv);
+                x.pg[j] = tab[min(x.tk / 16 + j, (t1 - 1) / 16)];
+                if (x.pg[j] >= a.cache_tokens / 16) {
+                    bad = true;
+                    x.pg[j] = 0;
+                }
             }
+            return x;
+        };
+        u32x4 kr[NJ][U];
+        uint32_t vr[NJ][4][VD];
+        auto load_k = [&](const Step &x) __attribute__((always_inline)) {
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; j++) {
+                const uint8_t *p = kh + (size_t)x.pg[j] * (16 * HD) + koff;
+#pragma unroll
+                for (int u = 0; u < U; u++) kr[j][u] = ld_once<RT == 1>((const u32x4 *)(p + 64 * u));
+            }
+        };
+        auto load_v = [&](const Step &x) __attribute__((always_inline)) {
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; j++) {
+                const uint8_t *p = vh + (size_t)x.pg[j] * (16 * HD) + voff;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    if (VD == 2) *(u32x2 *)vr[j][r] = ld_once<RT == 1>((const u32x2 *)(p + r * HD));
+                    else vr[j][r][0] = ld_once<RT == 1>((const uint32_t *)(p + r * HD));
+                }
+            }
+        };
+        uint32_t ksb[NJ], vsb[NJ];  // this step's scales
+        auto load_s = [&](const Step &x) __attribute__((always_inline)) {
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; j++) {
+                ksb[j] = ksc[(size_t)x.pg[j] * a.nkv];
+                vsb[j] = vsc[(size_t)x.pg[j] * a.nkv];
+            }
+        };
+        Step x = {}, nx = {};
+        if (wave < nstep) {
+            x = step(wave);
+            load_k(x);
+            load_v(x);
+            load_s(x);
+            if (wave + W < nstep) nx = step(wave + W);
+        }
+        // the rows' q as operand fragments: dims 64 u + 16 lg + 8 h .. (the scale's sign in them)
+        half8 qf[RT][NQ][2 * U];
+        float cf[RT];  // products to base-2 scores, but for the block's scale
+        uint32_t lim[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const uint32_t r = row0 + min(16 * rt + li, nrow - 1), i = r / a.G;
+            lim[rt] = min(seq.lim(i), t1);
+            const T *qp = (const T *)(a.q + (uint64_t)(seq.row + i) * a.q_row) + (size_t)(kvh * a.G + r % a.G) * HD + 16 * lg;
+            float v[2 * U][8], mx = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2 * U; k++) {
+                ld8(qp + 64 * (k / 2) + 8 * (k % 2), v[k]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k][e]));
+            }
+            int e = 0;  // q is scaled by 2^-e
+            if (NQ > 1) {
+                mx = xor32_max(xor16_max(mx));
+                const uint32_t E = __float_as_uint(mx) >> 23;
+                if (E < 255) e = (int)E - 141;  // (E == 0, subnormal or zero rows: a smaller maximum)
+            }
+            const float sign = copysignf(1.f, a.scale);
+#pragma unroll
+            for (int k = 0; k < 2 * U; k++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    float y = (NQ > 1 ? ldexpf(v[k][i], -e) : v[k][i]) * sign;
+#pragma unroll
+                    for (int p = 0; p < NQ; p++) {
+                        qf[rt][p][k][i] = (_Float16)y;
+                        y -= (float)qf[rt][p][k][i];
+                    }
+                }
+            cf[rt] = fabsf(ldexpf(a.scale, a.scale_exp + e));
+        }
+        floatx4 o[RT][ND];
+        float m[RT], l[RT];  // the row's reference (every lg alike), this lane's share of its sum
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            m[rt] = -INFINITY;
+            l[rt] = 0.f;
+#pragma unroll
+            for (int n = 0; n < ND; n++) o[rt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+        // the weights and products of step x; `more`: the next step's loads on the way.
+        // (The last step is code of its own: a load that may not be there would make
+        // the compiler wait for V before the scores.)
+        auto work = [&](auto more) __attribute__((always_inline)) {
+            Block<F> b[NJ];
+            bool ok = true;
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; j++) {
+                b[j].set(scalar(ksb[j]), scalar(vsb[j]));
+                ok = ok && b[j].ok;
+            }
+            floatx4 d[RT][NJ];
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; j++) {
+                half8 kf[2 * U];
+#pragma unroll
+                for (int k = 0; k < 2 * U; k++)
+                    kf[k] = row8<F>(kr[j][k / 2][2 * (k % 2)], kr[j][k / 2][2 * (k % 2) + 1]);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    d[rt][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int p = NQ - 1; p >= 0; p--)
+#pragma unroll
+                        for (int k = 0; k < 2 * U; k++)
+                            d[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], qf[rt][p][k], d[rt][j], 0, 0, 0);
+                }
+            }
+            if constexpr (more) {
+                load_k(nx);
+                load_s(nx);
+            }
+            const bool whole = ok && x.tk + KB <= min(every, t1);
+            half8 pf[RT][PV][NJ / 2];
+            float f[RT];
             if (!whole) {
+                // V of tokens past the part: zero (0 times what the cache holds there may be NaN)
+#pragma unroll
+                for (uint32_t j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int y = 0; y < VD; y++) vr[j][r][y] = x.tk + 16 * j + 4 * lg + r >= t1 ? 0u : vr[j][r][y];
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                float sc[NJ][4], mb = -INFINITY;
+#pragma unroll
+                for (uint32_t j = 0; j < NJ; j++) {
+                    const float ck = score_factor(cf[rt], b[j].ks);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) sc[j][r] = fmaf(d[rt][j][r], ck, b[j].lv);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (uint32_t j = 0; j < NJ; j++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const bool out = x.tk + 16 * j + 4 * lg + r >= lim[rt];
+                            sc[j][r] = out ? -INFINITY : b[j].ok ? sc[j][r] : NAN;
+                        }
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) mb = fmaxf(mb, sc[j][r]);
+                mb = xor32_max(xor16_max(mb));
+                // (the largest weight is 2^14: what fp16's subnormals lose of the others is 2^-39 of it)
+                const float mn = fmaxf(m[rt], mb - 14.f), ms = mn == -INFINITY ? 0.f : mn;
+                f[rt] = __builtin_amdgcn_exp2f(m[rt] - ms);  // (m = -inf: 0)
+                m[rt] = mn;
+                float ls = 0.f;
 #pragma unroll
                 for (uint32_t j = 0; j < NJ; j++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const bool out = x.tk + 16 * j + 4 * lg + r >= lim[rt];
-                        sc[j][r] = out ? -INFINITY : b[j].ok ? sc[j][r] : NAN;
+                        float p = __builtin_amdgcn_exp2f(sc[j][r] - ms);
+                        ls = fmaf(p, b[j].iv, ls);
+#pragma unroll
+                        for (int k = 0; k < PV; k++) {
+                            pf[rt][k][j / 2][4 * (j % 2) + r] = (_Float16)p;
+                            p -= (float)pf[rt][k][j / 2][4 * (j % 2) + r];
+                        }
                     }
+                l[rt] = fmaf(l[rt], f[rt], ls);
+            }
+            if (F == ZH_I8) {
+#pragma unroll
+                for (uint32_t j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int y = 0; y < VD; y++) vr[j][r][y] ^= 0x80808080u;
             }
 #pragma unroll
-            for (uint32_t j = 0; j < NJ; j++)
+            for (int n = 0; n < ND; n += 2) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) mb = fmaxf(mb, sc[j][r]);
-            mb = xor32_max(xor16_max(mb));
-            // (the largest weight is 2^14: what fp16's subnormals lose of the others is 2^-39 of it)
-            const float mn = fmaxf(m[rt], mb - 14.f), ms = mn == -INFINITY ? 0.f : mn;
-            f[rt] = __builtin_amdgcn_exp2f(m[rt] - ms);  // (m = -inf: 0)
-            m[rt] = mn;
-            float ls = 0.f;
+                for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-            for (uint32_t j = 0; j < NJ; j++)
+                    for (int r = 0; r < 4; r++) {
+                        o[rt][n][r] *= f[rt];
+                        o[rt][n + 1][r] *= f[rt];
+                    }
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float p = __builtin_amdgcn_exp2f(sc[j][r] - ms);
-                    ls = fmaf(p, b[j].iv, ls);
+                for (uint32_t jj = 0; jj < NJ / 2; jj++) {
+                    half2v e[2][4];  // dims n and n + 1: token pairs of the two pages
 #pragma unroll
-                    for (int k = 0; k < PV; k++) {
-                        pf[rt][k][j / 2][4 * (j % 2) + r] = (_Float16)p;
-                        p -= (float)pf[rt][k][j / 2][4 * (j % 2) + r];
+                    for (int i = 0; i < 4; i++)
+                        pair2<F>(vr[2 * jj + i / 2][2 * (i % 2)][n / 4], vr[2 * jj + i / 2][2 * (i % 2) + 1][n / 4], n, e[0][i],
+                                 e[1][i]);
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        const half8 vf = {e[y][0].x, e[y][0].y, e[y][1].x, e[y][1].y, e[y][2].x, e[y][2].y, e[y][3].x, e[y][3].y};
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                            for (int p = PV - 1; p >= 0; p--)
+                                o[rt][n + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][p][jj], o[rt][n + y], 0, 0, 0);
                     }
                 }
-            l[rt] = fmaf(l[rt], f[rt], ls);
-        }
-        if (F == ZH_I8) {
-#pragma unroll
-            for (uint32_t j = 0; j < NJ; j++)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int y = 0; y < VD; y++) vr[j][r][y] ^= 0x80808080u;
-        }
-#pragma unroll
-        for (int n = 0; n < ND; n += 2) {
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    o[rt][n][r] *= f[rt];
-                    o[rt][n + 1][r] *= f[rt];
-                }
-#pragma unroll
-            for (uint32_t jj = 0; jj < NJ / 2; jj++) {
-                half2v e[2][4];  // dims n and n + 1: token pairs of the two pages
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    pair2<F>(vr[2 * jj + i / 2][2 * (i % 2)][n / 4], vr[2 * jj + i / 2][2 * (i % 2) + 1][n / 4], n, e[0][i],
-                             e[1][i]);
-#pragma unroll
-                for (int y = 0; y < 2; y++) {
-                    const half8 vf = {e[y][0].x, e[y][0].y, e[y][1].x, e[y][1].y, e[y][2].x, e[y][2].y, e[y][3].x, e[y][3].y};
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                        for (int p = PV - 1; p >= 0; p--)
-                            o[rt][n + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][p][jj], o[rt][n + y], 0, 0, 0);
-                }
             }
-        }
-        if constexpr (more) load_v(nx);
-    };
-    if (wave < nstep) {
-        for (uint32_t st = wave + W; st < nstep; st += W) {
-            const Step nn = st + W < nstep ? step(st + W) : nx;
-            work(std::true_type{});
-            x = nx;
-            nx = nn;
-        }
-        work(std::false_type{});
-    }
-    if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
-    // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
-    const size_t p0 = ((size_t)blockIdx.x * 2 + slot) * ROWS;
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        __syncthreads();  // (the words below have been read)
-        const float ls = xor32_sum(xor16_sum(l[rt]));
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-            for (int n = 0; n < ND; n += 4)
-                *(f32x4 *)(so + (wave * 16 + li) * LD + ND * (4 * lg + r) + n) =
-                    f32x4{o[rt][n][r], o[rt][n + 1][r], o[rt][n + 2][r], o[rt][n + 3][r]};
-        if (lg == 0) {
-            sm[wave * 16 + li] = m[rt];
-            sl[wave * 16 + li] = ls;
-        }
-        __syncthreads();
-        for (uint32_t i = tid; i < 16 * (HD / 4); i += 64 * W) {
-            const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
-            if (16 * rt + r >= nrow) break;
-            const uint32_t R = 16 * rt + r, qi = R / a.G, h = kvh * a.G + R % a.G;
-            float M = sm[r], L = 0.f;
-            f32x4 O = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 1; k < W; k++) M = fmaxf(M, sm[k * 16 + r]);
-            const float Ms = M == -INFINITY ? 0.f : M;
-#pragma unroll
-            for (int k = 0; k < W; k++) {
-                const float fk = __builtin_amdgcn_exp2f(sm[k * 16 + r] - Ms);
-                const f32x4 v = *(const f32x4 *)(so + (k * 16 + r) * LD + d);
-                O.x = fmaf(v.x, fk, O.x);
-                O.y = fmaf(v.y, fk, O.y);
-                O.z = fmaf(v.z, fk, O.z);
-                O.w = fmaf(v.w, fk, O.w);
-                L = fmaf(sl[k * 16 + r], fk, L);
+            if constexpr (more) load_v(nx);
+        };
+        if (wave < nstep) {
+            for (uint32_t st = wave + W; st < nstep; st += W) {
+                const Step nn = st + W < nstep ? step(st + W) : nx;
+                work(std::true_type{});
+                x = nx;
+                nx = nn;
             }
-            if (direct) {
-                const f32x4 v = seq.lim(qi) ? f32x4{O.x / L, O.y / L, O.z / L, O.w / L} : f32x4{0.f, 0.f, 0.f, 0.f};
-                st_out<T>(a, seq.row + qi, h, d, HD, v);
-            } else {
-                const size_t pr = p0 + 16 * rt + r;
-                *(f32x4 *)(a.part + pr * HD + d) = O;
-                if (d == 0) {
-                    a.stat[2 * pr] = M;
-                    a.stat[2 * pr + 1] = L;
+            work(std::false_type{});
+        }
+        if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+        // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
+        const size_t p0 = ((size_t)blockIdx.x * 2 + slot) * ROWS;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            __syncthreads();  // (the words below have been read)
+            const float ls = xor32_sum(xor16_sum(l[rt]));
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int n = 0; n < ND; n += 4)
+                    *(f32x4 *)(so + (wave * 16 + li) * LD + ND * (4 * lg + r) + n) =
+                        f32x4{o[rt][n][r], o[rt][n + 1][r], o[rt][n + 2][r], o[rt][n + 3][r]};
+            if (lg == 0) {
+                sm[wave * 16 + li] = m[rt];
+                sl[wave * 16 + li] = ls;
+            }
+            __syncthreads();
+            for (uint32_t i = tid; i < 16 * (HD / 4); i += 64 * W) {
+                const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
+                if (16 * rt + r >= nrow) break;
+                const uint32_t R = row0 + 16 * rt + r, qi = R / a.G, h = kvh * a.G + R % a.G;
+                float M = sm[r], L = 0.f;
+                f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 1; k < W; k++) M = fmaxf(M, sm[k * 16 + r]);
+                const float Ms = M == -INFINITY ? 0.f : M;
+#pragma unroll
+                for (int k = 0; k < W; k++) {
+                    const float fk = __builtin_amdgcn_exp2f(sm[k * 16 + r] - Ms);
+                    const f32x4 v = *(const f32x4 *)(so + (k * 16 + r) * LD + d);
+                    O.x = fmaf(v.x, fk, O.x);
+                    O.y = fmaf(v.y, fk, O.y);
+                    O.z = fmaf(v.z, fk, O.z);
+                    O.w = fmaf(v.w, fk, O.w);
+                    L = fmaf(sl[k * 16 + r], fk, L);
+                }
+                if (direct) {
+                    const f32x4 v = seq.lim(qi) ? f32x4{O.x / L, O.y / L, O.z / L, O.w / L} : f32x4{0.f, 0.f, 0.f, 0.f};
+                    st_out<T>(a, seq.row + qi, h, d, HD, v);
+                } else {
+                    const size_t pr = p0 + 16 * rt + r;
+                    *(f32x4 *)(a.part + pr * HD + d) = O;
+                    if (d == 0) {
+                        a.stat[2 * pr] = M;
+                        a.stat[2 * pr + 1] = L;
+                    }
                 }
             }
         }
-    }
     }
 }
 
-// Many rows: a workgroup takes NW x 32 of them (rows of a kv head in the order query,
+// Many rows: a workgroup takes 256 of them (rows of a kv head in the order query,
 // head), each wave 32, over K and V that pass through LDS once for all of them, in
 // stages of 64 tokens, as fp16: every thread converts its pieces on the way there, so
 // a code becomes fp16 once a workgroup and not once a wave.
@@ -550,7 +609,9 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
 // are computed. The reference moves only when a score passes it by 2^8 (the weights
 // then reach 2^12 in fp16 at most), so the output is rarely rescaled. A wave stops at
 // the last token that one of its rows sees.
-constexpr uint32_t TK = 64, TS = 3;  // tokens of a stage, stages in LDS
+constexpr int TW = 8;                          // waves of a workgroup
+constexpr uint32_t TILE = 32 * TW;             // its rows
+constexpr uint32_t TK = 64, TS = 3;            // tokens of a stage, stages in LDS
 template <int HD>
 constexpr uint32_t t_krow() { return 2 * HD + 16; }
 template <int HD>
@@ -560,34 +621,83 @@ constexpr uint32_t t_lds() { return TS * TK * (t_krow<HD>() + t_vrow<HD>()) + TS
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// The LDS tile `u` of a kv head: its sequence, and which of the sequence's tiles (the
-// last ones, which see the most tokens, first).
-ZH_DEV bool tile_of(const Kv8Attn &a, uint32_t rows, uint32_t u, uint32_t &s, uint32_t &tile, AttnSeq &seq) {
+// The LDS tiles of sequence s and the stages of its longest one.
+struct TileSeq {
+    uint32_t tiles, stages;
+};
+ZH_DEV TileSeq tile_seq(const Kv8Attn &a, uint32_t rows, uint32_t s) {
     bool bad = false;
+    const AttnSeq x = attn_seq(a, s, bad);
+    const uint64_t n = (uint64_t)x.n * a.G;
+    TileSeq t = {0, 1};
+    if (n > a.few) {
+        t.tiles = (uint32_t)((n + rows - 1) / rows);
+        t.stages = max((x.lim(x.n - 1) + TK - 1) / TK, 1u);
+    }
+    return t;
+}
+// The most stages of a workgroup where tiles are cut: about the least for which no more
+// workgroups than there are take all parts, so that the tiles of a long context are cut
+// into more parts than those of a short one. Every wave by itself. t0: the lane's
+// sequence's tiles (of the first 64).
+ZH_DEV uint32_t tile_share(const Kv8Attn &a, uint32_t rows, const TileSeq &t0) {
+    if (!a.tslots) return 1u << 30;
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t n = t0.tiles * t0.stages;
+    for (uint32_t s = lane + 64; s < a.n_seq; s += 64) {
+        const TileSeq t = tile_seq(a, rows, s);
+        n += t.tiles * t.stages;
+    }
+    uint32_t q = max((wave_total(n) + a.tslots - 1) / a.tslots, 4u);
+    while (q < 1u << 24) {  // (a part a tile always fits)
+        n = t0.tiles * ((t0.stages + q - 1) / q);
+        for (uint32_t s = lane + 64; s < a.n_seq; s += 64) {
+            const TileSeq t = tile_seq(a, rows, s);
+            n += t.tiles * ((t.stages + q - 1) / q);
+        }
+        if (wave_total(n) <= a.tslots) break;
+        q += (q + 7) / 8;
+    }
+    return q;
+}
+// A workgroup's part of a tile.
+struct TileJob {
+    AttnSeq seq;
+    uint32_t tile, part, c;  // parts of c stages
+};
+ZH_DEV TileSeq first_seqs(const Kv8Attn &a, uint32_t rows) {
+    const uint32_t lane = threadIdx.x & 63;
+    return lane < a.n_seq ? tile_seq(a, rows, lane) : TileSeq{0, 1};
+}
+// Workgroup `u` of a kv head: sequences in order, of each the last tiles (which see the
+// most tokens) first, of each tile the parts.
+ZH_DEV bool tile_job(const Kv8Attn &a, uint32_t rows, uint32_t u, TileJob &j) {
+    const TileSeq t0 = first_seqs(a, rows);
+    const uint32_t q = tile_share(a, rows, t0);
     auto count = [&](uint32_t i) {
-        const uint64_t n = (uint64_t)attn_seq(a, i, bad).n * a.G;
-        return n > a.few ? (uint32_t)((n + rows - 1) / rows) : 0u;
+        const TileSeq t = i < 64 ? t0 : tile_seq(a, rows, i);
+        return t.tiles * ((t.stages + q - 1) / q);
     };
-    uint32_t item;
+    uint32_t s, item;
     if (!kv8_find(a.n_seq, u, count, s, item)) return false;
-    seq = attn_seq(a, s, bad);
-    tile = (uint32_t)((uint64_t)seq.n * a.G + rows - 1) / rows - 1 - item;
+    s = scalar(s);
+    bool bad = false;
+    j.seq = attn_seq(a, s, bad);
+    const TileSeq t = tile_seq(a, rows, s);
+    const uint32_t p = (t.stages + q - 1) / q;
+    j.c = scalar((t.stages + p - 1) / p);
+    j.tile = scalar(t.tiles - 1 - item / p);
+    j.part = scalar(item % p);
     return true;
 }
-// The parts of a tile's `end` tokens, of `c` each.
-ZH_DEV uint32_t tile_parts(const Kv8Attn &a, uint32_t end, uint32_t &c) {
-    c = max((end + a.tparts - 1) / a.tparts, 1u);
-    c = (c + TK - 1) / TK * TK;
-    return (end + c - 1) / c;
-}
 
-template <int HD, int NP, int NW, uint32_t F, typename T>
-__global__ __launch_bounds__(64 * NW, HD == 128 && NW == 4 ? 1 : 2) void k_kv8_tile(Kv8Attn a) {
+template <int HD, int NP, uint32_t F, typename T>
+__global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
     constexpr int KS = HD / 16, DT = HD / 32;        // k-steps of the scores, 32-dim tiles of the output
     constexpr uint32_t KROW = t_krow<HD>(), VROW = t_vrow<HD>(), KST = TK * KROW, VST = TK * VROW;  // of a row, a stage
-    constexpr uint32_t ROWS = 32 * NW, NT = 64 * NW;
+    constexpr uint32_t ROWS = TILE, NT = 64 * TW;
     constexpr uint32_t CPR = HD / 16, PC = TK * CPR;  // 16-code pieces of a row and of a stage's K (or V)
-    constexpr uint32_t NPC = 2 * PC / NT, NL = PC > NT ? PC / NT : 1;  // a thread's pieces, rows
+    constexpr uint32_t NPC = 2 * PC / NT;             // a thread's pieces
     extern __shared__ __align__(16) uint8_t lds[];
     typedef __fp16 tr4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) tr4 lds_tr4;
@@ -595,76 +705,69 @@ __global__ __launch_bounds__(64 * NW, HD == 128 && NW == 4 ? 1 : 2) void k_kv8_t
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t i32 = lane % 32, h = lane / 32;
     // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
-    const uint32_t kvh = blockIdx.x % a.nkv, part = blockIdx.x / a.nkv % a.tparts, u = blockIdx.x / a.nkv / a.tparts;
-    uint32_t s, tile;
-    AttnSeq seq;
-    if (!tile_of(a, ROWS, u, s, tile, seq)) return;
-    const uint32_t rows = seq.n * a.G, r0 = tile * ROWS, w0 = r0 + wave * 32;
-    const uint32_t end = seq.lim((min(r0 + ROWS, rows) - 1) / a.G);
-    uint32_t c;
-    const uint32_t parts = tile_parts(a, end, c);
-    if (part && part >= parts) return;  // (rows without tokens: part 0 writes their zeros)
-    const uint32_t t0 = part * c, t1 = min(t0 + c, end), nst = t1 > t0 ? (t1 - t0 + TK - 1) / TK : 0u;
+    const uint32_t kvh = blockIdx.x % a.nkv;
+    if (!a.few && blockIdx.x == 0) {  // (no streamed rows: their launch would report these)
+        bool wrong = false;
+        for (uint32_t i = tid; i < a.n_seq; i += NT) attn_seq(a, i, wrong);
+        if (wrong) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+    }
+    TileJob job;
+    if (!tile_job(a, ROWS, blockIdx.x / a.nkv, job)) return;
+    const AttnSeq &seq = job.seq;
+    const uint32_t rows = seq.n * a.G, r0 = job.tile * ROWS, w0 = r0 + wave * 32;
+    const uint32_t end = scalar(seq.lim((min(r0 + ROWS, rows) - 1) / a.G)), t0 = job.part * job.c * TK;
+    if (job.part && t0 >= end) return;  // (rows without tokens: part 0 writes their zeros)
+    const uint32_t t1 = min(t0 + job.c * TK, end), nst = t1 > t0 ? (t1 - t0 + TK - 1) / TK : 0u;
     // the wave's rows: the stages that it takes, the tokens that all of them see
     const bool mine = w0 < rows;
-    const uint32_t wend = mine ? min(seq.lim((min(w0 + 32, rows) - 1) / a.G), t1) : 0u;
-    const uint32_t wst = wend > t0 ? (wend - t0 + TK - 1) / TK : 0u, every = mine ? min(seq.lim(w0 / a.G), t1) : 0u;
+    const uint32_t wend = mine ? min(scalar(seq.lim((min(w0 + 32, rows) - 1) / a.G)), t1) : 0u;
+    const uint32_t wst = wend > t0 ? (wend - t0 + TK - 1) / TK : 0u, every = mine ? min(scalar(seq.lim(w0 / a.G)), t1) : 0u;
     const uint32_t row = min(w0 + i32, rows - 1), qi = row / a.G, lim = min(seq.lim(qi), t1);
-    // ---- a thread's pieces of a stage: 16 codes of a token each
+    // ---- a thread's pieces of a stage: 16 codes of a token each, of K or V (HD 64) or of both
     const uint8_t *kh = a.kc + (size_t)kvh * a.cache_tokens * HD, *vh = a.vc + (size_t)kvh * a.cache_tokens * HD;
-    const uint32_t *tab = a.tables + (size_t)s * a.stride;
+    const uint32_t *tab = a.tables + (size_t)seq.s * a.stride;
     bool bad = false;
-    auto trow = [&](uint32_t i) { return (i * NT + tid) % PC / CPR; };  // piece i's token of the stage
-    const uint32_t col = tid % CPR;
-    const bool kfirst = PC >= NT || tid < PC;  // piece 0 is one of K
+    const uint32_t trow = tid % PC / CPR, col = tid % CPR;  // the token of the stage, 16 dims of it
+    const bool isk = NPC == 2 || tid < PC, scales = isk && col == 0 && trow % 16 == 0;
+    // (one address of each kind in a register: the ring's other slots lie at immediate
+    // offsets from it, which reach 64 KiB)
+    const uint32_t kput = opaque(isk ? trow * KROW + col * 32 : TS * KST + trow * VROW + col * 32);
+    const uint32_t vput = opaque(TS * KST + trow * VROW + col * 32), sput = opaque(TS * (KST + VST) + trow);
     struct Raw {
         u32x4 x[NPC];
-        uint32_t k[NL], v[NL];  // scales (of the threads that have a page's first piece of K)
+        uint32_t k, v;  // scales (of the threads that have a page's first piece of K)
     };
-    uint32_t pg[NL];
-    auto look = [&](uint32_t st) __attribute__((always_inline)) {
-#pragma unroll
-        for (uint32_t i = 0; i < NL; i++) pg[i] = tab[min((t0 + st * TK + trow(i)) / 16, (t1 - 1) / 16)];
-    };
+    uint32_t pg;
+    auto look = [&](uint32_t st) __attribute__((always_inline)) { pg = tab[min((t0 + st * TK + trow) / 16, (t1 - 1) / 16)]; };
     auto fetch = [&](Raw &r) __attribute__((always_inline)) {
-#pragma unroll
-        for (uint32_t i = 0; i < NL; i++)
-            if (pg[i] >= a.cache_tokens / 16) {
-                bad = true;
-                pg[i] = 0;
-            }
-#pragma unroll
-        for (uint32_t i = 0; i < NPC; i++) {
-            const uint8_t *base = (PC >= NT ? i < PC / NT : kfirst) ? kh : vh;
-            r.x[i] = *(const u32x4 *)(base + ((size_t)pg[i % NL] * 16 + trow(i) % 16) * HD + col * 16);
+        if (pg >= a.cache_tokens / 16) {
+            bad = true;
+            pg = 0;
         }
-#pragma unroll
-        for (uint32_t i = 0; i < NL; i++)
-            if (kfirst && col == 0 && trow(i) % 16 == 0) {
-                r.k[i] = ((const uint32_t *)a.ks)[(size_t)pg[i] * a.nkv + kvh];
-                r.v[i] = ((const uint32_t *)a.vs)[(size_t)pg[i] * a.nkv + kvh];
-            }
+        const size_t at = ((size_t)pg * 16 + trow % 16) * HD + col * 16;
+        r.x[0] = *(const u32x4 *)((isk ? kh : vh) + at);
+        if (NPC == 2) r.x[NPC - 1] = *(const u32x4 *)(vh + at);
+        if (scales) {
+            r.k = ((const uint32_t *)a.ks)[(size_t)pg * a.nkv + kvh];
+            r.v = ((const uint32_t *)a.vs)[(size_t)pg * a.nkv + kvh];
+        }
     };
     auto put = [&](uint32_t st, const Raw &r) __attribute__((always_inline)) {
         const uint32_t slot = st % TS;
 #pragma unroll
         for (uint32_t i = 0; i < NPC; i++) {
-            const uint32_t t = trow(i);
-            const bool isk = PC >= NT ? i < PC / NT : kfirst;
             u32x4 x = r.x[i];
             // V past the part: zero (0 times what the cache holds there may be NaN)
-            if (!isk && t0 + st * TK + t >= t1) x = u32x4{0, 0, 0, 0};
-            uint8_t *to = lds + (isk ? slot * KST + t * KROW : TS * KST + slot * VST + t * VROW) + col * 32;
+            if ((NPC == 2 ? i : !isk) && t0 + st * TK + trow >= t1) x = u32x4{0, 0, 0, 0};
+            uint8_t *to = lds + (i ? vput + slot * VST : kput + (isk ? slot * KST : slot * VST));
             *(half8 *)to = row8<F>(x.x, x.y);
             *(half8 *)(to + 16) = row8<F>(x.z, x.w);
         }
-#pragma unroll
-        for (uint32_t i = 0; i < NL; i++)
-            if (kfirst && col == 0 && trow(i) % 16 == 0) {
-                Block<F> b;
-                b.set(r.k[i], r.v[i]);
-                *(f32x4 *)(scl + (slot * 4 + trow(i) / 16) * 4) = f32x4{b.ks, b.lv, b.iv, b.ok ? 1.f : 0.f};
-            }
+        if (scales) {
+            Block<F> b;
+            b.set(r.k, r.v);
+            *(f32x4 *)(lds + sput + slot * 64) = f32x4{b.ks, b.lv, b.iv, b.ok ? 1.f : 0.f};
+        }
     };
     Raw raw;
     if (nst) {
@@ -722,7 +825,7 @@ __global__ __launch_bounds__(64 * NW, HD == 128 && NW == 4 ? 1 : 2) void k_kv8_t
     // 64 d, of tokens 4 h .. +3, and of those 8 on
     const uint32_t l16 = lane % 16;
     const uint8_t *const kp = lds + i32 * KROW + 16 * h;
-    const uint8_t *const vp = lds + TS * KST + (4 * h + l16 / 4) * VROW + 32 * (lane / 16 % 2) + 8 * (l16 % 4);
+    const uint8_t *const vp = lds + opaque(TS * KST + (4 * h + l16 / 4) * VROW + 32 * (lane / 16 % 2) + 8 * (l16 % 4));
     f32x16 sc, sn;  // products of the current and the next 32 tokens
     half8 kf[KS];   // K fragments of the next ones
     struct Half {   // of 32 tokens' two pages: scores' factors, weights' exponents and shares
@@ -732,7 +835,7 @@ __global__ __launch_bounds__(64 * NW, HD == 128 && NW == 4 ? 1 : 2) void k_kv8_t
     Half hc, hn;
     // (two pieces of f32 leave no registers for V beside the scores' products, nor for
     // all of K ahead of them)
-    constexpr bool LATE = NP == 2 && HD == 128 && NW == 8;
+    constexpr bool LATE = NP == 2 && HD == 128;
     constexpr int AHEAD = LATE ? KS / 2 : KS;
     auto load_k = [&](uint32_t slot, uint32_t kt, int k0, int k1) __attribute__((always_inline)) {
 #pragma unroll
@@ -896,7 +999,7 @@ __global__ __launch_bounds__(64 * NW, HD == 128 && NW == 4 ? 1 : 2) void k_kv8_t
     if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
     l = xor32_sum(l);
     if (w0 + i32 >= rows) return;
-    if (parts <= 1) {
+    if (end <= job.c * TK) {  // (one part)
         const bool none = seq.lim(qi) == 0;
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -908,7 +1011,7 @@ __global__ __launch_bounds__(64 * NW, HD == 128 && NW == 4 ? 1 : 2) void k_kv8_t
             }
         return;
     }
-    const size_t pr = (((size_t)u * a.nkv + kvh) * a.tparts + part) * ROWS + (row - r0);
+    const size_t pr = (size_t)blockIdx.x * ROWS + (row - r0);
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -968,105 +1071,129 @@ template <int HD, int RT, typename T>
 __global__ __launch_bounds__(256) void k_kv8_join(Kv8Attn a) {
     constexpr uint32_t N = HD / 4, PER = 256 / N, ROWS = 16 * RT;  // rows of a workgroup, of a tile
     const uint32_t item = blockIdx.x / (ROWS / PER), r = blockIdx.x % (ROWS / PER) * PER + threadIdx.x / N;
-    const uint32_t kvh = item % a.nkv, s = item / a.nkv;
+    const uint32_t kvh = item % a.nkv, tile = item / a.nkv % a.tiles, s = item / a.nkv / a.tiles;
     bool bad = false;
     const uint32_t lane = threadIdx.x & 63;
     const AttnSeq seq = attn_seq(a, s, bad);
-    const uint32_t nrow = seq.n * a.G;
-    if (nrow == 0 || nrow > a.few || r / (64 / N) * (64 / N) >= nrow) return;  // (uniform per wave)
-    const uint32_t u0 = lane < a.n_seq ? units_of(a, lane, bad) : 0u;
+    const uint32_t all_rows = seq.n * a.G, row0 = tile * ROWS;
+    if (row0 >= all_rows || all_rows > a.few) return;
+    const uint32_t nrow = min(ROWS, all_rows - row0);
+    if (r / (64 / N) * (64 / N) >= nrow) return;  // (uniform per wave)
+    const UnitSeq u0 = first_units(a, bad);
     const Share x = share(a, u0, bad);
     uint32_t before = 0;
-    for (uint32_t i = lane; i < s; i += 64) before += x.items(i < 64 ? u0 : units_of(a, i, bad));
-    before = wave_total(before);
-    const uint32_t units = units_of(a, s, bad);
-    uint32_t first = before, parts = x.items(units);
+    for (uint32_t i = lane; i < s; i += 64) before += x.items(i < 64 ? u0 : unit_seq(a, i, bad));
+    const uint32_t units = unit_seq(a, s, bad).units;
+    uint32_t first, parts;
     if (x.parts) {  // (parts of one length: the last ones may be empty)
-        const uint32_t c = (units + parts - 1) / parts;
+        const uint32_t p = (units + x.q - 1) / x.q, c = (units + p - 1) / p;
+        first = wave_total(before) + tile * p;
         parts = (units + c - 1) / c;
     } else {
-        first = before / x.q;
-        parts = (before + units - 1) / x.q - first + 1;
+        const uint32_t u = wave_total(before) + tile * units;
+        first = u / x.q;
+        parts = (u + units - 1) / x.q - first + 1;
     }
     if (parts <= 1) return;
-    const uint32_t R = min(r, nrow - 1), qi = R / a.G, h = kvh * a.G + R % a.G;
+    const uint32_t R = min(r, nrow - 1), qi = (row0 + R) / a.G, h = kvh * a.G + (row0 + R) % a.G;
     // (the first part begins with the sequence, the others in it)
     auto at = [&](uint32_t p) { return ((size_t)((first + p) * a.nkv + kvh) * 2 + (p ? 0u : 1u)) * ROWS + R; };
     const f32x4 v = join_row<HD>(a.part, a.stat, parts, at);
     if (r < nrow) st_out<T>(a, seq.row + qi, h, threadIdx.x % N * 4, HD, seq.lim(qi) ? v : f32x4{0.f, 0.f, 0.f, 0.f});
 }
 
-template <int HD, int NW, typename T>
+template <int HD, typename T>
 __global__ __launch_bounds__(256) void k_kv8_tile_join(Kv8Attn a) {
-    constexpr uint32_t N = HD / 4, PER = 256 / N, ROWS = 32 * NW;
+    constexpr uint32_t N = HD / 4, PER = 256 / N, ROWS = TILE;
     const uint32_t item = blockIdx.x / (ROWS / PER), r = blockIdx.x % (ROWS / PER) * PER + threadIdx.x / N;
-    const uint32_t kvh = item % a.nkv, u = item / a.nkv;
-    uint32_t s, tile;
-    AttnSeq seq;
-    if (!tile_of(a, ROWS, u, s, tile, seq)) return;
-    const uint32_t r0 = tile * ROWS, nrow = min(ROWS, seq.n * a.G - r0);
-    uint32_t c;
-    const uint32_t parts = tile_parts(a, seq.lim((r0 + nrow - 1) / a.G), c);
+    const uint32_t kvh = item % a.nkv, lane = threadIdx.x & 63;
+    const TileSeq t0 = first_seqs(a, ROWS);
+    const uint32_t q = tile_share(a, ROWS, t0);
+    auto get = [&](uint32_t i) { return i < 64 ? t0 : tile_seq(a, ROWS, i); };
+    uint32_t s, at_s, before = 0;
+    if (!kv8_find(a.n_seq, item / a.nkv, [&](uint32_t i) { return get(i).tiles; }, s, at_s)) return;
+    // the workgroups of the sequences before
+    for (uint32_t i = lane; i < s; i += 64) before += get(i).tiles * ((get(i).stages + q - 1) / q);
+    before = wave_total(before);
+    bool bad = false;
+    const AttnSeq seq = attn_seq(a, s, bad);
+    const TileSeq t = tile_seq(a, ROWS, s);
+    const uint32_t p = (t.stages + q - 1) / q, c = (t.stages + p - 1) / p * TK;
+    const uint32_t r0 = (t.tiles - 1 - at_s) * ROWS, nrow = min(ROWS, seq.n * a.G - r0);
+    const uint32_t parts = (seq.lim((r0 + nrow - 1) / a.G) + c - 1) / c;
     if (parts <= 1 || r / (64 / N) * (64 / N) >= nrow) return;  // (uniform per wave)
-    const uint32_t R = r0 + min(r, nrow - 1), qi = R / a.G, h = kvh * a.G + R % a.G;
-    auto at = [&](uint32_t p) { return ((size_t)item * a.tparts + p) * ROWS + (R - r0); };
+    const uint32_t R = r0 + min(r, nrow - 1), qi = R / a.G, h = kvh * a.G + R % a.G, first = before + at_s * p;
+    auto at = [&](uint32_t i) { return ((size_t)(first + i) * a.nkv + kvh) * ROWS + (R - r0); };
     const f32x4 v = join_row<HD>(a.tpart, a.tstat, parts, at);
     if (r < nrow) st_out<T>(a, seq.row + qi, h, threadIdx.x % N * 4, HD, seq.lim(qi) ? v : f32x4{0.f, 0.f, 0.f, 0.f});
 }
 
 // How a call is cut (the same for every call of these sizes).
 struct Kv8Plan {
-    uint32_t rt, few, groups, least;           // streamed
-    uint32_t nw, items, tparts, tblocks;       // LDS tiles (nw 0: none)
+    uint32_t rt, few, tiles, groups, least;    // streamed
+    uint32_t items, tslots;                    // LDS tiles (items 0: none)
     uint64_t stat_off, tpart_off, tstat_off, bytes;  // of ws
 };
 constexpr uint32_t LEAST = 4;    // units of a share at least
-constexpr uint32_t FEW = 32;     // rows that are streamed
+// Rows of a sequence and kv head that are streamed, in tiles of 32 that each read K and V
+// (through the L2s) again, where LDS tiles of 256 rows would be emptier than that costs.
+// us streamed / on LDS tiles, head_dim 128: f16 36 rows of 16 sequences of 2000 tokens 31 /
+// 52, of 40 62 / 154, 128 of 16 45 / 57, of 40 117 / 146, 160 of 16 65 / 62, of 40 139 /
+// 146, 192 of 16 71 / 64; f32 128 of 16 52 / 66, 192 of 16 81 / 82, of 40 of 4000 374 / 400,
+// 256 of 16 98 / 94; one sequence of 30000 tokens f16 128 rows 44 / 46, 256 74 / 55.
+constexpr uint32_t few_rows(bool f32) { return f32 ? 192 : 128; }
+// Sequences from which on the few rows of some are streamed in a launch of their own
+// before the tiles of others; below, they take emptier tiles. us with / without, 512 rows
+// after 2000 tokens and n decode rows at 1000 and at 8000 tokens, f16: n = 0 51 / 47, 4 59
+// and 67 / 53 and 67, 8 70 and 104 / 68 and 103, 15 102 and 127 / 91 and 166
+constexpr uint32_t MIXED = 9;
 constexpr uint32_t TILE_FIX = 5; // a tile launch's start and end, in stages
 
 constexpr uint64_t kv8_one(uint32_t hd) { return hd == 64 ? 768 : 512; }
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t n_rows, uint32_t max_rows, uint32_t max_len,
-              Kv8Plan &p) {
+              bool f32, Kv8Plan &p) {
     const uint64_t G = nh / kv->n_kv_heads, rows = max_rows * G, nkv = kv->n_kv_heads, hd = kv->head_dim;
     p = {};
     if (n_rows * G >= 1ull << 31) return false;
     p.rt = rows <= 16 ? 1 : 2;
-    p.few = 16 * p.rt;
-    const uint64_t jobs = kv->n_seq * nkv, slots = (p.rt == 1 ? 3ull : 2ull) * cus;
+    p.few = rows <= few_rows(f32) ? (uint32_t)rows : kv->n_seq < MIXED ? 0 : few_rows(f32);
+    p.tiles = ceil_div(p.few, 16 * p.rt);
+    const uint64_t jobs = kv->n_seq * nkv * p.tiles, slots = (p.rt == 1 ? 3ull : 2ull) * cus;
     // one workgroup a sequence: few short ones, or so many that they even out by themselves
     const bool whole = (jobs <= cus && max_len <= kv8_one(hd) + kv8_one(hd) * jobs / cus) || jobs >= 8 * slots;
     p.least = whole ? 0 : LEAST;
-    const uint64_t units = kv->n_seq * (uint64_t)ceil_div(max_len, CUT);
-    p.groups = whole ? kv->n_seq
+    const uint64_t units = kv->n_seq * (uint64_t)ceil_div(max_len, CUT) * p.tiles;
+    p.groups = whole ? kv->n_seq * p.tiles
                      : (uint32_t)std::min<uint64_t>(std::max<uint64_t>(slots / nkv, 1), (units + LEAST - 1) / LEAST);
     if (units >= 1ull << 31 || p.groups * nkv >= 1ull << 23) return false;  // (a launch has fewer than 2^32 threads)
-    const uint64_t parts = whole ? 0 : 2ull * p.groups * nkv * 16 * p.rt;
+    const uint64_t parts = whole || !p.few ? 0 : 2ull * p.groups * nkv * 16 * p.rt;
     uint64_t tparts = 0;
     if (rows > p.few) {
-        p.nw = rows > 128 ? 8 : 4;
-        const uint64_t tr = 32 * p.nw;
+        const uint64_t tr = TILE;
         // a sequence of n rows takes at most (n + tr - 1) / tr tiles, and n / (few + 1) sequences take any
+        // (and all rows at least so many, which the parts are chosen for)
         const uint64_t seqs = std::min<uint64_t>(kv->n_seq, n_rows * G / (p.few + 1));
-        const uint64_t items = (n_rows * G + seqs * (tr - 1)) / tr, tj = items * nkv;
+        const uint64_t items = (n_rows * G + seqs * (tr - 1)) / tr, tj = (n_rows * G + tr - 1) / tr * nkv;
         // the parts that fill 1 to 4 rounds of one workgroup per CU, by the rounds' stages
         const uint32_t top = ceil_div(max_len, 256);
-        uint32_t n = 1;
-        uint64_t best = ~0ull;
+        uint64_t best = ~0ull, slots = 0;
         for (uint64_t r = 1; r <= 4; r++) {
             const uint32_t fit = (uint32_t)(r * cus / tj), k = fit < 1 ? 1u : fit < top ? fit : top;
             const uint64_t cost = ceil_div(tj * k, cus) * (uint64_t)(ceil_div(ceil_div(max_len, k), TK) + TILE_FIX);
             if (cost < best) {
                 best = cost;
-                n = k;
+                slots = k == 1 ? 0 : std::max<uint64_t>(items, ceil_div(tj * k, cus) * (uint64_t)cus / nkv);
             }
         }
+        // (uncut, where the kernels' 32-bit sums of all sequences' stages could pass their
+        // range, whatever row_start says)
+        if (kv->n_seq * ((rows + tr - 1) / tr) * ceil_div(max_len, TK) >= 1ull << 30) slots = 0;
         p.items = (uint32_t)items;
-        p.tparts = n;
-        if (tj * n >= 1ull << 22 || items * nkv * tr >= 1ull << 27) return false;
-        p.tblocks = (uint32_t)(tj * n);
-        tparts = n == 1 ? 0 : tj * n * tr;
+        p.tslots = (uint32_t)slots;
+        if (std::max(items, slots) * nkv >= 1ull << 22 || items * nkv * tr >= 1ull << 27) return false;
+        tparts = slots * nkv * tr;
     }
     p.stat_off = parts * hd * 4;
     p.tpart_off = p.stat_off + parts * 8;
@@ -1108,7 +1235,7 @@ extern "C" int zh_check_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: rows overlap", who);
     const uint64_t qb = ((n - 1) * r->q_stride + w) * size, ob = ((n - 1) * r->out_stride + w) * size;
     Kv8Plan p;
-    if (!kv8_plan(cus, kv, r->n_heads, r->n_rows, r->max_rows, r->max_len, p))
+    if (!kv8_plan(cus, kv, r->n_heads, r->n_rows, r->max_rows, r->max_len, r->type == ZH_F32, p))
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: too large", who);
     if (!kv_in_range(r->q, r->q_off, qb) || !kv_in_range(r->out, r->out_off, ob) ||
         (p.bytes && !kv_in_range(r->ws, 0, p.bytes)))
@@ -1130,13 +1257,31 @@ extern "C" int zh_check_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
     return ZH_OK;
 }
 
-// zh_flash_attn_kv8_ws of a device of `cus` CUs (exported for the tests).
+// zh_flash_attn_kv8_ws of a device of `cus` CUs (exported for the tests): what kv8_plan
+// asks for at most, over smaller calls too, so every term grows with the sizes.
 extern "C" uint64_t zh_check_attn_kv8_ws(const zh_kv8_batch *kv, uint32_t n_heads, uint32_t n_rows, uint32_t max_rows,
                                          uint32_t max_len, uint32_t cus) {
     Kv8Plan p;
-    if (!kv8_shape_ok(kv, n_heads, n_rows, max_rows, max_len) || !kv8_plan(cus, kv, n_heads, n_rows, max_rows, max_len, p))
+    if (!kv8_shape_ok(kv, n_heads, n_rows, max_rows, max_len) ||
+        !kv8_plan(cus, kv, n_heads, n_rows, max_rows, max_len, false, p) ||
+        !kv8_plan(cus, kv, n_heads, n_rows, max_rows, max_len, true, p))
         return 0;
-    return std::max<uint64_t>(16, p.bytes);
+    const uint64_t nkv = kv->n_kv_heads, G = n_heads / nkv, rows = max_rows * G;
+    // streamed: two parts of a tile's rows in each workgroup
+    auto streamed = [&](uint64_t few, uint64_t tile, uint64_t slots) {
+        const uint64_t units = kv->n_seq * (uint64_t)ceil_div(max_len, CUT) * ceil_div(few, tile);
+        return 2 * std::min<uint64_t>(std::max<uint64_t>(slots / nkv, 1), (units + LEAST - 1) / LEAST) * nkv * tile;
+    };
+    uint64_t parts = streamed(std::min<uint64_t>(rows, 16), 16, 3ull * cus);
+    if (rows > 16) parts = std::max(parts, streamed(std::min<uint64_t>(rows, few_rows(true)), 32, 2ull * cus));
+    // LDS tiles: cut ones are at most two a CU before that
+    if (rows > few_rows(false) && max_len > 256) {
+        const uint64_t all = std::min<uint64_t>(n_rows * G, 2ull * cus / nkv * TILE), tj = ceil_div(all, TILE) * nkv;
+        const uint64_t seqs = std::max(std::min<uint64_t>(kv->n_seq, MIXED - 1), std::min<uint64_t>(kv->n_seq, all / few_rows(false)));
+        const uint64_t rounds = std::min<uint64_t>(4, ceil_div(tj * ceil_div(max_len, 256), cus));
+        parts += std::max<uint64_t>((all + seqs * (TILE - 1)) / TILE, rounds * cus / nkv) * nkv * TILE;
+    }
+    return parts * (kv->head_dim * 4 + 8);
 }
 
 extern "C" uint64_t zh_flash_attn_kv8_ws(zh_ctx *c, const zh_kv8_batch *kv, uint32_t n_heads, uint32_t n_rows,
@@ -1150,25 +1295,25 @@ static int attn_launch(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p) {
     ZH_LAUNCH_CHECK(c);
     if (p.least) {
         const uint32_t per = 256 / (HD / 4);
-        hipLaunchKernelGGL((k_kv8_join<HD, RT, T>), dim3(a.n_seq * a.nkv * (16 * RT / per)), dim3(256), 0, c->stream, a);
+        hipLaunchKernelGGL((k_kv8_join<HD, RT, T>), dim3(a.n_seq * a.nkv * a.tiles * (16 * RT / per)), dim3(256), 0, c->stream, a);
         ZH_LAUNCH_CHECK(c);
     }
     return ZH_OK;
 }
 
-template <int HD, int NP, int NW, uint32_t F, typename T>
+template <int HD, int NP, uint32_t F, typename T>
 static int tile_launch(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p) {
     static std::atomic<bool> attr[64];  // by device
     if (c->device >= 64 || !attr[c->device].load(std::memory_order_relaxed)) {
-        ZH_HIP(c, hipFuncSetAttribute((const void *)k_kv8_tile<HD, NP, NW, F, T>,
+        ZH_HIP(c, hipFuncSetAttribute((const void *)k_kv8_tile<HD, NP, F, T>,
                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)t_lds<HD>()));
         if (c->device < 64) attr[c->device].store(true, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL((k_kv8_tile<HD, NP, NW, F, T>), dim3(p.tblocks), dim3(64 * NW), t_lds<HD>(), c->stream, a);
+    hipLaunchKernelGGL((k_kv8_tile<HD, NP, F, T>), dim3((p.tslots ? p.tslots : p.items) * a.nkv), dim3(64 * TW), t_lds<HD>(), c->stream, a);
     ZH_LAUNCH_CHECK(c);
-    if (p.tparts > 1) {
+    if (p.tslots) {
         const uint32_t per = 256 / (HD / 4);
-        hipLaunchKernelGGL((k_kv8_tile_join<HD, NW, T>), dim3(p.items * a.nkv * (32 * NW / per)), dim3(256), 0, c->stream, a);
+        hipLaunchKernelGGL((k_kv8_tile_join<HD, T>), dim3(p.items * a.nkv * (TILE / per)), dim3(256), 0, c->stream, a);
         ZH_LAUNCH_CHECK(c);
     }
     return ZH_OK;
@@ -1176,9 +1321,8 @@ static int tile_launch(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p) {
 
 template <int HD, int NP, uint32_t F, typename T>
 static int attn_rt(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p) {
-    const int rc = p.rt == 1 ? attn_launch<HD, NP, 1, F, T>(c, a, p) : attn_launch<HD, NP, 2, F, T>(c, a, p);
-    if (rc || !p.nw) return rc;
-    return p.nw == 8 ? tile_launch<HD, NP, 8, F, T>(c, a, p) : tile_launch<HD, NP, 4, F, T>(c, a, p);
+    const int rc = !p.few ? ZH_OK : p.rt == 1 ? attn_launch<HD, NP, 1, F, T>(c, a, p) : attn_launch<HD, NP, 2, F, T>(c, a, p);
+    return rc || !p.items ? rc : tile_launch<HD, NP, F, T>(c, a, p);
 }
 template <int HD, uint32_t F>
 static int attn_type(zh_ctx *c, const Kv8Attn &a, const Kv8Plan &p, uint32_t type) {
@@ -1192,7 +1336,7 @@ extern "C" int zh_flash_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
     const zh_attn_rows x = with_strides(kv, rows), *r = &x;
     zh_device_scope dev(c);
     Kv8Plan p;
-    kv8_plan((uint32_t)c->cu_count, kv, r->n_heads, r->n_rows, r->max_rows, r->max_len, p);
+    kv8_plan((uint32_t)c->cu_count, kv, r->n_heads, r->n_rows, r->max_rows, r->max_len, r->type == ZH_F32, p);
     Kv8Attn a = {};
     const uint64_t size = r->type == ZH_F32 ? 4 : 2;
     a.q = (const uint8_t *)r->q->ptr + r->q_off;
@@ -1221,8 +1365,9 @@ extern "C" int zh_flash_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
     a.tpart = p.bytes ? (float *)((char *)r->ws->ptr + p.tpart_off) : nullptr;
     a.tstat = p.bytes ? (float *)((char *)r->ws->ptr + p.tstat_off) : nullptr;
     a.few = p.few;
-    a.items = p.items;
-    a.tparts = p.tparts;
+    a.tslots = p.tslots;
+    a.rt = 16 * p.rt;
+    a.tiles = p.tiles;
     a.groups = p.groups;
     a.least = p.least;
     // (64 bits: a scale of any size times log2 e)
