@@ -350,9 +350,9 @@ int zh_kv_copy_pages(zh_ctx *ctx, const zh_kv_caches *dst, const zh_kv_caches *s
 enum { ZH_I8 = 24, ZH_E4M3 = 256 };
 /* One layer's caches, the page tables of a batch (as in zh_kv_batch) and the
  * batch's rows: sequence s has the rows row_start[s] .. row_start[s + 1] - 1 of
- * the call (u32 [n_seq + 1], ascending; NULL: row s alone, or none where
- * seq_lens[s] is 0) and, these among them, seq_lens[s] tokens; its rows are its
- * last ones, in order. A sequence may have no rows; rows outside every sequence
+ * the call (u32 [n_seq + 1], ascending; NULL: row s alone, which the write passes
+ * over where seq_lens[s] is 0) and, these among them, seq_lens[s] tokens; its rows
+ * are its last ones, in order. A sequence may have no rows; rows outside every sequence
  * are left as they were. Tables, row_start and seq_lens are read on the device:
  * where row_start falls or passes the call's rows, a sequence has more rows than
  * tokens (the first ones are left out) or more tokens than its table holds, or a

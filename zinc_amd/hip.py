@@ -570,7 +570,7 @@ class Context:
         """n_tokens tokens in pages of src (KvCaches) quantised into pages of dst (Kv8Caches)."""
         d, n = _u32_array(dst_pages)
         s, ns = _u32_array(src_pages)
-        if n != ns or n != -(-n_tokens // 16):
+        if n_tokens < 0 or n != ns or n != -(-n_tokens // 16):
             raise ValueError("one source and one destination page per 16 tokens")
         self.check(lib().zh_kv8_pack_pages(self.h, dst.ptr, src.ptr, d, s, n_tokens))
 
