@@ -395,11 +395,12 @@ typedef struct zh_attn_rows {
  * outside the cache reads as page 0, and the next zh_sync then returns
  * ZH_ERR_INVALID_ARGUMENT. A row of a sequence without tokens is zero. What a row
  * may not see does not enter its result, whatever the cache holds there (NaN codes
- * of tokens of the same call excepted). ZH_F32: q and the probabilities in two fp16 pieces each
- * (22 bits); ZH_F16: the probabilities in two, or in one in a call of many rows
- * (max_rows of more than 128 query rows of a kv head); sums and softmax in 32 bits. Allocates
- * nothing and adds in a fixed order; calls that may overlap (other contexts,
- * replayed graphs) need a ws each. attn_scale finite. */
+ * of tokens of the same call excepted). ZH_F32: q and the probabilities in two
+ * fp16 pieces each (22 bits); ZH_F16: the probabilities in two, or in one in a
+ * call of many rows (max_rows of more than 128 query rows of a kv head); sums and
+ * softmax in 32 bits, and a score past 2^127 (in base 2) makes its row NaN.
+ * Allocates nothing and adds in a fixed order; calls that may overlap (other
+ * contexts, replayed graphs) need a ws each. attn_scale finite. */
 int zh_flash_attn_kv8(zh_ctx *ctx, const zh_kv8_batch *kv, const zh_attn_rows *rows);
 /* Bytes of ws for a call of these sizes and for every call of fewer sequences or
  * rows, a smaller max_rows or max_len, of either type (0: refused sizes). A call is

@@ -240,5 +240,5 @@ def test_attention(zh, ctx, fmt, t, case):
     starts = None if all(c == 1 for c in counts) else np.concatenate([[0], np.cumsum(counts)])
     q, got = attend(zh, ctx, rng, cache, tables, counts, lens, G, t, starts)
     want, *terms = expect(cache, tables, q, counts, lens, hd ** -0.5)
-    tiled = max(counts) * G > 32
+    tiled = max(counts) * G > 128
     close(got, want, tolerance(cache, t, want, *terms, lens, floor=-29 if tiled else -39))

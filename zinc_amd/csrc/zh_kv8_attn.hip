@@ -79,11 +79,10 @@ ZH_DEV AttnSeq attn_seq(const Kv8Attn &a, uint32_t s, bool &bad) {
 }
 
 // What takes the products of a row's q, scaled by 2^-e, times a block's scale to
-// base-2 scores. Kept in [2^-120, 2^80]: products lie below 2^32 in steps of 2^-48 at
-// least, so below that range every weight is 1 and above it all but a row's largest
-// are 0, as without the bounds; within it no score is infinite, and none that is
-// masked (-inf) meets a factor of 0.
-ZH_DEV float score_factor(float c, float scale) { return fminf(fmaxf(c * scale, 0x1p-120f), 0x1p80f); }
+// base-2 scores. 2^-120 at least: products lie below 2^32, so every weight is 1 there, as
+// without the bound, and no score that is masked (-inf) meets a factor of 0. A score
+// past the range of 32 bits makes its row NaN.
+ZH_DEV float score_factor(float c, float scale) { return fmaxf(c * scale, 0x1p-120f); }
 
 // A block's scales as the kernels take them: the scores' factor, the weights'
 // exponent and what takes a weight to its share of the sum; `ok` false: it reads as NaN
@@ -473,8 +472,9 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 3 : 2) void k_kv8_attn(Kv8Attn a)
 #pragma unroll
                     for (int r = 0; r < 4; r++) mb = fmaxf(mb, sc[j][r]);
                 mb = xor32_max(xor16_max(mb));
-                // (the largest weight is 2^14: what fp16's subnormals lose of the others is 2^-39 of it)
-                const float mn = fmaxf(m[rt], mb - 14.f), ms = mn == -INFINITY ? 0.f : mn;
+                // (the largest weight is 2^14: what fp16's subnormals lose of the others is 2^-39 of
+                // it; scores of 2^24 on have steps of 2 and more, and no room for 14 exactly)
+                const float mn = fmaxf(m[rt], fabsf(mb) < 0x1p24f ? mb - 14.f : mb), ms = mn == -INFINITY ? 0.f : mn;
                 f[rt] = __builtin_amdgcn_exp2f(m[rt] - ms);  // (m = -inf: 0)
                 m[rt] = mn;
                 float ls = 0.f;
@@ -923,8 +923,19 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
 #pragma unroll
         for (uint32_t kt = 0; kt < 2; kt++) {
             half8 pf[NP][2], vf[2][DT];
-            const float b = m == -INFINITY ? 0.f : 4.f - m;
-            const float bl[2] = {hc.lv[0] + b, hc.lv[1] + b};
+            const float ms = m == -INFINITY ? 0.f : m;
+            float bl[2] = {hc.lv[0] + (4.f - ms), hc.lv[1] + (4.f - ms)};
+            // where m's own rounding passes 1/4, the scores are rounded as it was before it is
+            // taken from them
+            if (__builtin_amdgcn_ballot_w64(fabsf(ms) >= 0x1p22f)) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) sc[r] = fmaf(sc[r], hc.ck[r / 8], hc.lv[r / 8]) - ms;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    hc.ck[j] = 1.f;
+                    bl[j] = 4.f;
+                }
+            }
             float mx = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; r++) sn[r] = 0.f;
