@@ -311,6 +311,9 @@ MIXED = [  # counts, lens, heads per kv head, kv heads, head_dim
     ([140, 0, 1] * 30, None, 1, 1, 64),
     ([11] * 20, None, 3, 1, 128),                                   # tiles of 32 that cut a row's heads
     ([5] * 9, [2000] * 9, 71, 1, 64),
+    ([50, 1] * 5 + [200], [2500, 1300] * 5 + [1700], 2, 1, 64),     # row tiles in shares, and LDS tiles
+    ([20, 3, 40] * 14, [2500, 77, 640] * 14, 2, 1, 64),
+    ([1] * 90, [1800, 900, 2500] * 30, 4, 2, 128),
 ]
 
 
@@ -333,6 +336,8 @@ SHAPES = [  # streamed, in one workgroup a sequence and in shares; LDS tiles who
     ([40, 7], [60, 300], 3, 1, 128),
     ([260, 3], [700, 300], 1, 2, 64),
     ([300], [4000], 1, 1, 128),
+    ([40, 7], [2600, 300], 3, 1, 128),
+    ([60, 1, 20], [1500, 3000, 2200], 2, 1, 64),
 ]
 
 

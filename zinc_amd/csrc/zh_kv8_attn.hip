@@ -1164,7 +1164,17 @@ constexpr uint32_t TILE_FIX = 5; // a tile launch's start and end, in stages
 // for three: 48 sequences of 3000 tokens f16 42.5 us for 39.1, f32 46.6 for 41.2; 16 rows,
 // four for three: no faster).
 constexpr uint64_t kv8_slots(uint32_t rt, uint64_t hd) { return rt == 1 || hd == 64 ? 3 : 2; }
-constexpr uint64_t kv8_one(uint32_t hd) { return hd == 64 ? 768 : 512; }
+// The max_len up to which a workgroup takes a whole sequence and row tile: it goes through
+// its tokens one step after the other, where shares are even, but begin anew, and wait for
+// memory, in every sequence that they reach into, and are joined. us whole / in shares, 8
+// kv heads, lengths up to the given one, f16: head_dim 128, 16 sequences 1000 tokens 11.9 /
+// 13.4, 1600 15.7 / 13.6; 48 1000 19.2 / 22.7, 2000 34.9 / 33.0, 4000 61 / 47; 192 2000 87 /
+// 94, 6000 244 / 215; 600 400 58 / 117; 20 rows 16 1000 16.3 / 18.0, 2000 28 / 24.5; 64 2000
+// 40 / 50, 4000 68 / 70; head_dim 64, 16 1300 11.6 / 11.6, 64 2000 20 / 23.5, 4000 36 / 31.5.
+// (So many that they even out by themselves: 3200 of 8000 593 / 579.)
+constexpr uint64_t kv8_one(uint32_t rt, uint64_t hd, uint64_t jobs, uint64_t cus) {
+    return rt == 2 ? 800 + 1300 * jobs / cus : hd == 64 ? 1250 + 900 * jobs / cus : 1000 + 500 * jobs / cus;
+}
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t n_rows, uint32_t max_rows, uint32_t max_len,
@@ -1176,8 +1186,8 @@ bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t n_rows
     p.few = rows <= few_rows(f32) ? (uint32_t)rows : kv->n_seq < MIXED ? 0 : few_rows(f32);
     p.tiles = ceil_div(p.few, 16 * p.rt);
     const uint64_t jobs = kv->n_seq * nkv * p.tiles, slots = kv8_slots(p.rt, hd) * cus;
-    // one workgroup a sequence: few short ones, or so many that they even out by themselves
-    const bool whole = (jobs <= cus && max_len <= kv8_one(hd) + kv8_one(hd) * jobs / cus) || jobs >= 8 * slots;
+    // one workgroup a sequence and row tile
+    const bool whole = max_len <= kv8_one(p.rt, hd, jobs, cus) || jobs >= 8 * slots;
     p.least = whole ? 0 : LEAST;
     const uint64_t units = kv->n_seq * (uint64_t)ceil_div(max_len, CUT) * p.tiles;
     p.groups = whole ? kv->n_seq * p.tiles
