@@ -229,6 +229,10 @@ ZH_DEV UnitSeq first_units(const Kv8Attn &a, bool &bad) {
 //   permutes before they become fp16; column li of output tile n is dim HD/16 li + n.
 // NP pieces of q (scaled by a power of two to a maximum in [2^14, 2^15)) as sums of
 // fp16 values, 2 of the weights: 22 bits of each.
+// Bound by HBM where the sequences are long (64 of 16384 tokens, 8 kv heads of 128: 315 us,
+// 6.4 TB/s), by 8 to 10 us of start, last steps and the waves' joining where not (48 ragged
+// ones to 4096 tokens, f32 i8: 41 us, 4.9 TB/s; 16 of 4096 25 us, 5.1); 24 sequences of 20
+// rows at 3000 tokens, head_dim 64, 16 us: 11 steps one after the other in every wave.
 template <int HD, int NP, int RT, uint32_t F, typename T>
 __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_attn(Kv8Attn a) {
     constexpr uint32_t KB = 16 * NJ;
@@ -606,7 +610,11 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
 //   address (swizzled pieces took 24 registers of addresses, and 12 others to scratch,
 //   whose reloads wait for the loads on the way).
 // The products of the next 32 tokens' scores run while the current ones' weights
-// are computed. The reference moves only when a score passes it by 2^8 (the weights
+// are computed. 4096 rows after 8192 tokens, 32 heads of 128 in f16, 687 GFLOP in 715 us
+// (960 TFLOP/s): the matrix units are busy for 42% of the cycles, vector instructions
+// (half of them the exponentials' and weights') for 52%, and the clock falls to 1.9 GHz
+// under both; without exponentials, maxima, fragment reads and copies the products alone
+// took 552 us. The reference moves only when a score passes it by 2^8 (the weights
 // then reach 2^12 in fp16 at most), so the output is rarely rescaled. A wave stops at
 // the last token that one of its rows sees.
 constexpr int TW = 8;                          // waves of a workgroup
@@ -1035,6 +1043,8 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
     }
 }
 
+// (Launches of their own, 4.3 us for 16 sequences of 4096 tokens, a chain of four loads; 12 us
+// for 777 rows of 28 heads on LDS tiles, 30 MB of parts.)
 // Joins the parts of a row: HD / 4 lanes, of 4 dims each, take the parts'
 // statistics, as many at a time, then all of them the parts' sums, 8 loads of 16
 // bytes in flight. Part p is row at(p) of part and stat.
@@ -1148,10 +1158,11 @@ struct Kv8Plan {
 constexpr uint32_t LEAST = 4;    // units of a share at least
 // Rows of a sequence and kv head that are streamed, in tiles of 32 that each read K and V
 // (through the L2s) again, where LDS tiles of 256 rows would be emptier than that costs.
-// us streamed / on LDS tiles, head_dim 128: f16 36 rows of 16 sequences of 2000 tokens 31 /
-// 52, of 40 62 / 154, 128 of 16 45 / 57, of 40 117 / 146, 160 of 16 65 / 62, of 40 139 /
-// 146, 192 of 16 71 / 64; f32 128 of 16 52 / 66, 192 of 16 81 / 82, of 40 of 4000 374 / 400,
-// 256 of 16 98 / 94; one sequence of 30000 tokens f16 128 rows 44 / 46, 256 74 / 55.
+// us streamed / on LDS tiles, head_dim 128, sequences of 2000 tokens: f16 36 rows of 16 31 /
+// 52, of 40 63 / 137, 128 of 4 26 / 27, of 16 43 / 55, of 40 94 / 152, 192 of 4 33 / 29, of
+// 16 60 / 63, 256 of 16 76 / 69; f32 128 of 16 54 / 66, of 40 116 / 188, 192 of 4 40 / 35, of
+// 16 70 / 81, of 40 160 / 207; one sequence of 30000 tokens, 128 rows f16 45 / 41, f32 50 /
+// 51, 256 rows 74 / 60 and 81 / 74.
 constexpr uint32_t few_rows(bool f32) { return f32 ? 192 : 128; }
 // Sequences from which on the few rows of some are streamed in a launch of their own
 // before the tiles of others; below, they take emptier tiles. us with / without, 512 rows
