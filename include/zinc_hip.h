@@ -352,11 +352,12 @@ enum { ZH_I8 = 24, ZH_E4M3 = 256 };
  * batch's rows: sequence s has the rows row_start[s] .. row_start[s + 1] - 1 of
  * the call (u32 [n_seq + 1], ascending; NULL: row s alone, which the write passes
  * over where seq_lens[s] is 0) and, these among them, seq_lens[s] tokens; its rows
- * are its last ones, in order. A sequence may have no rows; rows outside every sequence
- * are left as they were. Tables, row_start and seq_lens are read on the device:
- * where row_start falls or passes the call's rows, a sequence has more rows than
- * tokens (the first ones are left out) or more tokens than its table holds, or a
- * page lies outside the cache, the next zh_sync returns ZH_ERR_INVALID_ARGUMENT.
+ * are its last ones, in order. A sequence may have no rows (its length and pages
+ * are then not looked at); rows outside every sequence are left as they were.
+ * Tables, row_start and seq_lens are read on the device: where row_start falls or
+ * passes the call's rows, a sequence has more rows than tokens (the first ones are
+ * left out, in attention zero) or more tokens than its table holds, or a page lies
+ * outside the cache, the next zh_sync returns ZH_ERR_INVALID_ARGUMENT.
  * head_dim 64 or 128. */
 typedef struct zh_kv8_batch {
     zh_buf *k_cache, *v_cache, *k_scale, *v_scale;

@@ -520,6 +520,74 @@ def test_attention_of_malformed_batches(zh, ctx, case, t):  # noqa: F811
     run(lens=[0] * len(counts) if max(counts) == 1 else [1] * len(counts), max_len=max(lens))
 
 
+@pytest.mark.parametrize("t", [0, 1])
+@pytest.mark.parametrize("G", [4, 80])
+def test_sequences_without_rows(zh, ctx, G, t):  # noqa: F811
+    """Their lengths and pages may be anything, in a write and in attention, in both ways to
+    say whose the rows are."""
+    rng = np.random.default_rng(G)
+    counts, lens, hd, nkv = [2, 0, 3, 0, 0], [50, 1 << 31, 900, 0xFFFFFFFF, 7], 64, 1
+    live = [n if c else 0 for c, n in zip(counts, lens)]
+    tables, total = tables_for(rng, live, 1)
+    tables[1] = tables[3:] = 0xFFFFFF00
+    cache = Cache(ctx, rng, total, nkv, hd, E4M3)
+    kv = cache.batch(zh, tables, lens, starts_of(counts))
+    nq = 2
+    x = rng.normal(size=(5, nq + 2 * nkv, hd)).astype(np.float32)
+    write(zh, ctx, kv, x, nq, nkv, hd)
+    cache.k, cache.v, cache.ks, cache.vs = stored(cache, tables, counts, live, x, nq)
+    caches_agree(cache, cache.get(), (cache.k, cache.v, cache.ks, cache.vs))
+    cache.put()
+    q, got = attend(zh, ctx, rng, cache, tables, counts, lens, G, t, starts_of(counts), max_len=912)
+    agree(cache, tables, q, got, counts, live, t)
+    # a row a sequence, fewer rows than sequences
+    order = [0, 2, 1, 3, 4]
+    q, got = attend(zh, ctx, rng, cache, tables[order], [1, 1], u32(lens)[order], G, t, None, max_len=912)
+    agree(cache, tables[order], q, got, [1, 1], [live[i] for i in order[:2]], t)
+
+
+@pytest.mark.parametrize("t", [0, 1])
+@pytest.mark.parametrize("counts,lens,G", [([1, 1, 1], [40, 700, 2600], 4), ([3, 50, 9], [3, 400, 77], 4), ([90, 1], [300, 20], 4)])
+def test_stacked_rows_in_place(zh, ctx, t, counts, lens, G):  # noqa: F811
+    """Rows q | k | v | room of one buffer: q rotated in place, its result in the room; k and v
+    as they were."""
+    rng = np.random.default_rng(sum(lens))
+    nkv, hd = 2, 64
+    nq, T = G * nkv, sum(counts)
+    tables, total = tables_for(rng, lens, 1)
+    cache = Cache(ctx, rng, total, nkv, hd, (I8, E4M3)[t])
+    cache.ks[:] = cache.vs[:] = 2.0 ** -5
+    cache.put()
+    kv = cache.batch(zh, tables, lens, None if max(counts) == 1 else starts_of(counts))
+    w, W = (nq + 2 * nkv) * hd, (2 * nq + 2 * nkv) * hd + 16
+    x = rng.normal(size=(T, W)).astype(NP_TYPE[t])
+    b, size = ctx.upload(x), x.itemsize
+    freq = (1e4 ** (-np.arange(0, hd, 2) / hd)).astype(np.float32)
+    same_rows = dict(q_stride=W, k_stride=W, v_stride=W, q_out_stride=W)
+    ctx.qk_norm_rope_kv8_write_batched(kv, zh.QkvRows(q=b, k=b, v=b, q_out=b, k_off=nq * hd * size,
+                                                      v_off=(nq + nkv) * hd * size, type=t, pos=None, n_rows=T,
+                                                      n_q_heads=nq, inv_freq=ctx.upload(freq), rope_dim=hd, **same_rows))
+    ws = ctx.alloc(ctx.flash_attn_kv8_ws(kv, nq, T, max(counts), max(lens)))
+    ctx.flash_attn_kv8(kv, zh.AttnRows(q=b, out=b, out_off=w * size, q_stride=W, out_stride=W, ws=ws, n_rows=T, type=t,
+                                       max_rows=max(counts), max_len=max(lens), n_heads=nq))
+    ctx.sync()
+    got = b.download(x.dtype, x.size).reshape(x.shape)
+    pos = np.concatenate([np.arange(n - c, n) for n, c in zip(lens, counts)])
+    h = x[:, :w].reshape(T, nq + 2 * nkv, hd)
+    turned = ref.turned(h[:, :nq + nkv], None, freq, pos, 1e-6, hd)
+    q = got[:, :nq * hd].reshape(T, nq, hd)
+    mag = np.abs(h[:, :nq]).astype(np.float64)
+    mag = np.concatenate([mag[..., :hd // 2] + mag[..., hd // 2:]] * 2, -1)
+    close(q.astype(np.float64), turned[:, :nq], 2.0 ** -19 * mag + np.abs(turned[:, :nq]) * 2.0 ** (-11 if t else -24) +
+          (2.0 ** -25 if t else 0))
+    assert np.array_equal(got[:, nq * hd:w], x[:, nq * hd:w]) and np.array_equal(got[:, W - 16:], x[:, W - 16:])
+    y = h.astype(np.float64)
+    y[:, nq:nq + nkv] = turned[:, nq:]
+    cache.k, cache.v, cache.ks, cache.vs = stored(cache, tables, counts, lens, y, nq)
+    caches_agree(cache, cache.get(), (cache.k, cache.v, cache.ks, cache.vs))
+    agree(cache, tables, q, got[:, w:w + nq * hd].reshape(q.shape).astype(np.float64), counts, lens, t)
+
+
 def expect_cut(cache, tables, q, counts, lens, cut):
     """The rows see the tokens below `cut` only."""
     parts, first = [], 0

@@ -74,7 +74,7 @@ ZH_DEV AttnSeq attn_seq(const Kv8Attn &a, uint32_t s, bool &bad) {
     x.all = end > first ? end - first : 0u;
     x.n = min(x.all, a.max_rows);
     x.cut = min(x.len, a.max_len);
-    if (x.all > a.max_rows || x.len > a.max_len || (a.row_start && x.all > x.len)) bad = true;
+    if (x.all > a.max_rows || (x.all && x.len > a.max_len) || (a.row_start && x.all > x.len)) bad = true;
     return x;
 }
 
