@@ -396,10 +396,9 @@ typedef struct zh_attn_rows {
  * outside the cache reads as page 0, and the next zh_sync then returns
  * ZH_ERR_INVALID_ARGUMENT. A row of a sequence without tokens is zero. What a row
  * may not see does not enter its result, whatever the cache holds there (NaN codes
- * of tokens of the same call excepted). ZH_F32: q and the probabilities in two
- * fp16 pieces each (22 bits); ZH_F16: the probabilities in two, or in one in a
- * call of many rows (max_rows of more than 128 query rows of a kv head); sums and
- * softmax in 32 bits, and a score past 2^127 (in base 2) makes its row NaN.
+ * of tokens of the same call excepted). The probabilities are held in two fp16
+ * pieces (22 bits), and so is q of ZH_F32; sums and softmax in 32 bits, and a score
+ * past 2^127 (in base 2) makes its row NaN.
  * Allocates nothing and adds in a fixed order; calls that may overlap (other
  * contexts, replayed graphs) need a ws each. attn_scale finite. */
 int zh_flash_attn_kv8(zh_ctx *ctx, const zh_kv8_batch *kv, const zh_attn_rows *rows);

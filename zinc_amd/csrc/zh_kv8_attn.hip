@@ -610,11 +610,11 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
 //   address (swizzled pieces took 24 registers of addresses, and 12 others to scratch,
 //   whose reloads wait for the loads on the way).
 // The products of the next 32 tokens' scores run while the current ones' weights
-// are computed. 4096 rows after 8192 tokens, 32 heads of 128 in f16, 687 GFLOP in 715 us
-// (960 TFLOP/s): the matrix units are busy for 42% of the cycles, vector instructions
-// (half of them the exponentials' and weights') for 52%, and the clock falls to 1.9 GHz
-// under both; without exponentials, maxima, fragment reads and copies the products alone
-// took 552 us. The reference moves only when a score passes it by 2^8 (the weights
+// are computed. Weights are in two pieces, as where rows are streamed: in one, f16 results
+// were 2.7e-4 off where their rounding alone is 2.1e-4 (4096 rows then 730 us for 960). 4096
+// rows after 8192 tokens, 32 heads of 128 in f16, 687 GFLOP (1030 with the second piece) in
+// 955 to 1000 us: the matrix units are busy for 50% of the cycles, vector instructions for
+// 58%, and the clock falls under both. The reference moves only when a score passes it by 2^8 (the weights
 // then reach 2^12 in fp16 at most), so the output is rarely rescaled. A wave stops at
 // the last token that one of its rows sees.
 constexpr int TW = 8;                          // waves of a workgroup
@@ -701,7 +701,7 @@ ZH_DEV bool tile_job(const Kv8Attn &a, uint32_t rows, uint32_t u, TileJob &j) {
 
 template <int HD, int NP, uint32_t F, typename T>
 __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
-    constexpr int KS = HD / 16, DT = HD / 32;        // k-steps of the scores, 32-dim tiles of the output
+    constexpr int KS = HD / 16, DT = HD / 32, PW = 2;  // k-steps of the scores, 32-dim tiles of the output, weights' pieces
     constexpr uint32_t KROW = t_krow<HD>(), VROW = t_vrow<HD>(), KST = TK * KROW, VST = TK * VROW;  // of a row, a stage
     constexpr uint32_t ROWS = TILE, NT = 64 * TW;
     constexpr uint32_t CPR = HD / 16, PC = TK * CPR;  // 16-code pieces of a row and of a stage's K (or V)
@@ -930,7 +930,7 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
         const uint32_t tk = t0 + st * TK;
 #pragma unroll
         for (uint32_t kt = 0; kt < 2; kt++) {
-            half8 pf[NP][2], vf[2][DT];
+            half8 pf[PW][2], vf[2][DT];
             const float ms = m == -INFINITY ? 0.f : m;
             float bl[2] = {hc.lv[0] + (4.f - ms), hc.lv[1] + (4.f - ms)};
             // where m's own rounding passes 1/4, the scores are rounded as it was before it is
@@ -953,7 +953,7 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
                     float p = __builtin_amdgcn_exp2f(fmaf(sc[r], hc.ck[r / 8], bl[r / 8]));
                     l = fmaf(p, hc.iv[r / 8], l);
 #pragma unroll
-                    for (int k = 0; k < NP; k++) {
+                    for (int k = 0; k < PW; k++) {
                         pf[k][r / 8][r % 8] = (_Float16)p;
                         p -= (float)pf[k][r / 8][r % 8];
                     }
@@ -987,7 +987,7 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
 #pragma unroll
             for (int d = 0; d < DT; d++) {
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
+                for (int p = PW - 1; p >= 0; p--)
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][d], pf[p][0], o[d], 0, 0, 0);
 #pragma unroll
                 for (int i = EARLY + (PAIRS - EARLY) * d / DT; i < EARLY + (PAIRS - EARLY) * (d + 1) / DT; i++) weights(i);
@@ -998,7 +998,7 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
 #pragma unroll
             for (int d = 0; d < DT; d++) {
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
+                for (int p = PW - 1; p >= 0; p--)
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[1][d], pf[p][1], o[d], 0, 0, 0);
                 if (d == 0) mx = largest(sn, hn);
                 __builtin_amdgcn_sched_barrier(0);
@@ -1158,16 +1158,19 @@ struct Kv8Plan {
 constexpr uint32_t LEAST = 4;    // units of a share at least
 // Rows of a sequence and kv head that are streamed, in tiles of 32 that each read K and V
 // (through the L2s) again, where LDS tiles of 256 rows would be emptier than that costs.
-// us streamed / on LDS tiles, head_dim 128, sequences of 2000 tokens: f16 36 rows of 16 31 /
-// 52, of 40 63 / 137, 128 of 4 26 / 27, of 16 43 / 55, of 40 94 / 152, 192 of 4 33 / 29, of
-// 16 60 / 63, 256 of 16 76 / 69; f32 128 of 16 54 / 66, of 40 116 / 188, 192 of 4 40 / 35, of
-// 16 70 / 81, of 40 160 / 207; one sequence of 30000 tokens, 128 rows f16 45 / 41, f32 50 /
-// 51, 256 rows 74 / 60 and 81 / 74.
-constexpr uint32_t few_rows(bool f32) { return f32 ? 192 : 128; }
+// us streamed / on LDS tiles, head_dim 128, sequences of 2000 tokens: f16 36 rows of 16 30 /
+// 52, 128 of 1 16 / 20, of 4 26 / 29, of 16 42 / 58, of 40 99 / 168, 192 of 1 20 / 24, of 4
+// 34 / 32, of 16 59 / 69, of 40 140 / 178, 256 of 4 26 / 34, of 16 82 / 77; f32 128 of 16 54 /
+// 66, of 40 116 / 188, 192 of 4 40 / 35, of 16 70 / 81, of 40 160 / 207; 100 of 500 f16 192
+// rows 119 / 119, 256 154 / 131; one of 30000 f16 128 rows 46 / 46, 192 65 / 57, 256 72 / 64, f32
+// 128 50 / 51, 256 81 / 74.
+constexpr uint32_t FEW = 192;
 // Sequences from which on the few rows of some are streamed in a launch of their own
 // before the tiles of others; below, they take emptier tiles. us with / without, 512 rows
-// after 2000 tokens and n decode rows at 1000 and at 8000 tokens, f16: n = 0 51 / 47, 4 59
-// and 67 / 53 and 67, 8 70 and 104 / 68 and 103, 15 102 and 127 / 91 and 166
+// after 2000 tokens and n decode rows at 1000, 2000, 4000 and 8000 tokens, f16: n = 0 60 / 58;
+// 4 64, 64, 67, 85 / 64, 61, 74, 88; 8 67, 78, 72, 94 / 61, 76, 80, 117; 12 73, 89, 81, 110 / 77,
+// 84, 126, 145; 15 75, 89, 118, 126 / 77, 84, 139, 190; f32 8 76, 88, 82, 106 / 67, 83, 89, 131; 15
+// 85, 100, 133, 141 / 86, 93, 153, 203
 constexpr uint32_t MIXED = 9;
 constexpr uint32_t TILE_FIX = 5; // a tile launch's start and end, in stages
 
@@ -1189,12 +1192,12 @@ constexpr uint64_t kv8_one(uint32_t rt, uint64_t hd, uint64_t jobs, uint64_t cus
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t n_rows, uint32_t max_rows, uint32_t max_len,
-              bool f32, Kv8Plan &p) {
+              Kv8Plan &p) {
     const uint64_t G = nh / kv->n_kv_heads, rows = max_rows * G, nkv = kv->n_kv_heads, hd = kv->head_dim;
     p = {};
     if (n_rows * G >= 1ull << 31) return false;
     p.rt = rows <= 16 ? 1 : 2;
-    p.few = rows <= few_rows(f32) ? (uint32_t)rows : kv->n_seq < MIXED ? 0 : few_rows(f32);
+    p.few = rows <= FEW ? (uint32_t)rows : kv->n_seq < MIXED ? 0 : FEW;
     p.tiles = ceil_div(p.few, 16 * p.rt);
     const uint64_t jobs = kv->n_seq * nkv * p.tiles, slots = kv8_slots(p.rt, hd) * cus;
     // one workgroup a sequence and row tile
@@ -1271,7 +1274,7 @@ extern "C" int zh_check_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: rows overlap", who);
     const uint64_t qb = ((n - 1) * r->q_stride + w) * size, ob = ((n - 1) * r->out_stride + w) * size;
     Kv8Plan p;
-    if (!kv8_plan(cus, kv, r->n_heads, r->n_rows, r->max_rows, r->max_len, r->type == ZH_F32, p))
+    if (!kv8_plan(cus, kv, r->n_heads, r->n_rows, r->max_rows, r->max_len, p))
         return zh_set_err(c, ZH_ERR_INVALID_ARGUMENT, "%s: too large", who);
     if (!kv_in_range(r->q, r->q_off, qb) || !kv_in_range(r->out, r->out_off, ob) ||
         (p.bytes && !kv_in_range(r->ws, 0, p.bytes)))
@@ -1299,8 +1302,7 @@ extern "C" uint64_t zh_check_attn_kv8_ws(const zh_kv8_batch *kv, uint32_t n_head
                                          uint32_t max_len, uint32_t cus) {
     Kv8Plan p;
     if (!kv8_shape_ok(kv, n_heads, n_rows, max_rows, max_len) ||
-        !kv8_plan(cus, kv, n_heads, n_rows, max_rows, max_len, false, p) ||
-        !kv8_plan(cus, kv, n_heads, n_rows, max_rows, max_len, true, p))
+        !kv8_plan(cus, kv, n_heads, n_rows, max_rows, max_len, p))
         return 0;
     const uint64_t nkv = kv->n_kv_heads, G = n_heads / nkv, rows = max_rows * G;
     // streamed: two parts of a tile's rows in each workgroup
@@ -1309,11 +1311,11 @@ extern "C" uint64_t zh_check_attn_kv8_ws(const zh_kv8_batch *kv, uint32_t n_head
         return 2 * std::min<uint64_t>(std::max<uint64_t>(slots / nkv, 1), (units + LEAST - 1) / LEAST) * nkv * tile;
     };
     uint64_t parts = streamed(std::min<uint64_t>(rows, 16), 16, kv8_slots(1, kv->head_dim) * cus);
-    if (rows > 16) parts = std::max(parts, streamed(std::min<uint64_t>(rows, few_rows(true)), 32, kv8_slots(2, kv->head_dim) * cus));
+    if (rows > 16) parts = std::max(parts, streamed(std::min<uint64_t>(rows, FEW), 32, kv8_slots(2, kv->head_dim) * cus));
     // LDS tiles: cut ones are at most two a CU before that
-    if (rows > few_rows(false) && max_len > 256) {
+    if (rows > FEW && max_len > 256) {
         const uint64_t all = std::min<uint64_t>(n_rows * G, 2ull * cus / nkv * TILE), tj = ceil_div(all, TILE) * nkv;
-        const uint64_t seqs = std::max(std::min<uint64_t>(kv->n_seq, MIXED - 1), std::min<uint64_t>(kv->n_seq, all / few_rows(false)));
+        const uint64_t seqs = std::max(std::min<uint64_t>(kv->n_seq, MIXED - 1), std::min<uint64_t>(kv->n_seq, all / FEW));
         const uint64_t rounds = std::min<uint64_t>(4, ceil_div(tj * ceil_div(max_len, 256), cus));
         parts += std::max<uint64_t>((all + seqs * (TILE - 1)) / TILE, rounds * cus / nkv) * nkv * TILE;
     }
@@ -1372,7 +1374,7 @@ extern "C" int zh_flash_attn_kv8(zh_ctx *c, const zh_kv8_batch *kv, const zh_att
     const zh_attn_rows x = with_strides(kv, rows), *r = &x;
     zh_device_scope dev(c);
     Kv8Plan p;
-    kv8_plan((uint32_t)c->cu_count, kv, r->n_heads, r->n_rows, r->max_rows, r->max_len, r->type == ZH_F32, p);
+    kv8_plan((uint32_t)c->cu_count, kv, r->n_heads, r->n_rows, r->max_rows, r->max_len, p);
     Kv8Attn a = {};
     const uint64_t size = r->type == ZH_F32 ? 4 : 2;
     a.q = (const uint8_t *)r->q->ptr + r->q_off;
