@@ -1,5 +1,5 @@
-"""How exact the 8-bit cache's operators are, in every form that a call can take: f16
-attention rounded once."""
+"""How exact attention over the 8-bit cache is, in every form that a call can take: f16
+results rounded once, sums of weights where V's scales lie far apart."""
 import kv8_ref as ref
 import numpy as np
 import pytest
@@ -39,3 +39,132 @@ def test_f16_attention_is_rounded_once(zh, ctx, fmt, case):  # noqa: F811
     close(got, want, tolerance(cache, 1, want, *terms, lens, floor=-29))
     for a, b in zip(starts[:-1], starts[1:]):
         assert relative_rms(got[a:b], want[a:b].astype(np.float16).astype(np.float64)) < 2.0 ** -13
+
+
+# ---------------------------------------------------------------------------
+# V blocks of scales that lie far apart
+# ---------------------------------------------------------------------------
+def scales_of(kind, pages, far):
+    """The pages' exponents of V's scale."""
+    p = np.arange(pages)
+    if kind == "alternating":
+        return np.where(p % 2, far, -far)
+    if kind == "rising":
+        return np.where(p < pages // 2, -far, far)
+    if kind == "falling":
+        return np.where(p < pages // 2, far, -far)
+    return np.where(p == pages - 1, far, -far) if kind == "last" else np.where(p == 0, far, -far)
+
+
+APART = [  # counts, lens, heads per kv head, kv heads, head_dim
+    ([1, 1], [32, 130], 2, 2, 64),                # one step; a few, in several waves
+    ([1, 1, 1], [3000, 900, 2100], 4, 1, 128),    # in shares, joined
+    ([9, 20], [400, 2600], 3, 1, 128),            # tiles of 32 rows
+    ([9, 20], [400, 2600], 3, 1, 64),
+    ([260], [700], 1, 1, 64),                     # LDS tiles whole, and cut
+    ([230, 2], [4000, 300], 1, 1, 128),
+]
+
+
+@pytest.mark.parametrize("zero", [False, True], ids=["small", "zero"])
+@pytest.mark.parametrize("kind", ["alternating", "rising", "falling", "last", "first"])
+@pytest.mark.parametrize("case", APART, ids=lambda c: f"{len(c[0])}x{max(c[0])}-{max(c[1])}-{c[4]}")
+def test_v_scales_far_apart(zh, ctx, case, kind, zero):  # noqa: F811
+    """Every token counts in the sum of weights, whatever its block's scale is: blocks of the
+    least scale (of small values, or all zeros) and of the largest, in one step of a wave, in
+    different ones, waves, parts; scores that are flat, and ones that favour the large blocks
+    by 2^14, which thousands of others outweigh together by no more than 2^-3."""
+    counts, lens, G, nkv, hd = case
+    rng = np.random.default_rng(sum(counts) + len(kind))
+    tables, total = tables_for(rng, lens, 1)
+    for far, fmt in ((64, E4M3), (55, I8)):
+        cache = Cache(ctx, rng, total, nkv, hd, fmt)
+        cache.k[:] = 0
+        one = ref.encode(np.ones(1), fmt)[0]
+        large = np.zeros(total, bool)
+        for s, n in enumerate(lens):
+            pages = tables[s, :-(-n // 16)]
+            e = scales_of(kind, len(pages), far)
+            cache.vs[pages] = (2.0 ** e)[:, None]
+            large[pages] = e > 0
+        cache.ks[:] = 1
+        if zero:
+            cache.v.reshape(nkv, total, 16, hd)[:, ~large] = 0
+        cache.k.reshape(nkv, total, 16, hd)[:, large] = one  # (scores of these: the sum of q)
+        cache.put()
+        T, starts = sum(counts), starts_of(counts)
+        for favour in (0.0, 14.0):
+            q = np.zeros((T, G * nkv, hd), np.float32)
+            q[..., ::2] = favour * np.log(2) / (hd // 2)
+            q, got = attend(zh, ctx, rng, cache, tables, counts, lens, G, 0, starts, scale=1.0, q=q)
+            want, *terms = expect(cache, tables, q, counts, lens, 1.0)
+            close(got, want, tolerance(cache, 0, want, *terms, lens, floor=-29))
+
+
+@pytest.mark.parametrize("case", APART, ids=lambda c: f"{len(c[0])}x{max(c[0])}-{max(c[1])}-{c[4]}")
+@pytest.mark.parametrize("t", [0, 1])
+def test_v_scales_of_a_page_each(zh, ctx, case, t):  # noqa: F811
+    """Random scores, and a scale for each page from 2^-64 on, up to 2^64 (f16: up to where
+    results end)."""
+    counts, lens, G, nkv, hd = case
+    rng = np.random.default_rng(sum(counts) + 5)
+    tables, total = tables_for(rng, lens, 1)
+    cache = Cache(ctx, rng, total, nkv, hd, E4M3)
+    for top in (64, -30) if t == 0 else (6,):
+        cache.vs[:] = 2.0 ** rng.integers(-64, top + 1, (total, nkv))
+        cache.put()
+        q, got = attend(zh, ctx, rng, cache, tables, counts, lens, G, t, starts_of(counts))
+        want, *terms = expect(cache, tables, q, counts, lens, hd ** -0.5)
+        close(got, want, tolerance(cache, t, want, *terms, lens, floor=-29))
+
+
+@pytest.mark.parametrize("case", APART, ids=lambda c: f"{len(c[0])}x{max(c[0])}-{max(c[1])}-{c[4]}")
+def test_v_scales_far_apart_under_scores_of_any_size(zh, ctx, case):  # noqa: F811
+    """All of the weight on the largest score, where it passes the next by a hundredth,
+    whatever the scales of V are: 1 exactly, times a value with an exponent of its own."""
+    counts, lens, G, nkv, hd = case
+    rng = np.random.default_rng(sum(counts) + 6)
+    tables, total = tables_for(rng, lens, 1)
+    cache = Cache(ctx, rng, total, nkv, hd, I8)
+    cache.vs[:] = 2.0 ** rng.integers(-64, 65, (total, nkv))
+    cache.put()
+    T, starts = sum(counts), starts_of(counts)
+    q = rng.normal(size=(T, G * nkv, hd)).astype(np.float32)
+    want, sure, first = np.zeros(q.shape), np.zeros(q.shape, bool), 0
+    for s, (c, n) in enumerate(zip(counts, lens)):
+        p = np.arange(n)
+        at = tables[s, p // 16].astype(np.int64) * 16 + p % 16
+        for h in range(nkv):
+            k = ref.decode(cache.k[h, at], I8) * cache.ks[at // 16, h][:, None]
+            v = ref.decode(cache.v[h, at], I8) * cache.vs[at // 16, h][:, None].astype(np.float64)
+            for i in range(c):
+                x = q[first + i, h * G:(h + 1) * G].astype(np.float64) @ k[:n - c + i + 1].T
+                top = np.sort(x, 1)
+                want[first + i, h * G:(h + 1) * G] = v[x.argmax(1)]
+                sure[first + i, h * G:(h + 1) * G] = (top[:, -1] - top[:, -2] > 0.01 * np.abs(x).max(1))[:, None]
+        first += c
+    assert sure.any()
+    for scale in (1e6, 1e7, 1e8, 1e12, 1e30):
+        q, got = attend(zh, ctx, rng, cache, tables, counts, lens, G, 0, starts, scale=scale, q=q)
+        close(got[sure], want[sure], np.abs(want[sure]) * 2.0 ** -20)
+
+
+@pytest.mark.parametrize("t", [0, 1])
+@pytest.mark.parametrize("case", APART + [([21], [300], 1, 2, 64), ([9, 8], [700, 90], 4, 1, 128)],
+                         ids=lambda c: f"{len(c[0])}x{max(c[0])}-{max(c[1])}-{c[4]}")
+def test_v_scales_far_apart_in_place(zh, ctx, case, t):  # noqa: F811
+    """The rows' results in their q's place: those of a call with an out of its own, bit for bit."""
+    counts, lens, G, nkv, hd = case
+    rng = np.random.default_rng(sum(counts) + 7)
+    tables, total = tables_for(rng, lens, 1)
+    cache = Cache(ctx, rng, total, nkv, hd, E4M3)
+    cache.vs[:] = 2.0 ** rng.choice([-64, 0, 30], (total, nkv))
+    cache.put()
+    T, nh, starts = sum(counts), G * nkv, starts_of(counts)
+    q, apart = attend(zh, ctx, rng, cache, tables, counts, lens, G, t, starts)
+    kv = cache.batch(zh, tables, lens, starts)
+    b = ctx.upload(q)
+    ws = ctx.alloc(ctx.flash_attn_kv8_ws(kv, nh, T, max(counts), max(lens)))
+    ctx.flash_attn_kv8(kv, zh.AttnRows(q=b, out=b, ws=ws, n_rows=T, max_rows=max(counts), max_len=max(lens), n_heads=nh, type=t))
+    ctx.sync()
+    assert np.array_equal(b.download(q.dtype, q.size).reshape(q.shape).astype(np.float64), apart)

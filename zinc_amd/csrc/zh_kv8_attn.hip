@@ -84,22 +84,47 @@ ZH_DEV AttnSeq attn_seq(const Kv8Attn &a, uint32_t s, bool &bad) {
 // past the range of 32 bits makes its row NaN.
 ZH_DEV float score_factor(float c, float scale) { return fmaxf(c * scale, 0x1p-120f); }
 
+// V's scales may lie 2^128 apart, and exp2 gives 0 below 2^-126. A weight that small adds
+// nothing to the products with V, but its share w_t / b_t, in a block of a small scale, may
+// be most of the sum. So where parts are joined, or sums moved to a reference far above,
+// they are multiplied by 2^d in two factors (Shift); and blocks of scales below 2^-24 or
+// above 2^8 (none of a cache of ordinary values) are marked, for their tokens' shares to be
+// taken without b: streamed rows, by going over the scores again (far_sum: code in the loop
+// cost rows of f32 in tiles of 32 5 to 10%), LDS tiles in a branch that adds what fell out
+// (0.5%). Between the two scales nothing that counts is lost: of a share w_t / b_t with w_t
+// below 2^-126, b_t 2^-24, it is 2^-102; the sum is 2^-60 at least (a weight of 2^4 or more
+// over 2^64), so tokens lose it 2^-42 each at most.
+constexpr uint32_t LOW = (127 - 24) << 23, HIGH = (127 + 8) << 23;
+struct Shift {
+    float a, b;
+    ZH_DEVM explicit Shift(float d) {
+        const float e = fmaxf(d, -126.f);
+        a = __builtin_amdgcn_exp2f(e);
+        b = __builtin_amdgcn_exp2f(d - e);
+    }
+    ZH_DEVM float both() const { return a * b; }
+};
+ZH_DEV float lost_share(float a, float iv) {  // what the weight's product with iv has not
+    return a < -126.f ? __builtin_amdgcn_exp2f(a + 64.f) * (iv * 0x1p-64f) - __builtin_amdgcn_exp2f(a) * iv : 0.f;
+}
+
 // A block's scales as the kernels take them: the scores' factor, the weights'
 // exponent and what takes a weight to its share of the sum; `ok` false: it reads as NaN
 // (and the others are harmless).
 template <uint32_t F>
 struct Block {
     float ks, lv, iv;
-    bool ok;
+    bool ok, apart;
+    ZH_DEVM static constexpr float unit() { return F == ZH_I8 ? 0x1p-10f : 1.f; }  // (the fp16 codes' of 1)
     ZH_DEVM void set(uint32_t k, uint32_t v) {
-        constexpr float unit = F == ZH_I8 ? 1024.f : 1.f;  // (of the fp16 codes)
         ok = kv8_scale_ok(k) && kv8_scale_ok(v);
         const uint32_t kb = ok ? k : 0x3F800000u, vb = ok ? v : 0x3F800000u;
+        apart = vb - LOW > HIGH - LOW;
         // (exact for powers of two; for others the exponent's fraction is within 2^-21)
         const float mant = __uint_as_float((vb & 0x7FFFFFu) | 0x3F800000u);
-        ks = __uint_as_float(kb) * unit;
+        ks = __uint_as_float(kb) * (1.f / unit());
         lv = (float)((int)(vb >> 23) - 127) + __builtin_amdgcn_logf(mant);
-        iv = __builtin_amdgcn_rcpf(mant) * __uint_as_float((254u - (vb >> 23)) << 23) * (1.f / unit);
+        iv = __builtin_amdgcn_rcpf(mant) * __uint_as_float((254u - (vb >> 23)) << 23) * unit();
     }
 };
 
@@ -365,13 +390,9 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
             if (wave + W < nstep) nx = step(wave + W);
         }
         // the rows' q as operand fragments: dims 64 u + 16 lg + 8 h .. (the scale's sign in them)
-        half8 qf[RT][NQ][2 * U];
-        float cf[RT];  // products to base-2 scores, but for the block's scale
-        uint32_t lim[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
+        auto load_q = [&](int rt, half8 (&qf)[NQ][2 * U], float &cf, uint32_t &lim) __attribute__((always_inline)) {
             const uint32_t r = row0 + min(16 * rt + li, nrow - 1), i = r / a.G;
-            lim[rt] = min(seq.lim(i), t1);
+            lim = min(seq.lim(i), t1);
             const T *qp = (const T *)(a.q + (uint64_t)(seq.row + i) * a.q_row) + (size_t)(kvh * a.G + r % a.G) * HD + 16 * lg;
             float v[2 * U][8], mx = 0.f;
 #pragma unroll
@@ -394,12 +415,17 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
                     float y = (NQ > 1 ? ldexpf(v[k][i], -e) : v[k][i]) * sign;
 #pragma unroll
                     for (int p = 0; p < NQ; p++) {
-                        qf[rt][p][k][i] = (_Float16)y;
-                        y -= (float)qf[rt][p][k][i];
+                        qf[p][k][i] = (_Float16)y;
+                        y -= (float)qf[p][k][i];
                     }
                 }
-            cf[rt] = fabsf(ldexpf(a.scale, a.scale_exp + e));
-        }
+            cf = fabsf(ldexpf(a.scale, a.scale_exp + e));
+        };
+        half8 qf[RT][NQ][2 * U];
+        float cf[RT];  // products to base-2 scores, but for the block's scale
+        uint32_t lim[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) load_q(rt, qf[rt], cf[rt], lim[rt]);
         floatx4 o[RT][ND];
         float m[RT], l[RT];  // the row's reference (every lg alike), this lane's share of its sum
 #pragma unroll
@@ -409,6 +435,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
 #pragma unroll
             for (int n = 0; n < ND; n++) o[rt][n] = floatx4{0.f, 0.f, 0.f, 0.f};
         }
+        bool far_apart = false;  // (some block's scale of V is)
         // the weights and products of step x; `more`: the next step's loads on the way.
         // (The last step is code of its own: a load that may not be there would make
         // the compiler wait for V before the scores.)
@@ -419,6 +446,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
             for (uint32_t j = 0; j < NJ; j++) {
                 b[j].set(scalar(ksb[j]), scalar(vsb[j]));
                 ok = ok && b[j].ok;
+                far_apart = far_apart || b[j].apart;
             }
             floatx4 d[RT][NJ];
 #pragma unroll
@@ -543,11 +571,44 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
             work(std::false_type{});
         }
         if (bad && lane == 0) atomicOr(a.err, ZH_DEVERR_KV_ROW);
+        // a lane's share of a row's sum again, from the scores without V's scales
+        auto far_sum = [&](int rt, float m) __attribute__((always_inline)) {
+            half8 qf[NQ][2 * U];
+            float cf, sum = 0.f;
+            uint32_t lim;
+            load_q(rt, qf, cf, lim);
+            const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+            for (uint32_t tk = t0 + KB * wave, j = 0; tk < t1; tk += j ? KB * W - 16 * (NJ - 1) : 16, j ^= 1) {
+                const uint32_t pg = scalar(tab[tk / 16]), page = pg < a.cache_tokens / 16 ? pg : 0u;
+                const uint8_t *at = kh + (size_t)page * (16 * HD) + koff;
+                Block<F> b;
+                b.set(scalar(ksc[(size_t)page * a.nkv]), scalar(vsc[(size_t)page * a.nkv]));
+                half8 kf[2 * U];
+#pragma unroll
+                for (int k = 0; k < 2 * U; k++) {
+                    const u32x2 c = *(const u32x2 *)(at + 64 * (k / 2) + 8 * (k % 2));
+                    kf[k] = row8<F>(c.x, c.y);
+                }
+                floatx4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int p = NQ - 1; p >= 0; p--)
+#pragma unroll
+                    for (int k = 0; k < 2 * U; k++) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], qf[p][k], d, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float s = fmaf(d[r], score_factor(cf, b.ks), b.lv) - ms - b.lv;
+                    sum += tk + 4 * lg + r >= lim ? 0.f : __builtin_amdgcn_exp2f(s) * b.unit();
+                }
+            }
+            return sum;
+        };
         // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
         const size_t p0 = ((size_t)blockIdx.x * 2 + slot) * ROWS;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             __syncthreads();  // (the words below have been read)
+            if (far_apart) l[rt] = far_sum(rt, m[rt]);  // (uniform per wave)
             const float ls = xor32_sum(xor16_sum(l[rt]));
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -571,13 +632,14 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
                 const float Ms = M == -INFINITY ? 0.f : M;
 #pragma unroll
                 for (int k = 0; k < W; k++) {
-                    const float fk = __builtin_amdgcn_exp2f(sm[k * 16 + r] - Ms);
+                    const Shift to(sm[k * 16 + r] - Ms);
+                    const float fk = to.both();
                     const f32x4 v = *(const f32x4 *)(so + (k * 16 + r) * LD + d);
                     O.x = fmaf(v.x, fk, O.x);
                     O.y = fmaf(v.y, fk, O.y);
                     O.z = fmaf(v.z, fk, O.z);
                     O.w = fmaf(v.w, fk, O.w);
-                    L = fmaf(sl[k * 16 + r], fk, L);
+                    L = fmaf(sl[k * 16 + r] * to.a, to.b, L);
                 }
                 if (direct) {
                     const f32x4 v = seq.lim(qi) ? f32x4{O.x / L, O.y / L, O.z / L, O.w / L} : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -709,7 +771,7 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
     extern __shared__ __align__(16) uint8_t lds[];
     typedef __fp16 tr4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) tr4 lds_tr4;
-    float *const scl = (float *)(lds + TS * (KST + VST));  // [stage][page]: Block's ks, lv, iv and ok
+    float *const scl = (float *)(lds + TS * (KST + VST));  // [stage][page]: Block's ks, lv, iv; 0 not ok, 2 apart, 1 else
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t i32 = lane % 32, h = lane / 32;
     // (kv heads fastest: with 8 of them every head's K and V stay in one XCD's L2)
@@ -774,7 +836,7 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
         if (scales) {
             Block<F> b;
             b.set(r.k, r.v);
-            *(f32x4 *)(lds + sput + slot * 64) = f32x4{b.ks, b.lv, b.iv, b.ok ? 1.f : 0.f};
+            *(f32x4 *)(lds + sput + slot * 64) = f32x4{b.ks, b.lv, b.iv, !b.ok ? 0.f : b.apart ? 2.f : 1.f};
         }
     };
     Raw raw;
@@ -839,6 +901,7 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
     struct Half {   // of 32 tokens' two pages: scores' factors, weights' exponents and shares
         float ck[2], lv[2], iv[2];
         bool ok;
+        uint32_t apart;
     };
     Half hc, hn;
     // (two pieces of f32 leave no registers for V beside the scores' products, nor for
@@ -859,16 +922,20 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
             x.iv[j] = b.z;
             ok *= b.w;
         }
-        x.ok = __builtin_amdgcn_readfirstlane(__float_as_uint(ok)) != 0;
+        const uint32_t all = __builtin_amdgcn_readfirstlane(__float_as_uint(ok));
+        x.ok = all != 0;
+        x.apart = all > 0x3F800000u;
     };
     // the reference, for scores up to mx: moved, and the sums with it, where one
     // passes it by 2^8
     auto refer = [&](float mx) __attribute__((always_inline)) {
         mx = xor32_max(mx);
         if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
-            const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            const float mn = fmaxf(m, mx);
+            const Shift to(m - (mn == -INFINITY ? 0.f : mn));
+            const float f = to.both();
             m = mn;
-            l *= f;
+            l = l * to.a * to.b;
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -935,14 +1002,20 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
             float bl[2] = {hc.lv[0] + (4.f - ms), hc.lv[1] + (4.f - ms)};
             // where m's own rounding passes 1/4, the scores are rounded as it was before it is
             // taken from them
-            if (__builtin_amdgcn_ballot_w64(fabsf(ms) >= 0x1p22f)) {
+            const uint64_t far = __builtin_amdgcn_ballot_w64(fabsf(ms) >= 0x1p22f);
+            if (far | hc.apart) {  // (one branch)
+                if (far) {
 #pragma unroll
-                for (int r = 0; r < 16; r++) sc[r] = fmaf(sc[r], hc.ck[r / 8], hc.lv[r / 8]) - ms;
+                    for (int r = 0; r < 16; r++) sc[r] = fmaf(sc[r], hc.ck[r / 8], hc.lv[r / 8]) - ms;
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    hc.ck[j] = 1.f;
-                    bl[j] = 4.f;
+                    for (int j = 0; j < 2; j++) {
+                        hc.ck[j] = 1.f;
+                        bl[j] = 4.f;
+                    }
                 }
+                if (hc.apart)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) l += lost_share(fmaf(sc[r], hc.ck[r / 8], bl[r / 8]), hc.iv[r / 8]);
             }
             float mx = 0.f;
 #pragma unroll
@@ -1064,13 +1137,14 @@ ZH_DEV f32x4 join_row(const float *part, const float *stat, uint32_t parts, A at
 #pragma unroll
         for (uint32_t x = 1; x < N; x *= 2) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
         const float mn = fmaxf(M, mx), ms = mn == -INFINITY ? 0.f : mn;
-        const float old = __builtin_amdgcn_exp2f(M - ms), w = l < n ? __builtin_amdgcn_exp2f(st.x - ms) : 0.f;
-        float ls = l < n ? st.y * w : 0.f;
+        const Shift old(M - ms), own(st.x - ms);
+        const float w = l < n ? own.both() : 0.f;
+        float ls = l < n ? st.y * own.a * own.b : 0.f;
 #pragma unroll
         for (uint32_t x = 1; x < N; x *= 2) ls += __shfl_xor(ls, x, 64);
         M = mn;
-        L = fmaf(L, old, ls);
-        O *= old;
+        L = fmaf(L * old.a, old.b, ls);
+        O *= old.both();
         for (uint32_t p = 0; p < n; p += U) {
             if (p)
 #pragma unroll
