@@ -29,9 +29,11 @@ bool kv8_batch_ok(const zh_kv8_batch *kv, uint32_t n_rows) {
 // q/k RMSNorm + RoPE + quantised KV write. The arithmetic of q is the fp16
 // cache's operator's (zh_kv.hip). k goes in 64 bits from the row to the code, its
 // angle as a fraction of a turn with the product's own rounding put back: a code
-// does not then depend on the order of 32-bit sums, and the same tokens leave the
-// same cache whatever batch they came in. That is 30 operations of half rate for
-// each element of k beside its loads, 2 us of the chip for 8192 rows of 8 heads.
+// does not then depend on the order of 32-bit sums, and tokens written in the same steps
+// leave the same cache whichever form takes them and whatever else is in their calls. (In
+// other steps the scales are the same at the end, not every code: see zh_kv8.h.) That is some
+// 30 operations for each element of k beside its loads, 6 us of all vector units for 8192
+// rows of 8 heads.
 //
 // Two forms. Sequences with several rows: a workgroup takes one page of one sequence
 // and some heads of q, k or v: thread (slot, l) holds slot `slot` of the page and 8
@@ -41,8 +43,8 @@ bool kv8_batch_ok(const zh_kv8_batch *kv, uint32_t n_rows) {
 // vectors of a row a workgroup, each on 16 (8) lanes, which reach for the page's other
 // slots themselves where the scale rises; in the first form 15 of 16 threads would idle
 // (250 rows of 8 heads 12.8 us, 5.3 so).
-// 8192 rows of 32 + 16 heads of 128 in f16 (100 MB read, 84 written) 44 us, 4.2 TB/s: bound by
-// HBM and by waiting for it (45% of the waves' cycles). A decode step of 61 sequences 4.7
+// 8192 rows of 32 + 16 heads of 128 in f16 (100 MB read, 84 written) 44 us, 4.2 TB/s: vector
+// instructions issue in 84% of the cycles, and waves wait for 45% of theirs. A decode step of 61 sequences 4.7
 // us: a chain of loads, length, page, scale and rows, and a launch.
 // ---------------------------------------------------------------------------
 namespace {
