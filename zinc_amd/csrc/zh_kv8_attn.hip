@@ -1254,14 +1254,20 @@ constexpr uint32_t TILE_FIX = 5; // a tile launch's start and end, in stages
 constexpr uint64_t kv8_slots(uint32_t rt, uint64_t hd) { return rt == 1 || hd == 64 ? 3 : 2; }
 // The max_len up to which a workgroup takes a whole sequence and row tile: it goes through
 // its tokens one step after the other, where shares are even, but begin anew, and wait for
-// memory, in every sequence that they reach into, and are joined. us whole / in shares, 8
-// kv heads, lengths up to the given one, f16: head_dim 128, 16 sequences 1000 tokens 11.9 /
-// 13.4, 1600 15.7 / 13.6; 48 1000 19.2 / 22.7, 2000 34.9 / 33.0, 4000 61 / 47; 192 2000 87 /
-// 94, 6000 244 / 215; 600 400 58 / 117; 20 rows 16 1000 16.3 / 18.0, 2000 28 / 24.5; 64 2000
-// 40 / 50, 4000 68 / 70; head_dim 64, 16 1300 11.6 / 11.6, 64 2000 20 / 23.5, 4000 36 / 31.5.
-// (So many that they even out by themselves: 3200 of 8000 593 / 579.)
-constexpr uint64_t kv8_one(uint32_t rt, uint64_t hd, uint64_t jobs, uint64_t cus) {
-    return rt == 2 ? 800 + 1300 * jobs / cus : hd == 64 ? 1250 + 900 * jobs / cus : 1000 + 500 * jobs / cus;
+// memory, in every sequence that they reach into, and are joined; and dealing out takes every
+// workgroup, of the join's too, a pass over all sequences. The host knows the longest length
+// only, so the rule lies between what batches of like lengths and what one long sequence among
+// short ones would have it be. us whole / in shares, 8 kv heads, f16, n of a length | n - 1 of
+// 200 tokens and one of it: head_dim 128, 16 of 1000 12.2 / 14.3, 1250 | 13.8 / 12.1; 64 of
+// 2000 46 / 53 | 21 / 16; 200 of 4000 276 / 281 | 51 / 43; 600 of 6000 1149 / 1200, 10375 | 134 /
+// 127; 800 of 13500 | 171 / 170, 27000 | 264 / 178; 1600 of 26000 | 344 / 452, 52000 | 540 / 453;
+// head_dim 64, 64 of 1900 28 / 32, 1525 | 14 / 13, 3050 | 22 / 14; 200 of 3800 159 / 146, 3437 | 32
+// / 28; 600 of 9000 855 / 910, 9062 | 82 / 72, 18125 | 130 / 72; 20 rows, head_dim 128, 16 of 1000
+// 17.4 / 20.1 | 16.5 / 14.7, 2000 29 / 25 | 26 / 15; 64 of 2400 61 / 67 | 34 / 29, 3400 90 / 94 | 45
+// / 30; 6400 of 300 and one of 30000, 1 kv head 313 / 790.
+constexpr uint64_t kv8_one(uint32_t rt, uint64_t hd, uint64_t n_seq, uint64_t jobs, uint64_t cus) {
+    const uint64_t even = rt == 2 ? 800 + 800 * jobs / cus : 1000 + (hd == 64 ? 450 : 500) * jobs / cus;
+    return std::max(even, n_seq * jobs * rt * hd / 64000);
 }
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
@@ -1275,7 +1281,8 @@ bool kv8_plan(uint32_t cus, const zh_kv8_batch *kv, uint32_t nh, uint32_t n_rows
     p.tiles = ceil_div(p.few, 16 * p.rt);
     const uint64_t jobs = kv->n_seq * nkv * p.tiles, slots = kv8_slots(p.rt, hd) * cus;
     // one workgroup a sequence and row tile
-    const bool whole = max_len <= kv8_one(p.rt, hd, jobs, cus) || jobs >= 8 * slots;
+    // (so many that the join would not fit a launch: always)
+    const bool whole = jobs >= 1u << 20 || max_len <= kv8_one(p.rt, hd, kv->n_seq, jobs, cus);
     p.least = whole ? 0 : LEAST;
     const uint64_t units = kv->n_seq * (uint64_t)ceil_div(max_len, CUT) * p.tiles;
     p.groups = whole ? kv->n_seq * p.tiles
