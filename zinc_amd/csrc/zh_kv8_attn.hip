@@ -604,11 +604,17 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
             return sum;
         };
         // ---- join the waves; lane li, lg: row li, dims ND (4 lg + r) + n
+        if (far_apart)  // (uniform per wave)
+#pragma unroll 1
+            for (int rt = 0; rt < RT; rt++) {
+                const float sum = far_sum(rt, m[RT == 1 ? 0 : rt ? RT - 1 : 0]);
+                if (RT == 1 || rt == 0) l[0] = sum;
+                else l[RT - 1] = sum;
+            }
         const size_t p0 = ((size_t)blockIdx.x * 2 + slot) * ROWS;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             __syncthreads();  // (the words below have been read)
-            if (far_apart) l[rt] = far_sum(rt, m[rt]);  // (uniform per wave)
             const float ls = xor32_sum(xor16_sum(l[rt]));
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -625,21 +631,31 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
                 const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
                 if (16 * rt + r >= nrow) break;
                 const uint32_t R = row0 + 16 * rt + r, qi = R / a.G, h = kvh * a.G + R % a.G;
-                float M = sm[r], L = 0.f;
+                float M = sm[r], low = M, L = 0.f;
                 f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 1; k < W; k++) M = fmaxf(M, sm[k * 16 + r]);
+                for (int k = 1; k < W; k++) {
+                    M = fmaxf(M, sm[k * 16 + r]);
+                    low = fminf(low, sm[k * 16 + r]);
+                }
                 const float Ms = M == -INFINITY ? 0.f : M;
 #pragma unroll
                 for (int k = 0; k < W; k++) {
-                    const Shift to(sm[k * 16 + r] - Ms);
-                    const float fk = to.both();
+                    const float fk = __builtin_amdgcn_exp2f(sm[k * 16 + r] - Ms);
                     const f32x4 v = *(const f32x4 *)(so + (k * 16 + r) * LD + d);
                     O.x = fmaf(v.x, fk, O.x);
                     O.y = fmaf(v.y, fk, O.y);
                     O.z = fmaf(v.z, fk, O.z);
                     O.w = fmaf(v.w, fk, O.w);
-                    L = fmaf(sl[k * 16 + r] * to.a, to.b, L);
+                    L = fmaf(sl[k * 16 + r], fk, L);
+                }
+                if (__builtin_amdgcn_ballot_w64(low - Ms < -126.f)) {
+                    L = 0.f;
+#pragma unroll
+                    for (int k = 0; k < W; k++) {
+                        const Shift to(sm[k * 16 + r] - Ms);
+                        L = fmaf(sl[k * 16 + r] * to.a, to.b, L);
+                    }
                 }
                 if (direct) {
                     const f32x4 v = seq.lim(qi) ? f32x4{O.x / L, O.y / L, O.z / L, O.w / L} : f32x4{0.f, 0.f, 0.f, 0.f};
