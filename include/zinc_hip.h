@@ -397,8 +397,9 @@ typedef struct zh_attn_rows {
  * ZH_ERR_INVALID_ARGUMENT. A row of a sequence without tokens is zero. What a row
  * may not see does not enter its result, whatever the cache holds there (NaN codes
  * of tokens of the same call excepted). The probabilities are held in two fp16
- * pieces (22 bits), and so is q of ZH_F32; sums and softmax in 32 bits, and a score
- * past 2^127 (in base 2) makes its row NaN.
+ * pieces (22 bits), and so is q of ZH_F32; sums and softmax in 32 bits. A score past
+ * 2^127 (in base 2) makes its row NaN, and so may a factor of it: attn_scale by the
+ * row's largest q, or by that and a block's scale.
  * Allocates nothing and adds in a fixed order; calls that may overlap (other
  * contexts, replayed graphs) need a ws each. attn_scale finite. */
 int zh_flash_attn_kv8(zh_ctx *ctx, const zh_kv8_batch *kv, const zh_attn_rows *rows);

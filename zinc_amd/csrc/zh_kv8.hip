@@ -44,8 +44,8 @@ bool kv8_batch_ok(const zh_kv8_batch *kv, uint32_t n_rows) {
 // slots themselves where the scale rises; in the first form 15 of 16 threads would idle
 // (250 rows of 8 heads 12.8 us, 5.3 so).
 // 8192 rows of 32 + 16 heads of 128 in f16 (100 MB read, 84 written) 44 us, 4.2 TB/s: vector
-// instructions issue in 84% of the cycles, and waves wait for 45% of theirs. A decode step of 61 sequences 4.7
-// us: a chain of loads, length, page, scale and rows, and a launch.
+// instructions issue in 86% of the cycles, and waves wait for 43% of theirs. A decode step of
+// 61 sequences 4.7 us: a chain of loads, length, page, scale and rows, and a launch.
 // ---------------------------------------------------------------------------
 namespace {
 
@@ -495,7 +495,7 @@ extern "C" int zh_qk_norm_rope_kv8_write_batched(zh_ctx *c, const zh_kv8_batch *
     // heads of a workgroup: the more of them, the fewer angles are taken and the more
     // loads are on the way. us at 4 heads of q and 1 of k (of v) / 8 and 2 / 16 and 4,
     // 32 + 16 heads of 128, f16: 100 rows 4.6 / 5.9 / 8.4, 333 6.0 / 6.8 / 8.7, 1000 11.8 /
-    // 10.2 / 12.0, 2500 21.8 / 18.8 / 16.6, 8192 71 / 51 / 46; f32 8192 80 / 70 / 75
+    // 10.2 / 12.0, 2500 21.8 / 18.8 / 16.6, 8192 71 / 51 / 46; f32 8192 80 / 70 / 75 (for a floor of 58)
     const bool big = units >= 128 && si == 2;
     a.q_heads = units < 48 ? 4 : big ? 16 : 8;
     a.kv_heads = units < 48 ? 1 : big ? 4 : 2;

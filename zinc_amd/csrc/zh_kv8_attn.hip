@@ -257,7 +257,9 @@ ZH_DEV UnitSeq first_units(const Kv8Attn &a, bool &bad) {
 // Bound by HBM where the sequences are long (64 of 16384 tokens, 8 kv heads of 128: 315 us,
 // 6.4 TB/s), by 8 to 10 us of start, last steps and the waves' joining where not (48 ragged
 // ones to 4096 tokens, f32 i8: 41 us, 4.9 TB/s; 16 of 4096 25 us, 5.1); 24 sequences of 20
-// rows at 3000 tokens, head_dim 64, 16 us: 11 steps one after the other in every wave.
+// rows at 3000 tokens, head_dim 64, 4 kv heads, 16 us: three steps in every wave, behind a
+// start of some five loads that depend on one another and the finding of its share; vector
+// instructions in 61% of the cycles, on 32 row slots.
 template <int HD, int NP, int RT, uint32_t F, typename T>
 __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_attn(Kv8Attn a) {
     constexpr uint32_t KB = 16 * NJ;
@@ -692,7 +694,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
 // were 2.7e-4 off where their rounding alone is 2.1e-4 (4096 rows then 730 us for 960). 4096
 // rows after 8192 tokens, 32 heads of 128 in f16, 687 GFLOP (1030 with the second piece) in
 // 955 to 1000 us: the matrix units are busy for 50% of the cycles, vector instructions for
-// 58%, and the clock falls under both. The reference moves only when a score passes it by 2^8 (the weights
+// 59%, and the clock falls under both. The reference moves only when a score passes it by 2^8 (the weights
 // then reach 2^12 in fp16 at most), so the output is rarely rescaled. A wave stops at
 // the last token that one of its rows sees.
 constexpr int TW = 8;                          // waves of a workgroup
@@ -1133,7 +1135,8 @@ __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
 }
 
 // (Launches of their own, 4.3 us for 16 sequences of 4096 tokens, a chain of four loads; 12 us
-// for 777 rows of 28 heads on LDS tiles, 30 MB of parts.)
+// for 777 rows of 28 heads on LDS tiles, 30 MB of parts: vector instructions in 91% of the
+// cycles, most of them to find a tile's parts from the whole batch in every wave.)
 // Joins the parts of a row: HD / 4 lanes, of 4 dims each, take the parts'
 // statistics, as many at a time, then all of them the parts' sums, 8 loads of 16
 // bytes in flight. Part p is row at(p) of part and stat.
