@@ -694,9 +694,9 @@ __global__ __launch_bounds__(64 * W, RT == 1 || HD == 64 ? 3 : 2) void k_kv8_att
 // were 2.7e-4 off where their rounding alone is 2.1e-4 (4096 rows then 730 us for 960). 4096
 // rows after 8192 tokens, 32 heads of 128 in f16, 687 GFLOP (1030 with the second piece) in
 // 955 to 1000 us: the matrix units are busy for 50% of the cycles, vector instructions for
-// 59%, and the clock falls under both. The reference moves only when a score passes it by 2^8 (the weights
-// then reach 2^12 in fp16 at most), so the output is rarely rescaled. A wave stops at
-// the last token that one of its rows sees.
+// 59%, and the clock falls under both. The reference moves only when a score passes it by
+// 2^8 (the weights then reach 2^12 in fp16 at most), so the output is rarely rescaled. A
+// wave stops at the last token that one of its rows sees.
 constexpr int TW = 8;                          // waves of a workgroup
 constexpr uint32_t TILE = 32 * TW;             // its rows
 constexpr uint32_t TK = 64, TS = 3;            // tokens of a stage, stages in LDS
@@ -781,7 +781,8 @@ ZH_DEV bool tile_job(const Kv8Attn &a, uint32_t rows, uint32_t u, TileJob &j) {
 
 template <int HD, int NP, uint32_t F, typename T>
 __global__ __launch_bounds__(64 * TW, 2) void k_kv8_tile(Kv8Attn a) {
-    constexpr int KS = HD / 16, DT = HD / 32, PW = 2;  // k-steps of the scores, 32-dim tiles of the output, weights' pieces
+    constexpr int KS = HD / 16, DT = HD / 32;        // k-steps of the scores, 32-dim tiles of the output
+    constexpr int PW = 2;                            // pieces of the weights
     constexpr uint32_t KROW = t_krow<HD>(), VROW = t_vrow<HD>(), KST = TK * KROW, VST = TK * VROW;  // of a row, a stage
     constexpr uint32_t ROWS = TILE, NT = 64 * TW;
     constexpr uint32_t CPR = HD / 16, PC = TK * CPR;  // 16-code pieces of a row and of a stage's K (or V)
